@@ -85,6 +85,14 @@ class MoELayer(C.Structure):
     ]
 
 
+class PagedKVDesc(C.Structure):
+    """tf_paged_kv."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_uint64), ("position_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("num_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("dtype", C.c_int)]
+
+
 _P = C.c_void_p
 _U32 = C.c_uint32
 _U64 = C.c_uint64
@@ -144,6 +152,17 @@ _PROTOS = {
     "tf_softcap_softmax": ([_P, _P, _I, _P, _U32, _U32, C.c_float, _P], _I),
     "tf_sample": ([_P, _P, _U32, C.c_float, _U32, C.c_float, _U64, _U32, _P, _P], _I),
     "tf_sample_topk64": ([_P, _P, _U32, C.c_float, C.c_float, _U64, _P, _P], _I),
+    "tf_kv_pages_workspace_bytes": ([_U32], C.c_size_t),
+    "tf_kv_pages_resize": ([_P, _P, _P, _U32, _P, _U32, _P, _U32, _P, _U32, _U32, _P, _P, _P, _P, _P, _P, _U32, _P,
+                            C.c_size_t, _P], _I),
+    "tf_rope_frequencies": ([_U32, C.c_double, _I, C.c_double, C.c_double, C.c_double, C.c_double,
+                             C.POINTER(C.c_double), C.POINTER(C.c_double)], _I),
+    "tf_rope_kv_write": ([_P, _P, _U64, _P, _U64, _P, _U64, _P, _U64, C.POINTER(PagedKVDesc), _P, _P, _P, _U32, _I,
+                          C.c_float, _I, _P, _P, C.c_float, _U32, _U32, _P], _I),
+    "tf_shared_prefix_attention_workspace_bytes": ([_P, C.POINTER(PagedKVDesc), _U32, _U32, _U32, _U32, _U32],
+                                                   C.c_size_t),
+    "tf_shared_prefix_attention": ([_P, _P, _U64, C.POINTER(PagedKVDesc), _P, _U32, _P, _U32, _P, _P, _U32, _U32, _U32,
+                                    _U32, C.c_float, _U32, _P, _U64, _P, _P, C.c_size_t, _P], _I),
     "tf_ep_flag_bytes": ([_U32], C.c_size_t),
     "tf_ep_ipc_alloc": ([_P, C.c_size_t, C.POINTER(_P), _P], _I),
     "tf_ep_ipc_open": ([_P, _P, C.POINTER(_P)], _I),

@@ -42,7 +42,7 @@ constexpr int kStageBytes = 2 * kHalfBytes + 4 * kScaleArr;  // 16 KB
 constexpr uint32_t kSpinLimit = 1u << 20;  // bounded mbarrier wait (error flag after)
 
 // Error bits written to the context's device status word.
-enum : uint32_t { kErrMbarTimeout = 1u, kErrBadExpert = 2u, kErrAlign = 4u };
+enum : uint32_t { kErrMbarTimeout = 1u, kErrBadExpert = 2u, kErrAlign = 4u, kErrBadPage = 8u };
 
 // Debug builds (-DTF_CHECKS) verify the alignment of every vector and bulk
 // access before issuing it; a violation records the site and address in the

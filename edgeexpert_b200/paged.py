@@ -1,0 +1,178 @@
+"""Serving a ragged batch: a paged KV cache whose requests have different
+lengths and share one long prefix.
+
+* ``KVPages.encode_resize``          request lengths -> page tables, slots, positions (on the device)
+* ``RotaryKVWrite.encode``           head norms + rotary positions; K and V into the tokens' slots
+* ``SharedPrefixAttention.encode``   attention over the shared prefix and each request's own pages
+
+The operators have no counterpart in the reference, which decodes one sequence
+from a contiguous cache.  Lengths, tables, slots and positions are int32 CUDA
+tensors; nothing is read back, so a step can be captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import (Context, PagedKVDesc, TFError, TF_ERR_INVALID_ARG, TF_OK, lib, ptr, status_string, stream_ptr)
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_SCALINGS = {None: 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4}
+
+
+def _heads(t, what: str) -> int:
+    """Token stride of a [tokens][heads][dim] tensor whose heads lie side by side."""
+    if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise TFError(TF_ERR_INVALID_ARG, f"{what} must be [tokens][heads][dim] with contiguous heads")
+    return t.stride(0)
+
+
+def _int32(**tensors):
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise TFError(TF_ERR_INVALID_ARG, f"{name} must be a contiguous int32 tensor")
+
+
+class PagedKV:
+    """One layer's K and V pools, [page][position][head][dim] tensors of one
+    dtype (fp16 or bf16) and of any strides with dim innermost: a
+    [page][head][position][dim] pool is passed as its transposed view."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+            raise TFError(TF_ERR_INVALID_ARG, "k and v must be alike: [page][position][head][dim], dim innermost")
+        if k.dtype not in _DTYPES:
+            raise TFError(TF_ERR_INVALID_ARG, f"cache dtype {k.dtype}: float16 or bfloat16")
+        self.k, self.v, self.dtype = k, v, k.dtype
+        self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = k.shape
+        self.desc = PagedKVDesc(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), self.num_pages,
+                                self.page_size, self.num_kv_heads, self.head_dim, _DTYPES[k.dtype])
+        self.ref = C.byref(self.desc)
+
+
+class KVPages:
+    """The page tables of a ragged batch (tf_kv_pages_resize)."""
+
+    def __init__(self, context: Context | None = None):
+        self.ctx = context or Context.get(torch.cuda.current_device())
+
+    @staticmethod
+    def workspace_bytes(num_requests: int) -> int:
+        return int(lib().tf_kv_pages_workspace_bytes(num_requests))
+
+    def encode_resize(self, seq_lens, targets, page_table, free_ring, free_state, seq_lens_out, free_state_out,
+                      token_starts, slots, positions, requests, page_size: int, workspace, position_base: int = 0,
+                      stream=None):
+        """Grow or shrink every request to its target length: pages move between
+        `free_ring` and `page_table` [requests][max_pages], and every token added
+        gets its slot, position and request (-1 beyond the last).  seq_lens_out /
+        free_state_out may be seq_lens / free_state.  free_state = {head, count,
+        requests refused, tokens added}."""
+        B, max_tokens = seq_lens.numel(), slots.numel()
+        _int32(seq_lens=seq_lens, targets=targets, page_table=page_table, free_ring=free_ring, free_state=free_state,
+               seq_lens_out=seq_lens_out, free_state_out=free_state_out, token_starts=token_starts, slots=slots,
+               positions=positions, requests=requests)
+        if (targets.numel() != B or seq_lens_out.numel() != B or token_starts.numel() != B + 1
+                or page_table.dim() != 2 or page_table.shape[0] != B or free_state.numel() != 4
+                or free_state_out.numel() != 4 or positions.numel() != max_tokens or requests.numel() != max_tokens):
+            raise TFError(TF_ERR_INVALID_ARG, "KVPages.encode_resize: sizes of the tensors do not agree")
+        st = lib().tf_kv_pages_resize(
+            self.ctx.handle, seq_lens.data_ptr(), targets.data_ptr(), B, page_table.data_ptr(), page_table.shape[1],
+            free_ring.data_ptr(), free_ring.numel(), free_state.data_ptr(), page_size, position_base,
+            seq_lens_out.data_ptr(), free_state_out.data_ptr(), token_starts.data_ptr(), slots.data_ptr(),
+            positions.data_ptr(), requests.data_ptr(), max_tokens, workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), stream_ptr(stream))
+        self.ctx.check(st, "KVPages.encode_resize")
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                     original_context: float = 0.0, low: float = 1.0, high: float = 32.0, device="cuda"):
+    """(radians per position of each pair as a float64 tensor, attention factor)
+    for RotaryKVWrite.  scaling: None, "linear", "base", "ramp" (low / high =
+    turns over the original context below which a pair is slowed fully and
+    above which it is kept) or "bands" (the same, linear in the turns)."""
+    if scaling not in _SCALINGS:
+        raise TFError(TF_ERR_INVALID_ARG, f"rope_frequencies: unknown scaling {scaling!r}")
+    out, mul = (C.c_double * max(1, rotary_dim // 2))(), C.c_double(1.0)
+    st = lib().tf_rope_frequencies(rotary_dim, theta, _SCALINGS[scaling], factor, original_context, low, high, out,
+                                   C.byref(mul))
+    if st != TF_OK:
+        raise TFError(st, f"rope_frequencies: {status_string(st)}")
+    return torch.tensor(list(out)[:rotary_dim // 2], dtype=torch.float64, device=device), mul.value
+
+
+class RotaryKVWrite:
+    """Per-head norms, rotary positions and the write into the paged cache
+    (tf_rope_kv_write)."""
+
+    def __init__(self, context: Context | None = None):
+        self.ctx = context or Context.get(torch.cuda.current_device())
+
+    def encode(self, q, k, v, q_out, kv: PagedKV, slots, positions, inv_freq, rotary_dim: int | None = None,
+               layout: str = "half", attention_factor: float = 1.0, q_weight=None, k_weight=None, norm: bool = False,
+               eps: float = 1e-6, stream=None):
+        """q, q_out [T][heads][dim], k, v [T][kv heads][dim] (views of a fused
+        projection are fine); q_out may be q."""
+        T, nq, hd = q.shape
+        rot = hd if rotary_dim is None else rotary_dim
+        if layout not in _LAYOUTS:
+            raise TFError(TF_ERR_INVALID_ARG, f"RotaryKVWrite.encode: unknown layout {layout!r}")
+        if not (q.dtype == k.dtype == v.dtype == q_out.dtype == kv.dtype):
+            raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: q, k, v, q_out and the cache must have one dtype")
+        shape = (T, kv.num_kv_heads, kv.head_dim)
+        if k.shape != shape or v.shape != shape or q_out.shape != q.shape or hd != kv.head_dim:
+            raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: shapes of q, k, v and the cache do not agree")
+        _int32(slots=slots, positions=positions)
+        if slots.numel() != T or positions.numel() != T or inv_freq.dtype != torch.float64 or inv_freq.numel() * 2 != rot:
+            raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: a slot and position per token, a float64 per pair")
+        for w in (q_weight, k_weight):
+            if w is not None and (w.dtype != torch.bfloat16 or w.numel() != hd or not w.is_contiguous()):
+                raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: norm weights are contiguous bf16 [head_dim]")
+        st = lib().tf_rope_kv_write(
+            self.ctx.handle, q.data_ptr(), _heads(q, "q"), k.data_ptr(), _heads(k, "k"), v.data_ptr(), _heads(v, "v"),
+            q_out.data_ptr(), _heads(q_out, "q_out"), kv.ref, slots.data_ptr(), positions.data_ptr(),
+            inv_freq.data_ptr(), rot, _LAYOUTS[layout], attention_factor, int(norm), ptr(q_weight), ptr(k_weight), eps,
+            T, nq, stream_ptr(stream))
+        self.ctx.check(st, "RotaryKVWrite.encode")
+
+
+class SharedPrefixAttention:
+    """Causal attention of a ragged batch behind a shared prefix
+    (tf_shared_prefix_attention)."""
+
+    def __init__(self, context: Context | None = None):
+        self.ctx = context or Context.get(torch.cuda.current_device())
+
+    def workspace_bytes(self, kv: PagedKV, num_q_heads: int, tokens: int, num_requests: int, prefix_len: int,
+                        max_query: int) -> int:
+        """Enough for every call with at most these sizes."""
+        return int(lib().tf_shared_prefix_attention_workspace_bytes(self.ctx.handle, kv.ref, num_q_heads, tokens,
+                                                                    num_requests, prefix_len, max_query))
+
+    def encode(self, q, kv: PagedKV, page_table, seq_lens, token_starts, out, workspace, prefix_pages=None,
+               prefix_len: int = 0, max_query: int = 1, scale: float | None = None, window: int = 0, lse=None,
+               stream=None):
+        """q, out [T][heads][dim]: request b's last positions are tokens
+        token_starts[b] .. token_starts[b+1].  `lse` (optional): float32
+        [T][heads].  scale None: dim ** -0.5."""
+        T, nq, hd = q.shape
+        B = seq_lens.numel()
+        if q.dtype != kv.dtype or out.dtype != kv.dtype or out.shape != q.shape or hd != kv.head_dim:
+            raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: q, out and the cache do not agree")
+        _int32(page_table=page_table, seq_lens=seq_lens, token_starts=token_starts)
+        if page_table.dim() != 2 or page_table.shape[0] != B or token_starts.numel() != B + 1:
+            raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: sizes of the tensors do not agree")
+        if prefix_len:
+            if prefix_pages is None or prefix_pages.numel() * kv.page_size < prefix_len:
+                raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: too few prefix pages")
+            _int32(prefix_pages=prefix_pages)
+        if lse is not None and (lse.dtype != torch.float32 or lse.numel() != T * nq or not lse.is_contiguous()):
+            raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: lse must be contiguous float32 [T][heads]")
+        st = lib().tf_shared_prefix_attention(
+            self.ctx.handle, q.data_ptr(), _heads(q, "q"), kv.ref, ptr(prefix_pages), prefix_len,
+            page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), token_starts.data_ptr(), B, max_query, T,
+            nq, hd ** -0.5 if scale is None else scale, window, out.data_ptr(), _heads(out, "out"), ptr(lse),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream_ptr(stream))
+        self.ctx.check(st, "SharedPrefixAttention.encode")

@@ -467,6 +467,119 @@ TF_API tf_status tf_sample(tf_context* ctx, const void* probs, uint32_t V, float
 TF_API tf_status tf_sample_topk64(tf_context* ctx, const void* probs, uint32_t V, float temperature, float top_p,
                                   uint64_t seed, void* out_token, void* stream);
 
+/* ---- serving a ragged batch: paged KV cache, rotary positions, shared prefix -----------------
+ * No reference counterpart (the reference decodes one sequence from a contiguous cache).
+ * B requests of different lengths share one pool of KV pages and, optionally, one long
+ * prefix.  A step is
+ *   tf_kv_pages_resize           lengths -> pages, token_starts, and per new token its slot,
+ *                                position and request, all on the device
+ *   tf_rope_kv_write             (per layer) head norms + rotation at each token's position,
+ *                                q to q_out, k and v to the tokens' slots
+ *   tf_shared_prefix_attention   (per layer) attention over the shared prefix, read once for
+ *                                the whole batch, and each request's own pages
+ * Lengths, page tables, slots and positions are int32 on the device; nothing is read back. */
+typedef enum { TF_DTYPE_F16 = 0, TF_DTYPE_BF16 = 1 } tf_dtype;
+
+/* A pool of `num_pages` pages of `page_size` positions.  Element (page p, position i, KV head
+ * h, dim e) of K is k[p*page_stride + i*position_stride + h*head_stride + e], strides in
+ * elements and multiples of 8, k and v 16-byte aligned: [page][position][head] and
+ * [page][head][position] pools, or K and V interleaved in a page, are all strides.  slot =
+ * page*page_size + i, num_pages*page_size < 2^31.  head_dim: a multiple of 8 up to 512. */
+typedef struct {
+    void* k;
+    void* v;
+    uint64_t page_stride, position_stride, head_stride;
+    uint32_t num_pages, page_size, num_kv_heads, head_dim;
+    tf_dtype dtype;
+} tf_paged_kv;
+
+/* Brings every request from seq_lens[b] to targets[b] positions.  pages(n) = ceil(n / page_size).
+ *   target < 0: left alone; target > max_pages*page_size: refused.
+ *   shorter (0 when finished): its trailing pages go to the back of the free ring.
+ *   longer: pages are taken from the front of the ring in request order and appended to
+ *     page_table[b] (int32 [num_requests][max_pages]); a request whose pages, summed with
+ *     those that all earlier requests ask for, exceed the free pages, or whose tokens exceed
+ *     max_tokens in the same way, is refused.  One that needs no page is only bound by tokens.
+ * Pages handed back in a call can be taken from the next call on.  Refused requests keep
+ * their length.  Outputs: seq_lens_out[b]; token_starts[num_requests + 1], the exclusive sum
+ * of the tokens added; for token i of request b's additions, in request order:
+ *   slots[i] = page*page_size + offset, positions[i] = position_base + index in the request,
+ *   requests[i] = b; entries from the last token up to max_tokens are -1.
+ * free_ring int32[num_pages] holds free page ids at [head, head + count) mod num_pages;
+ * free_state / free_state_out int32[4] = {head, count, requests refused, tokens added} (the
+ * last two are outputs).  seq_lens_out and free_state_out may be the input buffers.  With
+ * separate ones the call can be repeated with the same result.  max_tokens may be 0. */
+TF_API size_t tf_kv_pages_workspace_bytes(uint32_t num_requests);
+TF_API tf_status tf_kv_pages_resize(tf_context* ctx, const void* seq_lens, const void* targets, uint32_t num_requests,
+                                    void* page_table, uint32_t max_pages, void* free_ring, uint32_t num_pages,
+                                    const void* free_state, uint32_t page_size, uint32_t position_base,
+                                    void* seq_lens_out, void* free_state_out, void* token_starts, void* slots,
+                                    void* positions, void* requests, uint32_t max_tokens, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+typedef enum { TF_ROPE_HALF = 0, TF_ROPE_INTERLEAVED = 1 } tf_rope_layout;
+typedef enum {
+    TF_ROPE_SCALE_NONE = 0,
+    TF_ROPE_SCALE_LINEAR = 1, /* every frequency / factor */
+    TF_ROPE_SCALE_BASE = 2,   /* theta * factor^(rot / (rot - 2)) */
+    TF_ROPE_SCALE_RAMP = 3,   /* pairs of more than beta_fast turns over original_context keep their
+                               * frequency, those of fewer than beta_slow get it / factor, linear in
+                               * the pair index between; attention factor 0.1 ln(factor) + 1 */
+    TF_ROPE_SCALE_BANDS = 4   /* the same with low_factor / high_factor turns, linear in the turns;
+                               * attention factor 1 */
+} tf_rope_scaling;
+
+/* HOST function: inv_freq[i] (double, rotary_dim/2) = radians per position of pair i, and the
+ * factor that cos and sin are to be multiplied by.  low / high: beta_slow / beta_fast or
+ * low_factor / high_factor.  rotary_dim even, > 2 for TF_ROPE_SCALE_BASE. */
+TF_API tf_status tf_rope_frequencies(uint32_t rotary_dim, double theta, tf_rope_scaling scaling, double factor,
+                                     double original_context, double low, double high, double* inv_freq,
+                                     double* attention_factor);
+
+/* For T tokens, q [T][num_q_heads][head_dim], k and v [T][num_kv_heads][head_dim] (rows of heads
+ * contiguous, token strides in elements), all of kv->dtype:
+ *   norm != 0: x = x * rsqrt(mean(x^2) + eps) * w per head (w BF16, NULL = 1; v never has one)
+ *   the first rotary_dim dims of q and k: pairs (i, i + rotary_dim/2) or (2i, 2i + 1) turned by
+ *   positions[t] * inv_freq[i] (device double[rotary_dim/2]), cos and sin times attention_factor
+ * in fp32, rounded once; angles are reduced in 64 bits, so any int32 position keeps full accuracy.
+ * q goes to q_out (which may be q), k and v to the pool at slots[t].  A token with slots[t] < 0 is
+ * padding: its q_out row is 0 and nothing else is written.  A slot beyond the pool raises the
+ * context's device error bit and is treated the same way.  Two tokens must not share a slot.
+ * num_q_heads may be 0.  tf_qkv_epilogue is the form for one position and a contiguous cache (it
+ * rounds the norm to fp16 before it rotates). */
+TF_API tf_status tf_rope_kv_write(tf_context* ctx, const void* q, uint64_t q_stride, const void* k, uint64_t k_stride,
+                                  const void* v, uint64_t v_stride, void* q_out, uint64_t q_out_stride,
+                                  const tf_paged_kv* kv, const void* slots, const void* positions,
+                                  const void* inv_freq, uint32_t rotary_dim, tf_rope_layout layout,
+                                  float attention_factor, int norm, const void* q_weight, const void* k_weight,
+                                  float eps, uint32_t T, uint32_t num_q_heads, void* stream);
+
+/* Causal attention of a ragged batch behind a shared prefix.  Request b's query tokens are
+ * q[token_starts[b] .. token_starts[b+1]) (q [T][num_q_heads][head_dim], token stride q_stride
+ * elements), its n_b last positions: token j stands at p = prefix_len + seq_lens[b] - n_b + j and
+ * sees key positions in (p - window, p] (window 0: all up to p).  Positions below prefix_len
+ * are those of prefix_pages (int32[pages(prefix_len)], shared by every request, any length);
+ * position prefix_len + s is position s of page_table[b].  seq_lens counts the request's own
+ * positions, this step's tokens among them (their K and V already written).
+ *   out[t][h] = sum_p softmax_p(scale q.k_p) v_p, KV head h / (num_q_heads / num_kv_heads);
+ *   lse[t][h] (float, optional) = log sum_p exp(scale q.k_p).
+ * A row that sees nothing gives out 0 and lse -infinity; so do tokens from token_starts[B] up to T.
+ * max_query: host bound on any n_b (tokens beyond it give 0 and the device error bit, as does
+ * a page id outside the pool, whose positions are left out).  Positions that no row of the batch
+ * (for the prefix) or of the request (for its own pages) sees may hold anything, NaN included.
+ * scale > 0.  q, out 16-byte aligned, strides multiples of 8.  Any number of query heads per KV
+ * head.  workspace: caller-owned device scratch, contents arbitrary, one per concurrent call. */
+TF_API size_t tf_shared_prefix_attention_workspace_bytes(const tf_context* ctx, const tf_paged_kv* kv,
+                                                         uint32_t num_q_heads, uint32_t T, uint32_t num_requests,
+                                                         uint32_t prefix_len, uint32_t max_query);
+TF_API tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_stride, const tf_paged_kv* kv,
+                                            const void* prefix_pages, uint32_t prefix_len, const void* page_table,
+                                            uint32_t max_pages, const void* seq_lens, const void* token_starts,
+                                            uint32_t num_requests, uint32_t max_query, uint32_t T,
+                                            uint32_t num_q_heads, float scale, uint32_t window, void* out,
+                                            uint64_t out_stride, void* lse, void* workspace, size_t workspace_bytes,
+                                            void* stream);
+
 /* ---- expert parallelism (routed experts sharded over GPUs) ------------------------------
  * No reference counterpart (the reference streams experts from SSD on one GPU).
  * Experts are sharded in contiguous id ranges of experts_per_rank; the
