@@ -523,6 +523,36 @@ def test_attention_of_extreme_scores(cuda, counts, dtype, hd):
     batch.check(*batch.run())
 
 
+@pytest.mark.parametrize("counts,window,hd", [([3, 1], 0, 256), ([3, 2], 40, 64), ([90, 4], 0, 128), ([1] * 40, 64, 128)])
+def test_attention_of_keys_that_others_see(cuda, counts, window, hd):
+    """Infinities and NaN in keys and values that only some rows of a tile see
+    (the next token of a draft, a prefix position out of one row's window): the
+    others are as if they were not there, and those that see them are not finite."""
+    lens = [c + 13 + 5 * i for i, c in enumerate(counts)]
+    batch = Batch(100, lens, counts, 8, 4, hd, "fp16", 16, seed=11)
+    last = lens[0] - 1  # the last token of the first request, and a position late in the prefix
+    spots = [(int(batch.table[0, last // 16]), last % 16)]
+    if window:
+        spots.append((int(batch.prefix_pages[75 // 16]), 75 % 16))
+    for i, (page, at) in enumerate(spots):
+        batch.v[page, at, :, 0] = float("inf")
+        batch.v[page, at, 0, 1] = float("nan")
+        batch.k[page, at, 1, 0] = float("nan")
+    out, lse = (f64(x) for x in batch.run(window))
+    shared = f64(batch.both[0])
+    for b, (length, n) in enumerate(zip(lens, counts)):
+        own = f64(batch.both[1 + b])
+        keys, values = (np.concatenate([shared[i], own[i]]) for i in (0, 1))
+        at = 100 + length - n + np.arange(n)
+        t = slice(batch.starts[b], batch.starts[b + 1])
+        ro, rl, A, s = attention_reference(f64(batch.q[t]), keys, values, at, batch.scale, window)
+        hit = (at >= 100 + last) & (b == 0)
+        if window:
+            hit |= (at >= 75) & (at < 75 + window)
+        assert (np.abs(out[t] - ro)[~hit] <= ((2 * U[torch.float16] + 2 * s + 16 * E32) * A + 1e-4)[~hit]).all()
+        assert not np.isfinite(out[t][hit][..., 0]).any() and not np.isfinite(lse[t][hit][:, 2:4]).any()
+
+
 def test_attention_by_another_stream_strides_and_repeats(cuda):
     """q and out as slices of wider rows, another stream, no lse; the same bits every time."""
     batch = Batch(700, [90, 5, 300], [2, 1, 3], 16, 4, 128, "fp16", 16, seed=8)
