@@ -8,6 +8,7 @@
 #include <math.h>
 
 #include "tf_prefix_stream.cuh"
+#include "tf_prefix_tensor.cuh"
 
 using namespace tf;
 
@@ -118,6 +119,24 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_parts_kernel(const __gri
             const int rows = max(0, min(p.starts[p.B], p.T_tokens)) * p.G, row_tiles = (rows + p.stream.rows - 1) / p.stream.rows;
             add_stream(2, (kvh * row_tiles + grow / p.stream.rows) * prefix_tiles, prefix_tiles, grow % p.stream.rows);
         }
+        if (p.tensor.ctas) {
+            const int tile = grow / kTcRows, units = (p.tensor.base[tile + 1] - p.tensor.base[tile]) / p.nkv;
+            if (units) {
+                const int TU = p.tensor.base[(int)(((long long)p.T_tokens * p.G + kTcRows - 1) / kTcRows)];
+                const int unit = p.tensor.base[tile] + kvh * units;
+                const int c0 = cta_of(unit, TU, p.tensor.ctas), c1 = cta_of(unit + units - 1, TU, p.tensor.ctas);
+                if (c0 == c1 && by_tensor(p, r)) {  // the tensor kernel has written the result
+                    const float mark = p.tensor.first_md[row].x;
+                    if (mark != mark) attend_alone(p, b, r, j, h);
+                    continue;
+                }
+                parts.n[2] = 1;
+                parts.place[2] = row;
+                parts.n[3] = c1 - c0;
+                parts.place[3] = (long long)(c0 + 1) * kTcRows + grow % kTcRows;
+                parts.step[3] = kTcRows;
+            }
+        }
         const float* src[4] = {p.stream.first, p.stream.cont, p.tensor.first,
                                p.prefix_by_stream ? p.stream.cont : p.tensor.cont};
         const float2* src_md[4] = {p.stream.first_md, p.stream.cont_md, p.tensor.first_md,
@@ -179,8 +198,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_parts_kernel(const __gri
 }
 
 // ---- sizes and the workspace ---------------------------------------------------------
+// Rows up to which a request (or the whole batch, for the prefix) is the stream kernel's.
+constexpr int kFewRows = 32;
+
 struct Shape {
-    int hd, nt, stream_keys, stream_rows, stream_ctas, tensor_ctas;
+    int hd, tensor_above, nt, stream_keys, stream_rows, stream_ctas, tensor_ctas;
     bool prefix_by_stream;
 };
 
@@ -216,8 +238,12 @@ Shape shape_of_call(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, u
     const long long G = nq / kv->num_kv_heads;
     const long long own = std::min<long long>(max_query, T) * G;
     Shape s = shape_for(ctx, kv->head_dim, own);
-    s.prefix_by_stream = true;
-    s.tensor_ctas = ctx->num_sms;
+    const bool tensor = kv->head_dim <= 256;
+    s.prefix_by_stream = !tensor || T * G <= kFewRows;
+    // nothing for the tensor cores: no prefix of theirs and no request with many rows
+    const bool used = tensor && ((prefix_len && !s.prefix_by_stream) || own > kFewRows);
+    s.tensor_above = tensor ? kFewRows : 0x7FFFFFFF;
+    s.tensor_ctas = used ? ctx->num_sms : 0;
     return s;
 }
 
@@ -235,7 +261,7 @@ Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint
     };
     const size_t rows = (size_t)T * nq, G = nq / kv->num_kv_heads;
     // either kernel's grid and tile may be smaller in a call, never larger
-    const size_t cont[2] = {(size_t)ctx->num_sms * 2 * 64, (size_t)s.tensor_ctas * kTcRows};
+    const size_t cont[2] = {(size_t)ctx->num_sms * 2 * 64, (size_t)ctx->num_sms * kTcRows};
     const size_t bases[2] = {B + 1, (size_t)T * G / kTcRows + 2};
     for (int k = 0; k < 2; ++k) {
         l.base[k] = take(bases[k] * sizeof(int));
@@ -263,9 +289,30 @@ tf_status launch_stream(tf_context* ctx, const AttnParams<T>& p, cudaStream_t cs
     return cuda_check(ctx, cudaGetLastError(), name);
 }
 
+template <typename T, int HD>
+tf_status launch_tensor(tf_context* ctx, const AttnParams<T>& p, cudaStream_t cs, const char* name) {
+    using S = TensorShape<HD>;
+    static bool configured[64] = {};  // per instantiation, per device
+    const int dev = ctx->device & 63;
+    if (!configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(attention_many_rows_kernel<T, HD>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        if (e != cudaSuccess) return cuda_check(ctx, e, name);
+        configured[dev] = true;
+    }
+    attention_many_rows_kernel<T, HD><<<p.tensor.ctas, S::kThreads, S::kSmem, cs>>>(p);
+    return cuda_check(ctx, cudaGetLastError(), name);
+}
+
 template <typename T>
 tf_status launch(tf_context* ctx, const AttnParams<T>& p, const Shape& s, cudaStream_t cs, const char* name) {
     tf_status st = TF_OK;
+    if (s.tensor_ctas) {
+        st = s.hd == 64    ? launch_tensor<T, 64>(ctx, p, cs, name)
+             : s.hd == 128 ? launch_tensor<T, 128>(ctx, p, cs, name)
+                           : launch_tensor<T, 256>(ctx, p, cs, name);
+        if (st) return st;
+    }
     if (s.hd == 64)
         st = s.nt == 1 ? launch_stream<T, 64, 1>(ctx, p, cs, name) : launch_stream<T, 64, 4>(ctx, p, cs, name);
     else if (s.hd == 128)
@@ -362,7 +409,7 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
                                                                                               max_query - window + 1))
                              : 0;
         p.prefix_by_stream = shape.prefix_by_stream;
-        p.tensor_above = 0x7FFFFFFF;
+        p.tensor_above = shape.tensor_above;
         uint8_t* w = static_cast<uint8_t*>(workspace);
         Parts* parts[2] = {&p.stream, &p.tensor};
         for (int k = 0; k < 2; ++k) {

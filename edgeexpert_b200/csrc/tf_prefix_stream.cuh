@@ -206,13 +206,11 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
         }
     };
 
-    uint32_t masks[kStages];  // existing keys of the units in flight, oldest first
     look_up();
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
         issue(i);
         cp_async_commit();
-        masks[i] = next_mask;
         look_up();
     }
 
@@ -266,7 +264,7 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
                     }
                 }
                 row_lo[nt][i] = lo;
-                row_hi[nt][i] = hi;
+                row_hi[nt][i] = min(hi, cur.hi);
                 m[nt][i] = -INFINITY;
                 d[nt][i] = 0.f;
             }
@@ -354,7 +352,6 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
         const int fill = stage == 0 ? kStages - 1 : stage - 1;
         issue(fill);
         cp_async_commit();
-        masks[kStages - 1] = next_mask;
         look_up();
         cp_async_wait<kStages - 1>();
         __syncwarp();
@@ -373,7 +370,6 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
             for (int nt = 0; nt < NT; ++nt) mma_16x8<T>(ks & 1 ? s2[nt] : s[nt], a, qf[ks][nt][0], qf[ks][nt][1]);
         }
         const int key0 = cur.lo + cur.tile * S::kKeys + warp * 16;
-        const uint32_t mask = masks[0];
         uint32_t pf[NT][2];
         bool grew = false;
         float keep[NT][2];
@@ -382,7 +378,7 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = key0 + g + 8 * (i >> 1);
-                const bool ok = ((mask >> (g + 8 * (i >> 1))) & 1) && key >= row_lo[nt][i & 1] && key < row_hi[nt][i & 1];
+                const bool ok = key >= row_lo[nt][i & 1] && key < row_hi[nt][i & 1];
                 s[nt][i] = ok ? (s[nt][i] + s2[nt][i]) * sc : -INFINITY;
             }
 #pragma unroll
@@ -419,8 +415,6 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
             for (int nt = 0; nt < NT; ++nt) mma_16x8<T>(acc[mt][nt], a, pf[nt][0], pf[nt][1]);
         }
         __syncwarp();  // before this stage is filled again
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) masks[i] = masks[i + 1];
         stage = stage == kStages - 1 ? 0 : stage + 1;
         if (cur.tile == cur.tiles - 1 || u == u1 - 1) {
             end_job();

@@ -564,8 +564,8 @@ TF_API tf_status tf_rope_kv_write(tf_context* ctx, const void* q, uint64_t q_str
  *   out[t][h] = sum_p softmax_p(scale q.k_p) v_p, KV head h / (num_q_heads / num_kv_heads);
  *   lse[t][h] (float, optional) = log sum_p exp(scale q.k_p).
  * A row that sees nothing gives out 0 and lse -infinity; so do tokens from token_starts[B] up to T.
- * max_query: host bound on any n_b (tokens beyond it give 0 and the device error bit, as does
- * a page id outside the pool, whose positions are left out).  Positions that no row of the batch
+ * max_query: host bound on any n_b (tokens beyond it give 0 and the device error bit).  A page id
+ * outside the pool is not read and raises the bit too; rows that see it are unspecified.  Positions that no row of the batch
  * (for the prefix) or of the request (for its own pages) sees may hold anything, NaN included.
  * scale > 0.  q, out 16-byte aligned, strides multiples of 8.  Any number of query heads per KV
  * head.  workspace: caller-owned device scratch, contents arbitrary, one per concurrent call. */
