@@ -14,7 +14,8 @@ using namespace tf;
 
 namespace {
 
-constexpr int kJoinWarps = 8;
+constexpr int kThreads = 256;  // of the parts kernel: 8 warps, 255 registers a thread
+constexpr int kJoinRows = 128;  // rows a joining CTA looks at, at most
 
 // One warp, one row, key by key: the definition.  Only for rows whose joined
 // result is not finite: an infinity or NaN in a key that the row does not see,
@@ -62,121 +63,270 @@ __device__ void attend_alone(const AttnParams<T>& p, int b, const Request& r, in
     if (lane == 0 && p.lse) p.lse[(long long)t * p.nq + h] = d == 0.f ? -INFINITY : m + logf(d);
 }
 
-// The parts of one row, numbered.
-struct RowParts {
-    int n[4];             // first, cont of the stream kernel; first, cont of the tensor kernel
-    long long place[4];   // row of the first of them
-    int step[4];          // rows from one to the next
-};
+// Nanoseconds of an SM that a unit takes, for dealing the SMs to the two kinds
+// of work.  A streamed unit is bound by memory: 16 keys of K and V at an SM's
+// share of the bandwidth (6450 / 148 bytes a nanosecond).  A tensor unit is 64
+// (head_dim 256) or 128 keys for 128 rows.
+__host__ __device__ constexpr float few_unit_ns(int hd) { return 16.f * 4.f * hd / 43.6f; }
+__host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 64 ? 900.f : 700.f; }
 
-// Joins the parts of every row: one CTA per token, a warp per head.
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_parts_kernel(const __grid_constant__ AttnParams<T> p,
-                                                                     int stream_keys) {
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    // most batches have one token a request, and then b = t
-    int b = min(t, p.B - 1);
-    if (!(p.starts[b] <= t && t < p.starts[b + 1])) b = request_at(p, t);
-    Request r;
-    int j = 0;
-    bool live = b < p.B;
-    if (live) {
-        r = request_of(p, b);
-        j = t - r.start;
-        if (j >= r.used) {
-            live = false;
-            if (threadIdx.x == 0) atomicOr(p.err, kErrBadPage);
+// All parts of all rows, one CTA per SM.  Every CTA sums the units of both kinds
+// over the batch and finds its share: the first CTAs take the tensor cores' jobs,
+// as many as these need to finish when the others have streamed the rest.
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __grid_constant__ AttnParams<T> p) {
+    using S = StreamShape<HD, NT>;
+    extern __shared__ uint8_t raw[];
+    __shared__ int red[32], s_seg[S::kWarps], s_at[S::kWarps], s_tile, s_tile_at, s_tile_units;
+    __shared__ TensorBarriers bar;
+    __shared__ __align__(8) uint64_t full[S::kBars];
+    const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
+    const int grid = gridDim.x, cta = blockIdx.x;
+    constexpr bool kTensor = HD <= 256;
+
+    // thread i looks after requests [i*per, (i+1)*per) and a share of the row tiles
+    const int per = (p.B + kThreads - 1) / kThreads;
+    const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
+    int few_before, many_before = 0, many = 0, i0 = 0, i1 = 0;
+    const int few = stream_units<T, HD, NT>(p, red, b0, b1, few_before);
+    if constexpr (kTensor) {
+        const bool any = !p.prefix_few && (p.prefix_len || p.max_query * p.G > p.many_above);
+        const int row_tiles = any ? (int)(((long long)p.T_tokens * p.G + kTcRows - 1) / kTcRows) : 0;
+        const int per_tile = (row_tiles + kThreads - 1) / kThreads;
+        i0 = min(row_tiles, (int)threadIdx.x * per_tile);
+        i1 = min(row_tiles, i0 + per_tile);
+        if (any) many = all_tensor_units<T, HD>(p, red, i0, i1, many_before);
+    }
+    int many_ctas = 0;
+    if (many) {
+        const float m = many * many_unit_ns(HD), f = few * few_unit_ns(HD);
+        many_ctas = few ? max(1, min(grid - 1, __float2int_rn(grid * (m / (m + f))))) : grid;
+        many_ctas = min(many_ctas, many);
+    }
+    // no worker without a unit (a part is read back for every worker between a job's
+    // first and last); the few there may be are spread over the CTAs
+    const int few_ctas = grid - many_ctas, workers = min(few, few_ctas * S::kWarps);
+    if (cta == 0) {
+        if (threadIdx.x == 0) *p.deal = {few, workers, many, many_ctas};
+        StreamCursor c;
+        int at = few_before;
+        for (c.seg = b0; c.seg < b1; ++c.seg) {
+            stream_segment<T, HD, NT>(p, c);
+            p.few.base[c.seg] = at;
+            at += c.row_tiles * c.tiles * p.nkv;
+        }
+        if constexpr (kTensor) {
+            at = many_before;
+            for (int i = i0; i < i1; ++i) {
+                p.many.base[i] = at;
+                at += tensor_units<T, HD>(p, i) * p.nkv;
+                p.many.base[i + 1] = at;
+            }
         }
     }
-    const int prefix_tiles = (p.prefix_len - p.prefix_lo + stream_keys - 1) / stream_keys;
-    const int SU = p.stream.base[p.B];
-    for (int h = threadIdx.x >> 5; h < p.nq; h += kJoinWarps) {
-        const int kvh = h / p.G, grow = t * p.G + h % p.G;
-        const long long row = (long long)t * p.nq + h;
+    if (cta < many_ctas) {
+        if constexpr (kTensor) {
+            const int u0 = unit_begin(cta, many, many_ctas), u1 = unit_begin(cta + 1, many, many_ctas);
+            int at = many_before;
+            for (int i = i0; i < i1; ++i) {
+                const int units = tensor_units<T, HD>(p, i);
+                if (u0 >= at && u0 < at + units * p.nkv) {
+                    s_tile = i;
+                    s_tile_at = at;
+                    s_tile_units = units;
+                }
+                at += units * p.nkv;
+            }
+            __syncthreads();
+            tensor_cta<T, HD>(p, smem, bar, u0, u1, s_tile, s_tile_at, s_tile_units, cta);
+        }
+        return;
+    }
+    const int mine = cta - many_ctas;  // this CTA's workers: mine, mine + few_ctas, ...
+    if (mine >= workers) return;
+    auto begin_of = [&](int w) { return unit_begin(min(mine + w * few_ctas, workers), few, workers); };
+    {
+        StreamCursor c;
+        c.seg = -1;
+        stream_segment<T, HD, NT>(p, c);
+        const int prefix_units = c.row_tiles * c.tiles * p.nkv;
+        if (threadIdx.x < S::kWarps && begin_of(threadIdx.x) < prefix_units) {
+            s_seg[threadIdx.x] = -1;
+            s_at[threadIdx.x] = 0;
+        }
+        int at = few_before;
+        for (c.seg = b0; c.seg < b1; ++c.seg) {
+            stream_segment<T, HD, NT>(p, c);
+            const int units = c.row_tiles * c.tiles * p.nkv;
+            for (int w = 0; units && w < S::kWarps; ++w) {
+                const int u = begin_of(w);
+                if (u >= at && u < at + units) {
+                    s_seg[w] = c.seg;
+                    s_at[w] = at;
+                }
+            }
+            at += units;
+        }
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kBars; ++i) mbar_init(&full[i], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    const int warp = threadIdx.x >> 5;
+    const int worker = mine + warp * few_ctas;
+    if (warp >= S::kWarps || worker >= workers) return;
+    const int u0 = unit_begin(worker, few, workers), u1 = unit_begin(worker + 1, few, workers);
+    StreamCursor cur;
+    cur.seg = s_seg[warp];
+    stream_segment<T, HD, NT>(p, cur);
+    const int in = u0 - s_at[warp];
+    cur.tile = in % cur.tiles;
+    cur.rt = in / cur.tiles % cur.row_tiles;
+    cur.kvh = in / cur.tiles / cur.row_tiles;
+    stream_warp<T, HD, NT>(p, smem + warp * S::kTiles * S::kTile, full + warp * S::kTiles, cur, u0, u1, worker);
+}
+
+// The parts of one row: own keys' first and cont, then (prefix or tensor
+// cores') first and cont; cont places are a worker's rows apart.
+struct RowParts {
+    int n[4], place[4];
+    int b, j;  // request and token in it; b < 0: nothing to do, b = the batch's size: a row of zeros
+};
+
+// Joins the parts of every row.  A thread finds the parts of a row (and rows
+// that are finished drop out), a warp adds them up.
+template <typename T>
+__global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__ AttnParams<T> p, int rows_per_cta) {
+    __shared__ RowParts rows[kJoinRows];
+    const int lane = threadIdx.x & 31;
+    const int row0 = blockIdx.x * rows_per_cta, n_rows = min(rows_per_cta, p.T_tokens * p.nq - row0);
+    const Deal deal = *p.deal;
+    for (int i = threadIdx.x; i < n_rows; i += blockDim.x) {
+        RowParts x = {};
+        const int row = row0 + i, t = row / p.nq, h = row - t * p.nq, kvh = h / p.G, in_group = h - kvh * p.G;
+        // most batches have one token a request, and then b = t
+        int b = min(t, p.B - 1);
+        if (!(p.starts[b] <= t && t < p.starts[b + 1])) b = request_at(p, t);
+        x.b = b;
+        if (b < p.B) {
+            const Request r = request_of(p, b);
+            x.j = t - r.start;
+            if (x.j >= r.used) {
+                atomicOr(p.err, kErrBadPage);
+                x.b = p.B;
+            } else {
+                auto add_few = [&](int which, int unit, int tiles, int in_tile) {
+                    const int c0 = worker_of(unit, deal.few_units, deal.few_workers);
+                    const int c1 = worker_of(unit + tiles - 1, deal.few_units, deal.few_workers);
+                    x.n[which] = 1;
+                    x.place[which] = row;
+                    x.n[which + 1] = c1 - c0;
+                    x.place[which + 1] = (c0 + 1) * p.few.rows + in_tile;
+                };
+                const bool many = is_many(p, r);
+                const int from = own_lo(p, r), tiles = (r.len - (from & ~(kMaxRun - 1)) + 15) / 16;
+                if (r.len > from && !many) {
+                    const int own = x.j * p.G + in_group, row_tiles = (r.used * p.G + p.few.rows - 1) / p.few.rows;
+                    add_few(0, p.few.base[b] + (kvh * row_tiles + own / p.few.rows) * tiles, tiles, own % p.few.rows);
+                }
+                const int group_row = t * p.G + in_group;
+                const int prefix_tiles = (p.prefix_len - (p.prefix_lo & ~(kMaxRun - 1)) + 15) / 16;
+                if (p.prefix_few && p.prefix_len > p.prefix_lo) {
+                    const int live = max(0, min(p.starts[p.B], p.T_tokens)) * p.G;
+                    const int row_tiles = (live + p.few.rows - 1) / p.few.rows;
+                    add_few(2, (kvh * row_tiles + group_row / p.few.rows) * prefix_tiles, prefix_tiles,
+                            group_row % p.few.rows);
+                }
+                if (deal.many_workers) {
+                    const int tile = group_row / kTcRows, units = (p.many.base[tile + 1] - p.many.base[tile]) / p.nkv;
+                    if (units) {
+                        const int unit = p.many.base[tile] + kvh * units;
+                        const int c0 = worker_of(unit, deal.many_units, deal.many_workers);
+                        const int c1 = worker_of(unit + units - 1, deal.many_units, deal.many_workers);
+                        x.n[2] = 1;
+                        x.place[2] = row;
+                        x.n[3] = c1 - c0;
+                        x.place[3] = (c0 + 1) * kTcRows + group_row % kTcRows;
+                        if (c0 == c1 && many) {  // written where it was computed, unless it was not finite
+                            const float mark = p.many.first_md[row].x;
+                            x.n[2] = 0;
+                            x.b = mark == mark ? -1 : b;
+                            x.n[0] = mark == mark ? 0 : -1;
+                        }
+                    }
+                }
+            }
+        }
+        rows[i] = x;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x >> 5; i < n_rows; i += blockDim.x >> 5) {
+        const RowParts& x = rows[i];
+        if (x.b < 0) continue;
+        const int row = row0 + i, t = row / p.nq, h = row - t * p.nq;
         T* out = p.out + t * p.out_stride + (long long)h * p.hd;
-        if (!live) {
-            for (int e = lane; e < p.hd; e += 32) out[e] = from_float<T>(0.f);
-            if (lane == 0 && p.lse) p.lse[row] = -INFINITY;
-            continue;
-        }
-        RowParts parts = {};
-        auto add_stream = [&](int which, int unit, int tiles, int in_tile) {
-            const int c0 = cta_of(unit, SU, p.stream.ctas), c1 = cta_of(unit + tiles - 1, SU, p.stream.ctas);
-            parts.n[which] = 1;
-            parts.place[which] = row;
-            if (c1 > c0) {  // only one of a row's two stream jobs can be in a given cont place, but both may have some
-                parts.n[which + 1] = c1 - c0;
-                parts.place[which + 1] = (long long)(c0 + 1) * p.stream.rows + in_tile;
-                parts.step[which + 1] = p.stream.rows;
+        const int n0 = max(0, x.n[0]), n1 = n0 + x.n[1], n2 = n1 + x.n[2], n = n2 + x.n[3];
+        float top = -INFINITY, d = 0.f;
+        constexpr int E = kMaxPagedHeadDim / 128;
+        float4 o[E];
+#pragma unroll
+        for (int u = 0; u < E; ++u) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int base = 0; base < n; base += 32) {
+            // lane i has part base + i
+            const int part = base + lane;
+            const float* src = nullptr;
+            float2 md = make_float2(-INFINITY, 0.f);
+            if (part < n) {
+                const int k = part < n0 ? 0 : (part < n1 ? 1 : (part < n2 ? 2 : 3));
+                const int at = part - (k == 0 ? 0 : (k == 1 ? n0 : (k == 2 ? n1 : n2)));
+                const bool own_cont = k == 1 || (k == 3 && p.prefix_few);
+                const long long place = x.place[k] + (long long)at * (own_cont ? p.few.rows : kTcRows);
+                src = (k == 0 ? p.few.first : (k == 2 ? p.many.first : (own_cont ? p.few.cont : p.many.cont))) + place * p.hd;
+                md = (k == 0 ? p.few.first_md : (k == 2 ? p.many.first_md : (own_cont ? p.few.cont_md : p.many.cont_md)))[place];
             }
-        };
-        const int lo = own_lo(p, r), tiles = (r.len - lo + stream_keys - 1) / stream_keys;
-        if (tiles > 0 && !by_tensor(p, r)) {
-            const int rows = r.used * p.G, own = j * p.G + h % p.G, row_tiles = (rows + p.stream.rows - 1) / p.stream.rows;
-            add_stream(0, p.stream.base[b] + (kvh * row_tiles + own / p.stream.rows) * tiles, tiles, own % p.stream.rows);
-        }
-        if (p.prefix_by_stream && prefix_tiles > 0) {
-            const int rows = max(0, min(p.starts[p.B], p.T_tokens)) * p.G, row_tiles = (rows + p.stream.rows - 1) / p.stream.rows;
-            add_stream(2, (kvh * row_tiles + grow / p.stream.rows) * prefix_tiles, prefix_tiles, grow % p.stream.rows);
-        }
-        if (p.tensor.ctas) {
-            const int tile = grow / kTcRows, units = (p.tensor.base[tile + 1] - p.tensor.base[tile]) / p.nkv;
-            if (units) {
-                const int TU = p.tensor.base[(int)(((long long)p.T_tokens * p.G + kTcRows - 1) / kTcRows)];
-                const int unit = p.tensor.base[tile] + kvh * units;
-                const int c0 = cta_of(unit, TU, p.tensor.ctas), c1 = cta_of(unit + units - 1, TU, p.tensor.ctas);
-                if (c0 == c1 && by_tensor(p, r)) {  // the tensor kernel has written the result
-                    const float mark = p.tensor.first_md[row].x;
-                    if (mark != mark) attend_alone(p, b, r, j, h);
-                    continue;
+            float now = md.x;
+            for (int s = 16; s; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+            now = fmaxf(now, top);
+            const float ref = now == -INFINITY ? 0.f : now;
+            const float w = exp2_approx(md.x - ref);
+            float sum = md.y * w;
+            for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            const float keep = exp2_approx(top - ref);
+            d = d * keep + sum;
+            top = now;
+            if (base) {
+#pragma unroll
+                for (int u = 0; u < E; ++u) {
+                    o[u].x *= keep;
+                    o[u].y *= keep;
+                    o[u].z *= keep;
+                    o[u].w *= keep;
                 }
-                parts.n[2] = 1;
-                parts.place[2] = row;
-                parts.n[3] = c1 - c0;
-                parts.place[3] = (long long)(c0 + 1) * kTcRows + grow % kTcRows;
-                parts.step[3] = kTcRows;
             }
-        }
-        const float* src[4] = {p.stream.first, p.stream.cont, p.tensor.first,
-                               p.prefix_by_stream ? p.stream.cont : p.tensor.cont};
-        const float2* src_md[4] = {p.stream.first_md, p.stream.cont_md, p.tensor.first_md,
-                                   p.prefix_by_stream ? p.stream.cont_md : p.tensor.cont_md};
-        // the largest maximum, then the weighted sums
-        float top = -INFINITY;
+            const int here = min(32, n - base);
+#pragma unroll 4
+            for (int k = 0; k < here; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, w, k);
+                const float* from = reinterpret_cast<const float*>(
+                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k));
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            for (int i = lane; i < parts.n[k]; i += 32) {
-                const float2 md = src_md[k][parts.place[k] + (long long)i * parts.step[k]];
-                top = md.x != md.x ? md.x : fmaxf(top, md.x);
-            }
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float d = 0.f;
-        float4 o[kMaxPagedHeadDim / 128];
-#pragma unroll
-        for (int u = 0; u < kMaxPagedHeadDim / 128; ++u) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            for (int i = 0; i < parts.n[k]; ++i) {
-                const long long at = parts.place[k] + (long long)i * parts.step[k];
-                const float2 md = src_md[k][at];
-                if (md.x == -INFINITY && md.y == 0.f) continue;
-                const float w = exp2_approx(md.x - top);
-                d = fmaf(md.y, w, d);
-#pragma unroll
-                for (int u = 0; u < kMaxPagedHeadDim / 128; ++u) {
+                for (int u = 0; u < E; ++u) {
                     const int e = u * 128 + lane * 4;
-                    if (e >= p.hd) break;
-                    const float4 x = *reinterpret_cast<const float4*>(src[k] + at * p.hd + e);
-                    o[u].x = fmaf(x.x, w, o[u].x);
-                    o[u].y = fmaf(x.y, w, o[u].y);
-                    o[u].z = fmaf(x.z, w, o[u].z);
-                    o[u].w = fmaf(x.w, w, o[u].w);
+                    if (e < p.hd) {
+                        const float4 v = *reinterpret_cast<const float4*>(from + e);
+                        o[u].x = fmaf(v.x, wk, o[u].x);
+                        o[u].y = fmaf(v.y, wk, o[u].y);
+                        o[u].z = fmaf(v.z, wk, o[u].z);
+                        o[u].w = fmaf(v.w, wk, o[u].w);
+                    }
                 }
             }
+        }
         const float inv = d == 0.f ? 0.f : 1.f / d;
-        bool fine = isfinite(d);
+        bool fine = isfinite(d) && x.n[0] >= 0;
 #pragma unroll
-        for (int u = 0; u < kMaxPagedHeadDim / 128; ++u) {
+        for (int u = 0; u < E; ++u) {
             o[u].x *= inv;
             o[u].y *= inv;
             o[u].z *= inv;
@@ -184,71 +334,48 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_parts_kernel(const __gri
             fine &= isfinite(o[u].x) && isfinite(o[u].y) && isfinite(o[u].z) && isfinite(o[u].w);
         }
         if (!__all_sync(0xffffffffu, fine)) {
-            attend_alone(p, b, r, j, h);
+            attend_alone(p, x.b, request_of(p, x.b), x.j, h);
             continue;
         }
 #pragma unroll
-        for (int u = 0; u < kMaxPagedHeadDim / 128; ++u) {
+        for (int u = 0; u < E; ++u) {
             const int e = u * 128 + lane * 4;
-            if (e >= p.hd) break;
-            *reinterpret_cast<uint2*>(out + e) = make_uint2(Pair<T>::pack(o[u].x, o[u].y), Pair<T>::pack(o[u].z, o[u].w));
+            if (e < p.hd)
+                *reinterpret_cast<uint2*>(out + e) =
+                    make_uint2(Pair<T>::pack(o[u].x, o[u].y), Pair<T>::pack(o[u].z, o[u].w));
         }
         if (lane == 0 && p.lse) p.lse[row] = d == 0.f ? -INFINITY : (top + log2f(d)) * kLn2;
     }
 }
 
 // ---- sizes and the workspace ---------------------------------------------------------
-// Rows up to which a request (or the whole batch, for the prefix) is the stream kernel's.
+// Rows per KV head up to which a request streams its keys: a job's rows at
+// most, times two.  Beyond, the tensor cores' 128-row tile costs less than
+// streaming the keys again for every job's worth of rows.
 constexpr int kFewRows = 32;
 
 struct Shape {
-    int hd, tensor_above, nt, stream_keys, stream_rows, stream_ctas, tensor_ctas;
-    bool prefix_by_stream;
+    int hd, nt, few_rows;
+    bool prefix_few;
+    int many_above;
 };
-
-template <int HD, int NT>
-void stream_shape(const tf_context* ctx, Shape& s) {
-    using S = StreamShape<HD, NT>;
-    s.hd = HD;
-    s.nt = NT;
-    s.stream_keys = S::kKeys;
-    s.stream_rows = S::kRows;
-    const size_t per_sm = (size_t)ctx->max_smem_optin / (S::kSmem + 1024);
-    s.stream_ctas = ctx->num_sms * (int)std::max<size_t>(1, std::min<size_t>(S::kCtas, per_sm));
-}
 
 // Column tiles for `rows` query rows of a job: one up to eight rows, beyond
 // that as many as a warp's registers hold (512 / head_dim).
-Shape shape_for(const tf_context* ctx, uint32_t hd, long long rows) {
-    Shape s = {};
-    const bool few = rows <= 8;
-    if (hd <= 64)
-        few ? stream_shape<64, 1>(ctx, s) : stream_shape<64, 4>(ctx, s);
-    else if (hd <= 128)
-        few ? stream_shape<128, 1>(ctx, s) : stream_shape<128, 4>(ctx, s);
-    else if (hd <= 256)
-        few ? stream_shape<256, 1>(ctx, s) : stream_shape<256, 2>(ctx, s);
-    else
-        stream_shape<512, 1>(ctx, s);
-    return s;
-}
-
-Shape shape_of_call(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t prefix_len,
-                    uint32_t max_query) {
-    const long long G = nq / kv->num_kv_heads;
-    const long long own = std::min<long long>(max_query, T) * G;
-    Shape s = shape_for(ctx, kv->head_dim, own);
-    const bool tensor = kv->head_dim <= 256;
-    s.prefix_by_stream = !tensor || T * G <= kFewRows;
-    // nothing for the tensor cores: no prefix of theirs and no request with many rows
-    const bool used = tensor && ((prefix_len && !s.prefix_by_stream) || own > kFewRows);
-    s.tensor_above = tensor ? kFewRows : 0x7FFFFFFF;
-    s.tensor_ctas = used ? ctx->num_sms : 0;
+Shape shape_of_call(const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t max_query) {
+    const long long G = nq / kv->num_kv_heads, own = std::min<long long>(max_query, T) * G;
+    Shape s;
+    s.hd = kv->head_dim <= 64 ? 64 : (kv->head_dim <= 128 ? 128 : (kv->head_dim <= 256 ? 256 : 512));
+    s.nt = own <= 8 ? 1 : std::min(4, 512 / s.hd);
+    s.few_rows = s.nt * 8;
+    const bool tensor = s.hd <= 256;
+    s.prefix_few = !tensor || T * G <= kFewRows;
+    s.many_above = tensor ? kFewRows : 0x7FFFFFFF;
     return s;
 }
 
 struct Layout {
-    size_t first[2], first_md[2], cont[2], cont_md[2], base[2], bytes;
+    size_t first[2], first_md[2], cont[2], cont_md[2], base[2], deal, bytes;
 };
 
 Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t B, const Shape& s) {
@@ -260,9 +387,9 @@ Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint
         return here;
     };
     const size_t rows = (size_t)T * nq, G = nq / kv->num_kv_heads;
-    // either kernel's grid and tile may be smaller in a call, never larger
-    const size_t cont[2] = {(size_t)ctx->num_sms * 2 * 64, (size_t)ctx->num_sms * kTcRows};
-    const size_t bases[2] = {B + 1, (size_t)T * G / kTcRows + 2};
+    const size_t cont[2] = {(size_t)ctx->num_sms * (kThreads / 32) * s.few_rows, (size_t)ctx->num_sms * kTcRows};
+    const size_t bases[2] = {B, (size_t)T * G / kTcRows + 2};
+    l.deal = take(sizeof(Deal));
     for (int k = 0; k < 2; ++k) {
         l.base[k] = take(bases[k] * sizeof(int));
         l.first_md[k] = take(rows * sizeof(float2));
@@ -274,55 +401,61 @@ Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint
     return l;
 }
 
-template <typename T, int HD, int NT>
-tf_status launch_stream(tf_context* ctx, const AttnParams<T>& p, cudaStream_t cs, const char* name) {
-    using S = StreamShape<HD, NT>;
-    static bool configured[64] = {};  // per instantiation, per device
-    const int dev = ctx->device & 63;
-    if (!configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(attention_few_rows_kernel<T, HD, NT>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-        if (e != cudaSuccess) return cuda_check(ctx, e, name);
-        configured[dev] = true;
+// The pool in boxes of `keys` keys and `blocks` 64-dim blocks; false when it
+// cannot be described.  With one block a box, the dims of a head are not split
+// (dims beyond head_dim arrive as zeros).
+bool pool_map(CUtensorMap* m, const tf_paged_kv* kv, const void* base, uint32_t keys, uint32_t blocks) {
+    memset(m, 0, sizeof(*m));
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const bool split = blocks > 0;
+    cuuint64_t dims[5] = {split ? 64 : kv->head_dim, kv->page_size, split ? kv->head_dim / 64 : 1, kv->num_kv_heads,
+                          kv->num_pages};
+    cuuint64_t strides[4] = {kv->position_stride * 2, 128, kv->head_stride * 2, kv->page_stride * 2};
+    for (int i = 0; i < 4; ++i) {
+        if (dims[i + 1] == 1) strides[i] = 128;  // never used
+        if (strides[i] >= (1ull << 40)) return false;
     }
-    attention_few_rows_kernel<T, HD, NT><<<p.stream.ctas, S::kWarps * 32, S::kSmem, cs>>>(p);
-    return cuda_check(ctx, cudaGetLastError(), name);
+    cuuint32_t box[5] = {64, keys, split ? blocks : 1, 1, 1};
+    cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    return fn(m, kv->dtype == TF_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+              const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HD>
-tf_status launch_tensor(tf_context* ctx, const AttnParams<T>& p, cudaStream_t cs, const char* name) {
-    using S = TensorShape<HD>;
+template <typename T, int HD, int NT>
+tf_status launch_parts(tf_context* ctx, const AttnParams<T>& p, cudaStream_t cs, const char* name) {
+    constexpr int kMany = HD <= 256 ? TensorShape<HD>::kSmem : 0, kFew = StreamShape<HD, NT>::kSmem;
+    constexpr int kSmem = kMany > kFew ? kMany : kFew;
     static bool configured[64] = {};  // per instantiation, per device
     const int dev = ctx->device & 63;
     if (!configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(attention_many_rows_kernel<T, HD>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        cudaError_t e = cudaFuncSetAttribute(attention_parts_kernel<T, HD, NT>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return cuda_check(ctx, e, name);
         configured[dev] = true;
     }
-    attention_many_rows_kernel<T, HD><<<p.tensor.ctas, S::kThreads, S::kSmem, cs>>>(p);
+    attention_parts_kernel<T, HD, NT><<<ctx->num_sms, kThreads, kSmem, cs>>>(p);
     return cuda_check(ctx, cudaGetLastError(), name);
 }
 
 template <typename T>
 tf_status launch(tf_context* ctx, const AttnParams<T>& p, const Shape& s, cudaStream_t cs, const char* name) {
     tf_status st = TF_OK;
-    if (s.tensor_ctas) {
-        st = s.hd == 64    ? launch_tensor<T, 64>(ctx, p, cs, name)
-             : s.hd == 128 ? launch_tensor<T, 128>(ctx, p, cs, name)
-                           : launch_tensor<T, 256>(ctx, p, cs, name);
-        if (st) return st;
-    }
     if (s.hd == 64)
-        st = s.nt == 1 ? launch_stream<T, 64, 1>(ctx, p, cs, name) : launch_stream<T, 64, 4>(ctx, p, cs, name);
+        st = s.nt == 1 ? launch_parts<T, 64, 1>(ctx, p, cs, name) : launch_parts<T, 64, 4>(ctx, p, cs, name);
     else if (s.hd == 128)
-        st = s.nt == 1 ? launch_stream<T, 128, 1>(ctx, p, cs, name) : launch_stream<T, 128, 4>(ctx, p, cs, name);
+        st = s.nt == 1 ? launch_parts<T, 128, 1>(ctx, p, cs, name) : launch_parts<T, 128, 4>(ctx, p, cs, name);
     else if (s.hd == 256)
-        st = s.nt == 1 ? launch_stream<T, 256, 1>(ctx, p, cs, name) : launch_stream<T, 256, 2>(ctx, p, cs, name);
+        st = s.nt == 1 ? launch_parts<T, 256, 1>(ctx, p, cs, name) : launch_parts<T, 256, 2>(ctx, p, cs, name);
     else
-        st = launch_stream<T, 512, 1>(ctx, p, cs, name);
+        st = launch_parts<T, 512, 1>(ctx, p, cs, name);
     if (st) return st;
-    join_parts_kernel<T><<<p.T_tokens, kJoinWarps * 32, 0, cs>>>(p, s.stream_keys);
+    // a warp per row while that fills the GPU; then more rows a CTA
+    const int rows = p.T_tokens * p.nq;
+    const int per = std::min(kJoinRows, std::max(8, (rows / (ctx->num_sms * 4) + 7) / 8 * 8));
+    join_parts_kernel<T><<<(rows + per - 1) / per, 256, 0, cs>>>(p, per);
     return cuda_check(ctx, cudaGetLastError(), name);
 }
 
@@ -334,7 +467,7 @@ size_t tf_shared_prefix_attention_workspace_bytes(const tf_context* ctx, const t
                                                   uint32_t T, uint32_t num_requests, uint32_t prefix_len,
                                                   uint32_t max_query) {
     if (!ctx || !kv || kv->num_kv_heads == 0 || num_q_heads == 0 || num_q_heads % kv->num_kv_heads) return 0;
-    const Shape shape = shape_of_call(ctx, kv, num_q_heads, T, prefix_len, max_query);
+    const Shape shape = shape_of_call(kv, num_q_heads, T, max_query);
     return layout_of(ctx, kv, num_q_heads, T, num_requests, shape).bytes;
 }
 
@@ -369,16 +502,23 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
         !aligned16(workspace))
         return fail(ctx, TF_ERR_MISALIGNED, "%s: q, out and workspace 16-byte aligned, strides multiples of 8", name);
     const uint64_t G = num_q_heads / kv->num_kv_heads;
-    const Shape shape = shape_of_call(ctx, kv, num_q_heads, T, prefix_len, max_query);
-    const uint64_t row_tiles = std::min<uint64_t>(max_query, T) * G / shape.stream_rows + num_requests;
-    const uint64_t keys = (uint64_t)max_pages * kv->page_size / shape.stream_keys + 1;
-    if (row_tiles * keys * kv->num_kv_heads > 0x7FFFFFFFull ||
-        (T * G / shape.stream_rows + 1) * (prefix_len / shape.stream_keys + 1) * kv->num_kv_heads > 0x3FFFFFFFull)
-        return fail(ctx, TF_ERR_UNSUPPORTED_SHAPE, "%s: too many key tiles", name);
+    const Shape shape = shape_of_call(kv, num_q_heads, T, max_query);
+    const uint64_t row_tiles = T * G / shape.few_rows + std::min<uint64_t>(T, num_requests);
+    const uint64_t tiles = (uint64_t)max_pages * kv->page_size / 16 + prefix_len / 16 + 2;
+    if (row_tiles * tiles * kv->num_kv_heads > 0x7FFFFFFFull)
+        return fail(ctx, TF_ERR_UNSUPPORTED_SHAPE, "%s: too many keys", name);
     const Layout l = layout_of(ctx, kv, num_q_heads, T, num_requests, shape);
     const size_t need = l.bytes;
     if (workspace_bytes < need)
         return fail(ctx, TF_ERR_INVALID_ARG, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes, need);
+
+    KvMaps maps;
+    const uint32_t run = std::min<uint32_t>(kMaxRun, kv->page_size & (0u - kv->page_size));
+    const bool wide = run == 8 && kv->head_dim % 64 == 0;
+    const uint32_t blocks = wide ? shape.hd / 64 : 0;
+    if (!pool_map(&maps.k, kv, kv->k, run, blocks) || !pool_map(&maps.v, kv, kv->v, run, blocks) ||
+        !pool_map(&maps.v_row, kv, kv->v, 1, 0))
+        return fail(ctx, TF_ERR_UNSUPPORTED_SHAPE, "%s: the pool's sizes and strides cannot be described to TMA", name);
 
     auto fill = [&](auto& p) {
         using T_ = std::remove_const_t<std::remove_pointer_t<decltype(p.q)>>;
@@ -408,10 +548,10 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
         p.prefix_lo = window ? (int)std::max<long long>(0, std::min<long long>(prefix_len, (long long)prefix_len -
                                                                                               max_query - window + 1))
                              : 0;
-        p.prefix_by_stream = shape.prefix_by_stream;
-        p.tensor_above = shape.tensor_above;
+        p.prefix_few = shape.prefix_few;
+        p.many_above = shape.many_above;
         uint8_t* w = static_cast<uint8_t*>(workspace);
-        Parts* parts[2] = {&p.stream, &p.tensor};
+        Parts* parts[2] = {&p.few, &p.many};
         for (int k = 0; k < 2; ++k) {
             parts[k]->first = reinterpret_cast<float*>(w + l.first[k]);
             parts[k]->first_md = reinterpret_cast<float2*>(w + l.first_md[k]);
@@ -419,10 +559,15 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
             parts[k]->cont_md = reinterpret_cast<float2*>(w + l.cont_md[k]);
             parts[k]->base = reinterpret_cast<int*>(w + l.base[k]);
         }
-        p.stream.ctas = shape.stream_ctas;
-        p.stream.rows = shape.stream_rows;
-        p.tensor.ctas = shape.tensor_ctas;
-        p.tensor.rows = kTcRows;
+        p.few.rows = shape.few_rows;
+        p.many.rows = kTcRows;
+        p.deal = reinterpret_cast<Deal*>(w + l.deal);
+        p.run_shift = run == 8 ? 3 : (run == 4 ? 2 : (run == 2 ? 1 : 0));
+        p.page_shift = -1;
+        for (int i = 0; i < 31; ++i)
+            if (kv->page_size == (1u << i)) p.page_shift = i;
+        p.wide = wide;
+        p.maps = maps;
     };
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     if (kv->dtype == TF_DTYPE_F16) {

@@ -9,20 +9,35 @@ namespace tf {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTcRows = 128;  // query rows of a tensor tile
+constexpr int kMaxRun = 8;
 
-// Parts of rows.  A CTA works through a contiguous range of units (a unit is
-// one tile of keys of one job); the part it computes of a job goes to `first`
-// (at the row's own place) when it holds the job's first unit, and to `cont`
-// (at the CTA's place) otherwise: at most one of a CTA's jobs began before it.
-// o is not normalised; md = (m, d), m in units of log2.
+// Parts of rows.  A worker (a warp for few rows, a CTA for many) goes through a
+// contiguous range of units (a unit is one tile of keys of one job); the part
+// it computes of a job goes to `first` (at the row's own place) when it holds
+// the job's first unit, and to `cont` (at the worker's place) otherwise: at most
+// one of a worker's jobs began before it.  o is not normalised; md = (m, d), m
+// in units of log2.
 struct Parts {
     float* first;
     float2* first_md;
     float* cont;
     float2* cont_md;
-    int* base;  // first unit of each request (stream) or row tile (tensor); [count] = all units
-    int ctas;
-    int rows;  // rows a cont place holds
+    int* base;  // first unit of each request (few rows) or row tile (many rows)
+    int rows;   // rows a cont place holds
+};
+
+// The pool as TMA sees it: [page][head][64-dim block][position][64 dims], 128-byte
+// swizzle.  A tile of keys is kept as groups of eight keys, [group][block][8 keys]
+// [128 bytes], so a box of 8 keys and all blocks is one load ("wide") where pages
+// hold whole groups and head_dim whole blocks; otherwise a box is `run` keys and
+// one block.  rows: boxes of one key and one block.
+struct KvMaps {
+    CUtensorMap k, v, v_row;
+};
+
+// How the units were dealt, written by the first CTA for the joining kernel.
+struct Deal {
+    int few_units, few_workers, many_units, many_workers;
 };
 
 template <typename T>
@@ -39,10 +54,15 @@ struct AttnParams {
     float* lse;
     uint32_t* err;
     int prefix_len, prefix_lo, max_pages, B, max_query, T_tokens, nq, nkv, G, hd, window;
-    int prefix_by_stream;  // the stream kernel also reads the prefix (few rows)
-    int tensor_above;      // requests of more rows per KV head than this are the tensor kernel's
+    int prefix_few;   // the prefix is read by the streaming warps too (the batch has few rows)
+    int many_above;   // requests of more rows per KV head than this go to the tensor cores
     float scale;
-    Parts stream, tensor;
+    Parts few, many;
+    Deal* deal;
+    int run_shift;   // keys of a box, as a power of two: the largest up to 8 that divides the page size
+    int page_shift;  // the page size as a power of two, or -1 (a division per unit cost 150 clocks of its latency)
+    int wide;  // a box has all of a head's blocks
+    KvMaps maps;
 };
 
 // A request of the batch.
@@ -61,9 +81,13 @@ __device__ __forceinline__ Request request_of(const AttnParams<T>& p, int b) {
     return r;
 }
 
+// What runs once a job or segment is kept out of line here and below: inlined
+// wherever a cursor moves it made the kernel 247 KB of code, and the loops of its
+// warps, which share an instruction cache, spent half their time fetching it.
+
 // The last b with starts[b] <= t; B for tokens behind the last request.
 template <typename T>
-__device__ __forceinline__ int request_at(const AttnParams<T>& p, int t) {
+__device__ __noinline__ int request_at(const AttnParams<T>& p, int t) {
     int lo = 0, hi = p.B;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -92,13 +116,13 @@ __device__ __forceinline__ int own_lo(const AttnParams<T>& p, const Request& r) 
 }
 
 template <typename T>
-__device__ __forceinline__ bool by_tensor(const AttnParams<T>& p, const Request& r) {
-    return r.used * p.G > p.tensor_above;
+__device__ __forceinline__ bool is_many(const AttnParams<T>& p, const Request& r) {
+    return r.used * p.G > p.many_above;
 }
 
-// Units [c*U/N, (c+1)*U/N) are CTA c's.
+// Units [c*U/N, (c+1)*U/N) are worker c's.
 __device__ __forceinline__ int unit_begin(int c, int U, int N) { return (int)((long long)c * U / N); }
-__device__ __forceinline__ int cta_of(int u, int U, int N) { return (int)((((long long)u + 1) * N - 1) / U); }
+__device__ __forceinline__ int worker_of(int u, int U, int N) { return (int)((((long long)u + 1) * N - 1) / U); }
 
 // Exclusive sum of v over the block (up to 32 warps); *total receives the sum.
 __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
@@ -144,14 +168,124 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// 16-byte asynchronous copy; `bytes` 0 fills the destination with zeros.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Waits about two seconds at most, then reports it and returns false.
+__device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t* err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long since = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - since > 4000000000ll) {
+            atomicOr(err, kErrMbarTimeout);
+            return false;
+        }
+    return true;
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+
+// 5-D tiled TMA load (no multicast).
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int v, int w,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// One lane of a converged warp, known to the compiler as one.  The operands of
+// TMA and tcgen05 instructions live in uniform registers: issued under
+// `lane == 0` each becomes a loop over the lanes' values (46 clocks for an MMA
+// of 32, 87 for a TMA load), under this they go out back to back.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+// A tile of KEYS keys, by a converged warp.  Lane l has looked up the runs l, l +
+// 32, ...: the page, the place in it and (bit r) which of the run's keys exist.
+// Keys that do not exist arrive as zeros: a whole box from a page behind the
+// pool, and for V, whose every row meets a weight (0 * NaN would not be 0), key
+// by key where a run has both.
+template <int KEYS>
+struct TileKeys {
+    static constexpr int kMost = (KEYS + 31) / 32;
+    int page[kMost], in_page[kMost], have[kMost];
+};
+
+template <int HD, int KEYS, typename T>
+__device__ __forceinline__ void load_tile_keys(const AttnParams<T>& p, bool v, uint32_t tile, int head,
+                                               const TileKeys<KEYS>& k, uint64_t* bar) {
+    constexpr int kBlocks = HD / 64, kMost = TileKeys<KEYS>::kMost;
+    const CUtensorMap* map = v ? &p.maps.v : &p.maps.k;
+    const int lane = threadIdx.x & 31, run = 1 << p.run_shift, runs = KEYS >> p.run_shift, all = (1 << run) - 1;
+    const bool one = elect_one();
+    if (one) mbar_arrive_expect_tx(bar, KEYS * HD * 2);
+    bool complete = p.wide != 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) complete &= i * 32 + lane >= runs || k.have[i] == all;
+    if (__all_sync(0xffffffffu, complete)) {
+#pragma unroll 2
+        for (int r = 0; r < KEYS / 8; ++r) {
+            const int pg = __shfl_sync(0xffffffffu, k.page[0], r), in = __shfl_sync(0xffffffffu, k.in_page[0], r);
+            if (one) tma_load_5d(tile + r * (kBlocks * 1024), map, 0, in, 0, head, pg, bar);
+        }
+        __syncwarp();
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+#pragma unroll 1
+        for (int l = 0; l < min(32, runs - i * 32); ++l) {
+            const int pg = __shfl_sync(0xffffffffu, k.page[i], l), in = __shfl_sync(0xffffffffu, k.in_page[i], l);
+            const int have = __shfl_sync(0xffffffffu, k.have[i], l), first = (i * 32 + l) * run;
+            const uint32_t dst = tile + (first >> 3) * (kBlocks * 1024) + (first & 7) * 128;
+            const int from = have ? pg : p.kv.num_pages;
+            if (!one) continue;
+            if (!v || have == all || have == 0) {
+                if (p.wide)
+                    tma_load_5d(dst, map, 0, in, 0, head, from, bar);
+                else
+                    for (int b = 0; b < kBlocks; ++b) tma_load_5d(dst + b * 1024, map, b * 64, in, 0, head, from, bar);
+            } else {
+                for (int r = 0; r < run; ++r)
+                    for (int b = 0; b < kBlocks; ++b)
+                        tma_load_5d(dst + b * 1024 + r * 128, &p.maps.v_row, b * 64, in + r, 0, head,
+                                    (have >> r) & 1 ? pg : p.kv.num_pages, bar);
+            }
+        }
+    __syncwarp();
+}
+
+// The runs of the tile of keys that begins at position `pos0` of a segment
+// whose keys are [from, hi).
+template <int KEYS, typename T>
+__device__ __forceinline__ TileKeys<KEYS> look_up_keys(const AttnParams<T>& p, int seg, int pos0, int from, int hi) {
+    TileKeys<KEYS> k;
+    const int lane = threadIdx.x & 31, run = 1 << p.run_shift, runs = KEYS >> p.run_shift;
+#pragma unroll
+    for (int i = 0; i < TileKeys<KEYS>::kMost; ++i) {
+        const int pos = pos0 + ((i * 32 + lane) << p.run_shift);
+        const int a = max(0, from - pos), z = min(run, hi - pos);  // keys a .. z - 1 of the run exist
+        k.page[i] = k.in_page[i] = k.have[i] = 0;
+        if (i * 32 + lane < runs && a < z) {
+            const int at = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.kv.page_size;
+            k.in_page[i] = pos - at * p.kv.page_size;
+            k.have[i] = (1 << z) - (1 << a);
+            k.page[i] = seg < 0 ? p.prefix_pages[at] : p.table[(long long)seg * p.max_pages + at];
+        }
+    }
+    return k;
+}
+// Once the page ids are there: those outside the pool are reported and not read.
+template <int KEYS, typename T>
+__device__ __forceinline__ void check_keys(const AttnParams<T>& p, TileKeys<KEYS>& k) {
+#pragma unroll
+    for (int i = 0; i < TileKeys<KEYS>::kMost; ++i) {
+        asm volatile("" : "+r"(k.page[i]));  // not earlier: the id is waited for here
+        if (k.have[i] && (k.page[i] < 0 || k.page[i] >= p.kv.num_pages)) {
+            atomicOr(p.err, kErrBadPage);
+            k.have[i] = 0;
+        }
+    }
 }
 
 }  // namespace tf

@@ -3,12 +3,12 @@
 //
 // HBM-bound: K and V are read once, 4 * head_dim bytes a key, for 4 * head_dim
 // * rows operations.  Everything serves the stream of loads:
-//   * the units (64 keys of one request, KV head and row tile) are dealt evenly
-//     and contiguously, whatever the lengths; a CTA's stream of loads runs on
-//     across the requests it covers;
-//   * a warp owns 16 of a unit's keys and a ring of its own, filled by cp.async
-//     up to S - 1 units ahead, so warps wait for nobody until a job ends; page
-//     ids are looked up one unit before their loads are issued;
+//   * the units (16 keys of one request, KV head and row tile) are dealt evenly
+//     and contiguously to the warps, whatever the lengths.  A warp works for
+//     itself: its ring of K and V tiles is filled by its own cp.async and its
+//     loads run on across the jobs it covers, so no warp ever waits for another
+//     and one that begins or ends a job leaves the memory to the rest;
+//   * page ids are looked up one unit before their loads are issued;
 //   * scores are S^T = K Q^T and outputs O^T = V^T P^T: keys and dims fill the
 //     16-row side of mma.sync m16n8k16 and the few query rows its 8 columns, so
 //     one to eight rows cost one column tile and the accumulator of 256 dims is
@@ -57,162 +57,124 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 
 template <int HD, int NT>
 struct StreamShape {
-    static constexpr int kWarps = HD > 256 ? 2 : 4;
-    static constexpr int kKeys = kWarps * 16;                  // keys of a unit
-    static constexpr int kRows = NT * 8;                       // query rows of a job
-    static constexpr int kTile = 16 * HD * 2;                  // a warp's K (or V) tile, bytes
-    static constexpr int kStages = HD == 64 ? 6 : 3;           // K and V tiles per warp
-    static constexpr int kCtas = HD >= 256 ? 1 : 2;            // per SM
-    static constexpr int kJoinLd = 66;                         // floats per row while warps are joined
-    static constexpr int kRing = kWarps * kStages * 2 * kTile;
-    static constexpr int kSmem = kRing + kWarps * kRows * (kJoinLd + 2) * 4 + 1024;
+    static constexpr int kWarps = HD > 256 ? 4 : 8;  // that stream
+    static constexpr int kKeys = 16;                 // keys of a unit
+    static constexpr int kRows = NT * 8;             // query rows of a job
+    static constexpr int kTile = kKeys * HD * 2;     // bytes of a K (or V) tile
+    static constexpr int kTiles = HD >= 256 ? 3 : (HD == 128 ? 6 : 10);  // a warp's ring, K and V tiles in turn
+    static constexpr int kSmem = kWarps * kTiles * kTile + 1024;
+    static constexpr int kBars = kWarps * kTiles;
 };
 
-// Where a CTA is in its range of units.
+// Where a warp is in its range of units.
 struct StreamCursor {
     int seg;             // request, or -1: the prefix
     int kvh, rt, tile;   // KV head, row tile, key tile
     int row_tiles, tiles;
-    int lo, hi;          // keys of the segment
+    int lo, hi;          // keys of the segment; lo is rounded down to a box
+    int from;            // the first that any row sees
 };
 
 template <typename T, int HD, int NT>
 __device__ __forceinline__ void stream_segment(const AttnParams<T>& p, StreamCursor& c) {
     using S = StreamShape<HD, NT>;
     if (c.seg < 0) {
-        const int rows = p.prefix_by_stream ? max(0, min(p.starts[p.B], p.T_tokens)) * p.G : 0;
-        c.lo = p.prefix_lo;
+        const int rows = p.prefix_few ? max(0, min(p.starts[p.B], p.T_tokens)) * p.G : 0;
+        c.from = p.prefix_lo;
         c.hi = p.prefix_len;
         c.row_tiles = (rows + S::kRows - 1) / S::kRows;
     } else {
         const Request r = request_of(p, c.seg);
-        c.lo = own_lo(p, r);
+        c.from = own_lo(p, r);
         c.hi = r.len;
-        c.row_tiles = by_tensor(p, r) ? 0 : (r.used * p.G + S::kRows - 1) / S::kRows;
+        c.row_tiles = is_many(p, r) ? 0 : (r.used * p.G + S::kRows - 1) / S::kRows;
     }
-    c.tiles = c.row_tiles ? (c.hi - c.lo + S::kKeys - 1) / S::kKeys : 0;
+    c.lo = c.from & ~(kMaxRun - 1);
+    c.tiles = c.row_tiles && c.hi > c.from ? (c.hi - c.lo + S::kKeys - 1) / S::kKeys : 0;
 }
 
+// The first unit of the next job.
 template <typename T, int HD, int NT>
-__device__ __forceinline__ void stream_advance(const AttnParams<T>& p, StreamCursor& c) {
-    if (++c.tile < c.tiles) return;
+__device__ __noinline__ StreamCursor stream_next_job(const AttnParams<T>& p, StreamCursor c) {
     c.tile = 0;
-    if (++c.rt < c.row_tiles) return;
+    if (++c.rt < c.row_tiles) return c;
     c.rt = 0;
-    if (++c.kvh < p.nkv) return;
+    if (++c.kvh < p.nkv) return c;
     c.kvh = 0;
     do {
         ++c.seg;
-        if (c.seg >= p.B) return;
+        if (c.seg >= p.B) return c;
         stream_segment<T, HD, NT>(p, c);
     } while (c.tiles == 0);
+    return c;
+}
+template <typename T, int HD, int NT>
+__device__ __forceinline__ void stream_advance(const AttnParams<T>& p, StreamCursor& c) {
+    if (++c.tile >= c.tiles) c = stream_next_job<T, HD, NT>(p, c);
 }
 
+// The units of the whole batch; `before` those of the requests before this
+// thread's own [b0, b1).
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<HD, NT>::kCtas)
-    attention_few_rows_kernel(const __grid_constant__ AttnParams<T> p) {
-    using S = StreamShape<HD, NT>;
-    constexpr int kWarps = S::kWarps, kRows = S::kRows, kStages = S::kStages, CPR = HD / 8;
-    extern __shared__ uint8_t raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    float* join = reinterpret_cast<float*>(smem + S::kRing);         // [warp][row][kJoinLd]
-    float* join_md = join + kWarps * kRows * S::kJoinLd;             // [warp][row][2]
-    __shared__ int red[32], s_seg, s_at;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-
-    // ---- which units are mine -------------------------------------------------
-    // thread i sums the units of requests [i*per, (i+1)*per); the one whose sum
-    // contains my first unit finds the request
-    int U, u0, u1;
-    StreamCursor cur;
-    {
-        StreamCursor c;
-        c.seg = -1;
+__device__ __forceinline__ int stream_units(const AttnParams<T>& p, int* red, int b0, int b1, int& before) {
+    StreamCursor c;
+    c.seg = -1;
+    stream_segment<T, HD, NT>(p, c);
+    const int prefix_units = c.row_tiles * c.tiles * p.nkv;
+    int sum = 0, total;
+    for (c.seg = b0; c.seg < b1; ++c.seg) {
         stream_segment<T, HD, NT>(p, c);
-        const int prefix_units = c.row_tiles * c.tiles * p.nkv;
-        const int per = (p.B + blockDim.x - 1) / blockDim.x;
-        const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
-        int sum = 0;
-        for (c.seg = b0; c.seg < b1; ++c.seg) {
-            stream_segment<T, HD, NT>(p, c);
-            sum += c.row_tiles * c.tiles * p.nkv;
-        }
-        int at = prefix_units + block_scan(sum, red, &U);
-        U += prefix_units;
-        u0 = unit_begin(blockIdx.x, U, gridDim.x);
-        u1 = unit_begin(blockIdx.x + 1, U, gridDim.x);
-        if (threadIdx.x == 0 && (u0 < prefix_units || U == 0)) {
-            s_seg = -1;
-            s_at = 0;
-        }
-        for (c.seg = b0; c.seg < b1; ++c.seg) {
-            stream_segment<T, HD, NT>(p, c);
-            const int units = c.row_tiles * c.tiles * p.nkv;
-            if (blockIdx.x == 0) p.stream.base[c.seg] = at;
-            if (u0 >= at && u0 < at + units) {
-                s_seg = c.seg;
-                s_at = at;
-            }
-            at += units;
-        }
-        if (blockIdx.x == 0 && threadIdx.x == 0) p.stream.base[p.B] = U;
-        __syncthreads();
-        if (u0 >= u1) return;
-        cur.seg = s_seg;
-        stream_segment<T, HD, NT>(p, cur);
-        const int in = u0 - s_at;
-        cur.tile = in % cur.tiles;
-        cur.rt = in / cur.tiles % cur.row_tiles;
-        cur.kvh = in / cur.tiles / cur.row_tiles;
+        sum += c.row_tiles * c.tiles * p.nkv;
     }
-    StreamCursor ahead = cur;  // the unit whose page ids are looked up next
-    int left_ahead = u1 - u0;
+    before = prefix_units + block_scan(sum, red, &total);
+    return prefix_units + total;
+}
+
+// One warp: units [u0, u1) beginning at `cur`, as worker `worker`.
+template <typename T, int HD, int NT>
+__device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t ring, uint64_t* full, StreamCursor cur,
+                                            int u0, int u1, int worker) {
+    using S = StreamShape<HD, NT>;
+    constexpr int kRows = S::kRows, R = S::kTiles, kGroup8 = HD / 64 * 1024;  // bytes of eight keys
+    const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
 
     // ---- loads ------------------------------------------------------------------
-    const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * S::kTile;
-    long long next_off = 0;     // lane < 16: element offset of its key's row
-    uint32_t next_mask = 0;     // which of the 16 keys exist
+    StreamCursor ahead = cur;  // the unit whose page ids are looked up next
+    int left = u1 - u0;        // units not looked up yet
+    TileKeys<16> next, now;  // the unit after the one being loaded, and that one
+    int next_head = 0, now_head = 0;
     auto look_up = [&]() {
-        next_mask = 0;
-        if (left_ahead <= 0) return;
-        const int pos = ahead.lo + ahead.tile * S::kKeys + warp * 16 + (lane & 15);
-        bool ok = pos < ahead.hi;
-        next_off = 0;
-        if (ok) {
-            const int at = pos / p.kv.page_size;
-            const int page = ahead.seg < 0 ? p.prefix_pages[at] : p.table[(long long)ahead.seg * p.max_pages + at];
-            ok = page >= 0 && page < p.kv.num_pages;
-            if (ok)
-                next_off = page * p.kv.page_stride + (pos - at * p.kv.page_size) * p.kv.pos_stride +
-                           ahead.kvh * p.kv.head_stride;
-            else
-                atomicOr(p.err, kErrBadPage);
-        }
-        next_mask = __ballot_sync(0xffffffffu, ok) & 0xFFFFu;
-        --left_ahead;
-        stream_advance<T, HD, NT>(p, ahead);
+        next_head = ahead.kvh;
+        next = look_up_keys<16>(p, ahead.seg, ahead.lo + ahead.tile * S::kKeys, ahead.from, left > 0 ? ahead.hi : 0);
+        if (left-- > 0) stream_advance<T, HD, NT>(p, ahead);
     };
-    auto issue = [&](int stage) {  // loads of the keys last looked up
-        const uint32_t dst = ring + stage * 2 * S::kTile;
-#pragma unroll
-        for (int i = 0; i < 16 * CPR / 32; ++i) {
-            const int chunk = i * 32 + lane, row = chunk / CPR, c = chunk % CPR;
-            const long long off = __shfl_sync(0xffffffffu, next_off, row);
-            const int bytes = ((next_mask >> row) & 1) && c * 8 < p.hd ? 16 : 0;
-            const long long at = bytes ? off + c * 8 : 0;
-            const uint32_t to = dst + row * (HD * 2) + ((c ^ (row & 7)) << 4);
-            cp_async16(to, p.kv.k + at, bytes);
-            cp_async16(to + S::kTile, p.kv.v + at, bytes);
+    int fill = 0;  // ring place of the next tile to load
+    bool v_next = false;
+    auto load_tile = [&]() {
+        if (!v_next) {
+            now = next;
+            now_head = next_head;
+            check_keys(p, now);
         }
+        load_tile_keys<HD, 16>(p, v_next, ring + fill * S::kTile, now_head, now, full + fill);
+        if (!v_next) look_up();
+        v_next = !v_next;
+        fill = fill == R - 1 ? 0 : fill + 1;
     };
-
     look_up();
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-        issue(i);
-        cp_async_commit();
-        look_up();
-    }
+    // A tile's loads: bounded like every wait; after one that gave up the values
+    // are wrong, the error is reported and the units go on.
+    int slot = 0;
+    uint32_t phase = 0;
+    auto landed = [&]() { mbar_wait_limited(full + slot, phase, p.err); };
+    auto taken = [&]() {
+        if (++slot == R) {
+            slot = 0;
+            phase ^= 1;
+        }
+    };
+#pragma unroll 1
+    for (int i = 0; i < R - 1; ++i) load_tile();
 
     // ---- the job's rows -----------------------------------------------------------
     uint32_t qf[HD / 16][NT][2];
@@ -275,88 +237,44 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
         }
     };
 
-    // Joins the warps and writes the job's part.
+    // The job's part, straight from the registers: eight lanes write the 32
+    // bytes of eight dims of a row.
     bool from_start = cur.tile == 0;
     auto end_job = [&]() {
-        const int row0 = cur.rt * kRows;
+        // a row's part of the prefix goes where the tensor cores' would be
+        const Parts& to = cur.seg < 0 ? p.many : p.few;
+        float* po = from_start ? to.first : p.few.cont;
+        float2* pm = from_start ? to.first_md : p.few.cont_md;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float s = d[nt][i];
-                for (int o = 4; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (g == 0) {
-                    float* md = join_md + (warp * kRows + nt * 8 + 2 * tq + i) * 2;
-                    md[0] = m[nt][i];
-                    md[1] = s;
+                const int r = nt * 8 + 2 * tq + i, row = cur.rt * kRows + r;
+                const long long place = from_start ? (long long)(first_token + row / p.G) * p.nq + cur.kvh * p.G + row % p.G
+                                                   : (long long)worker * kRows + r;
+                float sum = d[nt][i];
+                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (r >= job_rows) continue;
+                if (g == 0) pm[place] = make_float2(m[nt][i], sum);
+                float* dst = po + place * p.hd + g;
+#pragma unroll
+                for (int mt = 0; mt < HD / 16; ++mt) {
+                    if (mt * 16 < p.hd) dst[mt * 16] = acc[mt][nt][i];
+                    if (mt * 16 + 8 < p.hd) dst[mt * 16 + 8] = acc[mt][nt][i + 2];
                 }
             }
-        __syncthreads();
-        float fac[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float top = -INFINITY;
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_md[(w * kRows + nt * 8 + 2 * tq + i) * 2]);
-                fac[nt][i] = m[nt][i] == -INFINITY ? 0.f : exp2_approx(m[nt][i] - top);
-            }
-        auto place = [&](int r) -> long long {  // row of `first` or `cont`
-            if (!from_start) return (long long)blockIdx.x * p.stream.rows + r;
-            const int row = row0 + r;
-            return (long long)(first_token + row / p.G) * p.nq + cur.kvh * p.G + row % p.G;
-        };
-        // a row's part of the prefix goes where the tensor kernel would have put it
-        const Parts& to = cur.seg < 0 ? p.tensor : p.stream;
-        float* po = from_start ? to.first : p.stream.cont;
-        float2* pm = from_start ? to.first_md : p.stream.cont_md;
-        for (int r = threadIdx.x; r < min(kRows, job_rows); r += blockDim.x) {
-            float top = -INFINITY, sum = 0.f;
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_md[(w * kRows + r) * 2]);
-            for (int w = 0; w < kWarps; ++w) {
-                const float mw = join_md[(w * kRows + r) * 2];
-                if (mw != -INFINITY) sum += join_md[(w * kRows + r) * 2 + 1] * exp2_approx(mw - top);
-            }
-            pm[place(r)] = make_float2(top, sum);
-        }
-#pragma unroll
-        for (int mt0 = 0; mt0 < HD / 16; mt0 += 4) {  // 64 dims at a time
-            if (mt0) __syncthreads();
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        join[(warp * kRows + nt * 8 + 2 * tq + (i & 1)) * S::kJoinLd + u * 16 + g + 8 * (i >> 1)] =
-                            acc[mt0 + u][nt][i] * fac[nt][i & 1];
-            __syncthreads();
-            for (int x = threadIdx.x; x < kRows * 64; x += blockDim.x) {
-                const int r = x >> 6, e = x & 63;
-                if (r >= job_rows || mt0 * 16 + e >= p.hd) continue;
-                float v = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) v += join[(w * kRows + r) * S::kJoinLd + e];
-                po[place(r) * p.hd + mt0 * 16 + e] = v;
-            }
-        }
-        __syncthreads();
     };
 
-    // ---- one unit -------------------------------------------------------------------
-    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_chunk = lane >> 4;      // K: keys x dims
+    // ---- units ------------------------------------------------------------------------
+    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_chunk = lane >> 4;        // K: keys x dims
     const int v_row = (lane & 7) + ((lane >> 4) & 1) * 8, v_chunk = (lane >> 3) & 1;  // V: dims x keys
-    int stage = 0;
     for (int u = u0; u < u1; ++u) {
         if (u == u0 || cur.tile == 0) begin_job();
-        const int fill = stage == 0 ? kStages - 1 : stage - 1;
-        issue(fill);
-        cp_async_commit();
-        look_up();
-        cp_async_wait<kStages - 1>();
-        __syncwarp();
-
-        const uint32_t kt = ring + stage * 2 * S::kTile, vt = kt + S::kTile;
+        __syncwarp();  // the tile before this one has been read by every lane
+        load_tile();
+        landed();
+        const uint32_t kt = ring + slot * S::kTile;
+        taken();
         float s[NT][4], s2[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -365,11 +283,11 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
             uint32_t a[4];
-            ldsm4(a, kt + k_row * (HD * 2) + (((ks * 2 + k_chunk) ^ (k_row & 7)) << 4));
+            ldsm4(a, kt + (k_row >> 3) * kGroup8 + (ks >> 2) * 1024 + (k_row & 7) * 128 + ((((ks & 3) * 2 + k_chunk) ^ (k_row & 7)) << 4));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_16x8<T>(ks & 1 ? s2[nt] : s[nt], a, qf[ks][nt][0], qf[ks][nt][1]);
         }
-        const int key0 = cur.lo + cur.tile * S::kKeys + warp * 16;
+        const int key0 = cur.lo + cur.tile * S::kKeys;
         uint32_t pf[NT][2];
         bool grew = false;
         float keep[NT][2];
@@ -407,22 +325,29 @@ __global__ void __launch_bounds__(StreamShape<HD, NT>::kWarps * 32, StreamShape<
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[mt][nt][i] *= keep[nt][i & 1];
         }
+        __syncwarp();  // K has been read
+        load_tile();
+        landed();
+        const uint32_t vt = ring + slot * S::kTile;
+        taken();
 #pragma unroll
         for (int mt = 0; mt < HD / 16; ++mt) {
             uint32_t a[4];
-            ldsm4_t(a, vt + v_row * (HD * 2) + (((mt * 2 + v_chunk) ^ (v_row & 7)) << 4));
+            ldsm4_t(a, vt + (v_row >> 3) * kGroup8 + (mt >> 2) * 1024 + (v_row & 7) * 128 + ((((mt & 3) * 2 + v_chunk) ^ (v_row & 7)) << 4));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_16x8<T>(acc[mt][nt], a, pf[nt][0], pf[nt][1]);
         }
-        __syncwarp();  // before this stage is filled again
-        stage = stage == kStages - 1 ? 0 : stage + 1;
         if (cur.tile == cur.tiles - 1 || u == u1 - 1) {
             end_job();
             from_start = true;
         }
         stream_advance<T, HD, NT>(p, cur);
     }
-    cp_async_wait<0>();
+    // what was loaded ahead (zeros) lands before the CTA may end
+    for (int i = 0; i < R - 1; ++i) {
+        landed();
+        taken();
+    }
 }
 
 }  // namespace tf

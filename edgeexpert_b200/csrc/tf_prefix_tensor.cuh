@@ -14,7 +14,7 @@
 //   S = Q K^T     A = Q (TMEM), B = K tile [keys][dims], K-major
 //   O += P V      A = P (TMEM), B = V tile [keys][dims], MN-major
 // Roles: warps 0-3 a row per thread (softmax, Q in, O out), warp 4 issues the
-// MMAs, warps 5-6 gather K and V by page into a ring of 128-byte-swizzled tiles.
+// MMAs, warps 5 and 6 fetch K and V by page into rings of 128-byte-swizzled tiles.
 // Scores of tile i+1 are computed while the softmax of tile i runs.
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
 // one its sums refer to: weights stay below 256, sums in fp32, and the quotient
@@ -29,11 +29,9 @@ template <int HD>
 struct TensorShape {
     static constexpr int kKeys = HD > 128 ? 64 : 128;     // keys of a unit
     static constexpr int kSlot = kKeys * HD * 2;          // bytes of a K or V tile
-    static constexpr int kSlots = HD > 64 ? 6 : 8;
-    static constexpr int kSmem = kSlots * kSlot + 1024;
+    static constexpr int kSlots = HD > 64 ? 3 : 4;        // of K, and as many of V behind them
+    static constexpr int kSmem = 2 * kSlots * kSlot + 1024;
     static constexpr int kColO = 0, kColQ = HD, kColS = HD + HD / 2;
-    static constexpr int kLoaders = 2;                    // warps; with two warps at most on a scheduler,
-    static constexpr int kThreads = 160 + 32 * kLoaders;  // a thread may have 255 registers
 };
 
 // tcgen05 pieces that only this kernel uses
@@ -85,12 +83,12 @@ __device__ __forceinline__ void tmem_ld_wait(float (&v)[N]) {
     for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
 
-// Descriptors of a tile [HD/64 blocks][keys][128 bytes], 16-byte chunk c of a
-// row stored at c ^ (row % 8).  K-major (K tile): rows are N, 8-row groups 1024
-// bytes apart.  MN-major (V tile): rows are K, 8-row groups 1024 bytes apart
-// (stride offset), 64-wide blocks of N `block` bytes apart (leading offset).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t leading) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+// Descriptors of a tile [group of 8 keys][64-dim block][8 keys][128 bytes], 16-byte
+// chunk c of a row stored at c ^ (row % 8).  K-major (K tile): keys are N, `stride`
+// from one group of eight to the next.  MN-major (V tile): keys are K, 64-wide
+// blocks of N `leading` bytes apart, groups of eight keys `stride` bytes apart.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
            (uint64_t)1u << 46 | (uint64_t)2u << 61;
 }
 template <typename T>
@@ -104,7 +102,8 @@ __device__ __forceinline__ constexpr uint32_t attention_idesc(int n, bool b_mn_m
 struct TensorCursor {
     int seg, last;   // -1: prefix, else request; the tile's last request
     int tile, tiles; // key tile of the segment
-    int lo, hi;      // keys of the segment
+    int lo, hi;      // keys of the segment; lo is rounded down to a box
+    int from;        // the first that any row sees
 };
 
 // Requests of row tile i: [first, last], first > last when it has no tokens.
@@ -119,12 +118,12 @@ template <typename T, int HD>
 __device__ __forceinline__ void tensor_segment(const AttnParams<T>& p, int i, TensorCursor& c) {
     c.tile = 0;
     if (c.seg < 0) {
-        c.lo = p.prefix_lo;
-        c.hi = p.prefix_by_stream ? p.prefix_lo : p.prefix_len;
+        c.from = p.prefix_lo;
+        c.hi = p.prefix_few ? p.prefix_lo : p.prefix_len;
     } else {
         const Request r = request_of(p, c.seg);
-        c.lo = c.hi = 0;
-        if (by_tensor(p, r)) {
+        c.from = c.hi = 0;
+        if (is_many(p, r)) {
             // its tokens in the tile, and what they see of its own keys
             const int j0 = max(0, (int)((long long)i * kTcRows / p.G) - r.start);
             const int j1 = min(r.used, (int)((((long long)i + 1) * kTcRows - 1) / p.G) + 1 - r.start);
@@ -132,19 +131,20 @@ __device__ __forceinline__ void tensor_segment(const AttnParams<T>& p, int i, Te
                 int lo, hi, unused;
                 seen_by(p, r, j0, lo, unused);
                 seen_by(p, r, j1 - 1, unused, hi);
-                c.lo = max(0, min(r.len, lo - p.prefix_len));
-                c.hi = max(c.lo, min(r.len, hi - p.prefix_len));
+                c.from = max(0, min(r.len, lo - p.prefix_len));
+                c.hi = max(c.from, min(r.len, hi - p.prefix_len));
             }
         }
     }
-    c.tiles = (c.hi - c.lo + TensorShape<HD>::kKeys - 1) / TensorShape<HD>::kKeys;
+    c.lo = c.from & ~(kMaxRun - 1);
+    c.tiles = c.hi > c.from ? (c.hi - c.lo + TensorShape<HD>::kKeys - 1) / TensorShape<HD>::kKeys : 0;
 }
 
 // First segment with keys of row tile i at or behind c.seg; false if none.
 template <typename T, int HD>
 __device__ __forceinline__ bool tensor_seek(const AttnParams<T>& p, int i, TensorCursor& c) {
     for (;;) {
-        if (c.seg > c.last || (c.seg >= 0 && p.max_query * p.G <= p.tensor_above)) return false;
+        if (c.seg > c.last || (c.seg >= 0 && p.max_query * p.G <= p.many_above)) return false;
         tensor_segment<T, HD>(p, i, c);
         if (c.tiles) return true;
         if (c.seg < 0) {
@@ -156,9 +156,9 @@ __device__ __forceinline__ bool tensor_seek(const AttnParams<T>& p, int i, Tenso
         }
     }
 }
+// The first unit of the next segment.
 template <typename T, int HD>
-__device__ __forceinline__ void tensor_advance(const AttnParams<T>& p, int i, TensorCursor& c) {
-    if (++c.tile < c.tiles) return;
+__device__ __noinline__ TensorCursor tensor_next_segment(const AttnParams<T>& p, int i, TensorCursor c) {
     if (c.seg < 0) {
         int first, last;
         requests_of_tile(p, i, first, last);
@@ -167,27 +167,28 @@ __device__ __forceinline__ void tensor_advance(const AttnParams<T>& p, int i, Te
         ++c.seg;
     }
     tensor_seek<T, HD>(p, i, c);
+    return c;
+}
+template <typename T, int HD>
+__device__ __forceinline__ void tensor_advance(const AttnParams<T>& p, int i, TensorCursor& c) {
+    if (++c.tile >= c.tiles) c = tensor_next_segment<T, HD>(p, i, c);
 }
 // The cursor at the `skip`-th unit of row tile i.
 template <typename T, int HD>
-__device__ __forceinline__ TensorCursor tensor_begin(const AttnParams<T>& p, int i, int skip) {
+__device__ __noinline__ TensorCursor tensor_begin(const AttnParams<T>& p, int i, int skip) {
     TensorCursor c;
     int first;
     requests_of_tile(p, i, first, c.last);
     c.seg = -1;
     while (tensor_seek<T, HD>(p, i, c) && skip >= c.tiles) {
         skip -= c.tiles;
-        c.tile = c.tiles - 1;
-        if (c.seg < 0)
-            c.seg = first;
-        else
-            ++c.seg;
+        c.seg = c.seg < 0 ? first : c.seg + 1;
     }
     c.tile = skip;
     return c;
 }
 template <typename T, int HD>
-__device__ __forceinline__ int tensor_units(const AttnParams<T>& p, int i) {
+__device__ __noinline__ int tensor_units(const AttnParams<T>& p, int i) {
     TensorCursor c;
     int first, units = 0;
     requests_of_tile(p, i, first, c.last);
@@ -200,75 +201,66 @@ __device__ __forceinline__ int tensor_units(const AttnParams<T>& p, int i) {
     return units;
 }
 
+// The units of all row tiles; `before` those before this thread's own [i0, i1).
 template <typename T, int HD>
-__global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
-    attention_many_rows_kernel(const __grid_constant__ AttnParams<T> p) {
-    using S = TensorShape<HD>;
-    constexpr int N = S::kKeys, CPR = HD / 8;
-    extern __shared__ uint8_t raw[];
-    __shared__ __align__(8) uint64_t full[S::kSlots], empty[S::kSlots], s_full[2], p_full[2], o_done[2], q_full,
-        drained;
-    __shared__ uint32_t s_tmem;
-    __shared__ int red[32], s_tile, s_at, s_units;
-    __shared__ volatile int s_dead;
-    const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row_tiles = (int)(((long long)p.T_tokens * p.G + kTcRows - 1) / kTcRows);
+__device__ __forceinline__ int all_tensor_units(const AttnParams<T>& p, int* red, int i0, int i1, int& before) {
+    int sum = 0, total;
+    for (int i = i0; i < i1; ++i) sum += tensor_units<T, HD>(p, i) * p.nkv;
+    before = block_scan(sum, red, &total);
+    return total;
+}
 
+struct TensorBarriers {
+    uint64_t full[2][4], empty[2][4], s_full[2],  // [K, V][slot]
+        p_full[2], o_done[2], q_full, drained;
+    uint32_t tmem;
+    volatile int dead;
+};
+
+// One CTA: units [u0, u1) of worker `worker`; the first is in row tile `tile`,
+// which begins at unit `tile_at` and has `tile_units` units a KV head.
+template <typename T, int HD>
+__device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring, TensorBarriers& bar, int u0, int u1,
+                                           int tile0, int tile_at, int tile_units, int worker) {
+    using S = TensorShape<HD>;
+    constexpr int N = S::kKeys;
+    const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kSlots; ++i) {
-            mbar_init(&full[i], S::kLoaders);
-            mbar_init(&empty[i], 1);
+            for (int kv = 0; kv < 2; ++kv) {
+                mbar_init(&bar.full[kv][i], 1);
+                mbar_init(&bar.empty[kv][i], 1);
+            }
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 128);
-            mbar_init(&o_done[i], 1);
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_full[i], 128);
+            mbar_init(&bar.o_done[i], 1);
         }
-        mbar_init(&q_full, 128);
-        mbar_init(&drained, 1);
+        mbar_init(&bar.q_full, 128);
+        mbar_init(&bar.drained, 1);
         fence_mbar_init();
-        s_dead = 0;
-        s_units = 0;
+        bar.dead = 0;
     }
-    // ---- which units are mine: sums over the row tiles, as in the stream kernel ----
-    int U, u0, u1;
-    {
-        const int per = (row_tiles + blockDim.x - 1) / blockDim.x;
-        const int i0 = min(row_tiles, (int)threadIdx.x * per), i1 = min(row_tiles, i0 + per);
-        int sum = 0;
-        for (int i = i0; i < i1; ++i) sum += tensor_units<T, HD>(p, i) * p.nkv;
-        int at = block_scan(sum, red, &U);
-        u0 = unit_begin(blockIdx.x, U, gridDim.x);
-        u1 = unit_begin(blockIdx.x + 1, U, gridDim.x);
-        for (int i = i0; i < i1; ++i) {
-            const int units = tensor_units<T, HD>(p, i);
-            if (blockIdx.x == 0) p.tensor.base[i] = at;
-            if (u0 >= at && u0 < at + units * p.nkv) {
-                s_tile = i;
-                s_at = at;
-                s_units = units;
-            }
-            at += units * p.nkv;
-        }
-        if (blockIdx.x == 0 && threadIdx.x == 0) p.tensor.base[row_tiles] = U;
-    }
-    if (u0 >= u1) return;  // the same for the whole CTA
-    if (warp == 4) tmem_alloc(&s_tmem, 512);
+    if (warp == 4) tmem_alloc(&bar.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = bar.tmem;
 
-    // Bounded waits: about a second, or until another warp gave up.
-    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        for (uint32_t i = 0; i < kSpinLimit; ++i) {
-            if (mbar_try_wait_sleep(bar, parity, 1000u)) return true;
-            if (s_dead) return false;
+    // Bounded waits: about two seconds, or until another warp gave up.
+    auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+        if (mbar_try_wait(b, parity)) return true;
+        const long long since = clock64();
+        while (!mbar_try_wait(b, parity)) {
+            if (bar.dead) return false;
+            if (clock64() - since > 4000000000ll) {
+                bar.dead = 1;
+                atomicOr(p.err, kErrMbarTimeout);
+                return false;
+            }
         }
-        s_dead = 1;
-        atomicOr(p.err, kErrMbarTimeout);
-        return false;
+        return true;
     };
     // Every role walks the CTA's jobs: (row tile, KV head, units [from, to) of `units`).
     struct Job {
@@ -276,9 +268,9 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
     };
     auto first_job = [&]() {
         Job j;
-        const int in = u0 - s_at;
-        j.tile = s_tile;
-        j.units = s_units;
+        const int in = u0 - tile_at;
+        j.tile = tile0;
+        j.units = tile_units;
         j.kvh = in / j.units;
         j.from = in % j.units;
         j.to = min(j.units, j.from + u1 - u0);
@@ -295,123 +287,105 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
         j.to = min(j.units, u1 - u);
     };
 
-    if (warp >= 5) {
-        // ---- loaders: tile after tile, K then V ---------------------------------
-        const int lw = warp - 5;
-        constexpr int kRows = N / S::kLoaders;          // of a tile, per warp
-        constexpr int kLag = 2;                         // tiles between a copy's issue and its hand-over
+    if (warp > 6) {
+        // no work
+    } else if (warp >= 5) {
+        // ---- loaders: warp 5 K, warp 6 V, tile after tile -------------------------------
+        const int kv = warp - 5;
         int it = 0;
         bool ok = true;
-        auto hand_over = [&](int tile) {
-            fence_proxy_async_smem();  // the copies are read by the tensor cores
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[tile % S::kSlots]);
-        };
         Job job = first_job();
         for (int u = u0; ok && u < u1;) {
             TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from);
-            for (int x = job.from; ok && x < job.to; ++x) {
-                long long off[kRows / 32];  // element offsets of the keys lane, lane + 32, ...
-                uint32_t mask[kRows / 32];  // which of them exist
-#pragma unroll
-                for (int w = 0; w < kRows / 32; ++w) {
-                    const int pos = c.lo + c.tile * N + lw * kRows + w * 32 + lane;
-                    bool have = false;
-                    off[w] = 0;
-                    if (pos < c.hi) {
-                        const int at = pos / p.kv.page_size;
-                        const int page = c.seg < 0 ? p.prefix_pages[at] : p.table[(long long)c.seg * p.max_pages + at];
-                        have = page >= 0 && page < p.kv.num_pages;
-                        if (have)
-                            off[w] = page * p.kv.page_stride + (pos - at * p.kv.page_size) * p.kv.pos_stride +
-                                     job.kvh * p.kv.head_stride;
-                        else
-                            atomicOr(p.err, kErrBadPage);
-                    }
-                    mask[w] = __ballot_sync(0xffffffffu, have);
+            TileKeys<N> next = look_up_keys<N>(p, c.seg, c.lo + c.tile * N, c.from, c.hi);
+            for (int x = job.from; ok && x < job.to; ++x, ++it) {
+                TileKeys<N> now = next;
+                check_keys(p, now);
+                if (x + 1 < job.to) {
+                    tensor_advance<T, HD>(p, job.tile, c);
+                    next = look_up_keys<N>(p, c.seg, c.lo + c.tile * N, c.from, c.hi);
                 }
-#pragma unroll 1
-                for (int kv = 0; kv < 2 && ok; ++kv, ++it) {
-                    const int slot = it % S::kSlots;
-                    ok = wait(&empty[slot], ((it / S::kSlots) & 1) ^ 1);
-                    if (!ok) break;
-                    const T* src = kv ? p.kv.v : p.kv.k;
-                    const uint32_t dst = ring + slot * S::kSlot;
-                    constexpr int kPer = 32 * CPR / 32;  // copies of 32 rows, per lane
-#pragma unroll
-                    for (int w = 0; w < kRows / 32; ++w)
-#pragma unroll 8
-                        for (int i = 0; i < kPer; ++i) {
-                            const int chunk = i * 32 + lane, rr = chunk / CPR, ch = chunk % CPR;
-                            const int row = lw * kRows + w * 32 + rr;
-                            const long long o = __shfl_sync(0xffffffffu, off[w], rr);
-                            const int bytes = ((mask[w] >> rr) & 1) && ch * 8 < p.hd ? 16 : 0;
-                            cp_async16(dst + (ch >> 3) * (N * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
-                                       src + (bytes ? o + ch * 8 : 0), bytes);
-                        }
-                    cp_async_commit();
-                    if (it >= kLag) {
-                        cp_async_wait<kLag>();
-                        hand_over(it - kLag);
-                    }
-                }
-                if (x + 1 < job.to) tensor_advance<T, HD>(p, job.tile, c);
+                const int slot = it % S::kSlots;
+                ok = __all_sync(0xffffffffu, wait(&bar.empty[kv][slot], ((it / S::kSlots) & 1) ^ 1));
+                if (ok)
+                    load_tile_keys<HD, N>(p, kv != 0, ring + (kv * S::kSlots + slot) * S::kSlot, job.kvh, now,
+                                          &bar.full[kv][slot]);
             }
             u += job.to - job.from;
             if (u < u1) next_job(job, u);
         }
-        cp_async_wait<0>();
-        if (ok)
-            for (int tile = max(0, it - kLag); tile < it; ++tile) hand_over(tile);
+        // after a wait that gave up: what is in flight lands before the CTA may end
+        if (!ok)
+            for (int i = max(0, it - 1 - S::kSlots); i < it - 1; ++i)
+                mbar_wait_limited(&bar.full[kv][i % S::kSlots], (i / S::kSlots) & 1, p.err);
     } else if (warp == 4) {
-        // ---- MMA issue: one thread ------------------------------------------------
-        if (lane == 0) {
+        // ---- MMA issue: one elected thread ------------------------------------------
+        if (elect_one()) {
+            constexpr uint32_t kGroup8 = HD / 64 * 1024;  // bytes of eight keys
             constexpr uint32_t idesc_s = attention_idesc<T>(N, false), idesc_o = attention_idesc<T>(HD, true);
-            int uc = 0, jobs = 0;  // units and jobs so far
+            struct Place {  // in a ring
+                int slot = 0;
+                uint32_t phase = 0;
+                __device__ __forceinline__ void next() {
+                    if (++slot == S::kSlots) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
+            } k, v;
+            uint32_t s_buf = 0, p_buf = 0, p_phase = 0, q_phase = 0;  // score buffers of the next S and P
             bool ok = true;
-            auto scores = [&](int x) {  // S[x % 2] = Q K^T of the CTA's x-th unit
-                const int it = 2 * x, slot = it % S::kSlots;
-                if (!wait(&full[slot], (it / S::kSlots) & 1)) return false;
-                tc_fence_after();
-                const uint32_t base = ring + slot * S::kSlot;
+            auto scores = [&]() {  // S = Q K^T of the next K tile
+                const uint32_t base = ring + k.slot * S::kSlot, to = tmem + S::kColS + s_buf * N;
+#pragma unroll 1  // four at a time: short enough to stay in the scheduler's instruction cache
+                for (int b = 0; b < HD / 64; ++b)
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks)
-                    umma_f16_ts(tmem + S::kColS + (x & 1) * N, tmem + S::kColQ + ks * 8,
-                                tile_desc(base + (ks >> 2) * (N * 128) + (ks & 3) * 32, 16), idesc_s, ks > 0);
-                umma_commit(&empty[slot]);
-                umma_commit(&s_full[x & 1]);
-                return true;
+                    for (int i = 0; i < 4; ++i)
+                        umma_f16_ts(to, tmem + S::kColQ + b * 32 + i * 8, tile_desc(base + b * 1024 + i * 32, 16, kGroup8),
+                                    idesc_s, b > 0 || i > 0);
+                umma_commit(&bar.s_full[s_buf]);
+                umma_commit(&bar.empty[0][k.slot]);
+                k.next();
+                s_buf ^= 1;
             };
             Job job = first_job();
             for (int u = u0; ok && u < u1;) {
                 const int n = job.to - job.from;
-                ok = wait(&q_full, jobs & 1);
+                ok = wait(&bar.q_full, q_phase) && wait(&bar.full[0][k.slot], k.phase);
+                if (!ok) break;
                 tc_fence_after();
-                ok = ok && scores(uc);
-                for (int x = 0; ok && x < n; ++x) {
-                    if (x + 1 < n) ok = scores(uc + x + 1);
-                    const int it = 2 * (uc + x) + 1, slot = it % S::kSlots;
-                    ok = ok && wait(&p_full[(uc + x) & 1], ((uc + x) >> 1) & 1) &&
-                         wait(&full[slot], (it / S::kSlots) & 1);
+                scores();
+                // The scores of unit x + 1, then O += P V of unit x: the softmax of x + 1 runs beside
+                // the second and the scores of x + 2.  About five MMAs can be queued, so behind PV's (128
+                // clocks each) there is time for the waits before the next scores, and behind those
+                // (32 clocks each) only for one: everything but the weights is waited for up front.
+                for (int x = 0; x < n; ++x) {
+                    const bool more = x + 1 < n;
+                    ok = wait(&bar.full[1][v.slot], v.phase) && (!more || wait(&bar.full[0][k.slot], k.phase));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t base = ring + slot * S::kSlot;
+                    if (more) scores();
+                    ok = wait(&bar.p_full[p_buf], p_phase);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t base = ring + (S::kSlots + v.slot) * S::kSlot, p_at = tmem + S::kColS + p_buf * N;
 #pragma unroll
                     for (int ks = 0; ks < N / 16; ++ks)
-                        umma_f16_ts(tmem + S::kColO, tmem + S::kColS + ((uc + x) & 1) * N + ks * 8,
-                                    tile_desc(base + ks * 2048, N * 128), idesc_o, x > 0 || ks > 0);
-                    umma_commit(&empty[slot]);
-                    umma_commit(&o_done[(uc + x) & 1]);
+                        umma_f16_ts(tmem + S::kColO, p_at + ks * 8, tile_desc(base + ks * 2 * kGroup8, 1024, kGroup8),
+                                    idesc_o, ks > 0 || x > 0);
+                    umma_commit(&bar.empty[1][v.slot]);
+                    umma_commit(&bar.o_done[p_buf]);
+                    v.next();
+                    p_phase ^= p_buf;
+                    p_buf ^= 1;
                 }
-                uc += n;
-                ++jobs;
+                q_phase ^= 1;
                 u += n;
                 if (u < u1) next_job(job, u);
             }
             // tensor memory is given back only when no MMA uses it, also after a wait that gave up
-            umma_commit(&drained);
-            for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait_sleep(&drained, 0, 1000u); ++i) {
-            }
+            umma_commit(&bar.drained);
+            mbar_wait_limited(&bar.drained, 0, p.err);
         }
         __syncwarp();
     } else {
@@ -423,7 +397,7 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
         // O holds everything up to unit uc - 1.  A barrier for even and one for odd units:
         // a commit covers all earlier MMAs, so the scores of unit uc being there means that
         // the phase before the one waited for here (unit uc - 3) is over.
-        auto o_ready = [&]() { return wait(&o_done[(uc - 1) & 1], ((uc - 1) >> 1) & 1); };
+        auto o_ready = [&]() { return wait(&bar.o_done[(uc - 1) & 1], ((uc - 1) >> 1) & 1); };
         Job job = first_job();
         for (int u = u0; ok && u < u1;) {
             const long long row = (long long)job.tile * kTcRows + threadIdx.x;
@@ -436,7 +410,7 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
                 const Request r = request_of(p, b);
                 if (t - r.start < r.used) {
                     seen_by(p, r, t - r.start, row_lo, row_hi);
-                    own = by_tensor(p, r);
+                    own = is_many(p, r);
                 } else {
                     b = p.B;
                 }
@@ -460,13 +434,13 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&q_full);
+                mbar_arrive(&bar.q_full);
             }
             float m = -INFINITY, d = 0.f;
             TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from);
             for (int x = job.from; x < job.to; ++x, ++uc) {
                 const int buf = uc & 1;
-                ok = wait(&s_full[buf], (uc >> 1) & 1);
+                ok = wait(&bar.s_full[buf], (uc >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t scol = mine + S::kColS + buf * N;
@@ -537,7 +511,7 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&p_full[buf]);
+                mbar_arrive(&bar.p_full[buf]);
                 if (x + 1 < job.to) tensor_advance<T, HD>(p, job.tile, c);
             }
             // ---- the job's part, or the result where nothing else belongs to it ------
@@ -547,8 +521,8 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
             const bool whole = job.from == 0 && job.to == job.units;
             const bool final = whole && own;
             const long long at = job.from == 0 ? (long long)t * p.nq + h
-                                               : (long long)blockIdx.x * kTcRows + threadIdx.x;
-            float* po = (job.from == 0 ? p.tensor.first : p.tensor.cont) + at * p.hd;
+                                               : (long long)worker * kTcRows + threadIdx.x;
+            float* po = (job.from == 0 ? p.many.first : p.many.cont) + at * p.hd;
             const float inv = d == 0.f ? 0.f : 1.f / d;
             bool fine = isfinite(d);
 #pragma unroll
@@ -581,9 +555,9 @@ __global__ void __launch_bounds__(TensorShape<HD>::kThreads, 1)
                 if (final) {
                     if (p.lse) p.lse[at] = d == 0.f ? -INFINITY : (m + log2f(d)) * kLn2;
                     // NaN here asks the joining kernel to compute the row by itself
-                    p.tensor.first_md[at] = make_float2(fine ? 0.f : __int_as_float(0x7fffffff), 0.f);
+                    p.many.first_md[at] = make_float2(fine ? 0.f : __int_as_float(0x7fffffff), 0.f);
                 } else {
-                    (job.from == 0 ? p.tensor.first_md : p.tensor.cont_md)[at] = make_float2(m, d);
+                    (job.from == 0 ? p.many.first_md : p.many.cont_md)[at] = make_float2(m, d);
                 }
             }
             tc_fence_before();
