@@ -66,9 +66,10 @@ __device__ void attend_alone(const AttnParams<T>& p, int b, const Request& r, in
 // Nanoseconds of an SM that a unit takes, for dealing the SMs to the two kinds
 // of work.  A streamed unit is bound by memory: 16 keys of K and V at an SM's
 // share of the bandwidth (6450 / 148 bytes a nanosecond).  A tensor unit is 64
-// (head_dim 256) or 128 keys for 128 rows.
+// (head_dim 256) or 128 keys for 128 rows: 600 ns by itself, but beside the
+// stream its loads take their turn behind the others'; measured 1400.
 __host__ __device__ constexpr float few_unit_ns(int hd) { return 16.f * 4.f * hd / 43.6f; }
-__host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 64 ? 900.f : 700.f; }
+__host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 64 ? 1400.f : 1000.f; }
 
 // All parts of all rows, one CTA per SM.  Every CTA sums the units of both kinds
 // over the batch and finds its share: the first CTAs take the tensor cores' jobs,
@@ -81,6 +82,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     __shared__ TensorBarriers bar;
     __shared__ __align__(8) uint64_t full[S::kBars];
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
+    griddep_launch_dependents();
     const int grid = gridDim.x, cta = blockIdx.x;
     constexpr bool kTensor = HD <= 256;
 
@@ -201,6 +203,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
     __shared__ RowParts rows[kJoinRows];
     const int lane = threadIdx.x & 31;
     const int row0 = blockIdx.x * rows_per_cta, n_rows = min(rows_per_cta, p.T_tokens * p.nq - row0);
+    griddep_wait();
     const Deal deal = *p.deal;
     for (int i = threadIdx.x; i < n_rows; i += blockDim.x) {
         RowParts x = {};
@@ -455,8 +458,17 @@ tf_status launch(tf_context* ctx, const AttnParams<T>& p, const Shape& s, cudaSt
     // a warp per row while that fills the GPU; then more rows a CTA
     const int rows = p.T_tokens * p.nq;
     const int per = std::min(kJoinRows, std::max(8, (rows / (ctx->num_sms * 4) + 7) / 8 * 8));
-    join_parts_kernel<T><<<(rows + per - 1) / per, 256, 0, cs>>>(p, per);
-    return cuda_check(ctx, cudaGetLastError(), name);
+    // launched while the parts' last CTAs still run; it waits for them before it reads
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows + per - 1) / per));
+    cfg.blockDim = dim3(256);
+    cfg.stream = cs;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cuda_check(ctx, cudaLaunchKernelEx(&cfg, join_parts_kernel<T>, p, per), name);
 }
 
 }  // namespace

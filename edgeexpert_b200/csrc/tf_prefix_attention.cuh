@@ -180,13 +180,17 @@ __device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity
     return true;
 }
 
+// What L2 should do with what is loaded: own keys are read once (by one job) and
+// leave first; prefix keys are read by every row tile and stay.
+enum : uint64_t { kLeaveFirst = 0x12F0000000000000ull, kStay = 0x14F0000000000000ull };
+
 // 5-D tiled TMA load (no multicast).
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int v, int w,
-                                            uint64_t* bar) {
+                                            uint64_t* bar, uint64_t hint) {
     asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-        "%6}], [%7];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(w), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, "
+        "%3, %4, %5, %6}], [%7], %8;" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(w), "r"(smem_u32(bar)), "l"(hint)
         : "memory");
 }
 
@@ -213,7 +217,7 @@ struct TileKeys {
 
 template <int HD, int KEYS, typename T>
 __device__ __forceinline__ void load_tile_keys(const AttnParams<T>& p, bool v, uint32_t tile, int head,
-                                               const TileKeys<KEYS>& k, uint64_t* bar) {
+                                               const TileKeys<KEYS>& k, uint64_t* bar, uint64_t hint) {
     constexpr int kBlocks = HD / 64, kMost = TileKeys<KEYS>::kMost;
     const CUtensorMap* map = v ? &p.maps.v : &p.maps.k;
     const int lane = threadIdx.x & 31, run = 1 << p.run_shift, runs = KEYS >> p.run_shift, all = (1 << run) - 1;
@@ -226,7 +230,7 @@ __device__ __forceinline__ void load_tile_keys(const AttnParams<T>& p, bool v, u
 #pragma unroll 2
         for (int r = 0; r < KEYS / 8; ++r) {
             const int pg = __shfl_sync(0xffffffffu, k.page[0], r), in = __shfl_sync(0xffffffffu, k.in_page[0], r);
-            if (one) tma_load_5d(tile + r * (kBlocks * 1024), map, 0, in, 0, head, pg, bar);
+            if (one) tma_load_5d(tile + r * (kBlocks * 1024), map, 0, in, 0, head, pg, bar, hint);
         }
         __syncwarp();
         return;
@@ -242,14 +246,14 @@ __device__ __forceinline__ void load_tile_keys(const AttnParams<T>& p, bool v, u
             if (!one) continue;
             if (!v || have == all || have == 0) {
                 if (p.wide)
-                    tma_load_5d(dst, map, 0, in, 0, head, from, bar);
+                    tma_load_5d(dst, map, 0, in, 0, head, from, bar, hint);
                 else
-                    for (int b = 0; b < kBlocks; ++b) tma_load_5d(dst + b * 1024, map, b * 64, in, 0, head, from, bar);
+                    for (int b = 0; b < kBlocks; ++b) tma_load_5d(dst + b * 1024, map, b * 64, in, 0, head, from, bar, hint);
             } else {
                 for (int r = 0; r < run; ++r)
                     for (int b = 0; b < kBlocks; ++b)
                         tma_load_5d(dst + b * 1024 + r * 128, &p.maps.v_row, b * 64, in + r, 0, head,
-                                    (have >> r) & 1 ? pg : p.kv.num_pages, bar);
+                                    (have >> r) & 1 ? pg : p.kv.num_pages, bar, hint);
             }
         }
     __syncwarp();

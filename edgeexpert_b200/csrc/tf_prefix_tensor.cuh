@@ -189,6 +189,11 @@ __device__ __noinline__ TensorCursor tensor_begin(const AttnParams<T>& p, int i,
 }
 template <typename T, int HD>
 __device__ __noinline__ int tensor_units(const AttnParams<T>& p, int i) {
+    if (p.max_query * p.G <= p.many_above) {  // the prefix alone, for any tile with a token of the batch
+        constexpr int N = TensorShape<HD>::kKeys;
+        const bool live = (int)((long long)i * kTcRows / p.G) < p.starts[p.B];
+        return live && p.prefix_len > p.prefix_lo ? (p.prefix_len - (p.prefix_lo & ~(kMaxRun - 1)) + N - 1) / N : 0;
+    }
     TensorCursor c;
     int first, units = 0;
     requests_of_tile(p, i, first, c.last);
@@ -309,7 +314,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                 ok = __all_sync(0xffffffffu, wait(&bar.empty[kv][slot], ((it / S::kSlots) & 1) ^ 1));
                 if (ok)
                     load_tile_keys<HD, N>(p, kv != 0, ring + (kv * S::kSlots + slot) * S::kSlot, job.kvh, now,
-                                          &bar.full[kv][slot]);
+                                          &bar.full[kv][slot], kStay);
             }
             u += job.to - job.from;
             if (u < u1) next_job(job, u);
