@@ -10,6 +10,19 @@ using namespace tf;
 
 namespace {
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // ---- page tables -------------------------------------------------------------
 struct ResizeParams {
     const int* seq_lens;
@@ -23,15 +36,26 @@ struct ResizeParams {
     int* slots;
     int* positions;
     int* requests;
-    int* plan;  // [0] head, [1] free count, then per request {old length, first page taken, first page given back}
+    int* plan;       // [0] head, [1] free count, then per request {old length, new length, first page taken, first given back}
+    int* starts_at;  // the starts as resize_fill reads them
     uint32_t* err;
     int B, max_pages, N, ps, base, max_tokens;
+    int most;  // positions a request's table can hold
 };
 
 constexpr int kResizeThreads = 1024;
 constexpr int kFillThreads = 256;
+constexpr uint32_t kSmallTokens = 1024, kSmallRequests = 256;
 
-__device__ __forceinline__ int pages_of(int n, int ps) { return (int)(((long long)n + ps - 1) / ps); }
+// (64-bit divisions would be most of a small call's time: lengths and page sizes are below 2^31)
+__device__ __forceinline__ int pages_of(int n, int ps) { return (int)(((unsigned)n + (unsigned)ps - 1u) / (unsigned)ps); }
+// Place head + x of a ring of N.
+__device__ __forceinline__ int ring_at(int head, long long x, int N) {
+    unsigned long long at = (unsigned long long)head + (unsigned long long)x;
+    if (at >= (unsigned)N) at -= (unsigned)N;
+    if (at >= (unsigned)N) at %= (unsigned)N;
+    return (int)at;
+}
 
 // Exclusive sum over the block's threads; *total receives the whole sum.
 __device__ long long block_exclusive_sum(long long v, long long* red, long long* total) {
@@ -65,10 +89,9 @@ struct Ask {
 
 __device__ __forceinline__ Ask ask_of(const ResizeParams& p, int b) {
     Ask a;
-    const long long most = (long long)p.max_pages * p.ps;
-    a.old_len = (int)max(0ll, min((long long)p.seq_lens[b], most));
+    a.old_len = max(0, min(p.seq_lens[b], p.most));
     a.target = p.targets[b];
-    const bool valid = a.target >= 0 && a.target <= most;
+    const bool valid = a.target >= 0 && a.target <= p.most;
     a.grow = valid && a.target > a.old_len;
     a.shrink = valid && a.target < a.old_len;
     const int d = (a.grow || a.shrink) ? pages_of(a.target, p.ps) - pages_of(a.old_len, p.ps) : 0;
@@ -90,7 +113,8 @@ __device__ void resize_plan(const ResizeParams& p) {
         s_taken = 0;
         s_refused = 0;
     }
-    const int head = (int)(((long long)p.state[0] % p.N + p.N) % p.N);
+    int head = p.state[0];
+    if (head < 0 || head >= p.N) head = (head % p.N + p.N) % p.N;
     const int free_count = max(0, min(p.state[1], p.N));
     const int per = (p.B + blockDim.x - 1) / blockDim.x;
     const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
@@ -139,20 +163,24 @@ __device__ void resize_plan(const ResizeParams& p) {
         const bool granted = paged && d <= p.max_tokens;
         if (granted && a.need) taken = (int)c;
         refused += (a.target > a.old_len && !granted) ? 1 : 0;
-        p.plan[2 + 3 * b] = a.old_len;
-        p.plan[3 + 3 * b] = first_page;
-        p.plan[4 + 3 * b] = first_back;
-        p.lens_out[b] = granted || a.shrink ? a.target : a.old_len;
-        p.starts[b + 1] = (int)min(d, fit);
+        const int len = granted || a.shrink ? a.target : a.old_len, start = (int)min(d, fit);
+        p.plan[2 + 4 * b] = a.old_len;
+        p.plan[3 + 4 * b] = len;
+        p.plan[4 + 4 * b] = first_page;
+        p.plan[5 + 4 * b] = first_back;
+        p.lens_out[b] = len;
+        p.starts[b + 1] = start;
+        if (p.starts_at != p.starts) p.starts_at[b + 1] = start;
     }
     if (taken) atomicMax(&s_taken, taken);
     if (refused) atomicAdd(&s_refused, refused);
     __syncthreads();  // also: every thread has read the state, which state_out may be
     if (threadIdx.x == 0) {
         p.starts[0] = 0;
+        p.starts_at[0] = 0;
         p.plan[0] = head;
         p.plan[1] = free_count;
-        p.state_out[0] = (int)(((long long)head + s_taken) % p.N);
+        p.state_out[0] = ring_at(head, s_taken, p.N);
         p.state_out[1] = (int)min((long long)p.N, (long long)free_count - s_taken + back_total);
         p.state_out[2] = s_refused;
         p.state_out[3] = (int)fit;
@@ -160,55 +188,96 @@ __device__ void resize_plan(const ResizeParams& p) {
 }
 
 // Pages handed out and back (a warp per request) and the tokens' slots (a
-// thread per token, its request found by bisection of the starts).  Pages
+// thread per four tokens, their request found by bisection of the starts).  Pages
 // taken and pages given back lie in disjoint parts of the ring, and tables are
 // written only beyond the old length, so nothing here waits for anything else.
 __device__ void resize_fill(const ResizeParams& p, int cta, int ctas) {
     const int head = p.plan[0], free_count = p.plan[1];
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     for (int b = cta * warps + (threadIdx.x >> 5); b < p.B; b += ctas * warps) {
-        const int old_len = p.plan[2 + 3 * b], len = p.lens_out[b];
+        const int old_len = p.plan[2 + 4 * b], len = p.plan[3 + 4 * b];
         const int have = pages_of(old_len, p.ps), want = pages_of(len, p.ps);
         int* row = p.table + (long long)b * p.max_pages;
         for (int j = lane; j < want - have; j += 32)
-            row[have + j] = p.ring[((long long)head + p.plan[3 + 3 * b] + j) % p.N];
+            row[have + j] = p.ring[ring_at(head, (long long)p.plan[4 + 4 * b] + j, p.N)];
         for (int j = lane; j < have - want; j += 32)
-            p.ring[((long long)head + free_count + p.plan[4 + 3 * b] + j) % p.N] = row[want + j];
+            p.ring[ring_at(head, (long long)free_count + p.plan[5 + 4 * b] + j, p.N)] = row[want + j];
     }
-    const int total = p.starts[p.B];
-    for (long long i = (long long)cta * blockDim.x + threadIdx.x; i < p.max_tokens; i += (long long)ctas * blockDim.x) {
-        int slot = -1, position = -1, request = -1;
-        if (i < total) {
-            int lo = 0, hi = p.B - 1;  // the last b with starts[b] <= i (an empty request shares its start with the next)
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (p.starts[mid] <= i)
-                    lo = mid;
+    const int total = p.starts_at[p.B];
+    const bool vec = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions) |
+                       reinterpret_cast<uintptr_t>(p.requests)) & 15) == 0;
+    for (long long i0 = 4 * ((long long)cta * blockDim.x + threadIdx.x); i0 < p.max_tokens;
+         i0 += 4ll * ctas * blockDim.x) {
+        // the last b with starts[b] <= i0 (an empty request shares its start with the next);
+        // from there on the requests follow each other
+        int b = 0;
+        if (i0 < total) {
+            int hi = p.B - 1;
+            while (b < hi) {
+                const int mid = (b + hi + 1) >> 1;
+                if (p.starts_at[mid] <= i0)
+                    b = mid;
                 else
                     hi = mid - 1;
             }
-            request = lo;
-            const int old_len = p.plan[2 + 3 * lo];
-            const int at = old_len + (int)(i - p.starts[lo]);
-            position = p.base + at;
+        }
+        int slot[4], position[4], request[4];
+        int start = p.starts_at[b], end = p.starts_at[b + 1], old_len = p.plan[2 + 4 * b], first = p.plan[4 + 4 * b];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long i = i0 + k;
+            slot[k] = position[k] = request[k] = -1;
+            if (i >= total) continue;
+            while (i >= end) {
+                ++b;
+                start = end;
+                end = p.starts_at[b + 1];
+                old_len = p.plan[2 + 4 * b];
+                first = p.plan[4 + 4 * b];
+            }
+            const int at = old_len + (int)(i - start);
+            request[k] = b;
+            position[k] = p.base + at;
             const int page_at = at / p.ps, have = pages_of(old_len, p.ps);
-            const int page = page_at < have
-                                 ? p.table[(long long)lo * p.max_pages + page_at]
-                                 : p.ring[((long long)head + p.plan[3 + 3 * lo] + page_at - have) % p.N];
+            // a page taken in this call is read from the ring: the table may be written by another CTA
+            const int page = page_at < have ? p.table[(long long)b * p.max_pages + page_at]
+                                            : p.ring[ring_at(head, (long long)first + page_at - have, p.N)];
             if (page >= 0 && page < p.N)
-                slot = page * p.ps + at - page_at * p.ps;
+                slot[k] = page * p.ps + at - page_at * p.ps;
             else
                 atomicOr(p.err, kErrBadPage);
         }
-        p.slots[i] = slot;
-        p.positions[i] = position;
-        p.requests[i] = request;
+        if (vec && i0 + 3 < p.max_tokens) {
+            *reinterpret_cast<int4*>(p.slots + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+            *reinterpret_cast<int4*>(p.positions + i0) = make_int4(position[0], position[1], position[2], position[3]);
+            *reinterpret_cast<int4*>(p.requests + i0) = make_int4(request[0], request[1], request[2], request[3]);
+        } else {
+            for (int k = 0; k < 4 && i0 + k < p.max_tokens; ++k) {
+                p.slots[i0 + k] = slot[k];
+                p.positions[i0 + k] = position[k];
+                p.requests[i0 + k] = request[k];
+            }
+        }
     }
 }
 
-__global__ void __launch_bounds__(kResizeThreads) resize_plan_kernel(ResizeParams p) { resize_plan(p); }
-
+// Up to a thousand tokens one CTA plans and fills (a launch costs more than
+// the filling) and passes the plan in shared memory; beyond, the second kernel fills with the whole GPU and is
+// launched while the first still plans.
+__global__ void __launch_bounds__(kSmallRequests) resize_small_kernel(ResizeParams p) {
+    __shared__ int plan[2 + 4 * kSmallRequests], starts[kSmallRequests + 1];
+    p.plan = plan;
+    p.starts_at = starts;
+    resize_plan(p);
+    __syncthreads();
+    resize_fill(p, 0, 1);
+}
+__global__ void __launch_bounds__(kResizeThreads) resize_plan_kernel(ResizeParams p) {
+    griddep_launch_dependents();
+    resize_plan(p);
+}
 __global__ void __launch_bounds__(kFillThreads) resize_fill_kernel(ResizeParams p) {
+    griddep_wait();
     resize_fill(p, blockIdx.x, gridDim.x);
 }
 
@@ -240,7 +309,168 @@ __device__ __forceinline__ float2 turn_of(int position, double f, float factor) 
     return make_float2(c * factor, s * factor);
 }
 
-// One CTA per token, a warp per head.
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+    const float r = a * c - b * s;
+    b = a * s + b * c;
+    a = r;
+}
+
+// Bandwidth-bound: every value is read once and written once.  A CTA takes
+// `tokens` tokens.  A warp takes 32 / (HD / 16) heads of one at a time, a lane two
+// 16-byte chunks of a head: the two halves of eight pairs (half layout), four
+// pairs in each (interleaved), or what is not turned; neighbouring lanes have
+// neighbouring chunks (two chunks side by side in a lane would touch every
+// 32-byte sector twice).  The loads of two such items are issued first; the
+// angles of the CTA's tokens are computed, once for all heads, while they are in
+// flight.  Cosines in registers instead (computed per warp) took 128 registers
+// and, at 16 warps an SM, 73 us for 8191 tokens of 32 heads of 256.
+constexpr int kRopeTable = 2048;  // cosines and sines a CTA keeps
+template <typename T, int HD>
+__global__ void __launch_bounds__(256, 4) rope_vec_kernel(RopeParams p, PagedView<T> kv, int tokens) {
+    constexpr int I = HD / 16, H = 32 / I;  // lanes of a head, heads of an item
+    constexpr int U = 2;
+    __shared__ __align__(16) float2 table[kRopeTable];
+    __shared__ long long cells[16];  // of the CTA's tokens in the pool; -1: padding
+    const int lane = threadIdx.x & 31, li = lane % I, sub = lane / I, warp = threadIdx.x >> 5;
+    const int heads = p.nq + 2 * p.nkv, passes = (heads + H - 1) / H;
+    const int t0 = blockIdx.x * tokens, items = min(tokens, p.T - t0) * passes;
+    const int half = p.rot >> 1, turned = p.rot / 16;  // lanes [0, turned) turn
+    int c0, c1;  // first elements of the two chunks
+    if (p.interleaved) {
+        c0 = li * 8;
+        c1 = HD / 2 + li * 8;
+    } else if (li < turned) {
+        c0 = li * 8;
+        c1 = half + li * 8;
+    } else {
+        c0 = p.rot + (li - turned) * 8;
+        c1 = c0 + (HD - p.rot) / 2;
+    }
+    uint4 a[U], b[U];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int item = base + u * 8 + warp;
+            a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (item >= items) continue;
+            const int local = tokens == 1 ? 0 : item / passes, t = t0 + local, h = (item - local * passes) * H + sub;
+            if (h < heads) {
+                const T* src = h < p.nq ? static_cast<const T*>(p.q) + t * p.q_stride + (long long)h * HD
+                               : h < p.nq + p.nkv
+                                   ? static_cast<const T*>(p.k) + t * p.k_stride + (long long)(h - p.nq) * HD
+                                   : static_cast<const T*>(p.v) + t * p.v_stride + (long long)(h - p.nq - p.nkv) * HD;
+                a[u] = __ldcs(reinterpret_cast<const uint4*>(src + c0));
+                b[u] = __ldcs(reinterpret_cast<const uint4*>(src + c1));
+            }
+        }
+    };
+    load(0);
+    for (int local = warp; local < min(tokens, p.T - t0); local += 8) {
+        if (lane == 0) {
+            const int slot = p.slots[t0 + local];
+            long long cell = -1;
+            if (slot >= kv.num_pages * kv.page_size) {
+                atomicOr(p.err, kErrBadPage);
+            } else if (slot >= 0) {
+                const int page = slot / kv.page_size;
+                cell = page * kv.page_stride + (slot - page * kv.page_size) * kv.pos_stride;
+            }
+            cells[local] = cell;
+        }
+    }
+    if (tokens == 1) {
+        for (int i = threadIdx.x; i < half; i += 256) table[i] = turn_of(p.positions[t0], p.inv_freq[i], p.factor);
+    } else {
+        for (int local = warp; local < min(tokens, p.T - t0); local += 8)
+            for (int i = lane; i < half; i += 32)
+                table[local * half + i] = turn_of(p.positions[t0 + local], p.inv_freq[i], p.factor);
+    }
+    __syncthreads();
+    for (int base = 0; base < items; base += U * 8) {
+        if (base) load(base);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int item = base + u * 8 + warp;
+            if (item >= items) break;  // the same for the whole warp
+            const int local = tokens == 1 ? 0 : item / passes, t = t0 + local, h = (item - local * passes) * H + sub;
+            const int which = h < p.nq ? 0 : (h < p.nq + p.nkv ? 1 : 2);
+            const long long cell = cells[local];
+            float x[8], y[8], sum = 0.f;
+            const T* ea = reinterpret_cast<const T*>(&a[u]);
+            const T* eb = reinterpret_cast<const T*>(&b[u]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = to_float(ea[i]);
+                y[i] = to_float(eb[i]);
+                sum = fmaf(x[i], x[i], sum);
+                sum = fmaf(y[i], y[i], sum);
+            }
+            if (p.norm) {
+#pragma unroll
+                for (int o = 1; o < I; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float inv = rsqrtf(sum / (float)HD + p.eps);
+                const __nv_bfloat16* wt = which == 0 ? p.q_weight : (which == 1 ? p.k_weight : nullptr);
+                uint4 w0 = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u), w1 = w0;  // ones
+                if (wt) {
+                    w0 = *reinterpret_cast<const uint4*>(wt + c0);
+                    w1 = *reinterpret_cast<const uint4*>(wt + c1);
+                }
+                const uint32_t* e0 = reinterpret_cast<const uint32_t*>(&w0);
+                const uint32_t* e1 = reinterpret_cast<const uint32_t*>(&w1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[2 * i] *= inv * __uint_as_float(e0[i] << 16);
+                    x[2 * i + 1] *= inv * __uint_as_float(e0[i] & 0xFFFF0000u);
+                    y[2 * i] *= inv * __uint_as_float(e1[i] << 16);
+                    y[2 * i + 1] *= inv * __uint_as_float(e1[i] & 0xFFFF0000u);
+                }
+            }
+            const float2* cs = table + local * half;
+            if (which < 2) {
+                if (p.interleaved) {
+                    if (c0 < p.rot) {
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            const float4 w = *reinterpret_cast<const float4*>(cs + c0 / 2 + i);
+                            turn(x[2 * i], x[2 * i + 1], w.x, w.y);
+                            turn(x[2 * i + 2], x[2 * i + 3], w.z, w.w);
+                        }
+                    }
+                    if (c1 < p.rot) {
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            const float4 w = *reinterpret_cast<const float4*>(cs + c1 / 2 + i);
+                            turn(y[2 * i], y[2 * i + 1], w.x, w.y);
+                            turn(y[2 * i + 2], y[2 * i + 3], w.z, w.w);
+                        }
+                    }
+                } else if (li < turned) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const float4 w = *reinterpret_cast<const float4*>(cs + li * 8 + i);
+                        turn(x[i], y[i], w.x, w.y);
+                        turn(x[i + 1], y[i + 1], w.z, w.w);
+                    }
+                }
+            }
+            if (h >= heads || (cell < 0 && which)) continue;
+            T* dst = which == 0 ? static_cast<T*>(p.q_out) + t * p.qo_stride + (long long)h * HD
+                     : which == 1 ? kv.k + cell + (h - p.nq) * kv.head_stride
+                                  : kv.v + cell + (h - p.nq - p.nkv) * kv.head_stride;
+            uint32_t r[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                r[i] = cell < 0 ? 0u : pack2<T>(x[2 * i], x[2 * i + 1]);
+                r[i + 4] = cell < 0 ? 0u : pack2<T>(y[2 * i], y[2 * i + 1]);
+            }
+            *reinterpret_cast<uint4*>(dst + c0) = make_uint4(r[0], r[1], r[2], r[3]);
+            *reinterpret_cast<uint4*>(dst + c1) = make_uint4(r[4], r[5], r[6], r[7]);
+        }
+    }
+}
+
+// Any head size, pairs that no 16-byte boundary meets, rows of any alignment: one
+// CTA per token, a warp per head, a row in shared memory.
 template <typename T>
 __global__ void __launch_bounds__(128) rope_kernel(RopeParams p, PagedView<T> kv) {
     __shared__ float2 turn[kMaxPagedHeadDim / 2];
@@ -297,11 +527,39 @@ __global__ void __launch_bounds__(128) rope_kernel(RopeParams p, PagedView<T> kv
     }
 }
 
+template <typename T>
+tf_status launch_rope(tf_context* ctx, const RopeParams& p, const tf_paged_kv* kv, cudaStream_t cs, const char* name) {
+    const PagedView<T> view = paged_view<T>(kv);
+    // whole chunks: a power-of-two head size, halves (or pairs) of 16-byte chunks, aligned rows
+    const bool chunks = (p.hd == 64 || p.hd == 128 || p.hd == 256 || p.hd == 512) && p.rot % (p.interleaved ? 8 : 16) == 0;
+    const bool aligned = aligned16(p.q_weight) && aligned16(p.k_weight) && aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.q_out) &&
+                         (p.T == 1 || (p.q_stride | p.k_stride | p.v_stride | p.qo_stride) % 8 == 0);
+    if (!chunks || !aligned) {
+        rope_kernel<T><<<p.T, 128, 0, cs>>>(p, view);
+        return cuda_check(ctx, cudaGetLastError(), name);
+    }
+    // sixteen items a CTA (two a warp, all loads in flight), but a CTA a token while that
+    // does not fill the GPU
+    const int H = 512 / p.hd, passes = (p.nq + 2 * p.nkv + H - 1) / H;
+    const int fit = std::min(16 / std::min(passes, 16), p.rot ? kRopeTable / std::max(1, p.rot / 2) : 16);
+    const int tokens = std::max(1, std::min<int>(fit, (int)(p.T / (4ll * ctx->num_sms))));
+    const unsigned ctas = (unsigned)(((long long)p.T + tokens - 1) / tokens);
+    if (p.hd == 64)
+        rope_vec_kernel<T, 64><<<ctas, 256, 0, cs>>>(p, view, tokens);
+    else if (p.hd == 128)
+        rope_vec_kernel<T, 128><<<ctas, 256, 0, cs>>>(p, view, tokens);
+    else if (p.hd == 256)
+        rope_vec_kernel<T, 256><<<ctas, 256, 0, cs>>>(p, view, tokens);
+    else
+        rope_vec_kernel<T, 512><<<ctas, 256, 0, cs>>>(p, view, tokens);
+    return cuda_check(ctx, cudaGetLastError(), name);
+}
+
 }  // namespace
 
 extern "C" {
 
-size_t tf_kv_pages_workspace_bytes(uint32_t num_requests) { return (2 + 3 * (size_t)num_requests) * sizeof(int); }
+size_t tf_kv_pages_workspace_bytes(uint32_t num_requests) { return (2 + 4 * (size_t)num_requests) * sizeof(int); }
 
 tf_status tf_kv_pages_resize(tf_context* ctx, const void* seq_lens, const void* targets, uint32_t num_requests,
                              void* page_table, uint32_t max_pages, void* free_ring, uint32_t num_pages,
@@ -344,6 +602,7 @@ tf_status tf_kv_pages_resize(tf_context* ctx, const void* seq_lens, const void* 
     p.positions = static_cast<int*>(positions);
     p.requests = static_cast<int*>(requests);
     p.plan = static_cast<int*>(workspace);
+    p.starts_at = p.starts;
     p.err = ctx->d_err;
     p.B = (int)num_requests;
     p.max_pages = (int)max_pages;
@@ -351,12 +610,26 @@ tf_status tf_kv_pages_resize(tf_context* ctx, const void* seq_lens, const void* 
     p.ps = (int)page_size;
     p.base = (int)position_base;
     p.max_tokens = (int)max_tokens;
+    p.most = (int)(max_pages * page_size);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    if (max_tokens <= kSmallTokens && num_requests <= kSmallRequests) {
+        resize_small_kernel<<<1, kSmallRequests, 0, cs>>>(p);
+        return cuda_check(ctx, cudaGetLastError(), name);
+    }
     resize_plan_kernel<<<1, kResizeThreads, 0, cs>>>(p);
-    const long long work = std::max<long long>((long long)max_tokens, 32ll * num_requests);
-    const int ctas = (int)std::min<long long>((work + kFillThreads - 1) / kFillThreads, 8ll * ctx->num_sms);
-    resize_fill_kernel<<<ctas, kFillThreads, 0, cs>>>(p);
-    return cuda_check(ctx, cudaGetLastError(), name);
+    const long long work = std::max<long long>(((long long)max_tokens + 3) / 4, 32ll * num_requests);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<long long>((work + kFillThreads - 1) / kFillThreads, 8ll * ctx->num_sms));
+    cfg.blockDim = dim3(kFillThreads);
+    cfg.stream = cs;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, resize_fill_kernel, p);
+    return cuda_check(ctx, e, name);
 }
 
 tf_status tf_rope_frequencies(uint32_t rotary_dim, double theta, tf_rope_scaling scaling, double factor,
@@ -446,11 +719,8 @@ tf_status tf_rope_kv_write(tf_context* ctx, const void* q, uint64_t q_stride, co
     p.interleaved = layout == TF_ROPE_INTERLEAVED;
     p.norm = norm != 0;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    if (kv->dtype == TF_DTYPE_F16)
-        rope_kernel<__half><<<T, 128, 0, cs>>>(p, paged_view<__half>(kv));
-    else
-        rope_kernel<__nv_bfloat16><<<T, 128, 0, cs>>>(p, paged_view<__nv_bfloat16>(kv));
-    return cuda_check(ctx, cudaGetLastError(), name);
+    return kv->dtype == TF_DTYPE_F16 ? launch_rope<__half>(ctx, p, kv, cs, name)
+                                     : launch_rope<__nv_bfloat16>(ctx, p, kv, cs, name);
 }
 
 }  // extern "C"

@@ -15,24 +15,35 @@ import ctypes as C
 
 import torch
 
-from ._lib import (Context, PagedKVDesc, TFError, TF_ERR_INVALID_ARG, TF_OK, lib, ptr, status_string, stream_ptr)
+from ._lib import Context, PagedKVDesc, TFError, TF_ERR_INVALID_ARG, TF_OK, lib, status_string
 
+_I32 = torch.int32
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {None: 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4}
 
 
+def _stream(stream, device: int) -> int:
+    """The raw stream of an encode call (these calls are made once a layer: the
+    stream objects of torch would cost as much as the launch)."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
 def _heads(t, what: str) -> int:
     """Token stride of a [tokens][heads][dim] tensor whose heads lie side by side."""
+    if t.is_contiguous() and t.dim() == 3:
+        return t.shape[1] * t.shape[2]
     if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
         raise TFError(TF_ERR_INVALID_ARG, f"{what} must be [tokens][heads][dim] with contiguous heads")
     return t.stride(0)
 
 
-def _int32(**tensors):
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise TFError(TF_ERR_INVALID_ARG, f"{name} must be a contiguous int32 tensor")
+def _int32(what: str, *tensors):
+    for t in tensors:
+        if t.dtype is not _I32 or not t.is_contiguous():
+            raise TFError(TF_ERR_INVALID_ARG, f"{what}: lengths, tables, slots and positions are contiguous int32 tensors")
 
 
 class PagedKV:
@@ -57,6 +68,7 @@ class KVPages:
 
     def __init__(self, context: Context | None = None):
         self.ctx = context or Context.get(torch.cuda.current_device())
+        self.call = lib().tf_kv_pages_resize
 
     @staticmethod
     def workspace_bytes(num_requests: int) -> int:
@@ -71,20 +83,20 @@ class KVPages:
         free_state_out may be seq_lens / free_state.  free_state = {head, count,
         requests refused, tokens added}."""
         B, max_tokens = seq_lens.numel(), slots.numel()
-        _int32(seq_lens=seq_lens, targets=targets, page_table=page_table, free_ring=free_ring, free_state=free_state,
-               seq_lens_out=seq_lens_out, free_state_out=free_state_out, token_starts=token_starts, slots=slots,
-               positions=positions, requests=requests)
+        _int32("KVPages.encode_resize", seq_lens, targets, page_table, free_ring, free_state, seq_lens_out,
+               free_state_out, token_starts, slots, positions, requests)
         if (targets.numel() != B or seq_lens_out.numel() != B or token_starts.numel() != B + 1
                 or page_table.dim() != 2 or page_table.shape[0] != B or free_state.numel() != 4
                 or free_state_out.numel() != 4 or positions.numel() != max_tokens or requests.numel() != max_tokens):
             raise TFError(TF_ERR_INVALID_ARG, "KVPages.encode_resize: sizes of the tensors do not agree")
-        st = lib().tf_kv_pages_resize(
+        st = self.call(
             self.ctx.handle, seq_lens.data_ptr(), targets.data_ptr(), B, page_table.data_ptr(), page_table.shape[1],
             free_ring.data_ptr(), free_ring.numel(), free_state.data_ptr(), page_size, position_base,
             seq_lens_out.data_ptr(), free_state_out.data_ptr(), token_starts.data_ptr(), slots.data_ptr(),
             positions.data_ptr(), requests.data_ptr(), max_tokens, workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), stream_ptr(stream))
-        self.ctx.check(st, "KVPages.encode_resize")
+            workspace.nbytes, _stream(stream, self.ctx.device))
+        if st:
+            self.ctx.check(st, "KVPages.encode_resize")
 
 
 def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
@@ -109,6 +121,7 @@ class RotaryKVWrite:
 
     def __init__(self, context: Context | None = None):
         self.ctx = context or Context.get(torch.cuda.current_device())
+        self.call = lib().tf_rope_kv_write
 
     def encode(self, q, k, v, q_out, kv: PagedKV, slots, positions, inv_freq, rotary_dim: int | None = None,
                layout: str = "half", attention_factor: float = 1.0, q_weight=None, k_weight=None, norm: bool = False,
@@ -124,18 +137,20 @@ class RotaryKVWrite:
         shape = (T, kv.num_kv_heads, kv.head_dim)
         if k.shape != shape or v.shape != shape or q_out.shape != q.shape or hd != kv.head_dim:
             raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: shapes of q, k, v and the cache do not agree")
-        _int32(slots=slots, positions=positions)
+        _int32("RotaryKVWrite.encode", slots, positions)
         if slots.numel() != T or positions.numel() != T or inv_freq.dtype != torch.float64 or inv_freq.numel() * 2 != rot:
             raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: a slot and position per token, a float64 per pair")
         for w in (q_weight, k_weight):
             if w is not None and (w.dtype != torch.bfloat16 or w.numel() != hd or not w.is_contiguous()):
                 raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: norm weights are contiguous bf16 [head_dim]")
-        st = lib().tf_rope_kv_write(
+        st = self.call(
             self.ctx.handle, q.data_ptr(), _heads(q, "q"), k.data_ptr(), _heads(k, "k"), v.data_ptr(), _heads(v, "v"),
             q_out.data_ptr(), _heads(q_out, "q_out"), kv.ref, slots.data_ptr(), positions.data_ptr(),
-            inv_freq.data_ptr(), rot, _LAYOUTS[layout], attention_factor, int(norm), ptr(q_weight), ptr(k_weight), eps,
-            T, nq, stream_ptr(stream))
-        self.ctx.check(st, "RotaryKVWrite.encode")
+            inv_freq.data_ptr(), rot, _LAYOUTS[layout], attention_factor, int(norm),
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+            T, nq, _stream(stream, self.ctx.device))
+        if st:
+            self.ctx.check(st, "RotaryKVWrite.encode")
 
 
 class SharedPrefixAttention:
@@ -144,6 +159,7 @@ class SharedPrefixAttention:
 
     def __init__(self, context: Context | None = None):
         self.ctx = context or Context.get(torch.cuda.current_device())
+        self.call = lib().tf_shared_prefix_attention
 
     def workspace_bytes(self, kv: PagedKV, num_q_heads: int, tokens: int, num_requests: int, prefix_len: int,
                         max_query: int) -> int:
@@ -161,18 +177,20 @@ class SharedPrefixAttention:
         B = seq_lens.numel()
         if q.dtype != kv.dtype or out.dtype != kv.dtype or out.shape != q.shape or hd != kv.head_dim:
             raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: q, out and the cache do not agree")
-        _int32(page_table=page_table, seq_lens=seq_lens, token_starts=token_starts)
+        _int32("SharedPrefixAttention.encode", page_table, seq_lens, token_starts)
         if page_table.dim() != 2 or page_table.shape[0] != B or token_starts.numel() != B + 1:
             raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: sizes of the tensors do not agree")
         if prefix_len:
             if prefix_pages is None or prefix_pages.numel() * kv.page_size < prefix_len:
                 raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: too few prefix pages")
-            _int32(prefix_pages=prefix_pages)
+            _int32("SharedPrefixAttention.encode", prefix_pages)
         if lse is not None and (lse.dtype != torch.float32 or lse.numel() != T * nq or not lse.is_contiguous()):
             raise TFError(TF_ERR_INVALID_ARG, "SharedPrefixAttention.encode: lse must be contiguous float32 [T][heads]")
-        st = lib().tf_shared_prefix_attention(
-            self.ctx.handle, q.data_ptr(), _heads(q, "q"), kv.ref, ptr(prefix_pages), prefix_len,
-            page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), token_starts.data_ptr(), B, max_query, T,
-            nq, hd ** -0.5 if scale is None else scale, window, out.data_ptr(), _heads(out, "out"), ptr(lse),
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream_ptr(stream))
-        self.ctx.check(st, "SharedPrefixAttention.encode")
+        st = self.call(
+            self.ctx.handle, q.data_ptr(), _heads(q, "q"), kv.ref, prefix_pages.data_ptr() if prefix_len else None,
+            prefix_len, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), token_starts.data_ptr(), B,
+            max_query, T, nq, hd ** -0.5 if scale is None else scale, window, out.data_ptr(), _heads(out, "out"),
+            None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.nbytes,
+            _stream(stream, self.ctx.device))
+        if st:
+            self.ctx.check(st, "SharedPrefixAttention.encode")
