@@ -22,7 +22,7 @@ constexpr int kJoinRows = 128;  // rows a joining CTA looks at, at most
 // but a neighbour in its tile does, reaches the tile's product as 0 * inf; here
 // such a key is not read.
 template <typename T>
-__device__ void attend_alone(const AttnParams<T>& p, int b, const Request& r, int j, int h) {
+__device__ __noinline__ void attend_alone(const AttnParams<T>& p, int b, const Request& r, int j, int h) {
     constexpr int E = kMaxPagedHeadDim / 32;
     const int lane = threadIdx.x & 31, kvh = h / p.G, t = r.start + j;
     float q[E], o[E], m = -INFINITY, d = 0.f;
@@ -78,7 +78,7 @@ template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __grid_constant__ AttnParams<T> p) {
     using S = StreamShape<HD, NT>;
     extern __shared__ uint8_t raw[];
-    __shared__ int red[32], s_seg[S::kWarps], s_at[S::kWarps], s_tile, s_tile_at, s_tile_units;
+    __shared__ int red[32], s_seg[S::kWarps], s_at[S::kWarps], s_begin[S::kWarps], s_tile, s_tile_at, s_tile_units;
     __shared__ TensorBarriers bar;
     __shared__ __align__(8) uint64_t full[S::kBars];
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
@@ -108,24 +108,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     // no worker without a unit (a part is read back for every worker between a job's
     // first and last); the few there may be are spread over the CTAs
     const int few_ctas = grid - many_ctas, workers = min(few, few_ctas * S::kWarps);
-    if (cta == 0) {
-        if (threadIdx.x == 0) *p.deal = {few, workers, many, many_ctas};
-        StreamCursor c;
-        int at = few_before;
-        for (c.seg = b0; c.seg < b1; ++c.seg) {
-            stream_segment<T, HD, NT>(p, c);
-            p.few.base[c.seg] = at;
-            at += c.row_tiles * c.tiles * p.nkv;
-        }
-        if constexpr (kTensor) {
-            at = many_before;
-            for (int i = i0; i < i1; ++i) {
-                p.many.base[i] = at;
-                at += tensor_units<T, HD>(p, i) * p.nkv;
-                p.many.base[i + 1] = at;
-            }
-        }
-    }
     if (cta < many_ctas) {
         if constexpr (kTensor) {
             const int u0 = unit_begin(cta, many, many_ctas), u1 = unit_begin(cta + 1, many, many_ctas);
@@ -146,13 +128,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     }
     const int mine = cta - many_ctas;  // this CTA's workers: mine, mine + few_ctas, ...
     if (mine >= workers) return;
-    auto begin_of = [&](int w) { return unit_begin(min(mine + w * few_ctas, workers), few, workers); };
+    if (threadIdx.x < S::kWarps) s_begin[threadIdx.x] = unit_begin(min(mine + (int)threadIdx.x * few_ctas, workers), few, workers);
+    __syncthreads();
     {
         StreamCursor c;
         c.seg = -1;
         stream_segment<T, HD, NT>(p, c);
         const int prefix_units = c.row_tiles * c.tiles * p.nkv;
-        if (threadIdx.x < S::kWarps && begin_of(threadIdx.x) < prefix_units) {
+        if (threadIdx.x < S::kWarps && s_begin[threadIdx.x] < prefix_units) {
             s_seg[threadIdx.x] = -1;
             s_at[threadIdx.x] = 0;
         }
@@ -161,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
             stream_segment<T, HD, NT>(p, c);
             const int units = c.row_tiles * c.tiles * p.nkv;
             for (int w = 0; units && w < S::kWarps; ++w) {
-                const int u = begin_of(w);
+                const int u = s_begin[w];
                 if (u >= at && u < at + units) {
                     s_seg[w] = c.seg;
                     s_at[w] = at;
@@ -178,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     const int warp = threadIdx.x >> 5;
     const int worker = mine + warp * few_ctas;
     if (warp >= S::kWarps || worker >= workers) return;
-    const int u0 = unit_begin(worker, few, workers), u1 = unit_begin(worker + 1, few, workers);
+    const int u0 = s_begin[warp], u1 = unit_begin(worker + 1, few, workers);
     StreamCursor cur;
     cur.seg = s_seg[warp];
     stream_segment<T, HD, NT>(p, cur);
@@ -204,10 +187,14 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
     const int lane = threadIdx.x & 31;
     const int row0 = blockIdx.x * rows_per_cta, n_rows = min(rows_per_cta, p.T_tokens * p.nq - row0);
     griddep_wait();
-    const Deal deal = *p.deal;
     for (int i = threadIdx.x; i < n_rows; i += blockDim.x) {
         RowParts x = {};
-        const int row = row0 + i, t = row / p.nq, h = row - t * p.nq, kvh = h / p.G, in_group = h - kvh * p.G;
+        const int row = row0 + i, t = row / p.nq;
+        // (read with the rest, used where it is there)
+        const Parts& second = p.prefix_few ? p.few : p.many;  // whose places the second two parts have
+        const int own_first = p.few.first_of[row], own_last = p.few.last_of[row];
+        const int other_first = p.many.first_of[row], other_last = p.many.last_of[row];
+        const float mark = p.many.first_md[row].x;
         // most batches have one token a request, and then b = t
         int b = min(t, p.B - 1);
         if (!(p.starts[b] <= t && t < p.starts[b + 1])) b = request_at(p, t);
@@ -219,44 +206,26 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
                 atomicOr(p.err, kErrBadPage);
                 x.b = p.B;
             } else {
-                auto add_few = [&](int which, int unit, int tiles, int in_tile) {
-                    const int c0 = worker_of(unit, deal.few_units, deal.few_workers);
-                    const int c1 = worker_of(unit + tiles - 1, deal.few_units, deal.few_workers);
-                    x.n[which] = 1;
-                    x.place[which] = row;
-                    x.n[which + 1] = c1 - c0;
-                    x.place[which + 1] = (c0 + 1) * p.few.rows + in_tile;
-                };
-                const bool many = is_many(p, r);
-                const int from = own_lo(p, r), tiles = (r.len - (from & ~(kMaxRun - 1)) + 15) / 16;
-                if (r.len > from && !many) {
-                    const int own = x.j * p.G + in_group, row_tiles = (r.used * p.G + p.few.rows - 1) / p.few.rows;
-                    add_few(0, p.few.base[b] + (kvh * row_tiles + own / p.few.rows) * tiles, tiles, own % p.few.rows);
+                const bool many = is_many(p, r), prefix = p.prefix_len > p.prefix_lo;
+                int lo, hi;
+                seen_by(p, r, x.j, lo, hi);
+                if (!many && r.len > own_lo(p, r)) {
+                    const int c0 = own_first >> p.few.shift;
+                    x.n[0] = 1;
+                    x.place[0] = row;
+                    x.n[1] = own_last - c0;
+                    x.place[1] = own_first + (1 << p.few.shift);
                 }
-                const int group_row = t * p.G + in_group;
-                const int prefix_tiles = (p.prefix_len - (p.prefix_lo & ~(kMaxRun - 1)) + 15) / 16;
-                if (p.prefix_few && p.prefix_len > p.prefix_lo) {
-                    const int live = max(0, min(p.starts[p.B], p.T_tokens)) * p.G;
-                    const int row_tiles = (live + p.few.rows - 1) / p.few.rows;
-                    add_few(2, (kvh * row_tiles + group_row / p.few.rows) * prefix_tiles, prefix_tiles,
-                            group_row % p.few.rows);
-                }
-                if (deal.many_workers) {
-                    const int tile = group_row / kTcRows, units = (p.many.base[tile + 1] - p.many.base[tile]) / p.nkv;
-                    if (units) {
-                        const int unit = p.many.base[tile] + kvh * units;
-                        const int c0 = worker_of(unit, deal.many_units, deal.many_workers);
-                        const int c1 = worker_of(unit + units - 1, deal.many_units, deal.many_workers);
-                        x.n[2] = 1;
-                        x.place[2] = row;
-                        x.n[3] = c1 - c0;
-                        x.place[3] = (c0 + 1) * kTcRows + group_row % kTcRows;
-                        if (c0 == c1 && many) {  // written where it was computed, unless it was not finite
-                            const float mark = p.many.first_md[row].x;
-                            x.n[2] = 0;
-                            x.b = mark == mark ? -1 : b;
-                            x.n[0] = mark == mark ? 0 : -1;
-                        }
+                if (prefix || (many && hi > lo)) {
+                    const int c0 = other_first >> second.shift;
+                    x.n[2] = 1;
+                    x.place[2] = row;
+                    x.n[3] = other_last - c0;
+                    x.place[3] = other_first + (1 << second.shift);
+                    if (many && other_last == c0) {  // written where it was computed, unless it was not finite
+                        x.n[2] = 0;
+                        x.n[0] = mark == mark ? 0 : -1;
+                        if (mark == mark) x.b = -1;
                     }
                 }
             }
@@ -284,7 +253,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
                 const int k = part < n0 ? 0 : (part < n1 ? 1 : (part < n2 ? 2 : 3));
                 const int at = part - (k == 0 ? 0 : (k == 1 ? n0 : (k == 2 ? n1 : n2)));
                 const bool own_cont = k == 1 || (k == 3 && p.prefix_few);
-                const long long place = x.place[k] + (long long)at * (own_cont ? p.few.rows : kTcRows);
+                const long long place = x.place[k] + (long long)at * (own_cont ? 1 << p.few.shift : kTcRows);
                 src = (k == 0 ? p.few.first : (k == 2 ? p.many.first : (own_cont ? p.few.cont : p.many.cont))) + place * p.hd;
                 md = (k == 0 ? p.few.first_md : (k == 2 ? p.many.first_md : (own_cont ? p.few.cont_md : p.many.cont_md)))[place];
             }
@@ -308,7 +277,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
                 }
             }
             const int here = min(32, n - base);
-#pragma unroll 4
+#pragma unroll 8
             for (int k = 0; k < here; ++k) {
                 const float wk = __shfl_sync(0xffffffffu, w, k);
                 const float* from = reinterpret_cast<const float*>(
@@ -352,10 +321,10 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
 }
 
 // ---- sizes and the workspace ---------------------------------------------------------
-// Rows per KV head up to which a request streams its keys: a job's rows at
-// most, times two.  Beyond, the tensor cores' 128-row tile costs less than
-// streaming the keys again for every job's worth of rows.
-constexpr int kFewRows = 32;
+// Rows per KV head up to which a request streams its keys (again for every job's
+// worth of rows, but then out of L2), and up to which the whole batch does so with
+// the prefix.  Beyond, the tensor cores' 128-row tile costs less.
+constexpr int kFewRows = 64, kFewPrefixRows = 32;
 
 struct Shape {
     int hd, nt, few_rows;
@@ -372,16 +341,16 @@ Shape shape_of_call(const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t max
     s.nt = own <= 8 ? 1 : std::min(4, 512 / s.hd);
     s.few_rows = s.nt * 8;
     const bool tensor = s.hd <= 256;
-    s.prefix_few = !tensor || T * G <= kFewRows;
+    s.prefix_few = !tensor || T * G <= kFewPrefixRows;
     s.many_above = tensor ? kFewRows : 0x7FFFFFFF;
     return s;
 }
 
 struct Layout {
-    size_t first[2], first_md[2], cont[2], cont_md[2], base[2], deal, bytes;
+    size_t first[2], first_md[2], cont[2], cont_md[2], first_of[2], last_of[2], bytes;
 };
 
-Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t B, const Shape& s) {
+Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint32_t T, const Shape& s) {
     Layout l;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -389,12 +358,11 @@ Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint
         at += (bytes + 255) & ~(size_t)255;
         return here;
     };
-    const size_t rows = (size_t)T * nq, G = nq / kv->num_kv_heads;
+    const size_t rows = (size_t)T * nq;
     const size_t cont[2] = {(size_t)ctx->num_sms * (kThreads / 32) * s.few_rows, (size_t)ctx->num_sms * kTcRows};
-    const size_t bases[2] = {B, (size_t)T * G / kTcRows + 2};
-    l.deal = take(sizeof(Deal));
     for (int k = 0; k < 2; ++k) {
-        l.base[k] = take(bases[k] * sizeof(int));
+        l.first_of[k] = take(rows * sizeof(int));
+        l.last_of[k] = take(rows * sizeof(int));
         l.first_md[k] = take(rows * sizeof(float2));
         l.cont_md[k] = take(cont[k] * sizeof(float2));
         l.first[k] = take(rows * kv->head_dim * sizeof(float));
@@ -480,7 +448,7 @@ size_t tf_shared_prefix_attention_workspace_bytes(const tf_context* ctx, const t
                                                   uint32_t max_query) {
     if (!ctx || !kv || kv->num_kv_heads == 0 || num_q_heads == 0 || num_q_heads % kv->num_kv_heads) return 0;
     const Shape shape = shape_of_call(kv, num_q_heads, T, max_query);
-    return layout_of(ctx, kv, num_q_heads, T, num_requests, shape).bytes;
+    return layout_of(ctx, kv, num_q_heads, T, shape).bytes;
 }
 
 tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_stride, const tf_paged_kv* kv,
@@ -519,7 +487,7 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
     const uint64_t tiles = (uint64_t)max_pages * kv->page_size / 16 + prefix_len / 16 + 2;
     if (row_tiles * tiles * kv->num_kv_heads > 0x7FFFFFFFull)
         return fail(ctx, TF_ERR_UNSUPPORTED_SHAPE, "%s: too many keys", name);
-    const Layout l = layout_of(ctx, kv, num_q_heads, T, num_requests, shape);
+    const Layout l = layout_of(ctx, kv, num_q_heads, T, shape);
     const size_t need = l.bytes;
     if (workspace_bytes < need)
         return fail(ctx, TF_ERR_INVALID_ARG, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes, need);
@@ -569,15 +537,17 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
             parts[k]->first_md = reinterpret_cast<float2*>(w + l.first_md[k]);
             parts[k]->cont = reinterpret_cast<float*>(w + l.cont[k]);
             parts[k]->cont_md = reinterpret_cast<float2*>(w + l.cont_md[k]);
-            parts[k]->base = reinterpret_cast<int*>(w + l.base[k]);
+            parts[k]->first_of = reinterpret_cast<int*>(w + l.first_of[k]);
+            parts[k]->last_of = reinterpret_cast<int*>(w + l.last_of[k]);
         }
-        p.few.rows = shape.few_rows;
-        p.many.rows = kTcRows;
-        p.deal = reinterpret_cast<Deal*>(w + l.deal);
+        p.few.shift = 2 + (shape.nt == 1 ? 1 : (shape.nt == 2 ? 2 : 3));  // log2(8 nt)
+        p.many.shift = 7;
         p.run_shift = run == 8 ? 3 : (run == 4 ? 2 : (run == 2 ? 1 : 0));
-        p.page_shift = -1;
-        for (int i = 0; i < 31; ++i)
+        p.page_shift = p.g_shift = -1;
+        for (int i = 0; i < 31; ++i) {
             if (kv->page_size == (1u << i)) p.page_shift = i;
+            if (G == (1u << i)) p.g_shift = i;
+        }
         p.wide = wide;
         p.maps = maps;
     };

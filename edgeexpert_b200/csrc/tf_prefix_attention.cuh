@@ -22,8 +22,11 @@ struct Parts {
     float2* first_md;
     float* cont;
     float2* cont_md;
-    int* base;  // first unit of each request (few rows) or row tile (many rows)
-    int rows;   // rows a cont place holds
+    // for every row: the worker of its job's first unit and the row's place in the job (first_of =
+    // worker << shift | place), and the worker of the last: what the joining kernel adds up
+    int* first_of;
+    int* last_of;
+    int shift;  // log2 of the rows a cont place holds
 };
 
 // The pool as TMA sees it: [page][head][64-dim block][position][64 dims], 128-byte
@@ -33,11 +36,6 @@ struct Parts {
 // one block.  rows: boxes of one key and one block.
 struct KvMaps {
     CUtensorMap k, v, v_row;
-};
-
-// How the units were dealt, written by the first CTA for the joining kernel.
-struct Deal {
-    int few_units, few_workers, many_units, many_workers;
 };
 
 template <typename T>
@@ -58,12 +56,18 @@ struct AttnParams {
     int many_above;   // requests of more rows per KV head than this go to the tensor cores
     float scale;
     Parts few, many;
-    Deal* deal;
     int run_shift;   // keys of a box, as a power of two: the largest up to 8 that divides the page size
+    int g_shift;     // the query heads of a KV head as a power of two, or -1
     int page_shift;  // the page size as a power of two, or -1 (a division per unit cost 150 clocks of its latency)
     int wide;  // a box has all of a head's blocks
     KvMaps maps;
 };
+
+// Row -> token of a job's rows (token * G + head in the group).
+template <typename T>
+__device__ __forceinline__ int token_of(const AttnParams<T>& p, int row) {
+    return p.g_shift >= 0 ? row >> p.g_shift : row / p.G;
+}
 
 // A request of the batch.
 struct Request {
@@ -120,9 +124,10 @@ __device__ __forceinline__ bool is_many(const AttnParams<T>& p, const Request& r
     return r.used * p.G > p.many_above;
 }
 
-// Units [c*U/N, (c+1)*U/N) are worker c's.
-__device__ __forceinline__ int unit_begin(int c, int U, int N) { return (int)((long long)c * U / N); }
-__device__ __forceinline__ int worker_of(int u, int U, int N) { return (int)((((long long)u + 1) * N - 1) / U); }
+// Units [c*U/N, (c+1)*U/N) are worker c's.  In double: the products are below 2^53, and a
+// quotient that is no whole number is further from one than its rounding (64-bit integer
+// divisions, a dozen of them at a kernel's start, took microseconds).
+__device__ __forceinline__ int unit_begin(int c, int U, int N) { return (int)floor((double)c * U / N); }
 
 // Exclusive sum of v over the block (up to 32 warps); *total receives the sum.
 __device__ __forceinline__ int block_scan(int v, int* red, int* total) {

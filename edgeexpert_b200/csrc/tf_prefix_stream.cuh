@@ -203,7 +203,8 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
         for (int nt = 0; nt < NT; ++nt) {
             const int rq = row0 + nt * 8 + g;  // the row whose q this lane holds
             const bool ok = nt * 8 + g < job_rows;
-            const T* qr = p.q + (long long)(first_token + rq / p.G) * p.q_stride + (cur.kvh * p.G + rq % p.G) * p.hd;
+            const int tq0 = token_of(p, rq);
+            const T* qr = p.q + (long long)(first_token + tq0) * p.q_stride + (cur.kvh * p.G + rq - tq0 * p.G) * p.hd;
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
@@ -216,7 +217,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
                 const int rs = row0 + nt * 8 + 2 * tq + i;
                 int lo = 0, hi = 0;
                 if (nt * 8 + 2 * tq + i < job_rows) {
-                    const int j = rs / p.G;
+                    const int j = token_of(p, rs);
                     if (prefix) {
                         const int b = request_at(p, j);
                         if (b < p.B) {
@@ -245,6 +246,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
     // bytes of eight dims of a row.
     bool from_start = cur.tile == 0;
     auto end_job = [&]() {
+        const bool to_end = cur.tile == cur.tiles - 1;
         // a row's part of the prefix goes where the tensor cores' would be
         const Parts& to = cur.seg < 0 ? p.many : p.few;
         float* po = from_start ? to.first : p.few.cont;
@@ -254,12 +256,17 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = nt * 8 + 2 * tq + i, row = cur.rt * kRows + r;
-                const long long place = from_start ? (long long)(first_token + row / p.G) * p.nq + cur.kvh * p.G + row % p.G
-                                                   : (long long)worker * kRows + r;
+                const int tr = token_of(p, row);
+                const long long of = (long long)(first_token + tr) * p.nq + cur.kvh * p.G + row - tr * p.G;
+                const long long place = from_start ? of : (long long)worker * kRows + r;
                 float sum = d[nt][i];
                 for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 if (r >= job_rows) continue;
-                if (g == 0) pm[place] = make_float2(m[nt][i], sum);
+                if (g == 0) {
+                    pm[place] = make_float2(m[nt][i], sum);
+                    if (from_start) to.first_of[of] = worker * kRows + r;
+                    if (to_end) to.last_of[of] = worker;
+                }
                 float* dst = po + place * p.hd + g;
 #pragma unroll
                 for (int mt = 0; mt < HD / 16; ++mt) {

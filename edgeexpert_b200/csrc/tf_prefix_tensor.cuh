@@ -525,8 +525,8 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
             tc_fence_after();
             const bool whole = job.from == 0 && job.to == job.units;
             const bool final = whole && own;
-            const long long at = job.from == 0 ? (long long)t * p.nq + h
-                                               : (long long)worker * kTcRows + threadIdx.x;
+            const long long of = (long long)t * p.nq + h;
+            const long long at = job.from == 0 ? of : (long long)worker * kTcRows + threadIdx.x;
             float* po = (job.from == 0 ? p.many.first : p.many.cont) + at * p.hd;
             const float inv = d == 0.f ? 0.f : 1.f / d;
             bool fine = isfinite(d);
@@ -557,6 +557,8 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                 }
             }
             if (live) {
+                if (job.from == 0) p.many.first_of[of] = worker * kTcRows + threadIdx.x;
+                if (job.to == job.units) p.many.last_of[of] = worker;
                 if (final) {
                     if (p.lse) p.lse[at] = d == 0.f ? -INFINITY : (m + log2f(d)) * kLn2;
                     // NaN here asks the joining kernel to compute the row by itself
