@@ -106,8 +106,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
         many_ctas = min(many_ctas, many);
     }
     // no worker without a unit (a part is read back for every worker between a job's
-    // first and last); the few there may be are spread over the CTAs
-    const int few_ctas = grid - many_ctas, workers = min(few, few_ctas * S::kWarps);
+    // first and last), and two at least where there are: a part more costs the joining
+    // kernel about what a unit costs here; few workers are spread over the CTAs
+    const int few_ctas = grid - many_ctas, workers = min((few + 1) / 2, few_ctas * S::kWarps);
     if (cta < many_ctas) {
         if constexpr (kTensor) {
             const int u0 = unit_begin(cta, many, many_ctas), u1 = unit_begin(cta + 1, many, many_ctas);
@@ -181,7 +182,7 @@ struct RowParts {
 
 // Joins the parts of every row.  A thread finds the parts of a row (and rows
 // that are finished drop out), a warp adds them up.
-template <typename T>
+template <typename T, int HD>
 __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__ AttnParams<T> p, int rows_per_cta) {
     __shared__ RowParts rows[kJoinRows];
     const int lane = threadIdx.x & 31;
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
         T* out = p.out + t * p.out_stride + (long long)h * p.hd;
         const int n0 = max(0, x.n[0]), n1 = n0 + x.n[1], n2 = n1 + x.n[2], n = n2 + x.n[3];
         float top = -INFINITY, d = 0.f;
-        constexpr int E = kMaxPagedHeadDim / 128;
+        constexpr int E = HD > 128 ? HD / 128 : 1;  // 16-byte pieces of a lane
         float4 o[E];
 #pragma unroll
         for (int u = 0; u < E; ++u) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -277,22 +278,33 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
                 }
             }
             const int here = min(32, n - base);
-#pragma unroll 8
-            for (int k = 0; k < here; ++k) {
-                const float wk = __shfl_sync(0xffffffffu, w, k);
-                const float* from = reinterpret_cast<const float*>(
-                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k));
+            constexpr int kFly = 16 / E;  // parts whose loads are in flight together
+            for (int k0 = 0; k0 < here; k0 += kFly) {
+                float4 v[kFly][E];
+                float wk[kFly];
 #pragma unroll
-                for (int u = 0; u < E; ++u) {
-                    const int e = u * 128 + lane * 4;
-                    if (e < p.hd) {
-                        const float4 v = *reinterpret_cast<const float4*>(from + e);
-                        o[u].x = fmaf(v.x, wk, o[u].x);
-                        o[u].y = fmaf(v.y, wk, o[u].y);
-                        o[u].z = fmaf(v.z, wk, o[u].z);
-                        o[u].w = fmaf(v.w, wk, o[u].w);
+                for (int k = 0; k < kFly; ++k) {
+                    const int l = min(k0 + k, 31);
+                    wk[k] = __shfl_sync(0xffffffffu, w, l);
+                    const float* from = reinterpret_cast<const float*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), l));
+#pragma unroll
+                    for (int u = 0; u < E; ++u) {
+                        const int e = u * 128 + lane * 4;
+                        v[k][u] = k0 + k < here && e < p.hd ? *reinterpret_cast<const float4*>(from + e)
+                                                            : make_float4(0.f, 0.f, 0.f, 0.f);
                     }
+                    if (k0 + k >= here) wk[k] = 0.f;
                 }
+#pragma unroll
+                for (int k = 0; k < kFly; ++k)
+#pragma unroll
+                    for (int u = 0; u < E; ++u) {
+                        o[u].x = fmaf(v[k][u].x, wk[k], o[u].x);
+                        o[u].y = fmaf(v[k][u].y, wk[k], o[u].y);
+                        o[u].z = fmaf(v[k][u].z, wk[k], o[u].z);
+                        o[u].w = fmaf(v[k][u].w, wk[k], o[u].w);
+                    }
             }
         }
         const float inv = d == 0.f ? 0.f : 1.f / d;
@@ -436,7 +448,14 @@ tf_status launch(tf_context* ctx, const AttnParams<T>& p, const Shape& s, cudaSt
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_check(ctx, cudaLaunchKernelEx(&cfg, join_parts_kernel<T>, p, per), name);
+    cudaError_t e;
+    if (s.hd <= 128)
+        e = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, 128>, p, per);
+    else if (s.hd == 256)
+        e = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, 256>, p, per);
+    else
+        e = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, 512>, p, per);
+    return cuda_check(ctx, e, name);
 }
 
 }  // namespace
