@@ -268,12 +268,14 @@ __global__ void __launch_bounds__(kSmallRequests) resize_small_kernel(ResizePara
     __shared__ int plan[2 + 4 * kSmallRequests], starts[kSmallRequests + 1];
     p.plan = plan;
     p.starts_at = starts;
+    griddep_wait();
     resize_plan(p);
     __syncthreads();
     resize_fill(p, 0, 1);
 }
 __global__ void __launch_bounds__(kResizeThreads) resize_plan_kernel(ResizeParams p) {
     griddep_launch_dependents();
+    griddep_wait();
     resize_plan(p);
 }
 __global__ void __launch_bounds__(kFillThreads) resize_fill_kernel(ResizeParams p) {
@@ -364,6 +366,7 @@ __global__ void __launch_bounds__(256, 4) rope_vec_kernel(RopeParams p, PagedVie
             }
         }
     };
+    griddep_wait();
     load(0);
     for (int local = warp; local < min(tokens, p.T - t0); local += 8) {
         if (lane == 0) {
@@ -476,6 +479,7 @@ __global__ void __launch_bounds__(128) rope_kernel(RopeParams p, PagedView<T> kv
     __shared__ float2 turn[kMaxPagedHeadDim / 2];
     __shared__ float row[4][kMaxPagedHeadDim];
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    griddep_wait();
     int slot = p.slots[t];
     if (slot >= kv.num_pages * kv.page_size) {
         if (threadIdx.x == 0) atomicOr(p.err, kErrBadPage);
@@ -535,8 +539,7 @@ tf_status launch_rope(tf_context* ctx, const RopeParams& p, const tf_paged_kv* k
     const bool aligned = aligned16(p.q_weight) && aligned16(p.k_weight) && aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.q_out) &&
                          (p.T == 1 || (p.q_stride | p.k_stride | p.v_stride | p.qo_stride) % 8 == 0);
     if (!chunks || !aligned) {
-        rope_kernel<T><<<p.T, 128, 0, cs>>>(p, view);
-        return cuda_check(ctx, cudaGetLastError(), name);
+        return cuda_check(ctx, launch_overlapped(rope_kernel<T>, p.T, 128, 0, cs, p, view), name);
     }
     // sixteen items a CTA (two a warp, all loads in flight), but a CTA a token while that
     // does not fill the GPU
@@ -544,15 +547,11 @@ tf_status launch_rope(tf_context* ctx, const RopeParams& p, const tf_paged_kv* k
     const int fit = std::min(16 / std::min(passes, 16), p.rot ? kRopeTable / std::max(1, p.rot / 2) : 16);
     const int tokens = std::max(1, std::min<int>(fit, (int)(p.T / (4ll * ctx->num_sms))));
     const unsigned ctas = (unsigned)(((long long)p.T + tokens - 1) / tokens);
-    if (p.hd == 64)
-        rope_vec_kernel<T, 64><<<ctas, 256, 0, cs>>>(p, view, tokens);
-    else if (p.hd == 128)
-        rope_vec_kernel<T, 128><<<ctas, 256, 0, cs>>>(p, view, tokens);
-    else if (p.hd == 256)
-        rope_vec_kernel<T, 256><<<ctas, 256, 0, cs>>>(p, view, tokens);
-    else
-        rope_vec_kernel<T, 512><<<ctas, 256, 0, cs>>>(p, view, tokens);
-    return cuda_check(ctx, cudaGetLastError(), name);
+    auto* kernel = p.hd == 64    ? rope_vec_kernel<T, 64>
+                   : p.hd == 128 ? rope_vec_kernel<T, 128>
+                   : p.hd == 256 ? rope_vec_kernel<T, 256>
+                                 : rope_vec_kernel<T, 512>;
+    return cuda_check(ctx, launch_overlapped(kernel, ctas, 256, 0, cs, p, view, tokens), name);
 }
 
 }  // namespace
@@ -613,22 +612,12 @@ tf_status tf_kv_pages_resize(tf_context* ctx, const void* seq_lens, const void* 
     p.most = (int)(max_pages * page_size);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     if (max_tokens <= kSmallTokens && num_requests <= kSmallRequests) {
-        resize_small_kernel<<<1, kSmallRequests, 0, cs>>>(p);
-        return cuda_check(ctx, cudaGetLastError(), name);
+        return cuda_check(ctx, launch_overlapped(resize_small_kernel, 1, kSmallRequests, 0, cs, p), name);
     }
-    resize_plan_kernel<<<1, kResizeThreads, 0, cs>>>(p);
     const long long work = std::max<long long>(((long long)max_tokens + 3) / 4, 32ll * num_requests);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)std::min<long long>((work + kFillThreads - 1) / kFillThreads, 8ll * ctx->num_sms));
-    cfg.blockDim = dim3(kFillThreads);
-    cfg.stream = cs;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, resize_fill_kernel, p);
+    const unsigned ctas = (unsigned)std::min<long long>((work + kFillThreads - 1) / kFillThreads, 8ll * ctx->num_sms);
+    cudaError_t e = launch_overlapped(resize_plan_kernel, 1, kResizeThreads, 0, cs, p);
+    if (e == cudaSuccess) e = launch_overlapped(resize_fill_kernel, ctas, kFillThreads, 0, cs, p);
     return cuda_check(ctx, e, name);
 }
 

@@ -1,6 +1,8 @@
 // tf_paged.cuh -- the paged KV cache as the kernels see it (tf_paged_kv), and the
 // element types of the serving operators.
 #pragma once
+#include <type_traits>
+
 #include "tf_context.cuh"
 
 namespace tf {
@@ -58,6 +60,24 @@ inline tf_status check_paged_kv(tf_context* ctx, const tf_paged_kv* kv, const ch
         (kv->num_pages > 1 && kv->page_stride < kv->head_dim))
         return fail(ctx, TF_ERR_INVALID_ARG, "%s: cache strides below head_dim", name);
     return TF_OK;
+}
+
+// A launch whose start-up overlaps the end of what is before it in the stream (the kernels
+// wait for that before they read anything).
+template <typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Args...), unsigned ctas, unsigned threads, size_t smem, cudaStream_t cs,
+                              const std::common_type_t<Args>&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = cs;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 inline tf_status enter(tf_context* ctx, const char* name) {

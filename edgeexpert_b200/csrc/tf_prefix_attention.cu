@@ -67,24 +67,25 @@ __device__ __noinline__ void attend_alone(const AttnParams<T>& p, int b, const R
 // of work.  A streamed unit is bound by memory: 16 keys of K and V at an SM's
 // share of the bandwidth (6450 / 148 bytes a nanosecond).  A tensor unit is 64
 // (head_dim 256) or 128 keys for 128 rows: 600 ns by itself, but beside the
-// stream its loads take their turn behind the others'; measured 1400.
+// stream its loads take their turn behind the others': 1500 measured, 2000 for 128 keys of 128.
 __host__ __device__ constexpr float few_unit_ns(int hd) { return 16.f * 4.f * hd / 43.6f; }
-__host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 64 ? 1400.f : 1000.f; }
+__host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 128 ? 1500.f : (hd > 64 ? 2000.f : 800.f); }
 
 // All parts of all rows, one CTA per SM.  Every CTA sums the units of both kinds
 // over the batch and finds its share: the first CTAs take the tensor cores' jobs,
 // as many as these need to finish when the others have streamed the rest.
-template <typename T, int HD, int NT>
+// kTensor false: a batch with nothing for the tensor cores, without their 100 KB of
+// code (a small call's time is launch, instruction fetches and dependent loads).
+template <typename T, int HD, int NT, bool kTensor>
 __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __grid_constant__ AttnParams<T> p) {
     using S = StreamShape<HD, NT>;
     extern __shared__ uint8_t raw[];
     __shared__ int red[32], s_seg[S::kWarps], s_at[S::kWarps], s_begin[S::kWarps], s_tile, s_tile_at, s_tile_units;
-    __shared__ TensorBarriers bar;
     __shared__ __align__(8) uint64_t full[S::kBars];
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
     griddep_launch_dependents();
+    griddep_wait();
     const int grid = gridDim.x, cta = blockIdx.x;
-    constexpr bool kTensor = HD <= 256;
 
     // thread i looks after requests [i*per, (i+1)*per) and a share of the row tiles
     const int per = (p.B + kThreads - 1) / kThreads;
@@ -111,6 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     const int few_ctas = grid - many_ctas, workers = min((few + 1) / 2, few_ctas * S::kWarps);
     if (cta < many_ctas) {
         if constexpr (kTensor) {
+            __shared__ TensorBarriers bar;
             const int u0 = unit_begin(cta, many, many_ctas), u1 = unit_begin(cta + 1, many, many_ctas);
             int at = many_before;
             for (int i = i0; i < i1; ++i) {
@@ -340,21 +342,22 @@ constexpr int kFewRows = 64, kFewPrefixRows = 32;
 
 struct Shape {
     int hd, nt, few_rows;
-    bool prefix_few;
+    bool prefix_few, tensor;  // tensor: there may be work for the tensor cores
     int many_above;
 };
 
 // Column tiles for `rows` query rows of a job: one up to eight rows, beyond
 // that as many as a warp's registers hold (512 / head_dim).
-Shape shape_of_call(const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t max_query) {
+Shape shape_of_call(const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t prefix_len, uint32_t max_query) {
     const long long G = nq / kv->num_kv_heads, own = std::min<long long>(max_query, T) * G;
     Shape s;
     s.hd = kv->head_dim <= 64 ? 64 : (kv->head_dim <= 128 ? 128 : (kv->head_dim <= 256 ? 256 : 512));
     s.nt = own <= 8 ? 1 : std::min(4, 512 / s.hd);
     s.few_rows = s.nt * 8;
-    const bool tensor = s.hd <= 256;
-    s.prefix_few = !tensor || T * G <= kFewPrefixRows;
-    s.many_above = tensor ? kFewRows : 0x7FFFFFFF;
+    const bool can = s.hd <= 256;
+    s.prefix_few = !can || T * G <= kFewPrefixRows;
+    s.many_above = can ? kFewRows : 0x7FFFFFFF;
+    s.tensor = can && ((prefix_len && !s.prefix_few) || own > kFewRows);
     return s;
 }
 
@@ -407,54 +410,56 @@ bool pool_map(CUtensorMap* m, const tf_paged_kv* kv, const void* base, uint32_t 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, bool kTensor>
 tf_status launch_parts(tf_context* ctx, const AttnParams<T>& p, cudaStream_t cs, const char* name) {
-    constexpr int kMany = HD <= 256 ? TensorShape<HD>::kSmem : 0, kFew = StreamShape<HD, NT>::kSmem;
+    constexpr int kMany = kTensor ? TensorShape<HD>::kSmem : 0, kFew = StreamShape<HD, NT>::kSmem;
     constexpr int kSmem = kMany > kFew ? kMany : kFew;
     static bool configured[64] = {};  // per instantiation, per device
     const int dev = ctx->device & 63;
     if (!configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(attention_parts_kernel<T, HD, NT>,
+        cudaError_t e = cudaFuncSetAttribute(attention_parts_kernel<T, HD, NT, kTensor>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return cuda_check(ctx, e, name);
         configured[dev] = true;
     }
-    attention_parts_kernel<T, HD, NT><<<ctx->num_sms, kThreads, kSmem, cs>>>(p);
-    return cuda_check(ctx, cudaGetLastError(), name);
+    return cuda_check(ctx, launch_overlapped(attention_parts_kernel<T, HD, NT, kTensor>, ctx->num_sms, kThreads, kSmem, cs, p),
+                      name);
 }
 
 template <typename T>
 tf_status launch(tf_context* ctx, const AttnParams<T>& p, const Shape& s, cudaStream_t cs, const char* name) {
     tf_status st = TF_OK;
+    auto parts = [&](auto hd, auto nt) {
+        constexpr int HD = decltype(hd)::value, NT = decltype(nt)::value;
+        if constexpr (HD <= 256) {
+            if (s.tensor) return launch_parts<T, HD, NT, true>(ctx, p, cs, name);
+        }
+        return launch_parts<T, HD, NT, false>(ctx, p, cs, name);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
     if (s.hd == 64)
-        st = s.nt == 1 ? launch_parts<T, 64, 1>(ctx, p, cs, name) : launch_parts<T, 64, 4>(ctx, p, cs, name);
+        st = s.nt == 1 ? parts(integral_constant<int, 64>(), one) : parts(integral_constant<int, 64>(), four);
     else if (s.hd == 128)
-        st = s.nt == 1 ? launch_parts<T, 128, 1>(ctx, p, cs, name) : launch_parts<T, 128, 4>(ctx, p, cs, name);
+        st = s.nt == 1 ? parts(integral_constant<int, 128>(), one) : parts(integral_constant<int, 128>(), four);
     else if (s.hd == 256)
-        st = s.nt == 1 ? launch_parts<T, 256, 1>(ctx, p, cs, name) : launch_parts<T, 256, 2>(ctx, p, cs, name);
+        st = s.nt == 1 ? parts(integral_constant<int, 256>(), one) : parts(integral_constant<int, 256>(), two);
     else
-        st = launch_parts<T, 512, 1>(ctx, p, cs, name);
+        st = parts(integral_constant<int, 512>(), one);
     if (st) return st;
     // a warp per row while that fills the GPU; then more rows a CTA
     const int rows = p.T_tokens * p.nq;
     const int per = std::min(kJoinRows, std::max(8, (rows / (ctx->num_sms * 4) + 7) / 8 * 8));
-    // launched while the parts' last CTAs still run; it waits for them before it reads
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((rows + per - 1) / per));
-    cfg.blockDim = dim3(256);
-    cfg.stream = cs;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    const unsigned ctas = (unsigned)((rows + per - 1) / per);
     cudaError_t e;
     if (s.hd <= 128)
-        e = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, 128>, p, per);
+        e = launch_overlapped(join_parts_kernel<T, 128>, ctas, 256, 0, cs, p, per);
     else if (s.hd == 256)
-        e = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, 256>, p, per);
+        e = launch_overlapped(join_parts_kernel<T, 256>, ctas, 256, 0, cs, p, per);
     else
-        e = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, 512>, p, per);
+        e = launch_overlapped(join_parts_kernel<T, 512>, ctas, 256, 0, cs, p, per);
     return cuda_check(ctx, e, name);
 }
 
@@ -466,7 +471,7 @@ size_t tf_shared_prefix_attention_workspace_bytes(const tf_context* ctx, const t
                                                   uint32_t T, uint32_t num_requests, uint32_t prefix_len,
                                                   uint32_t max_query) {
     if (!ctx || !kv || kv->num_kv_heads == 0 || num_q_heads == 0 || num_q_heads % kv->num_kv_heads) return 0;
-    const Shape shape = shape_of_call(kv, num_q_heads, T, max_query);
+    const Shape shape = shape_of_call(kv, num_q_heads, T, prefix_len, max_query);
     return layout_of(ctx, kv, num_q_heads, T, shape).bytes;
 }
 
@@ -501,7 +506,7 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
         !aligned16(workspace))
         return fail(ctx, TF_ERR_MISALIGNED, "%s: q, out and workspace 16-byte aligned, strides multiples of 8", name);
     const uint64_t G = num_q_heads / kv->num_kv_heads;
-    const Shape shape = shape_of_call(kv, num_q_heads, T, max_query);
+    const Shape shape = shape_of_call(kv, num_q_heads, T, prefix_len, max_query);
     const uint64_t row_tiles = T * G / shape.few_rows + std::min<uint64_t>(T, num_requests);
     const uint64_t tiles = (uint64_t)max_pages * kv->page_size / 16 + prefix_len / 16 + 2;
     if (row_tiles * tiles * kv->num_kv_heads > 0x7FFFFFFFull)
