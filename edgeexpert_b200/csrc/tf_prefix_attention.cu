@@ -67,9 +67,9 @@ __device__ __noinline__ void attend_alone(const AttnParams<T>& p, int b, const R
 // of work.  A streamed unit is bound by memory: 16 keys of K and V at an SM's
 // share of the bandwidth (6450 / 148 bytes a nanosecond).  A tensor unit is 64
 // (head_dim 256) or 128 keys for 128 rows: 600 ns by itself, but beside the
-// stream its loads take their turn behind the others': 1500 measured, 2000 for 128 keys of 128.
+// stream its loads take their turn behind the others': 1700 measured, 2300 for 128 keys of 128.
 __host__ __device__ constexpr float few_unit_ns(int hd) { return 16.f * 4.f * hd / 43.6f; }
-__host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 128 ? 1500.f : (hd > 64 ? 2000.f : 800.f); }
+__host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 128 ? 1700.f : (hd > 64 ? 2300.f : 900.f); }
 
 // All parts of all rows, one CTA per SM.  Every CTA sums the units of both kinds
 // over the batch and finds its share: the first CTAs take the tensor cores' jobs,
@@ -102,8 +102,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     }
     int many_ctas = 0;
     if (many) {
-        const float m = many * many_unit_ns(HD), f = few * few_unit_ns(HD);
-        many_ctas = few ? max(1, min(grid - 1, __float2int_rn(grid * (m / (m + f))))) : grid;
+        const float m = many * many_unit_ns(HD);
+        float f = few * few_unit_ns(HD);
+        if (f * 10.f < m) f *= 3.f;  // a small share: its warps wait for latencies, not for bandwidth
+        many_ctas = few ? max(1, min(grid - 1, (int)(grid * (m / (m + f))))) : grid;
         many_ctas = min(many_ctas, many);
     }
     // no worker without a unit (a part is read back for every worker between a job's

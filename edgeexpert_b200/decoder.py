@@ -306,18 +306,13 @@ class Decoder:
                                             stream=stream)
         self.launches += 1
 
-    def layer(self, i: int, position: int, stream=None):
-        """One decoder layer for the T tokens at `position` (cache slot)."""
-        cfg, L, T = self.cfg, self.w.layers[i], self.T
-        if T == 0:  # no tokens here: only serve this rank's experts
-            self._moe(i, stream)
-            return
-        d, hd, nq, nkv = cfg.d, cfg.head_dim, cfg.num_q_heads, cfg.num_kv_heads
-        ctx = self.ctx
+    def _attend(self, i: int, position: int, stream):
+        """normed -> attn: projections, head norms and rotation, cache write, attention."""
+        cfg, L, T, ctx = self.cfg, self.w.layers[i], self.T, self.ctx
+        hd, nq, nkv = cfg.head_dim, cfg.num_q_heads, cfg.num_kv_heads
         seq_stride = self.cache.ctx_len * nkv * hd
         kslot = self.cache.k[i, :, position]  # [T][nkv][hd], token stride seq_stride
         vslot = self.cache.v[i, :, position]
-        RMSNorm(ctx).encode(self.h, L.input_norm, self.normed, T, d, cfg.eps, stream=stream)
         self._proj(L.q, self.normed, self.q, stream)
         # K and V land straight in this position's cache slots (token stride = one sequence)
         self._proj(L.k, self.normed, kslot, stream, y_stride=seq_stride)
@@ -326,6 +321,16 @@ class Decoder:
                                      cfg.rope_theta, hd // 2, cfg.eps, kv_stride=seq_stride, stream=stream)
         Attention(ctx).encode(self.q, self.cache.k[i], self.cache.v[i], self.attn, hd, nq, nkv, T, position + 1,
                               self.attn_ws, seq_stride=seq_stride, stream=stream)
+
+    def layer(self, i: int, position: int, stream=None):
+        """One decoder layer for the T tokens at `position` (cache slot)."""
+        cfg, L, T = self.cfg, self.w.layers[i], self.T
+        if T == 0:  # no tokens here: only serve this rank's experts
+            self._moe(i, stream)
+            return
+        d, ctx = cfg.d, self.ctx
+        RMSNorm(ctx).encode(self.h, L.input_norm, self.normed, T, d, cfg.eps, stream=stream)
+        self._attend(i, position, stream)
         self._proj(L.o, self.attn, self.o, stream)
         FusedPostAttentionSetup(ctx).encode(self.h, self.o, self.dense_x, self.routed_x, self.router_x,
                                             L.post_attn_norm, L.pre_ffn, L.pre_ffn2, T, d, cfg.eps, stream=stream)

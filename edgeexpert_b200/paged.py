@@ -4,6 +4,7 @@ lengths and share one long prefix.
 * ``KVPages.encode_resize``          request lengths -> page tables, slots, positions (on the device)
 * ``RotaryKVWrite.encode``           head norms + rotary positions; K and V into the tokens' slots
 * ``SharedPrefixAttention.encode``   attention over the shared prefix and each request's own pages
+* ``PagedKVCache``, ``PagedDecoder``  the decoder of decoder.py on such a batch, with the three operators
 
 The operators have no counterpart in the reference, which decodes one sequence
 from a contiguous cache.  Lengths, tables, slots and positions are int32 CUDA
@@ -16,6 +17,7 @@ import ctypes as C
 import torch
 
 from ._lib import Context, PagedKVDesc, TFError, TF_ERR_INVALID_ARG, TF_OK, lib, status_string
+from .decoder import Decoder
 
 _I32 = torch.int32
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
@@ -194,3 +196,105 @@ class SharedPrefixAttention:
             _stream(stream, self.ctx.device))
         if st:
             self.ctx.check(st, "SharedPrefixAttention.encode")
+
+
+class PagedKVCache:
+    """The pools of every layer, and one set of page tables for all of them: a
+    request's position has the same slot in each layer.  The page tables live on
+    the device; `resize` is the only thing that changes them."""
+
+    def __init__(self, layers: int, num_kv_heads: int, head_dim: int, num_requests: int, num_pages: int,
+                 max_pages: int, max_tokens: int, page_size: int = 16, dtype=torch.float16, device="cuda",
+                 context: Context | None = None):
+        """num_pages: of each layer's pool; max_pages: of one request; max_tokens: added in one step."""
+        def i32(*shape, fill=0):
+            return torch.full(shape, fill, dtype=_I32, device=device)
+
+        shape = (layers, num_pages, page_size, num_kv_heads, head_dim)
+        self.k, self.v = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
+        self.layer = [PagedKV(self.k[i], self.v[i]) for i in range(layers)]
+        self.page_size, self.num_requests, self.max_tokens = page_size, num_requests, max_tokens
+        self.seq_lens, self.page_table = i32(num_requests), i32(num_requests, max_pages, fill=-1)
+        self.free_ring = torch.arange(num_pages, dtype=_I32, device=device)
+        self.free_state = torch.tensor([0, num_pages, 0, 0], dtype=_I32, device=device)
+        self.token_starts = i32(num_requests + 1)
+        self.slots, self.positions, self.requests = (i32(max_tokens, fill=-1) for _ in range(3))
+        self.prefix_pages, self.prefix_len = None, 0
+        self.pages = KVPages(context)
+        self.workspace = torch.empty(KVPages.workspace_bytes(num_requests), dtype=torch.uint8, device=device)
+
+    def resize(self, targets, stream=None):
+        """Bring the requests to `targets` positions of their own (int32, on the device; -1 leaves one
+        alone, 0 frees its pages).  free_state then holds {head, free pages, requests refused, tokens added}."""
+        self.pages.encode_resize(self.seq_lens, targets, self.page_table, self.free_ring, self.free_state,
+                                 self.seq_lens, self.free_state, self.token_starts, self.slots, self.positions,
+                                 self.requests, self.page_size, self.workspace, position_base=self.prefix_len,
+                                 stream=stream)
+
+    def share(self, request: int, length: int, stream=None):
+        """Make the `length` positions that `request` holds the prefix of all requests: its pages leave
+        the tables and stay out of the free ring.  The others must be empty."""
+        if self.prefix_len:
+            raise TFError(TF_ERR_INVALID_ARG, "PagedKVCache.share: there is a prefix already")
+        if not 0 < length <= self.page_table.shape[1] * self.page_size:
+            raise TFError(TF_ERR_INVALID_ARG, "PagedKVCache.share: no such positions")
+        with torch.cuda.stream(stream) if stream is not None else torch.cuda.stream(torch.cuda.current_stream()):
+            self.prefix_pages = self.page_table[request, :-(-length // self.page_size)].clone()
+            self.seq_lens[request] = 0
+        self.prefix_len = length
+
+
+class PagedDecoder(Decoder):
+    """The decoder on a ragged batch: a step adds any number of tokens to each
+    request (a prompt, a draft, one token, none), up to T in all, and gives the
+    next token after every one of them.  Rows beyond the tokens added are padding."""
+
+    def __init__(self, weights, T: int, cache: PagedKVCache, max_query: int = 1, context: Context | None = None,
+                 device=None):
+        """max_query: the most tokens a step adds to one request."""
+        super().__init__(weights, T, _NoContiguousCache(), context, device)
+        cfg = weights.cfg
+        if cache.max_tokens != T:
+            raise TFError(TF_ERR_INVALID_ARG, "PagedDecoder: the cache must take as many tokens a step")
+        self.kv, self.max_query = cache, max_query
+        dev = self.q.device
+        self.k_rows, self.v_rows = (torch.empty(T, cfg.num_kv_heads * cfg.head_dim, dtype=torch.float16, device=dev)
+                                    for _ in range(2))
+        self.inv_freq, self.rope_factor = rope_frequencies(cfg.head_dim, cfg.rope_theta, device=dev)
+        self.rope, self.attention = RotaryKVWrite(self.ctx), SharedPrefixAttention(self.ctx)
+        self.workspace = None
+
+    def _attend(self, i: int, position, stream):
+        cfg, L, T, kv = self.cfg, self.w.layers[i], self.T, self.kv
+        hd, nq, nkv = cfg.head_dim, cfg.num_q_heads, cfg.num_kv_heads
+        self._proj(L.q, self.normed, self.q, stream)
+        self._proj(L.k, self.normed, self.k_rows, stream)
+        self._proj(L.v, self.normed, self.v_rows, stream)
+        q = self.q.view(T, nq, hd)
+        self.rope.encode(q, self.k_rows.view(T, nkv, hd), self.v_rows.view(T, nkv, hd), q, kv.layer[i], kv.slots,
+                         kv.positions, self.inv_freq, attention_factor=self.rope_factor, q_weight=L.q_norm,
+                         k_weight=L.k_norm, norm=True, eps=cfg.eps, stream=stream)
+        self.attention.encode(q, kv.layer[i], kv.page_table, kv.seq_lens, kv.token_starts, self.attn.view(T, nq, hd),
+                              self.workspace, prefix_pages=kv.prefix_pages, prefix_len=kv.prefix_len,
+                              max_query=self.max_query, scale=1.0, stream=stream)
+
+    def step(self, token_ids, targets, stream=None):
+        """token_ids [T]: the tokens added, request after request; targets: every
+        request's length with them.  Next tokens in self.tokens, row by row of the
+        tokens added; kv.free_state tells whether every request was granted its pages."""
+        kv = self.kv
+        need = self.attention.workspace_bytes(kv.layer[0], self.cfg.num_q_heads, self.T, kv.num_requests, kv.prefix_len,
+                                              self.max_query)
+        if self.workspace is None or self.workspace.nbytes < need:
+            self.workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
+        kv.resize(targets, stream)
+        self.launches = 0
+        self.embed(token_ids, stream)
+        for i in range(self.cfg.layers):
+            self.layer(i, None, stream)
+        self.lm_head(stream)
+        return self.tokens
+
+
+class _NoContiguousCache:
+    ctx_len = 1  # Decoder sizes its own attention's scratch by it

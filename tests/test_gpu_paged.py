@@ -648,3 +648,66 @@ def test_attention_refusals(cuda):
         with pytest.raises(TFError):
             Context.get(0).check_device()
     no_device_error()
+
+
+# ------------------------------------------------------------ the whole path ----
+def test_paged_decoder_agrees_with_sequences_decoded_alone(cuda):
+    """A shared system prompt prefilled once, three users' prompts prefilled
+    together behind it, then tokens one at a time (one user finishing on the
+    way), against the contiguous decoder on each whole sequence by itself.  Two
+    layers, each within 2e-3 of the formulas on either side: 8e-3 between them."""
+    import oracle as O
+    from edgeexpert_b200.decoder import Decoder, DecoderConfig, KVCache, synthetic_decoder
+    from edgeexpert_b200.paged import PagedDecoder, PagedKVCache
+    cfg = DecoderConfig(d=256, f=128, fs=128, num_experts=16, top_k=8, num_q_heads=4, num_kv_heads=2, head_dim=64,
+                        vocab=1000, layers=2, max_context=64)
+    dev = torch.device("cuda", 0)
+    gen = torch.Generator(device=dev).manual_seed(7)
+    weights = synthetic_decoder(cfg, dev, gen)
+    rng = np.random.default_rng(3)
+    prefix, users = rng.integers(0, 1000, 21), [rng.integers(0, 1000, n) for n in (6, 2, 9)]
+    first = [3, 1, 5]  # of each user's tokens, the prompt
+
+    alone = []  # the last hidden state after every position of prefix + user
+    for user in users:
+        dec = Decoder(weights, 1, KVCache(cfg, 1, dev))
+        rows = []
+        for pos, token in enumerate(np.concatenate([prefix, user])):
+            dec.step(i32([token]), pos)
+            rows.append(f64(dec.h)[0].copy())
+        alone.append(rows)
+
+    def close(row, want):
+        assert O.rel_error(row.astype(np.float32), want.astype(np.float32)) < 8e-3
+
+    cache = PagedKVCache(cfg.layers, cfg.num_kv_heads, cfg.head_dim, 3, 24, 6, 21, page_size=4)
+    dec = PagedDecoder(weights, 21, cache, max_query=21)
+    dec.step(i32(prefix), i32([21, -1, -1]))
+    assert cache.free_state.tolist()[1:] == [24 - 6, 0, 21]
+    for pos in range(21):
+        close(f64(dec.h)[pos], alone[0][pos])
+    cache.share(0, 21)
+
+    def step(added, targets):
+        ids = np.zeros(21, np.int64)
+        ids[:sum(map(len, added))] = np.concatenate(added)
+        dec.step(i32(ids), i32(targets))
+        assert cache.free_state.tolist()[2:] == [0, sum(map(len, added))]
+        return f64(dec.h)
+
+    h = step([u[:n] for u, n in zip(users, first)], first)
+    row = 0
+    for u, n in enumerate(first):
+        for j in range(n):
+            close(h[row], alone[u][21 + j])
+            row += 1
+    at = list(first)
+    for _ in range(4):
+        live = [u for u in range(3) if at[u] < len(users[u])]
+        targets = [at[u] + 1 if u in live else 0 for u in range(3)]
+        h = step([users[u][at[u]:at[u] + 1] for u in live], targets)
+        for row, u in enumerate(live):
+            close(h[row], alone[u][21 + at[u]])
+            at[u] += 1
+    assert at == [6, 2, 9]
+    no_device_error()
