@@ -484,6 +484,7 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
                                      float scale, uint32_t window, void* out, uint64_t out_stride, void* lse,
                                      void* workspace, size_t workspace_bytes, void* stream) {
     const char* name = "tf_shared_prefix_attention";
+    max_query = std::min(max_query, T);  // no request has more
     tf_status s = enter(ctx, name);
     if (s) return s;
     s = check_paged_kv(ctx, kv, name);

@@ -598,6 +598,14 @@ def test_attention_in_a_graph(cuda):
         batch.both = keep
 
 
+def test_attention_with_a_loose_bound_on_the_queries(cuda):
+    """max_query far above any request's tokens changes nothing but the kernel chosen."""
+    batch = Batch(150, [90, 40, 7], [70, 1, 3], 16, 4, 128, "bf16", 16, seed=21)
+    for bound in (70, 1000, 2 ** 31 - 1, 2 ** 32 - 1):
+        batch.check(*batch.run(max_query=bound))
+    no_device_error()
+
+
 def test_attention_far_into_a_pool(cuda):
     """Element offsets beyond 2^32 and byte offsets beyond 2^33."""
     from edgeexpert_b200.paged import PagedKV, SharedPrefixAttention
