@@ -59,8 +59,9 @@ __device__ __forceinline__ int ring_at(int head, long long x, int N) {
 
 // Exclusive sum over the block's threads; *total receives the whole sum.
 __device__ long long block_exclusive_sum(long long v, long long* red, long long* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     long long incl = v;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long u = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += u;
@@ -68,17 +69,14 @@ __device__ long long block_exclusive_sum(long long v, long long* red, long long*
     __syncthreads();  // red may still be read from the previous sum
     if (lane == 31) red[warp] = incl;
     __syncthreads();
-    if (warp == 0) {
-        long long w = lane < (int)(blockDim.x >> 5) ? red[lane] : 0;
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += u;
-        }
-        red[lane] = w;
+    long long before = 0, all = 0;
+    for (int w = 0; w < warps; ++w) {
+        const long long x = red[w];
+        before += w < warp ? x : 0;
+        all += x;
     }
-    __syncthreads();
-    *total = red[31];
-    return (warp ? red[warp - 1] : 0) + incl - v;
+    *total = all;
+    return before + incl - v;
 }
 
 struct Ask {
@@ -100,6 +98,10 @@ __device__ __forceinline__ Ask ask_of(const ResizeParams& p, int b) {
     return a;
 }
 
+// Bound by latency until there are hundreds of thousands of tokens: a decode step
+// of 32 requests takes 8 us on the GPU (three sums, a bisection, dependent loads),
+// 1000 requests 13 us, 1.02 million admitted tokens (12.7 MB written) 15 us.
+//
 // Who gets what, by three sums over the requests in order: pages asked for
 // and given back, tokens of those whose pages are there, and (to close the
 // gap after the first request without room for its tokens) the largest token
@@ -119,14 +121,14 @@ __device__ void resize_plan(const ResizeParams& p) {
     const int per = (p.B + blockDim.x - 1) / blockDim.x;
     const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
 
-    long long need = 0, back = 0, total, back_total;
+    // pages asked for (below 2^31, like the table's entries) and given back, in one sum
+    long long both = 0, total;
     for (int b = b0; b < b1; ++b) {
         const Ask a = ask_of(p, b);
-        need += a.need;
-        back += a.back;
+        both += (long long)a.need + ((long long)a.back << 32);
     }
-    const long long need0 = block_exclusive_sum(need, red, &total);
-    const long long back0 = block_exclusive_sum(back, red, &back_total);
+    const long long both0 = block_exclusive_sum(both, red, &total);
+    const long long need0 = both0 & 0xFFFFFFFFll, back0 = both0 >> 32, back_total = total >> 32;
 
     long long c = need0, added = 0;
     for (int b = b0; b < b1; ++b) {
@@ -324,8 +326,9 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
 // neighbouring chunks (two chunks side by side in a lane would touch every
 // 32-byte sector twice).  The loads of two such items are issued first; the
 // angles of the CTA's tokens are computed, once for all heads, while they are in
-// flight.  Cosines in registers instead (computed per warp) took 128 registers
-// and, at 16 warps an SM, 73 us for 8191 tokens of 32 heads of 256.
+// flight.  8191 tokens of 32 heads of 256 (268 MB): 50 us, 5.3 TB/s; 256 tokens 10
+// us, 4 of them on the GPU.  Cosines in registers instead (computed per warp) took 128 registers
+// and, at 16 warps an SM, 73 us.
 constexpr int kRopeTable = 2048;  // cosines and sines a CTA keeps
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, 4) rope_vec_kernel(RopeParams p, PagedView<T> kv, int tokens) {

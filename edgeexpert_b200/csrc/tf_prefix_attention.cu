@@ -4,7 +4,15 @@
 // For a query row at position p, with the keys split in any way into parts i:
 //   m_i = max s, d_i = sum e^(s - m_i), o_i = sum e^(s - m_i) v   over the part's visible keys,
 //   M = max m_i, D = sum d_i e^(m_i - M), out = sum o_i e^(m_i - M) / D, lse = M + log D,
-// so the shared prefix can be one part and the request's own pages another.
+// so the shared prefix can be one part and the request's own pages another: the
+// prefix is read once for the rows of the whole batch (by the tensor cores, or by
+// the streaming warps when there are few rows), own keys once each.
+//   attention_parts_kernel   all parts of all rows, one CTA per SM, two kinds of work
+//   join_parts_kernel        M, D, out and lse of every row that has more than one part
+// Measured with both (16 query / 8 KV heads of 256): 256 requests behind 4096
+// shared positions with 1 to 1001 of their own, 1.09 GB: 212 us, 5.1 TB/s; 32
+// behind 2048 with up to 2048, 286 MB: 70 us; 2 behind 317: 18 us (17 on the GPU:
+// launch, sums over the batch, one unit, join).
 #include <math.h>
 
 #include "tf_prefix_stream.cuh"

@@ -15,6 +15,13 @@
 //     64 registers.  P^T comes from S^T by transposing 8x8 tiles in registers.
 // The tensor cores run at a few percent here; tcgen05's 64-row tiles would be
 // nearly empty.
+// Measured (16 query / 8 KV heads of 256, fp16): 256 requests of 500 keys on
+// average, no prefix, 1.05 GB: 207 us with the join, 5.1 TB/s; the warps end
+// between 137 and 208 us, 175 on average (the SMs do not get equal shares of the
+// memory).  Shares taken from a counter for the last 40 % instead: 183 us, but 2
+// to 11 us more for smaller batches (the counter's reset, restarts of the rings).
+// Four warps a CTA on the keys of one job, joined in shared memory: 71 us instead
+// of 55 us for 32 requests of 1024 keys (every join stopped all four).
 #pragma once
 #include "tf_prefix_attention.cuh"
 

@@ -16,6 +16,14 @@
 // Roles: warps 0-3 a row per thread (softmax, Q in, O out), warp 4 issues the
 // MMAs, warps 5 and 6 fetch K and V by page into rings of 128-byte-swizzled tiles.
 // Scores of tile i+1 are computed while the softmax of tile i runs.
+// Bound: MMAs alone take 1030 clocks a unit of 64 keys of 256 (measured, S and O
+// interleaved); with all SMs at work a unit takes 1600, because K and V tiles
+// arrive at 40 bytes a clock and SM, 10.6 TB/s over all SMs, from L2.  24 prompts
+// of 1 to 300 tokens behind 2050 shared positions (16/8 heads of 256): 230 us
+// with the join, 560 TFLOP/s.  Pairs of CTAs (cta_group::2) halve those bytes,
+// but the second CTA's weights have to be reported to the first every unit: 257
+// us at best.  Beside the stream a unit takes about 1.7 us, waiting for loads
+// behind the stream's; bringing tiles into L2 ten units ahead made it 1.9.
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
 // one its sums refer to: weights stay below 256, sums in fp32, and the quotient
 // at the end does not depend on the reference.
@@ -369,6 +377,10 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                     ok = wait(&bar.full[1][v.slot], v.phase) && (!more || wait(&bar.full[0][k.slot], k.phase));
                     if (!ok) break;
                     tc_fence_after();
+                    // S of unit x + 1 lies over P of unit x - 1: its product is over before that is overwritten
+                    // (queued MMAs run in order, but only for one accumulator is that promised; 0.5 % slower)
+                    if (more && x > 0) ok = wait(&bar.o_done[p_buf ^ 1], p_phase ^ p_buf ^ 1);
+                    if (!ok) break;
                     if (more) scores();
                     ok = wait(&bar.p_full[p_buf], p_phase);
                     if (!ok) break;

@@ -132,19 +132,21 @@ class RotaryKVWrite:
         projection are fine); q_out may be q."""
         T, nq, hd = q.shape
         rot = hd if rotary_dim is None else rotary_dim
+        dtype = kv.dtype
         if layout not in _LAYOUTS:
             raise TFError(TF_ERR_INVALID_ARG, f"RotaryKVWrite.encode: unknown layout {layout!r}")
-        if not (q.dtype == k.dtype == v.dtype == q_out.dtype == kv.dtype):
+        if q.dtype is not dtype or k.dtype is not dtype or v.dtype is not dtype or q_out.dtype is not dtype:
             raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: q, k, v, q_out and the cache must have one dtype")
-        shape = (T, kv.num_kv_heads, kv.head_dim)
-        if k.shape != shape or v.shape != shape or q_out.shape != q.shape or hd != kv.head_dim:
+        shape = k.shape
+        if shape != v.shape or shape != (T, kv.num_kv_heads, kv.head_dim) or q_out.shape != q.shape or hd != kv.head_dim:
             raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: shapes of q, k, v and the cache do not agree")
         _int32("RotaryKVWrite.encode", slots, positions)
-        if slots.numel() != T or positions.numel() != T or inv_freq.dtype != torch.float64 or inv_freq.numel() * 2 != rot:
+        if slots.numel() != T or positions.numel() != T or inv_freq.dtype is not torch.float64 or inv_freq.numel() * 2 != rot:
             raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: a slot and position per token, a float64 per pair")
-        for w in (q_weight, k_weight):
-            if w is not None and (w.dtype != torch.bfloat16 or w.numel() != hd or not w.is_contiguous()):
-                raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: norm weights are contiguous bf16 [head_dim]")
+        if q_weight is not None or k_weight is not None:
+            for w in (q_weight, k_weight):
+                if w is not None and (w.dtype is not torch.bfloat16 or w.numel() != hd or not w.is_contiguous()):
+                    raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: norm weights are contiguous bf16 [head_dim]")
         st = self.call(
             self.ctx.handle, q.data_ptr(), _heads(q, "q"), k.data_ptr(), _heads(k, "k"), v.data_ptr(), _heads(v, "v"),
             q_out.data_ptr(), _heads(q_out, "q_out"), kv.ref, slots.data_ptr(), positions.data_ptr(),
