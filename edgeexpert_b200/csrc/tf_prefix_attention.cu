@@ -98,15 +98,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     // thread i looks after requests [i*per, (i+1)*per) and a share of the row tiles
     const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
-    int few_before, many_before = 0, many = 0, i0 = 0, i1 = 0;
+    int few_before, many_before = 0, many = 0, i0 = 0, i1 = 0, per_row_tile = 0;
     const int few = stream_units<T, HD, NT>(p, red, b0, b1, few_before);
     if constexpr (kTensor) {
-        const bool any = !p.prefix_few && (p.prefix_len || p.max_query * p.G > p.many_above);
-        const int row_tiles = any ? (int)(((long long)p.T_tokens * p.G + kTcRows - 1) / kTcRows) : 0;
-        const int per_tile = (row_tiles + kThreads - 1) / kThreads;
-        i0 = min(row_tiles, (int)threadIdx.x * per_tile);
-        i1 = min(row_tiles, i0 + per_tile);
-        if (any) many = all_tensor_units<T, HD>(p, red, i0, i1, many_before);
+        const bool own = p.max_query * p.G > p.many_above;  // requests may have own keys here
+        if (!own && !p.prefix_few) {
+            // the prefix alone: the same for every row tile with a token of the batch
+            const int live = (int)(((long long)max(0, min(p.starts[p.B], p.T_tokens)) * p.G + kTcRows - 1) / kTcRows);
+            per_row_tile = tensor_units<T, HD>(p, 0) * p.nkv;
+            many = live * per_row_tile;
+        } else if (own) {
+            const int row_tiles = (int)(((long long)p.T_tokens * p.G + kTcRows - 1) / kTcRows);
+            const int per_tile = (row_tiles + kThreads - 1) / kThreads;
+            i0 = min(row_tiles, (int)threadIdx.x * per_tile);
+            i1 = min(row_tiles, i0 + per_tile);
+            many = all_tensor_units<T, HD>(p, red, i0, i1, many_before);
+        }
     }
     int many_ctas = 0;
     if (many) {
@@ -124,15 +131,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
         if constexpr (kTensor) {
             __shared__ TensorBarriers bar;
             const int u0 = unit_begin(cta, many, many_ctas), u1 = unit_begin(cta + 1, many, many_ctas);
-            int at = many_before;
-            for (int i = i0; i < i1; ++i) {
-                const int units = tensor_units<T, HD>(p, i);
-                if (u0 >= at && u0 < at + units * p.nkv) {
-                    s_tile = i;
-                    s_tile_at = at;
-                    s_tile_units = units;
+            if (per_row_tile) {
+                if (threadIdx.x == 0) {
+                    s_tile = u0 / per_row_tile;
+                    s_tile_at = u0 / per_row_tile * per_row_tile;
+                    s_tile_units = per_row_tile / p.nkv;
                 }
-                at += units * p.nkv;
+            } else {
+                int at = many_before;
+                for (int i = i0; i < i1; ++i) {
+                    const int units = tensor_units<T, HD>(p, i);
+                    if (u0 >= at && u0 < at + units * p.nkv) {
+                        s_tile = i;
+                        s_tile_at = at;
+                        s_tile_units = units;
+                    }
+                    at += units * p.nkv;
+                }
             }
             __syncthreads();
             tensor_cta<T, HD>(p, smem, bar, u0, u1, s_tile, s_tile_at, s_tile_units, cta);
