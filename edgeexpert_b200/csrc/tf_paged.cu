@@ -69,14 +69,18 @@ __device__ long long block_exclusive_sum(long long v, long long* red, long long*
     __syncthreads();  // red may still be read from the previous sum
     if (lane == 31) red[warp] = incl;
     __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < warps; ++w) {
-        const long long x = red[w];
-        before += w < warp ? x : 0;
-        all += x;
+    if (warp == 0) {
+        long long w = lane < warps ? red[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += u;
+        }
+        red[lane] = w;
     }
-    *total = all;
-    return before + incl - v;
+    __syncthreads();
+    *total = red[31];
+    return (warp ? red[warp - 1] : 0) + incl - v;
 }
 
 struct Ask {
