@@ -204,20 +204,31 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
 // cores') first and cont; cont places are a worker's rows apart.
 struct RowParts {
     int n[4], place[4];
-    int b, j;  // request and token in it; b < 0: nothing to do, b = the batch's size: a row of zeros
+    int row;
+    int b, j;  // request and token in it; b = the batch's size: a row of zeros
 };
 
-// Joins the parts of every row.  A thread finds the parts of a row (and rows
-// that are finished drop out), a warp adds them up.
+// Joins the parts of every row.  A thread finds the parts of a row (rows that
+// are finished drop out; the others in any order), a warp adds them up.  Bound by
+// latency: two rounds of dependent loads to find a row's parts, then two for each
+// row of a warp.  So as many CTAs as fit: 3 an SM with 32 registers of loads in
+// flight (58,000 rows of which a third have two parts, with the parts kernel: 205
+// us; 218 with 2 an SM and twice the loads; 229 without dropping finished rows
+// before the warps take theirs).
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__ AttnParams<T> p, int rows_per_cta) {
+__global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constant__ AttnParams<T> p, int rows_per_cta) {
     __shared__ RowParts rows[kJoinRows];
+    __shared__ int left;
     const int lane = threadIdx.x & 31;
     const int row0 = blockIdx.x * rows_per_cta, n_rows = min(rows_per_cta, p.T_tokens * p.nq - row0);
+    if (threadIdx.x == 0) left = 0;
+    __syncthreads();
     griddep_wait();
     for (int i = threadIdx.x; i < n_rows; i += blockDim.x) {
         RowParts x = {};
         const int row = row0 + i, t = row / p.nq;
+        bool done = false;
+        x.row = row;
         // (read with the rest, used where it is there)
         const Parts& second = p.prefix_few ? p.few : p.many;  // whose places the second two parts have
         const int own_first = p.few.first_of[row], own_last = p.few.last_of[row];
@@ -253,18 +264,17 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
                     if (many && other_last == c0) {  // written where it was computed, unless it was not finite
                         x.n[2] = 0;
                         x.n[0] = mark == mark ? 0 : -1;
-                        if (mark == mark) x.b = -1;
+                        done = mark == mark;
                     }
                 }
             }
         }
-        rows[i] = x;
+        if (!done) rows[atomicAdd(&left, 1)] = x;
     }
     __syncthreads();
-    for (int i = threadIdx.x >> 5; i < n_rows; i += blockDim.x >> 5) {
+    for (int i = threadIdx.x >> 5; i < left; i += blockDim.x >> 5) {
         const RowParts& x = rows[i];
-        if (x.b < 0) continue;
-        const int row = row0 + i, t = row / p.nq, h = row - t * p.nq;
+        const int row = x.row, t = row / p.nq, h = row - t * p.nq;
         T* out = p.out + t * p.out_stride + (long long)h * p.hd;
         const int n0 = max(0, x.n[0]), n1 = n0 + x.n[1], n2 = n1 + x.n[2], n = n2 + x.n[3];
         float top = -INFINITY, d = 0.f;
@@ -305,7 +315,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__
                 }
             }
             const int here = min(32, n - base);
-            constexpr int kFly = 16 / E;  // parts whose loads are in flight together
+            constexpr int kFly = 8 / E;  // parts whose loads are in flight together
             for (int k0 = 0; k0 < here; k0 += kFly) {
                 float4 v[kFly][E];
                 float wk[kFly];
@@ -474,9 +484,9 @@ tf_status launch(tf_context* ctx, const AttnParams<T>& p, const Shape& s, cudaSt
     else
         st = parts(integral_constant<int, 512>(), one);
     if (st) return st;
-    // a warp per row while that fills the GPU; then more rows a CTA
+    // a warp per row while that fills the GPU; then more rows a CTA, in four rounds of CTAs
     const int rows = p.T_tokens * p.nq;
-    const int per = std::min(kJoinRows, std::max(8, (rows / (ctx->num_sms * 4) + 7) / 8 * 8));
+    const int per = std::min(kJoinRows, std::max(8, (rows / (ctx->num_sms * 12) + 7) / 8 * 8));
     const unsigned ctas = (unsigned)((rows + per - 1) / per);
     cudaError_t e;
     if (s.hd <= 128)
