@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     __shared__ int red[32], s_seg[S::kWarps], s_at[S::kWarps], s_begin[S::kWarps], s_tile, s_tile_at, s_tile_units;
     __shared__ __align__(8) uint64_t full[S::kBars];
     const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();  // the joining kernel may read what this one may
     const int grid = gridDim.x, cta = blockIdx.x;
 
     // thread i looks after requests [i*per, (i+1)*per) and a share of the row tiles
@@ -223,49 +223,59 @@ __global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constan
     const int row0 = blockIdx.x * rows_per_cta, n_rows = min(rows_per_cta, p.T_tokens * p.nq - row0);
     if (threadIdx.x == 0) left = 0;
     __syncthreads();
+    const int row = row0 + threadIdx.x;
+    const bool mine = threadIdx.x < n_rows;  // (a thread for each: kJoinRows <= threads)
+    static_assert(kJoinRows <= 256);
+    RowParts x = {};
+    Request r = {};
+    bool many = false, own = false, other = false;
+    x.b = p.B;
+    if (mine) {
+        // what the caller wrote is complete: the parts kernel lets this one start after its own wait
+        const int t = row / p.nq;
+        // most batches have one token a request, and then b = t
+        x.b = min(t, p.B - 1);
+        if (!(p.starts[x.b] <= t && t < p.starts[x.b + 1])) x.b = request_at(p, t);
+        if (x.b < p.B) {
+            r = request_of(p, x.b);
+            x.j = t - r.start;
+            int lo, hi;
+            seen_by(p, r, x.j, lo, hi);
+            many = is_many(p, r);
+            own = !many && r.len > own_lo(p, r);
+            other = p.prefix_len > p.prefix_lo || (many && hi > lo);
+        }
+    }
     griddep_wait();
-    for (int i = threadIdx.x; i < n_rows; i += blockDim.x) {
-        RowParts x = {};
-        const int row = row0 + i, t = row / p.nq;
+    if (mine) {
         bool done = false;
         x.row = row;
-        // (read with the rest, used where it is there)
+        // (read together, used where it is there)
         const Parts& second = p.prefix_few ? p.few : p.many;  // whose places the second two parts have
         const int own_first = p.few.first_of[row], own_last = p.few.last_of[row];
         const int other_first = p.many.first_of[row], other_last = p.many.last_of[row];
         const float mark = p.many.first_md[row].x;
-        // most batches have one token a request, and then b = t
-        int b = min(t, p.B - 1);
-        if (!(p.starts[b] <= t && t < p.starts[b + 1])) b = request_at(p, t);
-        x.b = b;
-        if (b < p.B) {
-            const Request r = request_of(p, b);
-            x.j = t - r.start;
-            if (x.j >= r.used) {
-                atomicOr(p.err, kErrBadPage);
-                x.b = p.B;
-            } else {
-                const bool many = is_many(p, r), prefix = p.prefix_len > p.prefix_lo;
-                int lo, hi;
-                seen_by(p, r, x.j, lo, hi);
-                if (!many && r.len > own_lo(p, r)) {
-                    const int c0 = own_first >> p.few.shift;
-                    x.n[0] = 1;
-                    x.place[0] = row;
-                    x.n[1] = own_last - c0;
-                    x.place[1] = own_first + (1 << p.few.shift);
-                }
-                if (prefix || (many && hi > lo)) {
-                    const int c0 = other_first >> second.shift;
-                    x.n[2] = 1;
-                    x.place[2] = row;
-                    x.n[3] = other_last - c0;
-                    x.place[3] = other_first + (1 << second.shift);
-                    if (many && other_last == c0) {  // written where it was computed, unless it was not finite
-                        x.n[2] = 0;
-                        x.n[0] = mark == mark ? 0 : -1;
-                        done = mark == mark;
-                    }
+        if (x.b < p.B && x.j >= r.used) {
+            atomicOr(p.err, kErrBadPage);
+            x.b = p.B;
+        } else if (x.b < p.B) {
+            if (own) {
+                const int c0 = own_first >> p.few.shift;
+                x.n[0] = 1;
+                x.place[0] = row;
+                x.n[1] = own_last - c0;
+                x.place[1] = own_first + (1 << p.few.shift);
+            }
+            if (other) {
+                const int c0 = other_first >> second.shift;
+                x.n[2] = 1;
+                x.place[2] = row;
+                x.n[3] = other_last - c0;
+                x.place[3] = other_first + (1 << second.shift);
+                if (many && other_last == c0) {  // written where it was computed, unless it was not finite
+                    x.n[2] = 0;
+                    x.n[0] = mark == mark ? 0 : -1;
+                    done = mark == mark;
                 }
             }
         }
