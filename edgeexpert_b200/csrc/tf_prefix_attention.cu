@@ -10,8 +10,8 @@
 //   attention_parts_kernel   all parts of all rows, one CTA per SM, two kinds of work
 //   join_parts_kernel        M, D, out and lse of every row that has more than one part
 // Measured with both (16 query / 8 KV heads of 256): 256 requests behind 4096
-// shared positions with 1 to 1001 of their own, 1.09 GB: 212 us, 5.1 TB/s; 32
-// behind 2048 with up to 2048, 286 MB: 70 us; 2 behind 317: 18 us (17 on the GPU:
+// shared positions with 1 to 1001 of their own, 1.09 GB: 213 us, 5.1 TB/s; 32
+// behind 2048 with up to 2048, 286 MB: 69 us; 2 behind 317: 18 us (17 on the GPU:
 // launch, sums over the batch, one unit, join).
 #include <math.h>
 

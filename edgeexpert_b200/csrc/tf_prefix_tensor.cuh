@@ -17,13 +17,15 @@
 // MMAs, warps 5 and 6 fetch K and V by page into rings of 128-byte-swizzled tiles.
 // Scores of tile i+1 are computed while the softmax of tile i runs.
 // Bound: MMAs alone take 1030 clocks a unit of 64 keys of 256 (measured, S and O
-// interleaved); with all SMs at work a unit takes 1600, because K and V tiles
-// arrive at 40 bytes a clock and SM, 10.6 TB/s over all SMs, from L2.  24 prompts
-// of 1 to 300 tokens behind 2050 shared positions (16/8 heads of 256): 230 us
-// with the join, 560 TFLOP/s.  Pairs of CTAs (cta_group::2) halve those bytes,
-// but the second CTA's weights have to be reported to the first every unit: 257
-// us at best.  Beside the stream a unit takes about 1.7 us, waiting for loads
-// behind the stream's; bringing tiles into L2 ten units ahead made it 1.9.
+// interleaved); with all SMs at work a unit takes 1600 inside a job, because K and
+// V tiles arrive at 40 bytes a clock and SM, 10.6 TB/s over all SMs, from L2.  24
+// prompts of 1 to 300 tokens behind 2050 shared positions (16/8 heads of 256): 217
+// us with the join, 595 TFLOP/s; 116 units a CTA from 9 us on, ending at 151 to
+// 178 us, 1.33 us a unit with the changes of job (Q in, pipeline drained, O out).
+// Pairs of CTAs (cta_group::2) halve the bytes, but the second CTA's weights have
+// to be reported to the first every unit: 257 us at best, against 231 then.
+// Beside the stream a unit takes about 1.7 us, waiting for loads behind the
+// stream's; bringing tiles into L2 ten units ahead made it 1.9.
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
 // one its sums refer to: weights stay below 256, sums in fp32, and the quotient
 // at the end does not depend on the reference.
