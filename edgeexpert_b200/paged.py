@@ -265,6 +265,7 @@ class PagedDecoder(Decoder):
         self.inv_freq, self.rope_factor = rope_frequencies(cfg.head_dim, cfg.rope_theta, device=dev)
         self.rope, self.attention = RotaryKVWrite(self.ctx), SharedPrefixAttention(self.ctx)
         self.workspace = None
+        self.ids = torch.zeros(T, dtype=_I32, device=dev)  # the tokens of a step's rows
 
     def _attend(self, i: int, position, stream):
         cfg, L, T, kv = self.cfg, self.w.layers[i], self.T, self.kv
@@ -280,18 +281,34 @@ class PagedDecoder(Decoder):
                               self.workspace, prefix_pages=kv.prefix_pages, prefix_len=kv.prefix_len,
                               max_query=self.max_query, scale=1.0, stream=stream)
 
+    def _resize(self, token_ids, targets, stream):
+        """The page tables brought to `targets`, and self.ids = the tokens of the requests that
+        were granted.  The list holds the tokens of all that asked, the rows those of the granted
+        ones alone; a request whose tokens the list does not hold to the end is refused."""
+        kv, n = self.kv, token_ids.numel()
+        before = kv.seq_lens.clone()
+        asked = (targets - before).clamp_(min=0)
+        ends = asked.cumsum(0)  # of the requests' tokens in the list
+        kv.resize(torch.where((ends > n) & (asked > 0), 2 ** 31 - 1, targets), stream)
+        first = ends - asked - before - kv.prefix_len  # + a token's position = its place in the list
+        at = (first[kv.requests.clamp(min=0)] + kv.positions).clamp_(0, n - 1)
+        torch.mul(token_ids[at], kv.requests >= 0, out=self.ids)
+
     def step(self, token_ids, targets, stream=None):
-        """token_ids [T]: the tokens added, request after request; targets: every
-        request's length with them.  Next tokens in self.tokens, row by row of the
-        tokens added; kv.free_state tells whether every request was granted its pages."""
+        """token_ids [T]: the tokens to add, request after request, of every request that is to
+        grow; targets: every request's length with them.  A request that can't have its pages
+        is refused and keeps its length; the others are as if it had not asked.  Next tokens in
+        self.tokens, row by row of the tokens added: row i is position kv.positions[i] of request
+        kv.requests[i], and kv.free_state tells how many requests were refused."""
         kv = self.kv
         need = self.attention.workspace_bytes(kv.layer[0], self.cfg.num_q_heads, self.T, kv.num_requests, kv.prefix_len,
                                               self.max_query)
         if self.workspace is None or self.workspace.nbytes < need:
             self.workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
-        kv.resize(targets, stream)
+        with torch.cuda.stream(stream):  # (None: the current one)
+            self._resize(token_ids, targets, stream)
         self.launches = 0
-        self.embed(token_ids, stream)
+        self.embed(self.ids, stream)
         for i in range(self.cfg.layers):
             self.layer(i, None, stream)
         self.lm_head(stream)

@@ -1,0 +1,106 @@
+"""GPU tests of PagedDecoder where requests are refused, lists are short and
+batches are small, against the contiguous decoder on each sequence by itself.
+
+Two layers, each within 2e-3 of the formulas on either side: 8e-3 between
+them, as for the whole path in test_gpu_paged.py."""
+import numpy as np
+import pytest
+import torch
+
+import oracle as O
+from test_gpu_paged import f64, i32, no_device_error
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def model():
+    """(weights, last hidden states of a sequence by position)."""
+    from edgeexpert_b200.decoder import Decoder, DecoderConfig, KVCache, synthetic_decoder
+    cfg = DecoderConfig(d=256, f=128, fs=128, num_experts=16, top_k=8, num_q_heads=4, num_kv_heads=2, head_dim=64,
+                        vocab=1000, layers=2, max_context=64)
+    dev = torch.device("cuda", 0)
+    weights = synthetic_decoder(cfg, dev, torch.Generator(device=dev).manual_seed(7))
+
+    def alone(tokens):
+        dec = Decoder(weights, 1, KVCache(cfg, 1, dev))
+        rows = []
+        for pos, token in enumerate(tokens):
+            dec.step(i32([token]), pos)
+            rows.append(f64(dec.h)[0].copy())
+        return rows
+
+    return weights, alone
+
+
+def paged(weights, requests, pages, max_pages, T, page_size, max_query):
+    from edgeexpert_b200.paged import PagedDecoder, PagedKVCache
+    cfg = weights.cfg
+    cache = PagedKVCache(cfg.layers, cfg.num_kv_heads, cfg.head_dim, requests, pages, max_pages, T, page_size=page_size)
+    return PagedDecoder(weights, T, cache, max_query=max_query), cache
+
+
+def close(row, want):
+    assert O.rel_error(row.astype(np.float32), want.astype(np.float32)) < 8e-3
+
+
+def padded(tokens, T):
+    ids = np.zeros(T, np.int64)
+    ids[:len(tokens)] = tokens
+    return i32(ids)
+
+
+class Users:
+    """Users whose tokens are offered until they are granted."""
+
+    def __init__(self, model, sizes, T, **kw):
+        rng = np.random.default_rng(sum(sizes))
+        self.weights, alone = model
+        self.tokens = [rng.integers(1, 1000, n) for n in sizes]
+        self.want = [alone(t) for t in self.tokens]
+        self.at, self.T = [0] * len(sizes), T
+        self.dec, self.cache = paged(self.weights, len(sizes), T=T, **kw)
+
+    def offer(self, targets, granted):
+        """A step to `targets`, of which exactly the requests in `granted` come about; the list
+        holds the tokens of every request that grows, as far as it goes."""
+        ids = np.concatenate([t[o:max(o, n)] for t, o, n in zip(self.tokens, self.at, targets)] + [np.zeros(0, np.int64)])
+        self.dec.step(padded(ids[:self.T], self.T), i32(targets))
+        grown = [(b, j) for b in granted for j in range(self.at[b], targets[b])]
+        asked = sum(n > o for o, n in zip(self.at, targets))
+        assert self.cache.free_state.tolist()[2:] == [asked - len(granted), len(grown)]
+        for b, n in enumerate(targets):
+            if b in granted or 0 <= n < self.at[b]:
+                self.at[b] = n
+        assert self.cache.seq_lens.tolist() == self.at
+        h = f64(self.dec.h)
+        for row, (b, j) in enumerate(grown):
+            close(h[row], self.want[b][j])
+        no_device_error()
+
+
+def test_a_refused_request_leaves_the_others_their_tokens(cuda, model):
+    """No page for a request in the middle and for the last one: those granted behind the first
+    get their own tokens, and the refused ones later."""
+    u = Users(model, [6, 6, 6, 3], T=12, pages=4, max_pages=3, page_size=4, max_query=4)
+    u.offer([4, 4, 3, 0], [0, 1, 2])
+    u.offer([5, 5, 4, 2], [0, 2])    # one free page: the first takes it, the third needs none
+    u.offer([6, 5, 5, 2], [0])
+    u.offer([0, 5, 5, 2], [])        # the first is finished; its pages can be taken from the next step on
+    u.offer([-1, 5, 5, 2], [1, 2])
+    u.offer([-1, 6, 6, -1], [1, 2])
+
+
+def test_a_request_longer_than_its_table_is_refused_alone(cuda, model):
+    u = Users(model, [3, 13, 4], T=16, pages=16, max_pages=3, page_size=4, max_query=13)
+    u.offer([2, 13, 1], [0, 2])      # 13 positions are more than three pages hold; its tokens are in the list
+    u.offer([3, 12, 1], [0, 1])
+
+
+def test_tokens_that_the_list_does_not_hold_are_not_added(cuda, model):
+    """The list ends at T tokens: a request whose tokens lie behind is refused, also where the
+    tokens before it are refused too and its own would fit."""
+    u = Users(model, [12, 6, 4], T=12, pages=2, max_pages=2, page_size=8, max_query=12)
+    u.offer([0, 1, 0], [1])
+    u.offer([10, 6, 2], [])          # no two pages for the first; the second's five are at 10..14 of the list
+    u.offer([7, 6, 2], [0, 1])       # the third's are at 12 and 13
