@@ -291,21 +291,29 @@ class PagedDecoder(Decoder):
         ends = asked.cumsum(0)  # of the requests' tokens in the list
         kv.resize(torch.where((ends > n) & (asked > 0), 2 ** 31 - 1, targets), stream)
         first = ends - asked - before - kv.prefix_len  # + a token's position = its place in the list
+        if n == 0:
+            self.ids.zero_()
+            return
         at = (first[kv.requests.clamp(min=0)] + kv.positions).clamp_(0, n - 1)
         torch.mul(token_ids[at], kv.requests >= 0, out=self.ids)
 
     def step(self, token_ids, targets, stream=None):
-        """token_ids [T]: the tokens to add, request after request, of every request that is to
-        grow; targets: every request's length with them.  A request that can't have its pages
+        """token_ids (up to T): the tokens to add, request after request, of every request that
+        is to grow; targets: every request's length with them.  Both int32, on the device.  A request that can't have its pages
         is refused and keeps its length; the others are as if it had not asked.  Next tokens in
         self.tokens, row by row of the tokens added: row i is position kv.positions[i] of request
         kv.requests[i], and kv.free_state tells how many requests were refused."""
         kv = self.kv
+        for t, what in ((token_ids, "token_ids"), (targets, "targets")):
+            if t.dtype is not _I32 or t.dim() != 1 or t.device != self.ids.device:
+                raise TFError(TF_ERR_INVALID_ARG, f"PagedDecoder.step: {what} must be a vector of int32 on {self.ids.device}")
+        if token_ids.numel() > self.T or targets.numel() != kv.num_requests:
+            raise TFError(TF_ERR_INVALID_ARG, "PagedDecoder.step: up to T tokens, a target per request")
         need = self.attention.workspace_bytes(kv.layer[0], self.cfg.num_q_heads, self.T, kv.num_requests, kv.prefix_len,
                                               self.max_query)
-        if self.workspace is None or self.workspace.nbytes < need:
-            self.workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
         with torch.cuda.stream(stream):  # (None: the current one)
+            if self.workspace is None or self.workspace.nbytes < need:
+                self.workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
             self._resize(token_ids, targets, stream)
         self.launches = 0
         self.embed(self.ids, stream)

@@ -104,3 +104,36 @@ def test_tokens_that_the_list_does_not_hold_are_not_added(cuda, model):
     u.offer([0, 1, 0], [1])
     u.offer([10, 6, 2], [])          # no two pages for the first; the second's five are at 10..14 of the list
     u.offer([7, 6, 2], [0, 1])       # the third's are at 12 and 13
+
+
+def test_lists_of_any_length_up_to_the_step(cuda, model):
+    """A list shorter than the step is the whole list: nothing behind it is read."""
+    u = Users(model, [9, 5], T=12, pages=16, max_pages=3, page_size=4, max_query=9)
+    whole = torch.full((40,), 10 ** 6, dtype=torch.int32, device="cuda")  # no token of the vocabulary behind the list
+    for targets in ([4, 1], [5, 2], [-1, 3], [-1, -1], [9, 5], [0, 0]):
+        ids = np.concatenate([t[o:max(o, n)] for t, o, n in zip(u.tokens, u.at, targets)])
+        whole[:len(ids)] = i32(ids)
+        u.dec.step(whole[:len(ids)], i32(targets))
+        rows = [(b, j) for b in range(2) for j in range(u.at[b], targets[b])]
+        h = f64(u.dec.h)
+        for row, (b, j) in enumerate(rows):
+            close(h[row], u.want[b][j])
+        u.at = [o if n < 0 else n for o, n in zip(u.at, targets)]
+        assert u.cache.seq_lens.tolist() == u.at
+    # a request whose tokens the short list does not hold is refused
+    u.dec.step(i32(u.tokens[0][:3]), i32([2, 2]))
+    assert u.cache.seq_lens.tolist() == [2, 0] and u.cache.free_state.tolist()[2:] == [1, 2]
+    no_device_error()
+
+
+def test_step_refusals(cuda, model):
+    from edgeexpert_b200._lib import TFError
+    dec, cache = paged(model[0], 2, T=12, pages=8, max_pages=3, page_size=4, max_query=4)
+    for ids, targets in ((torch.zeros(12, dtype=torch.int64, device="cuda"), i32([1, 1])), (i32(np.zeros(13)), i32([1, 1])),
+                         (i32(np.zeros((3, 4))), i32([1, 1])), (torch.zeros(12, dtype=torch.int32), i32([1, 1])),
+                         (i32(np.zeros(12)), i32([1])), (i32(np.zeros(12)), torch.tensor([1, 1], device="cuda")),
+                         (i32(np.zeros(12)), torch.ones(2, dtype=torch.int32))):
+        with pytest.raises(TFError):
+            dec.step(ids, targets)
+    assert cache.seq_lens.tolist() == [0, 0] and cache.free_state.tolist()[1] == 8
+    no_device_error()
