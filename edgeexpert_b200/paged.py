@@ -22,6 +22,7 @@ from .decoder import Decoder
 _I32 = torch.int32
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _LAYOUTS = {"half": 0, "interleaved": 1}
+_MAX_STEP = 256  # rows that tf_lm_head_greedy takes
 _SCALINGS = {None: 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4}
 
 
@@ -253,7 +254,10 @@ class PagedDecoder(Decoder):
 
     def __init__(self, weights, T: int, cache: PagedKVCache, max_query: int = 1, context: Context | None = None,
                  device=None):
-        """max_query: the most tokens a step adds to one request."""
+        """T: the most tokens of a step, up to 256 (the rows of the LM head).  max_query: the most
+        that a step adds to one request."""
+        if not 0 < T <= _MAX_STEP:
+            raise TFError(TF_ERR_INVALID_ARG, f"PagedDecoder: a step has 1 to {_MAX_STEP} tokens")
         super().__init__(weights, T, _NoContiguousCache(), context, device)
         cfg = weights.cfg
         if cache.max_tokens != T:

@@ -137,3 +137,15 @@ def test_step_refusals(cuda, model):
             dec.step(ids, targets)
     assert cache.seq_lens.tolist() == [0, 0] and cache.free_state.tolist()[1] == 8
     no_device_error()
+
+
+def test_steps_that_the_lm_head_cannot_take(cuda, model):
+    """Refused before anything is written, not at the end of the first step."""
+    from edgeexpert_b200._lib import TFError
+    for T in (0, 257):
+        with pytest.raises(TFError):
+            paged(model[0], 2, T=T, pages=80, max_pages=70, page_size=4, max_query=T)
+    dec, cache = paged(model[0], 1, T=256, pages=64, max_pages=64, page_size=4, max_query=256)
+    dec.step(i32(np.arange(256)), i32([256]))
+    assert cache.seq_lens.tolist() == [256] and ((dec.tokens >= 0) & (dec.tokens < 1000)).all()
+    no_device_error()
