@@ -208,6 +208,13 @@ struct RowParts {
     int b, j;  // request and token in it; b = the batch's size: a row of zeros
 };
 
+// The workers of a row's parts are among those that there are places for.  They always are where
+// a worker has written them; where none has (a wait gave up), the workspace may hold anything.
+__device__ __forceinline__ bool parts_exist(const Parts& p, int first_of, int last_of) {
+    const int first = first_of >> p.shift;
+    return first >= 0 && last_of >= first && last_of < p.places;
+}
+
 // Joins the parts of every row.  A thread finds the parts of a row (rows that
 // are finished drop out; the others in any order), a warp adds them up.  Bound by
 // latency: two rounds of dependent loads to find a row's parts, then two for each
@@ -239,6 +246,9 @@ __global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constan
         if (x.b < p.B) {
             r = request_of(p, x.b);
             x.j = t - r.start;
+            if (x.j < 0) x.b = p.B;  // before the first request: a row of zeros
+        }
+        if (x.b < p.B) {
             int lo, hi;
             seen_by(p, r, x.j, lo, hi);
             many = is_many(p, r);
@@ -255,7 +265,9 @@ __global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constan
         const int own_first = p.few.first_of[row], own_last = p.few.last_of[row];
         const int other_first = p.many.first_of[row], other_last = p.many.last_of[row];
         const float mark = p.many.first_md[row].x;
-        if (x.b < p.B && x.j >= r.used) {
+        const bool lost = (own && !parts_exist(p.few, own_first, own_last)) ||
+                          (other && !parts_exist(second, other_first, other_last));
+        if (x.b < p.B && (x.j >= r.used || lost)) {
             atomicOr(p.err, kErrBadPage);
             x.b = p.B;
         } else if (x.b < p.B) {
@@ -419,7 +431,7 @@ Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint
         return here;
     };
     const size_t rows = (size_t)T * nq;
-    const size_t cont[2] = {(size_t)ctx->num_sms * (kThreads / 32) * s.few_rows, (size_t)ctx->num_sms * kTcRows};
+    const size_t cont[2] = {(size_t)ctx->num_sms * (kThreads / 32) * s.few_rows, (size_t)ctx->num_sms * kTcRows};  // (Parts::places)
     for (int k = 0; k < 2; ++k) {
         l.first_of[k] = take(rows * sizeof(int));
         l.last_of[k] = take(rows * sizeof(int));
@@ -610,6 +622,8 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
             parts[k]->first_of = reinterpret_cast<int*>(w + l.first_of[k]);
             parts[k]->last_of = reinterpret_cast<int*>(w + l.last_of[k]);
         }
+        p.few.places = ctx->num_sms * (kThreads / 32);
+        p.many.places = ctx->num_sms;
         p.few.shift = 2 + (shape.nt == 1 ? 1 : (shape.nt == 2 ? 2 : 3));  // log2(8 nt)
         p.many.shift = 7;
         p.run_shift = run == 8 ? 3 : (run == 4 ? 2 : (run == 2 ? 1 : 0));

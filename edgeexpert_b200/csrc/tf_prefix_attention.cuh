@@ -26,7 +26,8 @@ struct Parts {
     // worker << shift | place), and the worker of the last: what the joining kernel adds up
     int* first_of;
     int* last_of;
-    int shift;  // log2 of the rows a cont place holds
+    int shift;   // log2 of the rows a cont place holds
+    int places;  // workers that cont has places for
 };
 
 // The pool as TMA sees it: [page][head][64-dim block][position][64 dims], 128-byte
@@ -89,7 +90,8 @@ __device__ __forceinline__ Request request_of(const AttnParams<T>& p, int b) {
 // wherever a cursor moves it made the kernel 247 KB of code, and the loops of its
 // warps, which share an instruction cache, spent half their time fetching it.
 
-// The last b with starts[b] <= t; B for tokens behind the last request.
+// The last b with starts[b] <= t; B for tokens behind the last request, and 0 for those before
+// the first one too (whose token index is negative then).
 template <typename T>
 __device__ __noinline__ int request_at(const AttnParams<T>& p, int t) {
     int lo = 0, hi = p.B;
@@ -102,6 +104,9 @@ __device__ __noinline__ int request_at(const AttnParams<T>& p, int t) {
     }
     return lo;
 }
+
+// Token j of request r is one of those that are computed.
+__device__ __forceinline__ bool is_used(const Request& r, int j) { return j >= 0 && j < r.used; }
 
 // Keys [lo, hi) that token j of request r sees, as positions of the whole sequence.
 template <typename T>

@@ -229,7 +229,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
                         const int b = request_at(p, j);
                         if (b < p.B) {
                             const Request rb = request_of(p, b);
-                            if (j - rb.start < rb.used) seen_by(p, rb, j - rb.start, lo, hi);
+                            if (is_used(rb, j - rb.start)) seen_by(p, rb, j - rb.start, lo, hi);
                         }
                     } else {
                         seen_by(p, r, j, lo, hi);

@@ -427,7 +427,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
             if (exists) b = request_at(p, t);
             if (b < p.B) {
                 const Request r = request_of(p, b);
-                if (t - r.start < r.used) {
+                if (is_used(r, t - r.start)) {
                     seen_by(p, r, t - r.start, row_lo, row_hi);
                     own = is_many(p, r);
                 } else {

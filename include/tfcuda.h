@@ -563,7 +563,8 @@ TF_API tf_status tf_rope_kv_write(tf_context* ctx, const void* q, uint64_t q_str
  * positions, this step's tokens among them (their K and V already written).
  *   out[t][h] = sum_p softmax_p(scale q.k_p) v_p, KV head h / (num_q_heads / num_kv_heads);
  *   lse[t][h] (float, optional) = log sum_p exp(scale q.k_p).
- * A row that sees nothing gives out 0 and lse -infinity; so do tokens from token_starts[B] up to T.
+ * A row that sees nothing gives out 0 and lse -infinity; so do tokens before token_starts[0] and
+ * from token_starts[B] up to T.
  * max_query: host bound on any n_b (tokens beyond it give 0 and the device error bit).  A page id
  * outside the pool is not read and raises the bit too; rows that see it are unspecified.  Positions that no row of the batch
  * (for the prefix) or of the request (for its own pages) sees may hold anything, NaN included.
