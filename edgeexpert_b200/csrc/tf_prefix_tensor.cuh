@@ -277,6 +277,9 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
         }
         return true;
     };
+    // For warps that stay together: given up by the whole warp or by none of it (votes and tensor
+    // memory instructions with lanes missing would wait for them for good).
+    auto wait_warp = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
     // Every role walks the CTA's jobs: (row tile, KV head, units [from, to) of `units`).
     struct Job {
         int tile, kvh, units, from, to;
@@ -321,7 +324,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                     next = look_up_keys<N>(p, c.seg, c.lo + c.tile * N, c.from, c.hi);
                 }
                 const int slot = it % S::kSlots;
-                ok = __all_sync(0xffffffffu, wait(&bar.empty[kv][slot], ((it / S::kSlots) & 1) ^ 1));
+                ok = wait_warp(&bar.empty[kv][slot], ((it / S::kSlots) & 1) ^ 1);
                 if (ok)
                     load_tile_keys<HD, N>(p, kv != 0, ring + (kv * S::kSlots + slot) * S::kSlot, job.kvh, now,
                                           &bar.full[kv][slot], kStay);
@@ -416,7 +419,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
         // O holds everything up to unit uc - 1.  A barrier for even and one for odd units:
         // a commit covers all earlier MMAs, so the scores of unit uc being there means that
         // the phase before the one waited for here (unit uc - 3) is over.
-        auto o_ready = [&]() { return wait(&bar.o_done[(uc - 1) & 1], ((uc - 1) >> 1) & 1); };
+        auto o_ready = [&]() { return wait_warp(&bar.o_done[(uc - 1) & 1], ((uc - 1) >> 1) & 1); };
         Job job = first_job();
         for (int u = u0; ok && u < u1;) {
             const long long row = (long long)job.tile * kTcRows + threadIdx.x;
@@ -459,7 +462,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
             TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from);
             for (int x = job.from; x < job.to; ++x, ++uc) {
                 const int buf = uc & 1;
-                ok = wait(&bar.s_full[buf], (uc >> 1) & 1);
+                ok = wait_warp(&bar.s_full[buf], (uc >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t scol = mine + S::kColS + buf * N;
