@@ -178,16 +178,17 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// Waits about two seconds at most, then reports it and returns false.
-__device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t* err) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long since = clock64();
+// Waits about two seconds at most (from `since` on), then reports it and returns false.
+__device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t* err, long long since) {
     while (!mbar_try_wait(bar, parity))
         if (clock64() - since > 4000000000ll) {
             atomicOr(err, kErrMbarTimeout);
             return false;
         }
     return true;
+}
+__device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t* err) {
+    return mbar_try_wait(bar, parity) || mbar_wait_limited(bar, parity, err, clock64());
 }
 
 // What L2 should do with what is loaded: own keys are read once (by one job) and

@@ -173,11 +173,11 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
         fill = fill == R - 1 ? 0 : fill + 1;
     };
     look_up();
-    // A tile's loads: bounded like every wait; after one that gave up the values
-    // are wrong, the error is reported and the units go on.
+    // A tile's loads: bounded like every wait, and given up by the whole warp or by none of it.
+    // A warp that gives up issues no more loads and leaves its jobs; the error is reported.
     int slot = 0;
     uint32_t phase = 0;
-    auto landed = [&]() { mbar_wait_limited(full + slot, phase, p.err); };
+    auto landed = [&]() { return __all_sync(0xffffffffu, mbar_wait_limited(full + slot, phase, p.err)) != 0; };
     auto taken = [&]() {
         if (++slot == R) {
             slot = 0;
@@ -286,11 +286,13 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
     // ---- units ------------------------------------------------------------------------
     const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_chunk = lane >> 4;        // K: keys x dims
     const int v_row = (lane & 7) + ((lane >> 4) & 1) * 8, v_chunk = (lane >> 3) & 1;  // V: dims x keys
+    bool ok = true;
     for (int u = u0; u < u1; ++u) {
         if (u == u0 || cur.tile == 0) begin_job();
         __syncwarp();  // the tile before this one has been read by every lane
         load_tile();
-        landed();
+        ok = landed();
+        if (!ok) break;
         const uint32_t kt = ring + slot * S::kTile;
         taken();
         float s[NT][4], s2[NT][4];
@@ -345,7 +347,8 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
         }
         __syncwarp();  // K has been read
         load_tile();
-        landed();
+        ok = landed();
+        if (!ok) break;
         const uint32_t vt = ring + slot * S::kTile;
         taken();
 #pragma unroll
@@ -361,9 +364,11 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
         }
         stream_advance<T, HD, NT>(p, cur);
     }
-    // what was loaded ahead (zeros) lands before the CTA may end
-    for (int i = 0; i < R - 1; ++i) {
-        landed();
+    // what was loaded ahead (zeros) lands before the CTA may end; after a wait that gave up, what
+    // lands within one more such time
+    const long long since = clock64();
+    for (int i = 0; i < (ok ? R - 1 : R); ++i) {
+        mbar_wait_limited(full + slot, phase, p.err, since);
         taken();
     }
 }

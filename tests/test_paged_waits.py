@@ -38,3 +38,12 @@ def test_no_wait_is_ignored():
     for role in (loaders, issue, rows):
         for line in re.findall(r"[^\n;{}]*(?<!\w)(?:wait|wait_warp|o_ready)\([^\n]*", role):
             assert re.search(r"\b(ok|return|o_ready)\b.*=|return|ok &&", line), line
+    stream = code("tf_prefix_stream.cuh").split("void stream_warp(", 1)[1]
+    assert "__all_sync(0xffffffffu, mbar_wait_limited(" in stream
+    for line in re.findall(r"[^\n]*\blanded\(\)[^\n]*\n[^\n]*", stream):
+        assert re.search(r"ok = landed\(\);\s+if \(!ok\) break;", line), line
+
+
+def test_a_streaming_warp_that_gave_up_lets_its_loads_land():
+    stream = code("tf_prefix_stream.cuh").split("void stream_warp(", 1)[1]
+    assert re.search(r"i < \(ok \? R - 1 : R\); \+\+i\) \{\s*mbar_wait_limited\(", stream)
