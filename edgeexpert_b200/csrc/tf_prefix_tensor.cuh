@@ -332,10 +332,12 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
             u += job.to - job.from;
             if (u < u1) next_job(job, u);
         }
-        // after a wait that gave up: what is in flight lands before the CTA may end
-        if (!ok)
-            for (int i = max(0, it - 1 - S::kSlots); i < it - 1; ++i)
-                mbar_wait_limited(&bar.full[kv][i % S::kSlots], (i / S::kSlots) & 1, p.err);
+        // what is in flight lands before the CTA may end: also what nobody waits for any more because
+        // another warp gave up
+        const long long since = clock64();
+        const int issued = ok ? it : it - 1;
+        for (int i = max(0, issued - S::kSlots); i < issued; ++i)
+            mbar_wait_limited(&bar.full[kv][i % S::kSlots], (i / S::kSlots) & 1, p.err, since);
     } else if (warp == 4) {
         // ---- MMA issue: one elected thread ------------------------------------------
         if (elect_one()) {

@@ -4,7 +4,8 @@ the rules that keep it from becoming a hang are checked here.
 
 * A warp whose lanes go on to votes or tensor memory instructions together
   gives a wait up together: every wait of such a role is one of the warp.
-* A warp that gave up doesn't wait (or load) on: the result of a wait is used."""
+* A warp that gave up doesn't wait (or load) on: the result of a wait is used.
+* Loads in flight land before the CTA ends, whoever gave up."""
 import re
 from pathlib import Path
 
@@ -42,6 +43,12 @@ def test_no_wait_is_ignored():
     assert "__all_sync(0xffffffffu, mbar_wait_limited(" in stream
     for line in re.findall(r"[^\n]*\blanded\(\)[^\n]*\n[^\n]*", stream):
         assert re.search(r"ok = landed\(\);\s+if \(!ok\) break;", line), line
+
+
+def test_the_tensor_loaders_see_their_loads_land():
+    _, loaders, _, _ = roles()
+    end = loaders.split("next_job(job, u);", 1)[1]
+    assert re.search(r"issued = ok \? it : it - 1;\s*for .*issued - S::kSlots.*\s*mbar_wait_limited\(", end)
 
 
 def test_a_streaming_warp_that_gave_up_lets_its_loads_land():
