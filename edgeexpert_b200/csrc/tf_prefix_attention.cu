@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
     int few_before, many_before = 0, many = 0, i0 = 0, i1 = 0, per_row_tile = 0;
     const int few = stream_units<T, HD, NT>(p, red, b0, b1, few_before);
+    if (p.window && cta == 0 && threadIdx.x == 0) *p.prefix_first = prefix_first(p);
     if constexpr (kTensor) {
         const bool own = p.max_query * p.G > p.many_above;  // requests may have own keys here
         if (!own && !p.prefix_few) {
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constan
     static_assert(kJoinRows <= 256);
     RowParts x = {};
     Request r = {};
-    bool many = false, own = false, other = false;
+    bool many = false, own = false, seen = false;
     x.b = p.B;
     if (mine) {
         // what the caller wrote is complete: the parts kernel lets this one start after its own wait
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constan
             seen_by(p, r, x.j, lo, hi);
             many = is_many(p, r);
             own = !many && r.len > own_lo(p, r);
-            other = p.prefix_len > p.prefix_lo || (many && hi > lo);
+            seen = hi > lo;
         }
     }
     griddep_wait();
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constan
         const int own_first = p.few.first_of[row], own_last = p.few.last_of[row];
         const int other_first = p.many.first_of[row], other_last = p.many.last_of[row];
         const float mark = p.many.first_md[row].x;
+        const bool other = x.b < p.B && (p.prefix_len > (p.window ? *p.prefix_first : 0) || (many && seen));
         const bool lost = (own && !parts_exist(p.few, own_first, own_last)) ||
                           (other && !parts_exist(second, other_first, other_last));
         if (x.b < p.B && (x.j >= r.used || lost)) {
@@ -419,7 +421,7 @@ Shape shape_of_call(const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t pre
 }
 
 struct Layout {
-    size_t first[2], first_md[2], cont[2], cont_md[2], first_of[2], last_of[2], bytes;
+    size_t first[2], first_md[2], cont[2], cont_md[2], first_of[2], last_of[2], prefix_first, bytes;
 };
 
 Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint32_t T, const Shape& s) {
@@ -440,6 +442,7 @@ Layout layout_of(const tf_context* ctx, const tf_paged_kv* kv, uint32_t nq, uint
         l.first[k] = take(rows * kv->head_dim * sizeof(float));
         l.cont[k] = take(cont[k] * kv->head_dim * sizeof(float));
     }
+    l.prefix_first = take(sizeof(int));
     l.bytes = at;
     return l;
 }
@@ -606,10 +609,6 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
         p.G = (int)G;
         p.window = (int)window;
         p.scale = scale;
-        // no row stands before prefix_len - max_query
-        p.prefix_lo = window ? (int)std::max<long long>(0, std::min<long long>(prefix_len, (long long)prefix_len -
-                                                                                              max_query - window + 1))
-                             : 0;
         p.prefix_few = shape.prefix_few;
         p.many_above = shape.many_above;
         uint8_t* w = static_cast<uint8_t*>(workspace);
@@ -622,6 +621,7 @@ tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint64_t q_
             parts[k]->first_of = reinterpret_cast<int*>(w + l.first_of[k]);
             parts[k]->last_of = reinterpret_cast<int*>(w + l.last_of[k]);
         }
+        p.prefix_first = reinterpret_cast<int*>(w + l.prefix_first);
         p.few.places = ctx->num_sms * (kThreads / 32);
         p.many.places = ctx->num_sms;
         p.few.shift = 2 + (shape.nt == 1 ? 1 : (shape.nt == 2 ? 2 : 3));  // log2(8 nt)

@@ -52,7 +52,8 @@ struct AttnParams {
     long long out_stride;
     float* lse;
     uint32_t* err;
-    int prefix_len, prefix_lo, max_pages, B, max_query, T_tokens, nq, nkv, G, hd, window;
+    int* prefix_first;  // the first prefix position that any row sees, for the joining kernel (calls with a window)
+    int prefix_len, max_pages, B, max_query, T_tokens, nq, nkv, G, hd, window;
     int prefix_few;   // the prefix is read by the streaming warps too (the batch has few rows)
     int many_above;   // requests of more rows per KV head than this go to the tensor cores
     float scale;
@@ -114,6 +115,23 @@ __device__ __forceinline__ void seen_by(const AttnParams<T>& p, const Request& r
     const int at = p.prefix_len + r.len - (r.n - j);
     hi = at + 1;
     lo = p.window ? max(0, at - p.window + 1) : 0;
+}
+
+// The first prefix position that any row of the batch sees, as the parts kernel keeps it: positions
+// before it have no rows, and pages of them may belong to others by now.
+__device__ __forceinline__ int& shared_prefix_first() {
+    __shared__ int first;
+    return first;
+}
+template <typename T>
+__device__ __forceinline__ int prefix_first(const AttnParams<T>& p) {
+    return p.window ? shared_prefix_first() : 0;
+}
+// Tiles of `keys` keys that hold the prefix from there on.
+template <typename T>
+__device__ __forceinline__ int prefix_tiles(const AttnParams<T>& p, int keys) {
+    const int first = prefix_first(p);
+    return p.prefix_len > first ? (p.prefix_len - (first & ~(kMaxRun - 1)) + keys - 1) / keys : 0;
 }
 
 // First of a request's own positions that any of its rows sees.

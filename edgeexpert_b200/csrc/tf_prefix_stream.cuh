@@ -82,12 +82,18 @@ struct StreamCursor {
     int from;            // the first that any row sees
 };
 
+// Rows that have the prefix here.
+template <typename T>
+__device__ __forceinline__ int stream_prefix_rows(const AttnParams<T>& p) {
+    return p.prefix_few ? max(0, min(p.starts[p.B], p.T_tokens)) * p.G : 0;
+}
+
 template <typename T, int HD, int NT>
 __device__ __forceinline__ void stream_segment(const AttnParams<T>& p, StreamCursor& c) {
     using S = StreamShape<HD, NT>;
     if (c.seg < 0) {
-        const int rows = p.prefix_few ? max(0, min(p.starts[p.B], p.T_tokens)) * p.G : 0;
-        c.from = p.prefix_lo;
+        const int rows = stream_prefix_rows(p);
+        c.from = prefix_first(p);
         c.hi = p.prefix_len;
         c.row_tiles = (rows + S::kRows - 1) / S::kRows;
     } else {
@@ -121,19 +127,31 @@ __device__ __forceinline__ void stream_advance(const AttnParams<T>& p, StreamCur
 }
 
 // The units of the whole batch; `before` those of the requests before this
-// thread's own [b0, b1).
+// thread's own [b0, b1).  With a window also the first prefix position that any row sees.
 template <typename T, int HD, int NT>
 __device__ __forceinline__ int stream_units(const AttnParams<T>& p, int* red, int b0, int b1, int& before) {
+    using S = StreamShape<HD, NT>;
+    if (p.window) {
+        if (threadIdx.x == 0) shared_prefix_first() = p.prefix_len;
+        __syncthreads();
+    }
+    const int rows = stream_prefix_rows(p);
     StreamCursor c;
-    c.seg = -1;
-    stream_segment<T, HD, NT>(p, c);
-    const int prefix_units = c.row_tiles * c.tiles * p.nkv;
-    int sum = 0, total;
+    int sum = 0, total, first = p.prefix_len;
     for (c.seg = b0; c.seg < b1; ++c.seg) {
         stream_segment<T, HD, NT>(p, c);
         sum += c.row_tiles * c.tiles * p.nkv;
+        if (p.window) {
+            const Request r = request_of(p, c.seg);
+            int lo = first, hi;
+            if (r.used) seen_by(p, r, 0, lo, hi);
+            first = min(first, lo);
+        }
     }
-    before = prefix_units + block_scan(sum, red, &total);
+    if (p.window && first < p.prefix_len) atomicMin(&shared_prefix_first(), first);
+    before = block_scan(sum, red, &total);
+    const int prefix_units = (rows + S::kRows - 1) / S::kRows * prefix_tiles(p, S::kKeys) * p.nkv;
+    before += prefix_units;
     return prefix_units + total;
 }
 

@@ -128,8 +128,8 @@ template <typename T, int HD>
 __device__ __forceinline__ void tensor_segment(const AttnParams<T>& p, int i, TensorCursor& c) {
     c.tile = 0;
     if (c.seg < 0) {
-        c.from = p.prefix_lo;
-        c.hi = p.prefix_few ? p.prefix_lo : p.prefix_len;
+        c.from = prefix_first(p);
+        c.hi = p.prefix_few ? c.from : p.prefix_len;
     } else {
         const Request r = request_of(p, c.seg);
         c.from = c.hi = 0;
@@ -200,9 +200,7 @@ __device__ __noinline__ TensorCursor tensor_begin(const AttnParams<T>& p, int i,
 template <typename T, int HD>
 __device__ __noinline__ int tensor_units(const AttnParams<T>& p, int i) {
     if (p.max_query * p.G <= p.many_above) {  // the prefix alone, for any tile with a token of the batch
-        constexpr int N = TensorShape<HD>::kKeys;
-        const bool live = (int)((long long)i * kTcRows / p.G) < p.starts[p.B];
-        return live && p.prefix_len > p.prefix_lo ? (p.prefix_len - (p.prefix_lo & ~(kMaxRun - 1)) + N - 1) / N : 0;
+        return (int)((long long)i * kTcRows / p.G) < p.starts[p.B] ? prefix_tiles(p, TensorShape<HD>::kKeys) : 0;
     }
     TensorCursor c;
     int first, units = 0;

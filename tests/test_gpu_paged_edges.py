@@ -30,3 +30,40 @@ def test_tokens_before_the_first_request(cuda, case):
     no_device_error()
     batch.check(out, lse)
     assert (out[:before] == 0).all() and (lse[:before] == -float("inf")).all()
+
+
+# a window that ends behind the prefix for every row, for some, and one that ends inside it
+OUT_OF_SIGHT = [([70, 61, 90], [1, 2, 4], 16, 4, 128, "bf16", 50), ([60] * 40, [1] * 40, 16, 8, 256, "fp16", 60),
+                ([80, 200, 66], [1, 66, 1], 16, 8, 64, "fp16", 14), ([30], [1], 2, 2, 320, "fp16", 20),
+                ([3, 9, 40], [1, 1, 1], 16, 8, 256, "fp16", 40)]
+
+
+@pytest.mark.parametrize("case", range(len(OUT_OF_SIGHT)))
+def test_prefix_pages_that_no_row_sees(cuda, case):
+    """Page ids of the prefix that lie out of every row's window may be anything (the pages have
+    been given to others): nothing is reported and nothing is read."""
+    lens, counts, nq, nkv, hd, dtype, window = OUT_OF_SIGHT[case]
+    batch = Batch(700, lens, counts, nq, nkv, hd, dtype, 16, seed=40 + case)
+    first = min(max(0, 700 + n - c - window + 1) for n, c in zip(lens, counts))  # the first position any row sees
+    batch.prefix_pages = batch.prefix_pages.copy()
+    batch.prefix_pages[:first // 16] = -1
+    out, lse = batch.run(window)
+    no_device_error()
+    batch.check(out, lse, window)
+
+
+def test_more_queries_than_announced_under_a_window(cuda):
+    """Tokens beyond max_query give 0 and the error bit; those within it are right, wherever they stand."""
+    from edgeexpert_b200._lib import Context, TFError
+    batch = Batch(200, [2, 30], [40, 1], 8, 4, 64, "fp16", 16, seed=50)
+    out, lse = batch.run(window=20, max_query=3)
+    with pytest.raises(TFError):
+        Context.get(0).check_device()
+    assert (out[3:40] == 0).all() and (lse[3:40] == -float("inf")).all()
+    shared, own = f64(batch.both[0]), f64(batch.both[1])
+    keys, values = (np.concatenate([shared[i], own[i]]) for i in (0, 1))
+    ro, rl, A, s = attention_reference(f64(batch.q[:3]), keys, values, 200 + 2 - 40 + np.arange(3), batch.scale, 20)
+    u = U[torch.float16]
+    assert (np.abs(f64(out[:3]) - ro) <= (2 * u + 2 * s + 16 * E32) * A + 242 * 2.0 ** -25 * 6 + 2.0 ** -25).all()
+    assert (np.abs(f64(lse[:3]) - rl) <= s + 300 * E32 + 8 * E32 * np.abs(rl) + 4 * E32).all()
+    no_device_error()
