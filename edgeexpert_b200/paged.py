@@ -235,13 +235,18 @@ class PagedKVCache:
                                  stream=stream)
 
     def share(self, request: int, length: int, stream=None):
-        """Make the `length` positions that `request` holds the prefix of all requests: its pages leave
-        the tables and stay out of the free ring.  The others must be empty."""
+        """Make the `length` positions that `request` holds, all of them, the prefix of all requests:
+        its pages leave the tables and stay out of the free ring for as long as the cache lives.
+        The others must be empty.  Reads the lengths back (once in the cache's life)."""
         if self.prefix_len:
             raise TFError(TF_ERR_INVALID_ARG, "PagedKVCache.share: there is a prefix already")
-        if not 0 < length <= self.page_table.shape[1] * self.page_size:
-            raise TFError(TF_ERR_INVALID_ARG, "PagedKVCache.share: no such positions")
-        with torch.cuda.stream(stream) if stream is not None else torch.cuda.stream(torch.cuda.current_stream()):
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, self.seq_lens.device)
+        with torch.cuda.stream(stream):  # (None: the current one)
+            held = self.seq_lens.tolist()
+            if length <= 0 or held != [length if b == request else 0 for b in range(self.num_requests)]:
+                raise TFError(TF_ERR_INVALID_ARG, f"PagedKVCache.share: the requests hold {held} positions; "
+                              f"request {request} must hold {length} and the others none")
             self.prefix_pages = self.page_table[request, :-(-length // self.page_size)].clone()
             self.seq_lens[request] = 0
         self.prefix_len = length

@@ -149,3 +149,18 @@ def test_steps_that_the_lm_head_cannot_take(cuda, model):
     dec.step(i32(np.arange(256)), i32([256]))
     assert cache.seq_lens.tolist() == [256] and ((dec.tokens >= 0) & (dec.tokens < 1000)).all()
     no_device_error()
+
+
+def test_a_prefix_shared_on_a_raw_stream(cuda, model):
+    """An integer names a stream here as it does in every other call."""
+    u = Users(model, [9, 12], T=12, pages=16, max_pages=3, page_size=4, max_query=12)
+    u.dec.step(i32(u.tokens[0][:6]), i32([6, -1]))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    u.cache.share(0, 6, stream=stream.cuda_stream)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert u.cache.prefix_len == 6 and u.cache.seq_lens.tolist() == [0, 0]
+    u.dec.step(i32(u.tokens[0][6:]), i32([3, -1]))
+    for row in range(3):
+        close(f64(u.dec.h)[row], u.want[0][6 + row])
+    no_device_error()
