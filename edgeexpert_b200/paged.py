@@ -142,8 +142,10 @@ class RotaryKVWrite:
         if shape != v.shape or shape != (T, kv.num_kv_heads, kv.head_dim) or q_out.shape != q.shape or hd != kv.head_dim:
             raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: shapes of q, k, v and the cache do not agree")
         _int32("RotaryKVWrite.encode", slots, positions)
-        if slots.numel() != T or positions.numel() != T or inv_freq.dtype is not torch.float64 or inv_freq.numel() * 2 != rot:
-            raise TFError(TF_ERR_INVALID_ARG, "RotaryKVWrite.encode: a slot and position per token, a float64 per pair")
+        if (slots.numel() != T or positions.numel() != T or inv_freq.dtype is not torch.float64
+                or inv_freq.numel() * 2 != rot or not inv_freq.is_contiguous()):
+            raise TFError(TF_ERR_INVALID_ARG,
+                          "RotaryKVWrite.encode: a slot and position per token, a contiguous float64 per pair")
         if q_weight is not None or k_weight is not None:
             for w in (q_weight, k_weight):
                 if w is not None and (w.dtype is not torch.bfloat16 or w.numel() != hd or not w.is_contiguous()):
@@ -308,14 +310,16 @@ class PagedDecoder(Decoder):
 
     def step(self, token_ids, targets, stream=None):
         """token_ids (up to T): the tokens to add, request after request, of every request that
-        is to grow; targets: every request's length with them.  Both int32, on the device.  A request that can't have its pages
-        is refused and keeps its length; the others are as if it had not asked.  Next tokens in
-        self.tokens, row by row of the tokens added: row i is position kv.positions[i] of request
-        kv.requests[i], and kv.free_state tells how many requests were refused."""
+        is to grow; targets: every request's length with them.  Both int32, on the device.  A
+        request that can't have its pages is refused and keeps its length; the others are as if
+        it had not asked.  Next tokens in self.tokens, row by row of the tokens added: row i is
+        position kv.positions[i] of request kv.requests[i], and kv.free_state tells how many
+        requests were refused."""
         kv = self.kv
         for t, what in ((token_ids, "token_ids"), (targets, "targets")):
             if t.dtype is not _I32 or t.dim() != 1 or t.device != self.ids.device:
-                raise TFError(TF_ERR_INVALID_ARG, f"PagedDecoder.step: {what} must be a vector of int32 on {self.ids.device}")
+                raise TFError(TF_ERR_INVALID_ARG,
+                              f"PagedDecoder.step: {what} must be a vector of int32 on {self.ids.device}")
         if token_ids.numel() > self.T or targets.numel() != kv.num_requests:
             raise TFError(TF_ERR_INVALID_ARG, "PagedDecoder.step: up to T tokens, a target per request")
         need = self.attention.workspace_bytes(kv.layer[0], self.cfg.num_q_heads, self.T, kv.num_requests, kv.prefix_len,

@@ -67,3 +67,14 @@ def test_more_queries_than_announced_under_a_window(cuda):
     assert (np.abs(f64(out[:3]) - ro) <= (2 * u + 2 * s + 16 * E32) * A + 242 * 2.0 ** -25 * 6 + 2.0 ** -25).all()
     assert (np.abs(f64(lse[:3]) - rl) <= s + 300 * E32 + 8 * E32 * np.abs(rl) + 4 * E32).all()
     no_device_error()
+
+
+def test_rope_frequencies_of_a_view(cuda):
+    """Frequencies are read side by side: a view with gaps is refused."""
+    from edgeexpert_b200._lib import TFError
+    from edgeexpert_b200.paged import PagedKV, RotaryKVWrite
+    z = torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda")
+    kc, vc = (torch.zeros(2, 4, 4, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    gaps = torch.ones(64, dtype=torch.float64, device="cuda")[::2]
+    with pytest.raises(TFError):
+        RotaryKVWrite().encode(z, z, z, torch.empty_like(z), PagedKV(kc, vc), i32([0, 1]), i32([0, 1]), gaps)
