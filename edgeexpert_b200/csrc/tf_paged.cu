@@ -650,7 +650,7 @@ tf_status tf_rope_frequencies(uint32_t rotary_dim, double theta, tf_rope_scaling
         auto pair_of = [&](double turns) { return rot * log(original_context / (turns * tau)) / (2.0 * log(theta)); };
         ramp_lo = fmax(floor(pair_of(high)), 0.0);
         ramp_hi = fmin(ceil(pair_of(low)), rot - 1.0);
-        *attention_factor = 0.1 * log(factor) + 1.0;
+        *attention_factor = factor > 1.0 ? 0.1 * log(factor) + 1.0 : 1.0;
     }
     for (uint32_t i = 0; i < rotary_dim / 2; ++i) {
         const double f = pow(theta, -2.0 * i / rot);

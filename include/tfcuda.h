@@ -524,7 +524,7 @@ typedef enum {
     TF_ROPE_SCALE_BASE = 2,   /* theta * factor^(rot / (rot - 2)) */
     TF_ROPE_SCALE_RAMP = 3,   /* pairs of more than beta_fast turns over original_context keep their
                                * frequency, those of fewer than beta_slow get it / factor, linear in
-                               * the pair index between; attention factor 0.1 ln(factor) + 1 */
+                               * the pair index between; attention factor 0.1 ln(factor) + 1, 1 for factors below 1 */
     TF_ROPE_SCALE_BANDS = 4   /* the same with low_factor / high_factor turns, linear in the turns;
                                * attention factor 1 */
 } tf_rope_scaling;

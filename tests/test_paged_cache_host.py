@@ -1,4 +1,5 @@
-"""CPU tests of the paged cache's own bookkeeping, on tables in host memory."""
+"""CPU tests of the paged cache's own bookkeeping, on tables in host memory, and of a
+frequency scaling at its end."""
 from types import SimpleNamespace
 
 import pytest
@@ -44,3 +45,12 @@ def test_a_request_becomes_the_prefix_once(length):
     assert cache.prefix_pages.tolist() == pages
     with pytest.raises(TFError):
         cache.share(1, length)
+
+
+@pytest.mark.parametrize("factor", [1e-6, 0.25, 0.5, 1.0])
+def test_a_context_that_is_not_extended_keeps_its_attention(factor):
+    """The ramp's attention factor makes up for a longer context; factors up to 1 leave it at 1
+    (0.1 ln(factor) + 1 would fall, below e^-10 to negative values)."""
+    from edgeexpert_b200.paged import rope_frequencies
+    _, mul = rope_frequencies(64, scaling="ramp", factor=factor, original_context=8192, device="cpu")
+    assert mul == 1.0
