@@ -209,9 +209,14 @@ __device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity
     return mbar_try_wait(bar, parity) || mbar_wait_limited(bar, parity, err, clock64());
 }
 
-// What L2 should do with what is loaded: own keys are read once (by one job) and
-// leave first; prefix keys are read by every row tile and stay.
-enum : uint64_t { kLeaveFirst = 0x12F0000000000000ull, kStay = 0x14F0000000000000ull };
+// What L2 should do with a tile: keys that one job reads, once, leave first; the prefix's, and own
+// keys that several row tiles read, stay.
+__device__ __forceinline__ uint64_t l2_policy(bool once) {
+    uint64_t first, last;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(last));
+    return once ? first : last;
+}
 
 // 5-D tiled TMA load (no multicast).
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int v, int w,
@@ -246,11 +251,12 @@ struct TileKeys {
 
 template <int HD, int KEYS, typename T>
 __device__ __forceinline__ void load_tile_keys(const AttnParams<T>& p, bool v, uint32_t tile, int head,
-                                               const TileKeys<KEYS>& k, uint64_t* bar, uint64_t hint) {
+                                               const TileKeys<KEYS>& k, uint64_t* bar, bool once) {
     constexpr int kBlocks = HD / 64, kMost = TileKeys<KEYS>::kMost;
     const CUtensorMap* map = v ? &p.maps.v : &p.maps.k;
     const int lane = threadIdx.x & 31, run = 1 << p.run_shift, runs = KEYS >> p.run_shift, all = (1 << run) - 1;
     const bool one = elect_one();
+    const uint64_t hint = l2_policy(once);
     if (one) mbar_arrive_expect_tx(bar, KEYS * HD * 2);
     bool complete = p.wide != 0;
 #pragma unroll

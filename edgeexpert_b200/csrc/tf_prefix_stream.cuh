@@ -168,7 +168,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
     int left = u1 - u0;        // units not looked up yet
     TileKeys<16> next, now;  // the unit after the one being loaded, and that one
     int next_head = 0, now_head = 0;
-    bool next_own = true, now_own = true;  // own keys, not the prefix's
+    bool next_own = true, now_own = true;  // own keys that no other row tile reads
     auto look_up = [&]() {
         next_head = ahead.kvh;
         next_own = ahead.seg >= 0 && ahead.row_tiles == 1;
@@ -185,7 +185,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
             check_keys(p, now);
         }
         load_tile_keys<HD, 16>(p, v_next, ring + fill * S::kTile, now_head, now, full + fill,
-                               now_own ? kLeaveFirst : kStay);
+                               now_own);
         if (!v_next) look_up();
         v_next = !v_next;
         fill = fill == R - 1 ? 0 : fill + 1;

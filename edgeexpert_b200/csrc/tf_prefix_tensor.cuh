@@ -325,7 +325,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                 ok = wait_warp(&bar.empty[kv][slot], ((it / S::kSlots) & 1) ^ 1);
                 if (ok)
                     load_tile_keys<HD, N>(p, kv != 0, ring + (kv * S::kSlots + slot) * S::kSlot, job.kvh, now,
-                                          &bar.full[kv][slot], kStay);
+                                          &bar.full[kv][slot], false);
             }
             u += job.to - job.from;
             if (u < u1) next_job(job, u);
