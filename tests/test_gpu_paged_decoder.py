@@ -164,3 +164,75 @@ def test_a_prefix_shared_on_a_raw_stream(cuda, model):
     for row in range(3):
         close(f64(u.dec.h)[row], u.want[0][6 + row])
     no_device_error()
+
+
+class Watched:
+    """A decoder whose routing inputs and choices are kept, layer by layer."""
+
+    def __init__(self, dec):
+        self.dec, self.layers, moe = dec, [], dec._moe
+
+        def watched(i, stream):
+            moe(i, stream)
+            self.layers.append((dec.router_x.cpu().numpy().copy(), dec.idx.cpu().numpy().copy()))
+
+        dec._moe = watched
+
+    def step(self, *args):
+        self.layers.clear()
+        self.dec.step(*args)
+        return f64(self.dec.h), list(self.layers)
+
+
+def bits(t):
+    t = t.contiguous()
+    return t.view(torch.int16).cpu().numpy().view(np.uint16) if t.is_floating_point() else t.cpu().numpy()
+
+
+@pytest.mark.parametrize("T", [1, 2, 5, 8])
+def test_steps_of_a_few_tokens(cuda, model, T):
+    """Up to eight rows the projections are GEMVs, and one row has its own path through the experts.
+
+    The choice of experts is not continuous: two states within the tolerance of each other may
+    choose differently where two logits nearly meet.  There the choice is checked against the
+    formula on the row's own state in 64 bits, and the row's result has nothing to be compared with."""
+    from edgeexpert_b200.decoder import Decoder, KVCache
+    weights, cfg, dev = model[0], model[0].cfg, torch.device("cuda", 0)
+    rng = np.random.default_rng(16)
+    users = [rng.integers(1, 1000, n) for n in (7, 9)]
+    want = []
+    for user in users:
+        dec = Watched(Decoder(weights, 1, KVCache(cfg, 1, dev)))
+        want.append([dec.step(i32([token]), pos) for pos, token in enumerate(user)])
+    dec, cache = paged(weights, 2, T=T, pages=16, max_pages=3, page_size=4, max_query=T)
+    dec, at, apart, compared = Watched(dec), [0, 0], set(), 0
+    while at != [7, 9]:
+        added, targets = [], []
+        for b in range(2):
+            n = min(T - len(added), len(users[b]) - at[b])
+            targets.append(at[b] + n if n else -1)
+            added += [(b, j) for j in range(at[b], at[b] + n)]
+            at[b] += n
+        h, layers = dec.step(i32([users[b][j] for b, j in added]), i32(targets))
+        for row, (b, j) in enumerate(added):
+            (ho,), theirs = want[b][j]
+            for i, ((x, idx), (xo, idxo)) in enumerate(zip(layers, theirs)):
+                if b in apart:
+                    break
+                close(f64(torch.from_numpy(x[row])), f64(torch.from_numpy(xo[0])))
+                if set(idx[row]) != set(idxo[0]):
+                    M = weights.layers[i].moe
+                    logits = O.router_logits(bits(M.router_w), bits(M.router_s), bits(M.router_b),
+                                             x[row].view(np.uint16), bits(M.eff_scale))[1]
+                    chosen = np.isin(np.arange(cfg.num_experts), idx[row])
+                    # (fp32 sums of 256 products)
+                    assert logits[chosen].min() >= logits[~chosen].max() - 256 * 2.0 ** -23 * np.abs(logits).max()
+                    if i + 1 < cfg.layers:  # what later tokens of the request see of it is different too
+                        apart.add(b)
+                    break
+            else:
+                if b not in apart:
+                    close(h[row], ho)
+                    compared += 1
+    assert compared >= 12  # of sixteen
+    no_device_error()
