@@ -70,6 +70,12 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
+// Whether kernels are launched with programmatic dependent launch (TFCUDA_PDL=0 turns it off).
+inline bool dependent_launches() {
+    const char* env = getenv("TFCUDA_PDL");
+    return !(env && env[0] == '0');
+}
+
 // Largest dynamic shared memory an engine launch may request.
 template <class Pol, typename ST, int H = 0>
 size_t engine_smem_limit(tf_context* ctx) {
@@ -101,11 +107,10 @@ tf_status launch_engine(tf_context* ctx, const typename Pol::Params& p, size_t x
         configured[dev] = true;
     }
     const int grid = superjobs < ctx->num_sms ? superjobs : ctx->num_sms;
-    // Programmatic dependent launch (TFCUDA_PDL=0 turns it off): this grid's
-    // launch and set-up overlap the preceding kernel's tail; the kernel waits
-    // (griddepcontrol.wait) before reading anything that kernel produced.
-    const char* pdl_env = getenv("TFCUDA_PDL");
-    const bool pdl = !(pdl_env && pdl_env[0] == '0');
+    // Programmatic dependent launch: this grid's launch and set-up overlap the
+    // preceding kernel's tail; the kernel waits (griddepcontrol.wait) before
+    // reading anything that kernel produced.
+    const bool pdl = dependent_launches();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kWarps * 32 * (1 + H));

@@ -76,7 +76,7 @@ cudaError_t launch_overlapped(void (*kernel)(Args...), unsigned ctas, unsigned t
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = dependent_launches() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 

@@ -1,6 +1,8 @@
 """GPU tests of the serving operators at the edges of what their callers may
 pass: what rows do not see, bounds that are not met, views, tokens outside
 every request.  References and tolerances are those of test_gpu_paged.py."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -78,3 +80,39 @@ def test_rope_frequencies_of_a_view(cuda):
     gaps = torch.ones(64, dtype=torch.float64, device="cuda")[::2]
     with pytest.raises(TFError):
         RotaryKVWrite().encode(z, z, z, torch.empty_like(z), PagedKV(kc, vc), i32([0, 1]), i32([0, 1]), gaps)
+
+
+@pytest.mark.parametrize("switch", ["0", "1", None])
+def test_dependent_launches_can_be_switched_off(cuda, monkeypatch, switch):
+    """TFCUDA_PDL=0 holds for these operators as for all others: no edge between two of their
+    kernels is a programmatic one."""
+    from edgeexpert_b200.paged import PagedKV, SharedPrefixAttention
+    batch = Batch(100, [20, 30], [1, 1], 8, 4, 64, "fp16", 16, seed=70)
+    op, kv = SharedPrefixAttention(), PagedKV(batch.k, batch.v)
+    ws = torch.empty(op.workspace_bytes(kv, 8, 2, 2, 100, 1), dtype=torch.uint8, device="cuda")
+    args = (i32(batch.table), i32(batch.lens), i32(batch.starts))
+    pages, out, lse = i32(batch.prefix_pages), torch.zeros_like(batch.q), torch.zeros(2, 8, device="cuda")
+
+    def call():
+        op.encode(batch.q, kv, *args, out, ws, prefix_pages=pages, prefix_len=100, lse=lse)
+
+    monkeypatch.delenv("TFCUDA_PDL", raising=False)
+    if switch is not None:
+        monkeypatch.setenv("TFCUDA_PDL", switch)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+        call()
+    raw, count = C.c_void_p(int(graph.raw_cuda_graph())), C.c_size_t(0)
+    edges = C.CDLL("libcuda.so.1").cuGraphGetEdges_v2
+    assert edges(raw, None, None, None, C.byref(count)) == 0 and count.value == 3  # four kernels in a row
+    ends, data = [(C.c_void_p * 3)() for _ in range(2)], (C.c_uint8 * 24)()  # data: 8 bytes an edge, the third its type
+    assert edges(raw, *ends, data, C.byref(count)) == 0
+    assert [data[8 * i + 2] for i in range(3)] == [0 if switch == "0" else 1] * 3
+    out.zero_()
+    graph.instantiate()
+    graph.replay()
+    torch.cuda.synchronize()
+    batch.check(out, lse)
