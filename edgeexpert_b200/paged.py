@@ -298,7 +298,7 @@ class PagedDecoder(Decoder):
         ones alone; a request whose tokens the list does not hold to the end is refused."""
         kv, n = self.kv, token_ids.numel()
         before = kv.seq_lens.clone()
-        asked = (targets - before).clamp_(min=0)
+        asked = torch.maximum(targets, before) - before
         ends = asked.cumsum(0)  # of the requests' tokens in the list
         kv.resize(torch.where((ends > n) & (asked > 0), 2 ** 31 - 1, targets), stream)
         first = ends - asked - before - kv.prefix_len  # + a token's position = its place in the list

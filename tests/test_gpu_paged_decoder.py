@@ -120,6 +120,11 @@ def test_lists_of_any_length_up_to_the_step(cuda, model):
             close(h[row], u.want[b][j])
         u.at = [o if n < 0 else n for o, n in zip(u.at, targets)]
         assert u.cache.seq_lens.tolist() == u.at
+    # any negative target leaves a request alone
+    u.dec.step(i32(u.tokens[0][:3]), i32([3, -1]))
+    u.dec.step(i32(u.tokens[1][:2]), torch.tensor([-2 ** 31, 2], dtype=torch.int32, device="cuda"))
+    assert u.cache.seq_lens.tolist() == [3, 2] and u.cache.free_state.tolist()[2:] == [0, 2]
+    u.dec.step(i32([]), i32([0, 0]))
     # a request whose tokens the short list does not hold is refused
     u.dec.step(i32(u.tokens[0][:3]), i32([2, 2]))
     assert u.cache.seq_lens.tolist() == [2, 0] and u.cache.free_state.tolist()[2:] == [1, 2]
