@@ -268,8 +268,10 @@ __device__ void resize_fill(const ResizeParams& p, int cta, int ctas) {
 }
 
 // Up to a thousand tokens one CTA plans and fills (a launch costs more than
-// the filling) and passes the plan in shared memory; beyond, the second kernel fills with the whole GPU and is
-// launched while the first still plans.
+// the filling: 8.7 us for 32 requests of which each grows by a token, 12.3 for 1000 with two
+// kernels) and passes the plan in shared memory; beyond, the second kernel fills with the whole GPU
+// and is launched while the first still plans.  The rule does not know how many pages come back: 256
+// requests of 250 pages that finish together take 119 us here and would take 14 with two kernels.
 __global__ void __launch_bounds__(kSmallRequests) resize_small_kernel(ResizeParams p) {
     __shared__ int plan[2 + 4 * kSmallRequests], starts[kSmallRequests + 1];
     p.plan = plan;

@@ -10,9 +10,9 @@
 //   attention_parts_kernel   all parts of all rows, one CTA per SM, two kinds of work
 //   join_parts_kernel        M, D, out and lse of every row that has more than one part
 // Measured with both (16 query / 8 KV heads of 256): 256 requests behind 4096
-// shared positions with 1 to 1001 of their own, 1.09 GB: 213 us, 5.1 TB/s; 32
-// behind 2048 with up to 2048, 286 MB: 69 us; 2 behind 317: 18 us (17 on the GPU:
-// launch, sums over the batch, one unit, join).
+// shared positions with 1 to 1001 of their own, 1.09 GB: 215 to 221 us by machine,
+// 5.0 TB/s; 32 behind 2048 with up to 2048, 286 MB: 70 us; 2 behind 317: 18 us (17
+// on the GPU: launch, sums over the batch, one unit, join).
 #include <math.h>
 
 #include "tf_prefix_stream.cuh"
@@ -222,7 +222,7 @@ __device__ __forceinline__ bool parts_exist(const Parts& p, int first_of, int la
 // row of a warp.  So as many CTAs as fit: 3 an SM with 32 registers of loads in
 // flight (58,000 rows of which a third have two parts, with the parts kernel: 205
 // us; 218 with 2 an SM and twice the loads; 229 without dropping finished rows
-// before the warps take theirs).
+// before the warps take theirs; by itself, cold, 29 us).
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, 3) join_parts_kernel(const __grid_constant__ AttnParams<T> p, int rows_per_cta) {
     __shared__ RowParts rows[kJoinRows];

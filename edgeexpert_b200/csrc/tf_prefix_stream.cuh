@@ -5,9 +5,9 @@
 // * rows operations.  Everything serves the stream of loads:
 //   * the units (16 keys of one request, KV head and row tile) are dealt evenly
 //     and contiguously to the warps, whatever the lengths.  A warp works for
-//     itself: its ring of K and V tiles is filled by its own cp.async and its
-//     loads run on across the jobs it covers, so no warp ever waits for another
-//     and one that begins or ends a job leaves the memory to the rest;
+//     itself: its ring of K and V tiles is filled by its own TMA loads, which run
+//     on across the jobs it covers, so no warp ever waits for another and one
+//     that begins or ends a job leaves the memory to the rest;
 //   * page ids are looked up one unit before their loads are issued;
 //   * scores are S^T = K Q^T and outputs O^T = V^T P^T: keys and dims fill the
 //     16-row side of mma.sync m16n8k16 and the few query rows its 8 columns, so
@@ -351,7 +351,8 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
                 s[nt][i + 2] = exp2_approx(s[nt][i + 2] - ref);
                 d[nt][i] = d[nt][i] * keep[nt][i] + (s[nt][i] + s[nt][i + 2]);
             }
-            // weights go to the tensor cores in the cache's type (their sum is of the unrounded ones)
+            // weights go to the tensor cores in the cache's type, which their product with V has to have;
+            // each is off by half an ulp of it, their sum is of the unrounded ones
             pf[nt][0] = transpose8x8(Pair<T>::pack(s[nt][0], s[nt][1]));
             pf[nt][1] = transpose8x8(Pair<T>::pack(s[nt][2], s[nt][3]));
         }

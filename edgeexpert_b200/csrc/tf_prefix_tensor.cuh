@@ -28,7 +28,10 @@
 // stream's; bringing tiles into L2 ten units ahead made it 1.9.
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
 // one its sums refer to: weights stay below 256, sums in fp32, and the quotient
-// at the end does not depend on the reference.
+// at the end does not depend on the reference.  P is rounded to the cache's type,
+// as the product with V needs it; d sums the unrounded weights.  With that the
+// results for prompts of N(0, 1) keys and values are off by 2.9e-4 (fp16, relative
+// to the largest) where fp32 weights and a rounded result give 2.1e-4.
 #pragma once
 #include "tf_prefix_attention.cuh"
 #include "tf_umma.cuh"

@@ -566,8 +566,13 @@ TF_API tf_status tf_rope_kv_write(tf_context* ctx, const void* q, uint64_t q_str
  * A row that sees nothing gives out 0 and lse -infinity; so do tokens before token_starts[0] and
  * from token_starts[B] up to T.
  * max_query: host bound on any n_b (tokens beyond it give 0 and the device error bit).  A page id
- * outside the pool is not read and raises the bit too; rows that see it are unspecified.  Positions that no row of the batch
- * (for the prefix) or of the request (for its own pages) sees may hold anything, NaN included.
+ * outside the pool is not read and raises the bit too; rows that see it are unspecified.
+ * Positions that no row of the batch (for the prefix) or of the request (for its own pages) sees may
+ * hold anything, NaN included; page ids before the first position that one sees may be anything too.
+ * Scores, sums and lse are fp32.  The weights exp(s - max) are rounded to the cache's type before
+ * they meet V, on top of the result's own rounding: relative 2^-11 (fp16) or 2^-8 (bf16) of
+ * sum p|v| / sum p at most, about a third more error in all (2.9e-4 and 2.2e-3 of the largest result,
+ * where fp32 weights give 2.1e-4 and 1.7e-3).  out must not overlap q.
  * scale > 0.  q, out 16-byte aligned, strides multiples of 8.  Any number of query heads per KV
  * head.  workspace: caller-owned device scratch, contents arbitrary, one per concurrent call. */
 TF_API size_t tf_shared_prefix_attention_workspace_bytes(const tf_context* ctx, const tf_paged_kv* kv,
