@@ -76,6 +76,13 @@ __device__ __noinline__ void attend_alone(const AttnParams<T>& p, int b, const R
 // share of the bandwidth (6450 / 148 bytes a nanosecond).  A tensor unit is 64
 // (head_dim 256) or 128 keys for 128 rows: 600 ns by itself, but beside the
 // stream its loads take their turn behind the others': 1700 measured, 2300 for 128 keys of 128.
+// Fits, not laws; halved / as they are / doubled (us, cold, with a graph's launch):
+//   256: 32 decodes behind 2048, 1-2047 own     111 /  84 /  78     128, 1-200   76 / 68 / 82 (behind 4096)
+//        256 behind 4096, 1-1000 own            359 / 244 / 248
+//   128: 101 behind 1500, 0-900 own              70 /  57 /  61     128, 1-200   45 / 55 / 70
+//        256 behind 4096, 1-1000 own            125 / 127 / 142
+//    64: 101 behind 1500, 0-900 own              47 /  41 /  43     128, 1-200   41 / 45 / 53
+//        256 behind 4096, 1-1000 own             76 /  78 /  86
 __host__ __device__ constexpr float few_unit_ns(int hd) { return 16.f * 4.f * hd / 43.6f; }
 __host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 128 ? 1700.f : (hd > 64 ? 2300.f : 900.f); }
 
@@ -120,7 +127,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     if (many) {
         const float m = many * many_unit_ns(HD);
         float f = few * few_unit_ns(HD);
-        if (f * 10.f < m) f *= 3.f;  // a small share: its warps wait for latencies, not for bandwidth
+        // a small share: its warps wait for latencies, not for bandwidth (256 decodes behind 4096 with
+        // 1 to 30 own positions, head_dim 64: 45 us, 59 without; other batches the same, also with six)
+        if (f * 10.f < m) f *= 3.f;
         many_ctas = few ? max(1, min(grid - 1, (int)(grid * (m / (m + f))))) : grid;
         many_ctas = min(many_ctas, many);
     }

@@ -311,10 +311,10 @@ class PagedDecoder(Decoder):
     def step(self, token_ids, targets, stream=None):
         """token_ids (up to T): the tokens to add, request after request, of every request that
         is to grow; targets: every request's length with them.  Both int32, on the device.  A
-        request that can't have its pages is refused and keeps its length; the others are as if
-        it had not asked.  Next tokens in self.tokens, row by row of the tokens added: row i is
-        position kv.positions[i] of request kv.requests[i], and kv.free_state tells how many
-        requests were refused."""
+        request that can't have its pages is refused and keeps its length (what it asked for
+        counts before later requests' pages all the same); the others get their own tokens.  Next
+        tokens in self.tokens, row by row of the tokens added: row i is position kv.positions[i]
+        of request kv.requests[i], and kv.free_state tells how many requests were refused."""
         kv = self.kv
         for t, what in ((token_ids, "token_ids"), (targets, "targets")):
             if t.dtype is not _I32 or t.dim() != 1 or t.device != self.ids.device:
