@@ -93,6 +93,16 @@ class PagedKVDesc(C.Structure):
                 ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("dtype", C.c_int)]
 
 
+class LogitRulesDesc(C.Structure):
+    """tf_logit_rules."""
+
+    _fields_ = [(n, C.c_void_p) for n in (
+        "history", "history_lens", "prompt_lens", "repetition", "presence", "frequency", "bias_starts", "bias_tokens",
+        "bias_values", "allowed", "allowed_rows", "token_ids", "ancestors")] + [
+        (n, C.c_uint64) for n in ("history_stride", "allowed_stride")] + [
+        (n, C.c_uint32) for n in ("max_history", "bias_count", "allowed_count", "words")]
+
+
 _P = C.c_void_p
 _U32 = C.c_uint32
 _U64 = C.c_uint64
@@ -163,6 +173,15 @@ _PROTOS = {
                                                    C.c_size_t),
     "tf_shared_prefix_attention": ([_P, _P, _U64, C.POINTER(PagedKVDesc), _P, _U32, _P, _U32, _P, _P, _U32, _U32, _U32,
                                     _U32, C.c_float, _U32, _P, _U64, _P, _P, C.c_size_t, _P], _I),
+    "tf_draft_tree_plan": ([_P, _P, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _U32, _P], _I),
+    "tf_tree_attention_workspace_bytes": ([_P, C.POINTER(PagedKVDesc), _U32, _U32, _U32, _U32, _U32], C.c_size_t),
+    "tf_tree_attention": ([_P, _P, _U64, C.POINTER(PagedKVDesc), _P, _U32, _P, _U32, _P, _P, _U32, _P, _U32, _P, _U32,
+                           _U32, _U32, C.c_float, _U32, _P, _U64, _P, _P, C.c_size_t, _P], _I),
+    "tf_logit_rules_workspace_bytes": ([_U32, _U32], C.c_size_t),
+    "tf_logit_rules_apply": ([_P, _P, _U64, _P, _U64, _I, _U32, _U32, _P, _U32, _U32, C.POINTER(LogitRulesDesc), _P, _P,
+                              C.c_size_t, _P], _I),
+    "tf_draft_accept": ([_P, _P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _P, _P, C.POINTER(PagedKVDesc), _U64,
+                         _U32, _P, _U32, _P], _I),
     "tf_ep_flag_bytes": ([_U32], C.c_size_t),
     "tf_ep_ipc_alloc": ([_P, C.c_size_t, C.POINTER(_P), _P], _I),
     "tf_ep_ipc_open": ([_P, _P, C.POINTER(_P)], _I),
@@ -274,3 +293,10 @@ def ptr(t) -> C.c_void_p:
 
 
 stream_ptr = _stream_ptr
+
+
+def on_device(what: str, device: int, *tensors) -> None:
+    """Refuses tensors (None: left out) that are not on `device`: a kernel there cannot read them."""
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise TFError(TF_ERR_INVALID_ARG, f"{what}: a tensor on {t.device}, the context is on cuda:{device}")

@@ -1,4 +1,5 @@
-// tf_prefix_attention.cuh -- what the kernels of tf_shared_prefix_attention share:
+// tf_prefix_attention.cuh -- what the kernels of tf_shared_prefix_attention and (kTree)
+// tf_tree_attention share:
 // parameters, which rows see which keys, how work is dealt to CTAs, and where
 // the parts of a row's softmax are kept until they are joined.
 #pragma once
@@ -39,7 +40,9 @@ struct KvMaps {
     CUtensorMap k, v, v_row;
 };
 
-template <typename T>
+// kTree: a request's query tokens are the nodes of a drafted tree.  Each sees the history before
+// the nodes (hi of seen_by ends there) and those of the nodes whose bit is set in its ancestors.
+template <typename T, bool kTree>
 struct AttnParams {
     const T* q;
     long long q_stride;
@@ -51,6 +54,9 @@ struct AttnParams {
     T* out;
     long long out_stride;
     float* lse;
+    const uint32_t* ancestors;  // kTree: [tokens][words]
+    const int* positions;       // kTree, with a window: where the nodes stand
+    int words;
     uint32_t* err;
     int* prefix_first;  // the first prefix position that any row sees, for the joining kernel (calls with a window)
     int prefix_len, max_pages, B, max_query, T_tokens, nq, nkv, G, hd, window;
@@ -66,8 +72,8 @@ struct AttnParams {
 };
 
 // Row -> token of a job's rows (token * G + head in the group).
-template <typename T>
-__device__ __forceinline__ int token_of(const AttnParams<T>& p, int row) {
+template <typename T, bool kTree>
+__device__ __forceinline__ int token_of(const AttnParams<T, kTree>& p, int row) {
     return p.g_shift >= 0 ? row >> p.g_shift : row / p.G;
 }
 
@@ -76,8 +82,8 @@ struct Request {
     int start, n, used, len;  // first token, tokens, tokens within max_query, own positions
 };
 
-template <typename T>
-__device__ __forceinline__ Request request_of(const AttnParams<T>& p, int b) {
+template <typename T, bool kTree>
+__device__ __forceinline__ Request request_of(const AttnParams<T, kTree>& p, int b) {
     Request r;
     const int s0 = max(0, min(p.starts[b], p.T_tokens)), s1 = max(s0, min(p.starts[b + 1], p.T_tokens));
     r.start = s0;
@@ -93,8 +99,8 @@ __device__ __forceinline__ Request request_of(const AttnParams<T>& p, int b) {
 
 // The last b with starts[b] <= t; B for tokens behind the last request, and 0 for those before
 // the first one too (whose token index is negative then).
-template <typename T>
-__device__ __noinline__ int request_at(const AttnParams<T>& p, int t) {
+template <typename T, bool kTree>
+__device__ __noinline__ int request_at(const AttnParams<T, kTree>& p, int t) {
     int lo = 0, hi = p.B;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -110,11 +116,28 @@ __device__ __noinline__ int request_at(const AttnParams<T>& p, int t) {
 __device__ __forceinline__ bool is_used(const Request& r, int j) { return j >= 0 && j < r.used; }
 
 // Keys [lo, hi) that token j of request r sees, as positions of the whole sequence.
-template <typename T>
-__device__ __forceinline__ void seen_by(const AttnParams<T>& p, const Request& r, int j, int& lo, int& hi) {
-    const int at = p.prefix_len + r.len - (r.n - j);
-    hi = at + 1;
-    lo = p.window ? max(0, at - p.window + 1) : 0;
+template <typename T, bool kTree>
+__device__ __forceinline__ void seen_by(const AttnParams<T, kTree>& p, const Request& r, int j, int& lo, int& hi) {
+    if constexpr (kTree) {
+        hi = p.prefix_len + max(0, r.len - r.n);
+        lo = p.window ? max(0, max(hi, p.positions[r.start + j]) - p.window + 1) : 0;
+    } else {
+        const int at = p.prefix_len + r.len - (r.n - j);
+        hi = at + 1;
+        lo = p.window ? max(0, at - p.window + 1) : 0;
+    }
+}
+// The first key that any token of the request sees (nodes stand behind the history).
+template <typename T, bool kTree>
+__device__ __forceinline__ int seen_from(const AttnParams<T, kTree>& p, const Request& r) {
+    if constexpr (kTree) return p.window ? max(0, p.prefix_len + max(0, r.len - r.n) - p.window + 1) : 0;
+    int lo, hi;
+    seen_by(p, r, 0, lo, hi);
+    return lo;
+}
+// kTree: whether the token with these ancestors sees a node (of its own request).
+__device__ __forceinline__ bool sees_node(const uint32_t* ancestors, int words, int node) {
+    return node >= 0 && node < words * 32 && (ancestors[node >> 5] >> (node & 31) & 1u);
 }
 
 // The first prefix position that any row of the batch sees, as the parts kernel keeps it: positions
@@ -123,27 +146,25 @@ __device__ __forceinline__ int& shared_prefix_first() {
     __shared__ int first;
     return first;
 }
-template <typename T>
-__device__ __forceinline__ int prefix_first(const AttnParams<T>& p) {
+template <typename T, bool kTree>
+__device__ __forceinline__ int prefix_first(const AttnParams<T, kTree>& p) {
     return p.window ? shared_prefix_first() : 0;
 }
 // Tiles of `keys` keys that hold the prefix from there on.
-template <typename T>
-__device__ __forceinline__ int prefix_tiles(const AttnParams<T>& p, int keys) {
+template <typename T, bool kTree>
+__device__ __forceinline__ int prefix_tiles(const AttnParams<T, kTree>& p, int keys) {
     const int first = prefix_first(p);
     return p.prefix_len > first ? (p.prefix_len - (first & ~(kMaxRun - 1)) + keys - 1) / keys : 0;
 }
 
 // First of a request's own positions that any of its rows sees.
-template <typename T>
-__device__ __forceinline__ int own_lo(const AttnParams<T>& p, const Request& r) {
-    int lo, hi;
-    seen_by(p, r, 0, lo, hi);
-    return max(0, min(r.len, lo - p.prefix_len));
+template <typename T, bool kTree>
+__device__ __forceinline__ int own_lo(const AttnParams<T, kTree>& p, const Request& r) {
+    return max(0, min(r.len, seen_from(p, r) - p.prefix_len));
 }
 
-template <typename T>
-__device__ __forceinline__ bool is_many(const AttnParams<T>& p, const Request& r) {
+template <typename T, bool kTree>
+__device__ __forceinline__ bool is_many(const AttnParams<T, kTree>& p, const Request& r) {
     return r.used * p.G > p.many_above;
 }
 
@@ -249,8 +270,8 @@ struct TileKeys {
     int page[kMost], in_page[kMost], have[kMost];
 };
 
-template <int HD, int KEYS, typename T>
-__device__ __forceinline__ void load_tile_keys(const AttnParams<T>& p, bool v, uint32_t tile, int head,
+template <int HD, int KEYS, typename T, bool kTree>
+__device__ __forceinline__ void load_tile_keys(const AttnParams<T, kTree>& p, bool v, uint32_t tile, int head,
                                                const TileKeys<KEYS>& k, uint64_t* bar, bool once) {
     constexpr int kBlocks = HD / 64, kMost = TileKeys<KEYS>::kMost;
     const CUtensorMap* map = v ? &p.maps.v : &p.maps.k;
@@ -296,8 +317,8 @@ __device__ __forceinline__ void load_tile_keys(const AttnParams<T>& p, bool v, u
 
 // The runs of the tile of keys that begins at position `pos0` of a segment
 // whose keys are [from, hi).
-template <int KEYS, typename T>
-__device__ __forceinline__ TileKeys<KEYS> look_up_keys(const AttnParams<T>& p, int seg, int pos0, int from, int hi) {
+template <int KEYS, typename T, bool kTree>
+__device__ __forceinline__ TileKeys<KEYS> look_up_keys(const AttnParams<T, kTree>& p, int seg, int pos0, int from, int hi) {
     TileKeys<KEYS> k;
     const int lane = threadIdx.x & 31, run = 1 << p.run_shift, runs = KEYS >> p.run_shift;
 #pragma unroll
@@ -315,8 +336,8 @@ __device__ __forceinline__ TileKeys<KEYS> look_up_keys(const AttnParams<T>& p, i
     return k;
 }
 // Once the page ids are there: those outside the pool are reported and not read.
-template <int KEYS, typename T>
-__device__ __forceinline__ void check_keys(const AttnParams<T>& p, TileKeys<KEYS>& k) {
+template <int KEYS, typename T, bool kTree>
+__device__ __forceinline__ void check_keys(const AttnParams<T, kTree>& p, TileKeys<KEYS>& k) {
 #pragma unroll
     for (int i = 0; i < TileKeys<KEYS>::kMost; ++i) {
         asm volatile("" : "+r"(k.page[i]));  // not earlier: the id is waited for here

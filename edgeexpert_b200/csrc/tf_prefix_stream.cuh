@@ -83,13 +83,13 @@ struct StreamCursor {
 };
 
 // Rows that have the prefix here.
-template <typename T>
-__device__ __forceinline__ int stream_prefix_rows(const AttnParams<T>& p) {
+template <typename T, bool kTree>
+__device__ __forceinline__ int stream_prefix_rows(const AttnParams<T, kTree>& p) {
     return p.prefix_few ? max(0, min(p.starts[p.B], p.T_tokens)) * p.G : 0;
 }
 
-template <typename T, int HD, int NT>
-__device__ __forceinline__ void stream_segment(const AttnParams<T>& p, StreamCursor& c) {
+template <typename T, int HD, int NT, bool kTree>
+__device__ __forceinline__ void stream_segment(const AttnParams<T, kTree>& p, StreamCursor& c) {
     using S = StreamShape<HD, NT>;
     if (c.seg < 0) {
         const int rows = stream_prefix_rows(p);
@@ -107,8 +107,8 @@ __device__ __forceinline__ void stream_segment(const AttnParams<T>& p, StreamCur
 }
 
 // The first unit of the next job.
-template <typename T, int HD, int NT>
-__device__ __noinline__ StreamCursor stream_next_job(const AttnParams<T>& p, StreamCursor c) {
+template <typename T, int HD, int NT, bool kTree>
+__device__ __noinline__ StreamCursor stream_next_job(const AttnParams<T, kTree>& p, StreamCursor c) {
     c.tile = 0;
     if (++c.rt < c.row_tiles) return c;
     c.rt = 0;
@@ -121,15 +121,15 @@ __device__ __noinline__ StreamCursor stream_next_job(const AttnParams<T>& p, Str
     } while (c.tiles == 0);
     return c;
 }
-template <typename T, int HD, int NT>
-__device__ __forceinline__ void stream_advance(const AttnParams<T>& p, StreamCursor& c) {
+template <typename T, int HD, int NT, bool kTree>
+__device__ __forceinline__ void stream_advance(const AttnParams<T, kTree>& p, StreamCursor& c) {
     if (++c.tile >= c.tiles) c = stream_next_job<T, HD, NT>(p, c);
 }
 
 // The units of the whole batch; `before` those of the requests before this
 // thread's own [b0, b1).  With a window also the first prefix position that any row sees.
-template <typename T, int HD, int NT>
-__device__ __forceinline__ int stream_units(const AttnParams<T>& p, int* red, int b0, int b1, int& before) {
+template <typename T, int HD, int NT, bool kTree>
+__device__ __forceinline__ int stream_units(const AttnParams<T, kTree>& p, int* red, int b0, int b1, int& before) {
     using S = StreamShape<HD, NT>;
     if (p.window) {
         if (threadIdx.x == 0) shared_prefix_first() = p.prefix_len;
@@ -143,9 +143,7 @@ __device__ __forceinline__ int stream_units(const AttnParams<T>& p, int* red, in
         sum += c.row_tiles * c.tiles * p.nkv;
         if (p.window) {
             const Request r = request_of(p, c.seg);
-            int lo = first, hi;
-            if (r.used) seen_by(p, r, 0, lo, hi);
-            first = min(first, lo);
+            if (r.used) first = min(first, seen_from(p, r));
         }
     }
     if (p.window && first < p.prefix_len) atomicMin(&shared_prefix_first(), first);
@@ -156,8 +154,8 @@ __device__ __forceinline__ int stream_units(const AttnParams<T>& p, int* red, in
 }
 
 // One warp: units [u0, u1) beginning at `cur`, as worker `worker`.
-template <typename T, int HD, int NT>
-__device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t ring, uint64_t* full, StreamCursor cur,
+template <typename T, int HD, int NT, bool kTree>
+__device__ __forceinline__ void stream_warp(const AttnParams<T, kTree>& p, uint32_t ring, uint64_t* full, StreamCursor cur,
                                             int u0, int u1, int worker) {
     using S = StreamShape<HD, NT>;
     constexpr int kRows = S::kRows, R = S::kTiles, kGroup8 = HD / 64 * 1024;  // bytes of eight keys
@@ -208,6 +206,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
     // ---- the job's rows -----------------------------------------------------------
     uint32_t qf[HD / 16][NT][2];
     int row_lo[NT][2], row_hi[NT][2];
+    int row_bits[NT][2], node0 = 0x7FFFFFFF;  // kTree: where the rows' ancestors are, the first node's key
     float m[NT][2], d[NT][2], acc[HD / 16][NT][4];
     const float sc = p.scale * kLog2e;
     int job_rows = 0, first_token = 0;
@@ -222,6 +221,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
             job_rows = r.used * p.G;
             first_token = r.start;
         }
+        if constexpr (kTree) node0 = prefix ? 0x7FFFFFFF : r.len - r.n;
         const int row0 = cur.rt * kRows;
         job_rows -= row0;
 #pragma unroll
@@ -241,6 +241,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
             for (int i = 0; i < 2; ++i) {  // rows whose scores it holds
                 const int rs = row0 + nt * 8 + 2 * tq + i;
                 int lo = 0, hi = 0;
+                if constexpr (kTree) row_bits[nt][i] = -1;
                 if (nt * 8 + 2 * tq + i < job_rows) {
                     const int j = token_of(p, rs);
                     if (prefix) {
@@ -253,6 +254,7 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
                         seen_by(p, r, j, lo, hi);
                         lo -= p.prefix_len;
                         hi -= p.prefix_len;
+                        if constexpr (kTree) row_bits[nt][i] = (r.start + j) * p.words;
                     }
                 }
                 row_lo[nt][i] = lo;
@@ -334,7 +336,10 @@ __device__ __forceinline__ void stream_warp(const AttnParams<T>& p, uint32_t rin
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = key0 + g + 8 * (i >> 1);
-                const bool ok = key >= row_lo[nt][i & 1] && key < row_hi[nt][i & 1];
+                bool ok = key >= row_lo[nt][i & 1] && key < row_hi[nt][i & 1];
+                if constexpr (kTree)
+                    if (key >= node0 && key < cur.hi && row_bits[nt][i & 1] >= 0)
+                        ok = sees_node(p.ancestors + row_bits[nt][i & 1], p.words, key - node0);
                 s[nt][i] = ok ? (s[nt][i] + s2[nt][i]) * sc : -INFINITY;
             }
 #pragma unroll

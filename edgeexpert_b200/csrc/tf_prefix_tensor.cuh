@@ -120,15 +120,15 @@ struct TensorCursor {
 };
 
 // Requests of row tile i: [first, last], first > last when it has no tokens.
-template <typename T>
-__device__ __forceinline__ void requests_of_tile(const AttnParams<T>& p, int i, int& first, int& last) {
+template <typename T, bool kTree>
+__device__ __forceinline__ void requests_of_tile(const AttnParams<T, kTree>& p, int i, int& first, int& last) {
     const long long rows = (long long)p.T_tokens * p.G, row0 = (long long)i * kTcRows;
     first = request_at(p, (int)(row0 / p.G));
     last = min(p.B - 1, request_at(p, (int)((min(rows, row0 + kTcRows) - 1) / p.G)));
 }
 
-template <typename T, int HD>
-__device__ __forceinline__ void tensor_segment(const AttnParams<T>& p, int i, TensorCursor& c) {
+template <typename T, int HD, bool kTree>
+__device__ __forceinline__ void tensor_segment(const AttnParams<T, kTree>& p, int i, TensorCursor& c) {
     c.tile = 0;
     if (c.seg < 0) {
         c.from = prefix_first(p);
@@ -136,7 +136,10 @@ __device__ __forceinline__ void tensor_segment(const AttnParams<T>& p, int i, Te
     } else {
         const Request r = request_of(p, c.seg);
         c.from = c.hi = 0;
-        if (is_many(p, r)) {
+        if constexpr (kTree) {
+            c.from = own_lo(p, r);
+            c.hi = r.len;
+        } else if (is_many(p, r)) {
             // its tokens in the tile, and what they see of its own keys
             const int j0 = max(0, (int)((long long)i * kTcRows / p.G) - r.start);
             const int j1 = min(r.used, (int)((((long long)i + 1) * kTcRows - 1) / p.G) + 1 - r.start);
@@ -153,9 +156,13 @@ __device__ __forceinline__ void tensor_segment(const AttnParams<T>& p, int i, Te
     c.tiles = c.hi > c.from ? (c.hi - c.lo + TensorShape<HD>::kKeys - 1) / TensorShape<HD>::kKeys : 0;
 }
 
+// kTree: a job's keys are one segment, the prefix for the rows of the whole batch or a request's
+// own for its own rows (seg, see TreeJobs); trees are small, so tiles across requests would read
+// the keys of all of them for every row.
+//
 // First segment with keys of row tile i at or behind c.seg; false if none.
-template <typename T, int HD>
-__device__ __forceinline__ bool tensor_seek(const AttnParams<T>& p, int i, TensorCursor& c) {
+template <typename T, int HD, bool kTree>
+__device__ __forceinline__ bool tensor_seek(const AttnParams<T, kTree>& p, int i, TensorCursor& c) {
     for (;;) {
         if (c.seg > c.last || (c.seg >= 0 && p.max_query * p.G <= p.many_above)) return false;
         tensor_segment<T, HD>(p, i, c);
@@ -170,8 +177,8 @@ __device__ __forceinline__ bool tensor_seek(const AttnParams<T>& p, int i, Tenso
     }
 }
 // The first unit of the next segment.
-template <typename T, int HD>
-__device__ __noinline__ TensorCursor tensor_next_segment(const AttnParams<T>& p, int i, TensorCursor c) {
+template <typename T, int HD, bool kTree>
+__device__ __noinline__ TensorCursor tensor_next_segment(const AttnParams<T, kTree>& p, int i, TensorCursor c) {
     if (c.seg < 0) {
         int first, last;
         requests_of_tile(p, i, first, last);
@@ -182,14 +189,20 @@ __device__ __noinline__ TensorCursor tensor_next_segment(const AttnParams<T>& p,
     tensor_seek<T, HD>(p, i, c);
     return c;
 }
-template <typename T, int HD>
-__device__ __forceinline__ void tensor_advance(const AttnParams<T>& p, int i, TensorCursor& c) {
-    if (++c.tile >= c.tiles) c = tensor_next_segment<T, HD>(p, i, c);
+template <typename T, int HD, bool kTree>
+__device__ __forceinline__ void tensor_advance(const AttnParams<T, kTree>& p, int i, TensorCursor& c) {
+    if (++c.tile >= c.tiles && !kTree) c = tensor_next_segment<T, HD>(p, i, c);
 }
-// The cursor at the `skip`-th unit of row tile i.
-template <typename T, int HD>
-__device__ __noinline__ TensorCursor tensor_begin(const AttnParams<T>& p, int i, int skip) {
+// The cursor at the `skip`-th unit of row tile i (kTree: of segment seg).
+template <typename T, int HD, bool kTree>
+__device__ __noinline__ TensorCursor tensor_begin(const AttnParams<T, kTree>& p, int i, int skip, int seg) {
     TensorCursor c;
+    if constexpr (kTree) {
+        c.seg = c.last = seg;
+        tensor_segment<T, HD>(p, i, c);
+        c.tile = skip;
+        return c;
+    }
     int first;
     requests_of_tile(p, i, first, c.last);
     c.seg = -1;
@@ -200,8 +213,8 @@ __device__ __noinline__ TensorCursor tensor_begin(const AttnParams<T>& p, int i,
     c.tile = skip;
     return c;
 }
-template <typename T, int HD>
-__device__ __noinline__ int tensor_units(const AttnParams<T>& p, int i) {
+template <typename T, int HD, bool kTree>
+__device__ __noinline__ int tensor_units(const AttnParams<T, kTree>& p, int i) {
     if (p.max_query * p.G <= p.many_above) {  // the prefix alone, for any tile with a token of the batch
         return (int)((long long)i * kTcRows / p.G) < p.starts[p.B] ? prefix_tiles(p, TensorShape<HD>::kKeys) : 0;
     }
@@ -217,9 +230,48 @@ __device__ __noinline__ int tensor_units(const AttnParams<T>& p, int i) {
     return units;
 }
 
+// kTree: the row tiles of segment seg that are the tensor cores', and the units of each.
+struct TreeSegment {
+    int row_tiles, units;
+};
+template <typename T, int HD, bool kTree>
+__device__ __noinline__ TreeSegment tree_segment(const AttnParams<T, kTree>& p, int seg) {
+    TreeSegment s{0, 0};
+    int rows;
+    if (seg < 0) {
+        rows = p.prefix_few ? 0 : max(0, min(p.starts[p.B], p.T_tokens)) * p.G;
+    } else {
+        const Request r = request_of(p, seg);
+        rows = is_many(p, r) ? r.used * p.G : 0;
+    }
+    if (rows == 0) return s;
+    TensorCursor c;
+    c.seg = seg;
+    tensor_segment<T, HD>(p, 0, c);
+    s.units = c.tiles;
+    s.row_tiles = s.units ? (rows + kTcRows - 1) / kTcRows : 0;
+    return s;
+}
+
+// kTree: the units of the prefix and of all requests; `before` those before this thread's own
+// requests [b0, b1).
+template <typename T, int HD, bool kTree>
+__device__ __forceinline__ int all_tree_units(const AttnParams<T, kTree>& p, int* red, int b0, int b1, int& before) {
+    int sum = 0, total;
+    for (int b = b0; b < b1; ++b) {
+        const TreeSegment s = tree_segment<T, HD>(p, b);
+        sum += s.row_tiles * s.units * p.nkv;
+    }
+    before = block_scan(sum, red, &total);
+    const TreeSegment s = tree_segment<T, HD>(p, -1);
+    const int prefix = s.row_tiles * s.units * p.nkv;
+    before += prefix;
+    return prefix + total;
+}
+
 // The units of all row tiles; `before` those before this thread's own [i0, i1).
-template <typename T, int HD>
-__device__ __forceinline__ int all_tensor_units(const AttnParams<T>& p, int* red, int i0, int i1, int& before) {
+template <typename T, int HD, bool kTree>
+__device__ __forceinline__ int all_tensor_units(const AttnParams<T, kTree>& p, int* red, int i0, int i1, int& before) {
     int sum = 0, total;
     for (int i = i0; i < i1; ++i) sum += tensor_units<T, HD>(p, i) * p.nkv;
     before = block_scan(sum, red, &total);
@@ -234,9 +286,10 @@ struct TensorBarriers {
 };
 
 // One CTA: units [u0, u1) of worker `worker`; the first is in row tile `tile`,
-// which begins at unit `tile_at` and has `tile_units` units a KV head.
-template <typename T, int HD>
-__device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring, TensorBarriers& bar, int u0, int u1,
+// which begins at unit `tile_at` and has `tile_units` units a KV head (kTree:
+// in segment `tile`, whose row tiles have `tile_units` units each).
+template <typename T, int HD, bool kTree>
+__device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32_t ring, TensorBarriers& bar, int u0, int u1,
                                            int tile0, int tile_at, int tile_units, int worker) {
     using S = TensorShape<HD>;
     constexpr int N = S::kKeys;
@@ -284,10 +337,23 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
     // Every role walks the CTA's jobs: (row tile, KV head, units [from, to) of `units`).
     struct Job {
         int tile, kvh, units, from, to;
+        int seg, row_tiles;  // kTree: tile is one of the segment's row tiles
     };
     auto first_job = [&]() {
         Job j;
         const int in = u0 - tile_at;
+        if constexpr (kTree) {
+            j.seg = tile0;
+            j.row_tiles = tree_segment<T, HD>(p, j.seg).row_tiles;
+            j.units = tile_units;
+            const int q = in / j.units;
+            j.from = in % j.units;
+            j.to = min(j.units, j.from + u1 - u0);
+            j.tile = j.seg < 0 ? q / p.nkv : q % j.row_tiles;
+            j.kvh = j.seg < 0 ? q % p.nkv : q / j.row_tiles;
+            return j;
+        }
+        j.seg = -1;
         j.tile = tile0;
         j.units = tile_units;
         j.kvh = in / j.units;
@@ -297,7 +363,22 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
     };
     auto next_job = [&](Job& j, int u) {  // u: units done
         j.from = 0;
-        if (++j.kvh == p.nkv) {
+        if constexpr (kTree) {
+            // a request's row tiles read the same keys one after the other; the prefix's KV heads
+            // the same rows
+            if (j.seg < 0 ? ++j.kvh < p.nkv : ++j.tile < j.row_tiles) {
+            } else if (j.seg < 0 ? ++j.tile < j.row_tiles : ++j.kvh < p.nkv) {
+                (j.seg < 0 ? j.kvh : j.tile) = 0;
+            } else {
+                TreeSegment s;
+                do {
+                    s = tree_segment<T, HD>(p, ++j.seg);
+                } while (s.units == 0);
+                j.units = s.units;
+                j.row_tiles = s.row_tiles;
+                j.kvh = j.tile = 0;
+            }
+        } else if (++j.kvh == p.nkv) {
             j.kvh = 0;
             do {
                 j.units = tensor_units<T, HD>(p, ++j.tile);
@@ -315,7 +396,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
         bool ok = true;
         Job job = first_job();
         for (int u = u0; ok && u < u1;) {
-            TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from);
+            TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from, job.seg);
             TileKeys<N> next = look_up_keys<N>(p, c.seg, c.lo + c.tile * N, c.from, c.hi);
             for (int x = job.from; ok && x < job.to; ++x, ++it) {
                 TileKeys<N> now = next;
@@ -426,16 +507,25 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
         Job job = first_job();
         for (int u = u0; ok && u < u1;) {
             const long long row = (long long)job.tile * kTcRows + threadIdx.x;
-            const bool exists = row < (long long)p.T_tokens * p.G;
-            const int t = exists ? (int)(row / p.G) : 0, h = job.kvh * p.G + (int)(row % p.G);
-            int b = p.B, row_lo = 0, row_hi = 0;
-            bool own = false;  // its own keys are this kernel's too
-            if (exists) b = request_at(p, t);
+            bool exists = row < (long long)p.T_tokens * p.G;
+            int t = exists ? (int)(row / p.G) : 0;
+            const int h = job.kvh * p.G + (int)(row % p.G);
+            int b = p.B, row_lo = 0, row_hi = 0, node0 = 0x7FFFFFFF;
+            bool own = false;  // its own keys are this kernel's too (kTree: are the job's)
+            if (kTree && job.seg >= 0) {
+                const Request r = request_of(p, job.seg);
+                exists = row < (long long)r.used * p.G;
+                t = exists ? r.start + (int)(row / p.G) : 0;
+                node0 = r.len - r.n;
+                if (exists) b = job.seg;
+            } else if (exists) {
+                b = request_at(p, t);
+            }
             if (b < p.B) {
                 const Request r = request_of(p, b);
                 if (is_used(r, t - r.start)) {
                     seen_by(p, r, t - r.start, row_lo, row_hi);
-                    own = is_many(p, r);
+                    own = kTree ? job.seg >= 0 : is_many(p, r);
                 } else {
                     b = p.B;
                 }
@@ -462,7 +552,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                 mbar_arrive(&bar.q_full);
             }
             float m = -INFINITY, d = 0.f;
-            TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from);
+            TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from, job.seg);
             for (int x = job.from; x < job.to; ++x, ++uc) {
                 const int buf = uc & 1;
                 ok = wait_warp(&bar.s_full[buf], (uc >> 1) & 1);
@@ -479,13 +569,33 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                 lo = max(0, lo - key0);
                 hi = min(min(hi, c.hi) - key0, N);
                 float s[N];
-                if (__any_sync(0xffffffffu, hi > lo)) {
+                uint32_t nodes[N / 32];  // kTree: of the tile's keys, the nodes that the row sees
+                bool any_node = false;
+                if constexpr (kTree) {
+#pragma unroll
+                    for (int w = 0; w < N / 32; ++w) nodes[w] = 0u;
+                    if (c.seg >= 0 && key0 + N > node0 && live) {
+                        const uint32_t* bits = p.ancestors + (long long)t * p.words;
+#pragma unroll
+                        for (int w = 0; w < N / 32; ++w) {
+                            // 32 bits from node `at` on; what lies before node 0 or behind the words is not set
+                            const int at = key0 + 32 * w - node0, word = at >> 5, end = c.hi - key0 - 32 * w;
+                            const uint32_t a = word >= 0 && word < p.words ? bits[word] : 0u;
+                            const uint32_t z = word >= -1 && word + 1 < p.words ? bits[word + 1] : 0u;
+                            nodes[w] = __funnelshift_r(a, z, at & 31);
+                            if (end < 32) nodes[w] &= end > 0 ? (1u << end) - 1u : 0u;
+                            any_node |= nodes[w] != 0u;
+                        }
+                    }
+                }
+                if (__any_sync(0xffffffffu, hi > lo || any_node)) {
 #pragma unroll
                     for (int i = 0; i < N; i += 32) tmem_ld32_async(scol + i, s + i);
                     tmem_ld_wait(s);
                     if (!__all_sync(0xffffffffu, lo == 0 && hi == N)) {
 #pragma unroll
-                        for (int i = 0; i < N; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
+                        for (int i = 0; i < N; ++i)
+                            s[i] = (i >= lo && i < hi) || (kTree && (nodes[i / 32] >> (i & 31) & 1u)) ? s[i] : -INFINITY;
                     }
                     float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -544,10 +654,11 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
             if (!ok) break;
             tc_fence_after();
             const bool whole = job.from == 0 && job.to == job.units;
-            const bool final = whole && own;
+            const Parts& to = kTree && own ? p.few : p.many;  // (kTree: of the prefix in many)
+            const bool final = whole && own && !(kTree && p.prefix_len > prefix_first(p));
             const long long of = (long long)t * p.nq + h;
             const long long at = job.from == 0 ? of : (long long)worker * kTcRows + threadIdx.x;
-            float* po = (job.from == 0 ? p.many.first : p.many.cont) + at * p.hd;
+            float* po = (job.from == 0 ? to.first : p.many.cont) + at * p.hd;
             const float inv = d == 0.f ? 0.f : 1.f / d;
             bool fine = isfinite(d);
 #pragma unroll
@@ -577,14 +688,14 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T>& p, uint32_t ring
                 }
             }
             if (live) {
-                if (job.from == 0) p.many.first_of[of] = worker * kTcRows + threadIdx.x;
-                if (job.to == job.units) p.many.last_of[of] = worker;
+                if (job.from == 0) to.first_of[of] = worker * kTcRows + threadIdx.x;
+                if (job.to == job.units) to.last_of[of] = worker;
                 if (final) {
                     if (p.lse) p.lse[at] = d == 0.f ? -INFINITY : (m + log2f(d)) * kLn2;
                     // NaN here asks the joining kernel to compute the row by itself
-                    p.many.first_md[at] = make_float2(fine ? 0.f : __int_as_float(0x7fffffff), 0.f);
+                    to.first_md[at] = make_float2(fine ? 0.f : __int_as_float(0x7fffffff), 0.f);
                 } else {
-                    (job.from == 0 ? p.many.first_md : p.many.cont_md)[at] = make_float2(m, d);
+                    (job.from == 0 ? to.first_md : p.many.cont_md)[at] = make_float2(m, d);
                 }
             }
             tc_fence_before();

@@ -66,6 +66,17 @@ class PagedKV:
         self.ref = C.byref(self.desc)
 
 
+class PagedKVLayers:
+    """The pools of all layers, [layer][page][position][head][dim]: `layer[i]` is layer i's PagedKV."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride():
+            raise TFError(TF_ERR_INVALID_ARG, "k and v must be alike: [layer][page][position][head][dim]")
+        self.layer = [PagedKV(k[i], v[i]) for i in range(k.shape[0])]
+        self.layers, self.layer_stride = k.shape[0], k.stride(0)
+        self.k, self.v, self.ref = k, v, self.layer[0].ref if self.layer else None
+
+
 class KVPages:
     """The page tables of a ragged batch (tf_kv_pages_resize)."""
 
@@ -217,7 +228,8 @@ class PagedKVCache:
 
         shape = (layers, num_pages, page_size, num_kv_heads, head_dim)
         self.k, self.v = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
-        self.layer = [PagedKV(self.k[i], self.v[i]) for i in range(layers)]
+        self.layers = PagedKVLayers(self.k, self.v)
+        self.layer = self.layers.layer
         self.page_size, self.num_requests, self.max_tokens = page_size, num_requests, max_tokens
         self.seq_lens, self.page_table = i32(num_requests), i32(num_requests, max_pages, fill=-1)
         self.free_ring = torch.arange(num_pages, dtype=_I32, device=device)

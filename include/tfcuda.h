@@ -478,7 +478,8 @@ TF_API tf_status tf_sample_topk64(tf_context* ctx, const void* probs, uint32_t V
  *   tf_shared_prefix_attention   (per layer) attention over the shared prefix, read once for
  *                                the whole batch, and each request's own pages
  * Lengths, page tables, slots and positions are int32 on the device; nothing is read back. */
-typedef enum { TF_DTYPE_F16 = 0, TF_DTYPE_BF16 = 1 } tf_dtype;
+/* (TF_DTYPE_F32: logits only) */
+typedef enum { TF_DTYPE_F16 = 0, TF_DTYPE_BF16 = 1, TF_DTYPE_F32 = 2 } tf_dtype;
 
 /* A pool of `num_pages` pages of `page_size` positions.  Element (page p, position i, KV head
  * h, dim e) of K is k[p*page_stride + i*position_stride + h*head_stride + e], strides in
@@ -585,6 +586,121 @@ TF_API tf_status tf_shared_prefix_attention(tf_context* ctx, const void* q, uint
                                             uint32_t num_q_heads, float scale, uint32_t window, void* out,
                                             uint64_t out_stride, void* lse, void* workspace, size_t workspace_bytes,
                                             void* stream);
+
+/* ---- drafted trees in a ragged batch -----------------------------------------------------------
+ * No reference counterpart (the reference decodes one token at a time).  A step checks, for each
+ * request, a tree of tokens that a drafter guessed: its nodes are the request's tokens of the step,
+ * every node behind its parent, node 0 (the token chosen last) the root.  A step is
+ *   tf_kv_pages_resize     pages and slots for all nodes, as for any tokens
+ *   tf_draft_tree_plan     parents -> positions (of the way down to a node) and ancestor bits
+ *   tf_rope_kv_write       (per layer) with those positions
+ *   tf_tree_attention      (per layer) every node sees the history and its ancestors
+ *   tf_logit_rules_apply   penalties, biases and grammar masks for every node, and its choice
+ *   tf_draft_accept        down each tree along the choices; K and V of the kept nodes move behind
+ *                          the history, and targets are what tf_kv_pages_resize shrinks to
+ * A plain token, or a prompt, is a chain.  Trees have up to 256 nodes. */
+
+/* parents (int32[T]): of token token_starts[b] + j, the index of its parent among the request's
+ * nodes (below j), or -1: a root.  Outputs:
+ *   positions[t] = position_base + seq_lens[b] - n_b + depth (a root's is 0; seq_lens counts the nodes)
+ *   ancestors (uint32[T][words]): bit i (word i / 32, from the lowest) = node i of the request is t's
+ *     own or on the way from the root to it.
+ * words * 32 >= max_query, the host's bound on any n_b.  Rows of no request, and nodes from max_query
+ * on (which raise the context's device error bit), get position -1 and no bits.  Another parent
+ * raises the bit too and counts as -1. */
+TF_API tf_status tf_draft_tree_plan(tf_context* ctx, const void* parents, const void* seq_lens, const void* token_starts,
+                                    uint32_t num_requests, uint32_t max_query, uint32_t T, uint32_t position_base,
+                                    void* positions, void* ancestors, uint32_t words, void* stream);
+
+/* tf_shared_prefix_attention with a node's ancestors in the place of the causal mask.  Request b's
+ * nodes are its last n_b positions (their K and V written).  Node j sees
+ *   the keys before them, that is the prefix and the request's own positions below seq_lens[b] - n_b
+ *     (window 0: all; otherwise those above positions[t] - window, a position below the history's
+ *     end counting as its end), and
+ *   position seq_lens[b] - n_b + i for every bit i < n_b of ancestors[t], itself only if its bit is set.
+ * Any bits are taken, not only a tree's.  window 0 or >= max_query (a node's ancestors are then inside
+ * it); positions may be NULL without one.  Everything else is as there: a row that sees nothing gives
+ * 0 and -infinity, rows of no request too. */
+TF_API size_t tf_tree_attention_workspace_bytes(const tf_context* ctx, const tf_paged_kv* kv, uint32_t num_q_heads,
+                                                uint32_t T, uint32_t num_requests, uint32_t prefix_len,
+                                                uint32_t max_query);
+TF_API tf_status tf_tree_attention(tf_context* ctx, const void* q, uint64_t q_stride, const tf_paged_kv* kv,
+                                   const void* prefix_pages, uint32_t prefix_len, const void* page_table,
+                                   uint32_t max_pages, const void* seq_lens, const void* token_starts,
+                                   uint32_t num_requests, const void* ancestors, uint32_t words, const void* positions,
+                                   uint32_t max_query, uint32_t T, uint32_t num_q_heads, float scale, uint32_t window,
+                                   void* out, uint64_t out_stride, void* lse, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* Rules on the logits of a batch.  B requests, T rows, row t of request b when token_starts[b] <= t <
+ * token_starts[b + 1]; every part may be NULL (0):
+ *   history (int32[B][history_stride], rows of max_history): the tokens of the request, the first
+ *     prompt_lens[b] of its history_lens[b] the prompt, the others its output
+ *   repetition, presence, frequency (float[B]): 1, 0, 0 where NULL
+ *   bias_starts (int32[B + 1]), bias_tokens (int32), bias_values (float), bias_count entries: for
+ *     request b the entries from bias_starts[b] to bias_starts[b + 1]; of a token's entries the last counts
+ *   allowed (uint32[allowed_count][allowed_stride]): bit v (word v / 32) = token v is allowed;
+ *     allowed_rows (int32[T]): the row's row of allowed, -1: none (NULL: row t)
+ *   token_ids (int32[T]) and ancestors (uint32[T][words]): the tokens of a drafted tree; the tokens of a
+ *     row's ancestors are part of its output
+ * Tokens outside [0, V) have no effect. */
+typedef struct {
+    const void* history;
+    const void* history_lens;
+    const void* prompt_lens;
+    const void* repetition;
+    const void* presence;
+    const void* frequency;
+    const void* bias_starts;
+    const void* bias_tokens;
+    const void* bias_values;
+    const void* allowed;
+    const void* allowed_rows;
+    const void* token_ids;
+    const void* ancestors;
+    uint64_t history_stride, allowed_stride;
+    uint32_t max_history, bias_count, allowed_count, words;
+} tf_logit_rules;
+
+/* For every row and token v, c = how often v is in the row's output:
+ *   z = logits[t][v]
+ *   v in the prompt or c > 0:  z = z > 0 ? z / repetition : z * repetition
+ *   z = z - frequency * c;  c > 0: z = z - presence;  z = z + bias;  v not allowed: z = -infinity
+ * in fp32, each step rounded; out[t][v] = z in the logits' type (row strides in elements; out may be
+ * logits).  tokens[t] (int32, optional) = the v with the largest z before that last rounding, the lowest
+ * of equals, NaN never; -1 when no z is above -infinity.  Rows of no request are left as they were.
+ * max_query: host bound on any request's rows (further rows are left alone and raise the device error
+ * bit, as does a row of allowed that does not exist, which counts as none).  With drafted trees at most
+ * 256.  Pointers need their elements' alignment, rows that begin on 16 bytes are faster.  workspace
+ * (8-byte aligned, one per concurrent call) is needed for tokens. */
+TF_API size_t tf_logit_rules_workspace_bytes(uint32_t T, uint32_t V);
+TF_API tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t logits_stride, void* out,
+                                      uint64_t out_stride, tf_dtype dtype, uint32_t V, uint32_t T,
+                                      const void* token_starts, uint32_t num_requests, uint32_t max_query,
+                                      const tf_logit_rules* rules, void* tokens, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* Down every tree: of the node at hand, the first child whose token is the choice made there
+ * (choices[t], by any sampler, so the kept tokens are distributed as without drafts) is kept and is
+ * the next at hand.  given (int32[B], NULL: 1): so many leading nodes are a chain of known tokens (the
+ * root, or the rest of a prompt) that is kept without a look; the walk begins at the last of them.
+ * Outputs, int32:
+ *   counts[b]           nodes kept (0 for a request without tokens)
+ *   paths[b][max_query] their indices among the request's nodes, -1 behind them
+ *   tokens[b][max_query] the choices at the last given node and at the kept ones behind it: the
+ *                       counts[b] - given[b] + 1 new tokens of the request, the last of them not in the
+ *                       cache yet (the next root); -1 behind them
+ *   targets[b] = seq_lens[b] - n_b + counts[b] (-1 without tokens), for tf_kv_pages_resize
+ * With num_layers > 0, K and V of kept node k move from position seq_lens[b] - n_b + paths[b][k] to
+ * seq_lens[b] - n_b + k of the request's own, in num_layers pools like kv, layer_stride elements (a
+ * multiple of 8) apart.  A position without a page in the pool is not moved and raises the device error
+ * bit; nodes from max_query on are not looked at and raise it too; so does a parent that is not below
+ * its node, which is not kept.  The outputs must not overlap the inputs. */
+TF_API tf_status tf_draft_accept(tf_context* ctx, const void* token_ids, const void* parents, const void* choices,
+                                 const void* given, const void* seq_lens, const void* token_starts,
+                                 uint32_t num_requests, uint32_t max_query, uint32_t T, void* counts, void* paths,
+                                 void* tokens, void* targets, const tf_paged_kv* kv, uint64_t layer_stride,
+                                 uint32_t num_layers, const void* page_table, uint32_t max_pages, void* stream);
 
 /* ---- expert parallelism (routed experts sharded over GPUs) ------------------------------
  * No reference counterpart (the reference streams experts from SSD on one GPU).
