@@ -256,7 +256,8 @@ def _prepare_logits(c, s, gen, host):
     if own:
         from edgeexpert_b200.sampling import LogitRules
         s["handle"] = LogitRules()
-        s["workspace"] = torch.empty(s["handle"].workspace_bytes(T, V), dtype=torch.uint8, device="cuda")
+        biases = 0 if s["bias_tokens"] is None else s["bias_tokens"].numel()
+        s["workspace"] = torch.empty(s["handle"].workspace_bytes(T, V, B, longest, biases), dtype=torch.uint8, device="cuda")
     return s
 
 
