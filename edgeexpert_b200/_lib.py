@@ -177,7 +177,7 @@ _PROTOS = {
     "tf_tree_attention_workspace_bytes": ([_P, C.POINTER(PagedKVDesc), _U32, _U32, _U32, _U32, _U32], C.c_size_t),
     "tf_tree_attention": ([_P, _P, _U64, C.POINTER(PagedKVDesc), _P, _U32, _P, _U32, _P, _P, _U32, _P, _U32, _P, _U32,
                            _U32, _U32, C.c_float, _U32, _P, _U64, _P, _P, C.c_size_t, _P], _I),
-    "tf_logit_rules_workspace_bytes": ([_U32, _U32], C.c_size_t),
+    "tf_logit_rules_workspace_bytes": ([_U32, _U32, _U32, _U32, _U32], C.c_size_t),
     "tf_logit_rules_apply": ([_P, _P, _U64, _P, _U64, _I, _U32, _U32, _P, _U32, _U32, C.POINTER(LogitRulesDesc), _P, _P,
                               C.c_size_t, _P], _I),
     "tf_draft_accept": ([_P, _P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _P, _P, C.POINTER(PagedKVDesc), _U64,

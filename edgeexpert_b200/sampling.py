@@ -62,9 +62,10 @@ class LogitRules:
         self.call = lib().tf_logit_rules_apply
 
     @staticmethod
-    def workspace_bytes(rows: int, vocab: int) -> int:
-        """Enough for every call with at most so many rows of so many tokens."""
-        return int(lib().tf_logit_rules_workspace_bytes(rows, vocab))
+    def workspace_bytes(rows: int, vocab: int, requests: int, history: int = 0, biases: int = 0) -> int:
+        """Enough for every call with at most these sizes (history: the width of `history`, biases: all
+        requests' entries)."""
+        return int(lib().tf_logit_rules_workspace_bytes(rows, vocab, requests, history, biases))
 
     @staticmethod
     def _vectors(n: int, dtype, what: str, *tensors):
@@ -78,7 +79,7 @@ class LogitRules:
                 t.shape[1] > 1 and t.stride(1) != 1):
             raise TFError(TF_ERR_INVALID_ARG, f"LogitRules.encode: {what} must be an int32 matrix, rows contiguous")
 
-    def encode(self, logits, out, token_starts, workspace=None, max_query: int = 1, history=None, history_lens=None,
+    def encode(self, logits, out, token_starts, workspace, max_query: int = 1, history=None, history_lens=None,
                prompt_lens=None, repetition=None, presence=None, frequency=None, bias_starts=None, bias_tokens=None,
                bias_values=None, allowed=None, allowed_rows=None, token_ids=None, ancestors=None, tokens=None,
                stream=None):
@@ -134,9 +135,7 @@ class LogitRules:
             if ancestors.dtype is not i32 or ancestors.dim() != 2 or ancestors.shape[0] != T or not ancestors.is_contiguous():
                 raise TFError(TF_ERR_INVALID_ARG, f"{what}: ancestors are a contiguous int32 [rows][words]")
             d.words = ancestors.shape[1]
-        if tokens is not None and workspace is None:
-            raise TFError(TF_ERR_INVALID_ARG, f"{what}: tokens need a workspace")
         st = self.call(self.ctx.handle, logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0),
                        _LOGITS[logits.dtype], V, T, token_starts.data_ptr(), B, max_query, C.byref(d), at(tokens),
-                       at(workspace), 0 if workspace is None else workspace.nbytes, stream_ptr(stream))
+                       workspace.data_ptr(), workspace.nbytes, stream_ptr(stream))
         self.ctx.check(st, what)

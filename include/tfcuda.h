@@ -671,9 +671,11 @@ typedef struct {
  * of equals, NaN never; -1 when no z is above -infinity.  Rows of no request are left as they were.
  * max_query: host bound on any request's rows (further rows are left alone and raise the device error
  * bit, as does a row of allowed that does not exist, which counts as none).  With drafted trees at most
- * 256.  Pointers need their elements' alignment, rows that begin on 16 bytes are faster.  workspace
- * (8-byte aligned, one per concurrent call) is needed for tokens. */
-TF_API size_t tf_logit_rules_workspace_bytes(uint32_t T, uint32_t V);
+ * 256.  V <= 393216.  Pointers need their elements' alignment, rows that begin on 16 bytes are faster.
+ * workspace: caller-owned device scratch (16-byte aligned, contents arbitrary, one per concurrent call);
+ * bytes for one call are enough for any with no larger numbers. */
+TF_API size_t tf_logit_rules_workspace_bytes(uint32_t T, uint32_t V, uint32_t num_requests, uint32_t max_history,
+                                             uint32_t bias_count);
 TF_API tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t logits_stride, void* out,
                                       uint64_t out_stride, tf_dtype dtype, uint32_t V, uint32_t T,
                                       const void* token_starts, uint32_t num_requests, uint32_t max_query,

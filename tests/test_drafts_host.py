@@ -17,7 +17,7 @@ def test_entry_points_refuse_a_null_context():
     assert lib.tf_tree_attention_workspace_bytes(z, C.byref(kv), 1, 1, 1, 1, 1) == 0
     assert lib.tf_logit_rules_apply(z, z, 1, z, 1, 2, 1, 1, z, 1, 1, C.byref(rules), z, z, 0, z) == bad
     assert lib.tf_draft_accept(z, z, z, z, z, z, z, 1, 1, 1, z, z, z, z, C.byref(kv), 0, 0, z, 0, z) == bad
-    assert lib.tf_logit_rules_workspace_bytes(3, 262144) >= 3 * 8
+    assert lib.tf_logit_rules_workspace_bytes(3, 262144, 2, 100, 5) >= 3 * 8 + 16 * (2 * 100 + 5 + 3)
 
 
 def test_layers_describe_strides():

@@ -61,6 +61,10 @@ class Rows:
             self.drafted = tokens(T)
             self.masks = masks_of([random_parents(rng, n) for n in counts])
 
+    def workspace(self, op, T):
+        return op.workspace_bytes(T, self.V, len(self.counts), self.history.shape[1],
+                                  0 if self.bias is None else len(self.bias[1]))
+
     def run(self, out=None, logits=None, tokens=True, max_query=None, stream=None, words=None):
         from edgeexpert_b200.sampling import LogitRules
         op = LogitRules()
@@ -85,9 +89,9 @@ class Rows:
             words = -(-max([1] + self.counts) // 32) if words is None else words
             kw.update(token_ids=i32(self.drafted), ancestors=words_of(self.masks, words, padding))
         for left in (0, 255):
-            ws = torch.full((op.workspace_bytes(T, V),), left, dtype=torch.uint8, device="cuda")
+            ws = torch.full((self.workspace(op, T),), left, dtype=torch.uint8, device="cuda")
             torch.cuda.synchronize()
-            op.encode(logits, out, i32(self.starts), ws if tokens else None, max_query=most, tokens=chosen, stream=stream,
+            op.encode(logits, out, i32(self.starts), ws, max_query=most, tokens=chosen, stream=stream,
                       **kw)
             torch.cuda.synchronize()
             if out.data_ptr() == logits.data_ptr():
@@ -205,7 +209,7 @@ def test_ties_infinities_and_nan(cuda, dtype):
     """Equal logits go to the lowest token, across chunks and lanes; infinities stay what they are; NaN is
     never chosen; a row of NaN and -infinity has no token."""
     V = 20000
-    rows = Rows([8], V, dtype, history=(0, 0), factors=False)
+    rows = Rows([10], V, dtype, history=(0, 0), factors=False)
     z = rows.logits
     z.zero_()
     z[1, 17000] = z[1, 17001] = z[1, 4100] = 9.0
@@ -217,10 +221,12 @@ def test_ties_infinities_and_nan(cuda, dtype):
     z[6] = float("-inf")
     z[6, V - 1] = torch.finfo(z.dtype).min
     z[7, 5], z[7, 0] = -0.0, -1.0
+    z[8, :18000], z[9, :18000] = -1.0, -1.0
+    z[8, 17], z[9, 18003] = -0.0, -0.0
     out, chosen = rows.run()
     assert torch.equal(out.nan_to_num(3.0), z.nan_to_num(3.0)) and torch.equal(out.isnan(), z.isnan())
     # (-0 is below +0 in no comparison: the lower token of the two)
-    assert chosen.tolist() == [0, 4100, 3, -1, -1, 0, V - 1, 1]
+    assert chosen.tolist() == [0, 4100, 3, -1, -1, 0, V - 1, 1, 17, 18000]
 
 
 def test_the_last_bias_of_a_token_counts(cuda):
@@ -239,7 +245,7 @@ def test_rules_in_a_graph(cuda):
     rep, pres, freq = (torch.from_numpy(x).cuda() for x in (rows.rep, rows.pres, rows.freq))
     ids, bits = i32(rows.drafted), words_of(rows.masks, 1)
     out, tokens = torch.zeros_like(rows.logits), i32(np.zeros(5))
-    ws = torch.empty(op.workspace_bytes(5, 9000), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(op.workspace_bytes(5, 9000, 2, 100), dtype=torch.uint8, device="cuda")
 
     def call():
         op.encode(rows.logits, out, starts, ws, max_query=3, history=history, history_lens=lens, prompt_lens=prompt,
@@ -291,7 +297,7 @@ def test_refusals(cuda):
     from edgeexpert_b200.sampling import LogitRules
     op = LogitRules()
     z = torch.zeros(4, 64, device="cuda")
-    ws = torch.empty(op.workspace_bytes(4, 64), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(op.workspace_bytes(4, 64, 2, 4, 1), dtype=torch.uint8, device="cuda")
     two = i32([1, 1])
 
     def call(logits=z, out=None, starts=i32([0, 2, 4]), ws=ws, max_query=2, tokens=i32([0] * 4), **kw):
@@ -303,7 +309,7 @@ def test_refusals(cuda):
     bits = i32(np.zeros((4, 1)))
     for bad in (dict(logits=z.double()), dict(out=z.half()), dict(out=z[:, :63]), dict(logits=z.t(), out=z.t()),
                 dict(logits=z[0]), dict(starts=torch.tensor([0, 2, 4], device="cuda")), dict(starts=i32([0])),
-                dict(max_query=0), dict(ws=None), dict(ws=ws[:8]), dict(tokens=i32([0] * 3)), dict(tokens=torch.zeros(4).cuda()),
+                dict(max_query=0), dict(ws=ws[:8]), dict(tokens=i32([0] * 3)), dict(tokens=torch.zeros(4).cuda()),
                 dict(history=i32([[1], [2]])), dict(history_lens=two), dict(prompt_lens=two),
                 dict(history=i32([[1]]), history_lens=two), dict(history=torch.zeros(2, 1).cuda(), history_lens=two),
                 dict(history=i32(np.zeros((2, 4))).t()[:2], history_lens=two), dict(repetition=torch.ones(3, device="cuda")),
