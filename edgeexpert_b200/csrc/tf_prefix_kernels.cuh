@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
             const int u0 = unit_begin(cta, many, many_ctas), u1 = unit_begin(cta + 1, many, many_ctas);
             if constexpr (kTree) {
                 const TreeSegment pre = tree_segment<T, HD>(p, -1);
-                if (threadIdx.x == 0 && u0 < pre.row_tiles * pre.units * p.nkv) {
+                if (threadIdx.x == 0 && u0 < tree_slots(p, pre)) {
                     s_tile = -1;
                     s_tile_at = 0;
                     s_tile_units = pre.units;
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
                 int at = many_before;
                 for (int b = b0; b < b1; ++b) {
                     const TreeSegment s = tree_segment<T, HD>(p, b);
-                    const int units = s.row_tiles * s.units * p.nkv;
+                    const int units = tree_slots(p, s);
                     if (u0 >= at && u0 < at + units) {
                         s_tile = b;
                         s_tile_at = at;
@@ -449,7 +449,7 @@ Shape shape_of_call(const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t pre
     const long long G = nq / kv->num_kv_heads, own = std::min<long long>(max_query, T) * G;
     Shape s;
     s.hd = kv->head_dim <= 64 ? 64 : (kv->head_dim <= 128 ? 128 : (kv->head_dim <= 256 ? 256 : 512));
-    s.nt = own <= 8 ? 1 : std::min(4, 512 / s.hd);
+    s.nt = own <= 8 || tree ? 1 : std::min(4, 512 / s.hd);
     s.few_rows = s.nt * 8;
     const bool can = s.hd <= 256;
     s.prefix_few = !can || T * G <= kFewPrefixRows;

@@ -234,6 +234,13 @@ __device__ __noinline__ int tensor_units(const AttnParams<T, kTree>& p, int i) {
 struct TreeSegment {
     int row_tiles, units;
 };
+// kTree: what a job costs besides its units (Q in, the pipeline filled and drained, O out), as units:
+// the work is dealt by both, so that CTAs with many short jobs get fewer.
+constexpr int kJobUnits = 6;
+template <typename T, bool kTree>
+__device__ __forceinline__ int tree_slots(const AttnParams<T, kTree>& p, const TreeSegment& s) {
+    return s.row_tiles * (s.units + kJobUnits) * p.nkv;
+}
 template <typename T, int HD, bool kTree>
 __device__ __noinline__ TreeSegment tree_segment(const AttnParams<T, kTree>& p, int seg) {
     TreeSegment s{0, 0};
@@ -253,18 +260,16 @@ __device__ __noinline__ TreeSegment tree_segment(const AttnParams<T, kTree>& p, 
     return s;
 }
 
-// kTree: the units of the prefix and of all requests; `before` those before this thread's own
+// kTree: the units (and jobs, as units) of the prefix and of all requests; `before` those before this thread's own
 // requests [b0, b1).
 template <typename T, int HD, bool kTree>
 __device__ __forceinline__ int all_tree_units(const AttnParams<T, kTree>& p, int* red, int b0, int b1, int& before) {
     int sum = 0, total;
     for (int b = b0; b < b1; ++b) {
-        const TreeSegment s = tree_segment<T, HD>(p, b);
-        sum += s.row_tiles * s.units * p.nkv;
+        sum += tree_slots(p, tree_segment<T, HD>(p, b));
     }
     before = block_scan(sum, red, &total);
-    const TreeSegment s = tree_segment<T, HD>(p, -1);
-    const int prefix = s.row_tiles * s.units * p.nkv;
+    const int prefix = tree_slots(p, tree_segment<T, HD>(p, -1));
     before += prefix;
     return prefix + total;
 }
@@ -276,6 +281,95 @@ __device__ __forceinline__ int all_tensor_units(const AttnParams<T, kTree>& p, i
     for (int i = i0; i < i1; ++i) sum += tensor_units<T, HD>(p, i) * p.nkv;
     before = block_scan(sum, red, &total);
     return total;
+}
+
+// kTree: the weights of a unit's N keys for a row (the calling thread's), in place of its scores at
+// column `scol`, and m and d brought up to date; false if a wait gave up.  The row sees keys [lo, hi) and,
+// from key `node_at` on, the nodes of its `ancestors`, up to key `end`.
+// A tree's jobs are short (a few units) and so are a CTA's (twenty or thirty units), and code is fetched
+// anew by every launch: the N scores of a row at once, unrolled, took 5 to 9 us the first time and 1.0 to
+// 1.7 us a unit of 128 keys from then on.  So 64 keys at a time by one short loop and in one pass: weights
+// are formed with the reference m that there is, and where a maximum has outgrown it by more than 2^8 the
+// new one is a whole power of two away, so that weights that have been rounded already are moved to it
+// without another error.  P of keys 64 w .. is written over scores that have been read.
+template <typename T, int N, typename Ready>
+__device__ __forceinline__ bool tree_weights(const uint32_t* ancestors, int words, int node_at, int lo, int hi, int end,
+                                             uint32_t scol, uint32_t ocol, int hd, float sc, float& m, float& d,
+                                             bool has_o, Ready& o_ready) {
+    // 32 keys from key k on that the row sees, as bits
+    auto seen = [&](int k) {
+        const int a = max(0, lo - k), z = min(32, hi - k);
+        uint32_t bits = z > a ? (0xFFFFFFFFu >> (32 - (z - a))) << a : 0u;
+        if (k + 32 > node_at) {
+            // 32 bits from node `at` on; what lies before node 0 or behind the words is not set
+            const int at = k - node_at, word = at >> 5, left = end - k;
+            const uint32_t x = word >= 0 && word < words ? ancestors[word] : 0u;
+            const uint32_t y = word >= -1 && word + 1 < words ? ancestors[word + 1] : 0u;
+            const uint32_t nodes = __funnelshift_r(x, y, at & 31);
+            bits |= left >= 32 ? nodes : (left > 0 ? nodes & ((1u << left) - 1u) : 0u);
+        }
+        return bits;
+    };
+#pragma unroll 1
+    for (int w = 0; w < N / 64; ++w) {
+        const uint32_t bits[2] = {seen(64 * w), seen(64 * w + 32)};
+        float s[64];
+        tmem_ld32_async(scol + 64 * w, s);
+        tmem_ld32_async(scol + 64 * w + 32, s + 32);
+        tmem_ld_wait(s);
+        if (!__all_sync(0xffffffffu, (bits[0] & bits[1]) == 0xFFFFFFFFu)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) s[i] = bits[i / 32] >> (i & 31) & 1u ? s[i] : -INFINITY;
+        }
+        float top4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < 64; ++i) top4[i & 3] = fmaxf(top4[i & 3], s[i]);
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
+        const bool grown = top > m + 8.f;
+        if (__any_sync(0xffffffffu, grown)) {
+            const float now = grown ? floorf(top) : m;
+            const float f = !grown || m == -INFINITY ? 1.f : exp2_approx(m - now);
+            d *= f;
+            m = now;
+            if (w) {  // this unit's weights so far
+                tmem_wait_st();
+#pragma unroll 1
+                for (int i = 0; i < 32 * w; i += 16) {
+                    uint32_t x[16];
+                    tmem_ld16(scol + i, x);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = Pair<T>::scaled(x[e], f);
+                    tmem_st16(scol + i, x);
+                }
+            }
+            if (has_o) {
+                if (!o_ready()) return false;
+                tc_fence_after();
+#pragma unroll 1
+                for (int i = 0; i < hd; i += 32) {
+                    float o[32];
+                    tmem_ld32_async(ocol + i, o);
+                    tmem_ld_wait(o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] *= f;
+                    tmem_st32(ocol + i, reinterpret_cast<uint32_t*>(o));
+                }
+            }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float d4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t weights[32];
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+            const float a = exp2_approx(fmaf(s[i], sc, -ref)), z = exp2_approx(fmaf(s[i + 1], sc, -ref));
+            d4[i & 2] += a;
+            d4[(i & 2) + 1] += z;
+            weights[i / 2] = Pair<T>::pack(a, z);
+        }
+        tmem_st32(scol + 32 * w, weights);
+        d += (d4[0] + d4[1]) + (d4[2] + d4[3]);
+    }
+    return true;
 }
 
 struct TensorBarriers {
@@ -338,6 +432,33 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
     struct Job {
         int tile, kvh, units, from, to;
         int seg, row_tiles;  // kTree: tile is one of the segment's row tiles
+        int at;              // kTree: where the job's share of [u0, u1) begins, its own cost first
+    };
+    // kTree: the next job.  A request's row tiles read the same keys one after the other; the
+    // prefix's KV heads the same rows.
+    auto step = [&](Job& j) {
+        j.at += j.units + kJobUnits;
+        if (j.seg < 0 ? ++j.kvh < p.nkv : ++j.tile < j.row_tiles) return;
+        if (j.seg < 0 ? ++j.tile < j.row_tiles : ++j.kvh < p.nkv) {
+            (j.seg < 0 ? j.kvh : j.tile) = 0;
+            return;
+        }
+        TreeSegment s;
+        do {
+            s = tree_segment<T, HD>(p, ++j.seg);
+        } while (s.units == 0);
+        j.units = s.units;
+        j.row_tiles = s.row_tiles;
+        j.kvh = j.tile = 0;
+    };
+    // kTree: this job's units in [u0, u1), or those of the first job behind it that has some; none
+    // (from = to) if there is none.
+    auto take = [&](Job& j) {
+        for (;; step(j)) {
+            j.from = max(0, u0 - j.at - kJobUnits);
+            j.to = max(j.from, min(j.units, u1 - j.at - kJobUnits));
+            if (j.from < j.to || j.at + j.units + kJobUnits >= u1) return;
+        }
     };
     auto first_job = [&]() {
         Job j;
@@ -346,11 +467,11 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
             j.seg = tile0;
             j.row_tiles = tree_segment<T, HD>(p, j.seg).row_tiles;
             j.units = tile_units;
-            const int q = in / j.units;
-            j.from = in % j.units;
-            j.to = min(j.units, j.from + u1 - u0);
+            const int q = in / (j.units + kJobUnits);
+            j.at = u0 - in % (j.units + kJobUnits);
             j.tile = j.seg < 0 ? q / p.nkv : q % j.row_tiles;
             j.kvh = j.seg < 0 ? q % p.nkv : q / j.row_tiles;
+            take(j);
             return j;
         }
         j.seg = -1;
@@ -364,21 +485,11 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
     auto next_job = [&](Job& j, int u) {  // u: units done
         j.from = 0;
         if constexpr (kTree) {
-            // a request's row tiles read the same keys one after the other; the prefix's KV heads
-            // the same rows
-            if (j.seg < 0 ? ++j.kvh < p.nkv : ++j.tile < j.row_tiles) {
-            } else if (j.seg < 0 ? ++j.tile < j.row_tiles : ++j.kvh < p.nkv) {
-                (j.seg < 0 ? j.kvh : j.tile) = 0;
-            } else {
-                TreeSegment s;
-                do {
-                    s = tree_segment<T, HD>(p, ++j.seg);
-                } while (s.units == 0);
-                j.units = s.units;
-                j.row_tiles = s.row_tiles;
-                j.kvh = j.tile = 0;
-            }
-        } else if (++j.kvh == p.nkv) {
+            step(j);
+            take(j);
+            return;
+        }
+        if (++j.kvh == p.nkv) {
             j.kvh = 0;
             do {
                 j.units = tensor_units<T, HD>(p, ++j.tile);
@@ -386,6 +497,8 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
         }
         j.to = min(j.units, u1 - u);
     };
+    // Units (kTree: and jobs' own) behind this job's.
+    auto after = [&](const Job& j, int u) { return kTree ? j.at + kJobUnits + j.units : u + j.to - j.from; };
 
     if (warp > 6) {
         // no work
@@ -395,7 +508,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
         int it = 0;
         bool ok = true;
         Job job = first_job();
-        for (int u = u0; ok && u < u1;) {
+        for (int u = u0; ok && u < u1 && job.from < job.to;) {
             TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from, job.seg);
             TileKeys<N> next = look_up_keys<N>(p, c.seg, c.lo + c.tile * N, c.from, c.hi);
             for (int x = job.from; ok && x < job.to; ++x, ++it) {
@@ -411,7 +524,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                     load_tile_keys<HD, N>(p, kv != 0, ring + (kv * S::kSlots + slot) * S::kSlot, job.kvh, now,
                                           &bar.full[kv][slot], false);
             }
-            u += job.to - job.from;
+            u = after(job, u);
             if (u < u1) next_job(job, u);
         }
         // what is in flight lands before the CTA may end: also what nobody waits for any more because
@@ -451,7 +564,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 s_buf ^= 1;
             };
             Job job = first_job();
-            for (int u = u0; ok && u < u1;) {
+            for (int u = u0; ok && u < u1 && job.from < job.to;) {
                 const int n = job.to - job.from;
                 ok = wait(&bar.q_full, q_phase) && wait(&bar.full[0][k.slot], k.phase);
                 if (!ok) break;
@@ -486,7 +599,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                     p_buf ^= 1;
                 }
                 q_phase ^= 1;
-                u += n;
+                u = after(job, u);
                 if (u < u1) next_job(job, u);
             }
             // tensor memory is given back only when no MMA uses it, also after a wait that gave up
@@ -498,6 +611,9 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
         // ---- a row per thread -------------------------------------------------------
         const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);  // this warp's lanes
         const float sc = p.scale * kLog2e;
+        // A tree's jobs are short: what each runs once is kept in short loops, since it is fetched anew
+        // (its last unit, with nodes, and the way out took 8 to 11 us unrolled).
+        constexpr bool kOnce = kTree;
         int uc = 0;
         bool ok = true;
         // O holds everything up to unit uc - 1.  A barrier for even and one for odd units:
@@ -505,7 +621,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
         // the phase before the one waited for here (unit uc - 3) is over.
         auto o_ready = [&]() { return wait_warp(&bar.o_done[(uc - 1) & 1], ((uc - 1) >> 1) & 1); };
         Job job = first_job();
-        for (int u = u0; ok && u < u1;) {
+        for (int u = u0; ok && u < u1 && job.from < job.to;) {
             const long long row = (long long)job.tile * kTcRows + threadIdx.x;
             bool exists = row < (long long)p.T_tokens * p.G;
             int t = exists ? (int)(row / p.G) : 0;
@@ -531,6 +647,10 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 }
             }
             const bool live = b < p.B;
+            // kTree: rows that are nobody's weigh what their neighbours do, or, where a warp has no other,
+            // nothing: their results go nowhere (a row of a product does not depend on another)
+            const bool warp_live = !kTree || __any_sync(0xffffffffu, live);
+            if (kTree && !live) row_hi = 0x7FFFFFFF;
             {  // Q to tensor memory
                 const T* q = p.q + t * p.q_stride + (long long)h * p.hd;
 #pragma unroll
@@ -562,40 +682,34 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 // the keys of this tile that the row sees: [lo, hi) of 0..N
                 const int key0 = c.lo + c.tile * N;
                 int lo = row_lo, hi = row_hi;
-                if (c.seg >= 0) {
+                if (c.seg >= 0 && !(kTree && !live)) {
                     lo = b == c.seg ? lo - p.prefix_len : 0;
                     hi = b == c.seg ? hi - p.prefix_len : 0;
                 }
                 lo = max(0, lo - key0);
                 hi = min(min(hi, c.hi) - key0, N);
-                float s[N];
-                uint32_t nodes[N / 32];  // kTree: of the tile's keys, the nodes that the row sees
-                bool any_node = false;
                 if constexpr (kTree) {
-#pragma unroll
-                    for (int w = 0; w < N / 32; ++w) nodes[w] = 0u;
-                    if (c.seg >= 0 && key0 + N > node0 && live) {
-                        const uint32_t* bits = p.ancestors + (long long)t * p.words;
-#pragma unroll
-                        for (int w = 0; w < N / 32; ++w) {
-                            // 32 bits from node `at` on; what lies before node 0 or behind the words is not set
-                            const int at = key0 + 32 * w - node0, word = at >> 5, end = c.hi - key0 - 32 * w;
-                            const uint32_t a = word >= 0 && word < p.words ? bits[word] : 0u;
-                            const uint32_t z = word >= -1 && word + 1 < p.words ? bits[word + 1] : 0u;
-                            nodes[w] = __funnelshift_r(a, z, at & 31);
-                            if (end < 32) nodes[w] &= end > 0 ? (1u << end) - 1u : 0u;
-                            any_node |= nodes[w] != 0u;
-                        }
+                    if (warp_live) {
+                        const int node_at = live ? node0 - key0 : N;
+                        ok = tree_weights<T, N>(p.ancestors + (long long)t * p.words, p.words, node_at, lo, hi,
+                                                min(N, c.hi - key0), scol, mine + S::kColO, HD, sc, m, d, x > job.from,
+                                                o_ready);
+                        if (!ok) break;
+                        tmem_wait_st();
                     }
+                    tc_fence_before();
+                    mbar_arrive(&bar.p_full[buf]);
+                    if (x + 1 < job.to) tensor_advance<T, HD>(p, job.tile, c);
+                    continue;
                 }
-                if (__any_sync(0xffffffffu, hi > lo || any_node)) {
+                float s[N];
+                if (__any_sync(0xffffffffu, hi > lo)) {
 #pragma unroll
                     for (int i = 0; i < N; i += 32) tmem_ld32_async(scol + i, s + i);
                     tmem_ld_wait(s);
                     if (!__all_sync(0xffffffffu, lo == 0 && hi == N)) {
 #pragma unroll
-                        for (int i = 0; i < N; ++i)
-                            s[i] = (i >= lo && i < hi) || (kTree && (nodes[i / 32] >> (i & 31) & 1u)) ? s[i] : -INFINITY;
+                        for (int i = 0; i < N; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
                     }
                     float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -610,7 +724,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                             ok = o_ready();
                             if (!ok) break;
                             tc_fence_after();
-#pragma unroll
+#pragma unroll(kOnce ? 1 : HD / 32)
                             for (int i = 0; i < HD; i += 32) {
                                 float o[32];
                                 tmem_ld32_async(mine + S::kColO + i, o);
@@ -661,7 +775,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
             float* po = (job.from == 0 ? to.first : p.many.cont) + at * p.hd;
             const float inv = d == 0.f ? 0.f : 1.f / d;
             bool fine = isfinite(d);
-#pragma unroll
+#pragma unroll(kOnce ? 1 : HD / 32)
             for (int i = 0; i < HD; i += 32) {
                 float o[32];
                 tmem_ld32_async(mine + S::kColO + i, o);
@@ -699,7 +813,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 }
             }
             tc_fence_before();
-            u += job.to - job.from;
+            u = after(job, u);
             if (u < u1) next_job(job, u);
         }
     }
