@@ -528,7 +528,7 @@ template <typename T, bool kTree>
 tf_status launch(tf_context* ctx, const AttnParams<T, kTree>& p, const Shape& s, cudaStream_t cs, const char* name) {
     tf_status st = TF_OK;
     auto parts = [&](auto hd, auto nt) {
-        constexpr int HD = decltype(hd)::value, NT = decltype(nt)::value;
+        constexpr int HD = decltype(hd)::value, NT = kTree ? 1 : decltype(nt)::value;
         if constexpr (HD <= 256) {
             if (s.tensor) return launch_parts<T, HD, NT, true>(ctx, p, cs, name);
         }

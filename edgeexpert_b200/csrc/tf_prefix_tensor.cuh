@@ -283,6 +283,21 @@ __device__ __forceinline__ int all_tensor_units(const AttnParams<T, kTree>& p, i
     return total;
 }
 
+// Waits about two seconds at most, or until another warp gave up; false then.
+__device__ __forceinline__ bool wait_unless(uint64_t* bar, uint32_t parity, volatile int* dead, uint32_t* err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long since = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*dead) return false;
+        if (clock64() - since > 4000000000ll) {
+            *dead = 1;
+            atomicOr(err, kErrMbarTimeout);
+            return false;
+        }
+    }
+    return true;
+}
+
 // kTree: the weights of a unit's N keys for a row (the calling thread's), in place of its scores at
 // column `scol`, and m and d brought up to date; false if a wait gave up.  The row sees keys [lo, hi) and,
 // from key `node_at` on, the nodes of its `ancestors`, up to key `end`.
@@ -292,10 +307,16 @@ __device__ __forceinline__ int all_tensor_units(const AttnParams<T, kTree>& p, i
 // are formed with the reference m that there is, and where a maximum has outgrown it by more than 2^8 the
 // new one is a whole power of two away, so that weights that have been rounded already are moved to it
 // without another error.  P of keys 64 w .. is written over scores that have been read.
-template <typename T, int N, typename Ready>
-__device__ __forceinline__ bool tree_weights(const uint32_t* ancestors, int words, int node_at, int lo, int hi, int end,
-                                             uint32_t scol, uint32_t ocol, int hd, float sc, float& m, float& d,
-                                             bool has_o, Ready& o_ready) {
+// Out of line, so that a warp without work can run it too, beforehand and to no end (`dry`): the code is then
+// on its way while the rows wait for their queries.
+struct TreeSums {
+    float m, d;
+    int ok;
+};
+template <typename T, int N, int HD>
+__device__ __noinline__ TreeSums tree_weights(const uint32_t* ancestors, int words, int node_at, int lo, int hi, int end,
+                                              uint32_t scol, uint32_t ocol, float sc, float m, float d, bool dry,
+                                              uint64_t* o_done, uint32_t parity, volatile int* dead, uint32_t* err) {
     // 32 keys from key k on that the row sees, as bits
     auto seen = [&](int k) {
         const int a = max(0, lo - k), z = min(32, hi - k);
@@ -312,7 +333,7 @@ __device__ __forceinline__ bool tree_weights(const uint32_t* ancestors, int word
     };
 #pragma unroll 1
     for (int w = 0; w < N / 64; ++w) {
-        const uint32_t bits[2] = {seen(64 * w), seen(64 * w + 32)};
+        const uint32_t bits[2] = {seen(64 * w), dry ? 0u : seen(64 * w + 32)};
         float s[64];
         tmem_ld32_async(scol + 64 * w, s);
         tmem_ld32_async(scol + 64 * w + 32, s + 32);
@@ -325,7 +346,7 @@ __device__ __forceinline__ bool tree_weights(const uint32_t* ancestors, int word
 #pragma unroll
         for (int i = 4; i < 64; ++i) top4[i & 3] = fmaxf(top4[i & 3], s[i]);
         const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
-        const bool grown = top > m + 8.f;
+        const bool grown = top > m + 8.f && !dry;
         if (__any_sync(0xffffffffu, grown)) {
             const float now = grown ? floorf(top) : m;
             const float f = !grown || m == -INFINITY ? 1.f : exp2_approx(m - now);
@@ -342,11 +363,11 @@ __device__ __forceinline__ bool tree_weights(const uint32_t* ancestors, int word
                     tmem_st16(scol + i, x);
                 }
             }
-            if (has_o) {
-                if (!o_ready()) return false;
+            if (o_done) {  // O of the units before
+                if (!__all_sync(0xffffffffu, wait_unless(o_done, parity, dead, err))) return {m, d, 0};
                 tc_fence_after();
 #pragma unroll 1
-                for (int i = 0; i < hd; i += 32) {
+                for (int i = 0; i < HD; i += 32) {
                     float o[32];
                     tmem_ld32_async(ocol + i, o);
                     tmem_ld_wait(o);
@@ -366,10 +387,10 @@ __device__ __forceinline__ bool tree_weights(const uint32_t* ancestors, int word
             d4[(i & 2) + 1] += z;
             weights[i / 2] = Pair<T>::pack(a, z);
         }
-        tmem_st32(scol + 32 * w, weights);
+        if (!dry) tmem_st32(scol + 32 * w, weights);
         d += (d4[0] + d4[1]) + (d4[2] + d4[3]);
     }
-    return true;
+    return {m, d, 1};
 }
 
 struct TensorBarriers {
@@ -412,19 +433,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
     const uint32_t tmem = bar.tmem;
 
     // Bounded waits: about two seconds, or until another warp gave up.
-    auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
-        if (mbar_try_wait(b, parity)) return true;
-        const long long since = clock64();
-        while (!mbar_try_wait(b, parity)) {
-            if (bar.dead) return false;
-            if (clock64() - since > 4000000000ll) {
-                bar.dead = 1;
-                atomicOr(p.err, kErrMbarTimeout);
-                return false;
-            }
-        }
-        return true;
-    };
+    auto wait = [&](uint64_t* b, uint32_t parity) -> bool { return wait_unless(b, parity, &bar.dead, p.err); };
     // For warps that stay together: given up by the whole warp or by none of it (votes and tensor
     // memory instructions with lanes missing would wait for them for good).
     auto wait_warp = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
@@ -501,7 +510,11 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
     auto after = [&](const Job& j, int u) { return kTree ? j.at + kJobUnits + j.units : u + j.to - j.from; };
 
     if (warp > 6) {
-        // no work
+        if constexpr (kTree) {  // no work: see tree_weights
+            const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            tree_weights<T, N, HD>(p.ancestors, 0, N, 0, N, N, mine + S::kColS, mine + S::kColO, 0.f, 0.f, 0.f, true,
+                                   nullptr, 0, &bar.dead, p.err);
+        }
     } else if (warp >= 5) {
         // ---- loaders: warp 5 K, warp 6 V, tile after tile -------------------------------
         const int kv = warp - 5;
@@ -691,9 +704,13 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 if constexpr (kTree) {
                     if (warp_live) {
                         const int node_at = live ? node0 - key0 : N;
-                        ok = tree_weights<T, N>(p.ancestors + (long long)t * p.words, p.words, node_at, lo, hi,
-                                                min(N, c.hi - key0), scol, mine + S::kColO, HD, sc, m, d, x > job.from,
-                                                o_ready);
+                        uint64_t* const before = x > job.from ? &bar.o_done[(uc - 1) & 1] : nullptr;
+                        const TreeSums sums = tree_weights<T, N, HD>(
+                            p.ancestors + (long long)t * p.words, p.words, node_at, lo, hi, min(N, c.hi - key0), scol,
+                            mine + S::kColO, sc, m, d, false, before, ((uc - 1) >> 1) & 1, &bar.dead, p.err);
+                        m = sums.m;
+                        d = sums.d;
+                        ok = sums.ok != 0;
                         if (!ok) break;
                         tmem_wait_st();
                     }
