@@ -295,8 +295,27 @@ def ptr(t) -> C.c_void_p:
 stream_ptr = _stream_ptr
 
 
+def raw_stream(stream, device: int) -> int:
+    """The raw stream of an encode call (these calls are made once a layer: the
+    stream objects of torch would cost as much as the launch)."""
+    if stream is None:
+        import torch
+        return torch._C._cuda_getCurrentRawStream(device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
 def on_device(what: str, device: int, *tensors) -> None:
     """Refuses tensors (None: left out) that are not on `device`: a kernel there cannot read them."""
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise TFError(TF_ERR_INVALID_ARG, f"{what}: a tensor on {t.device}, the context is on cuda:{device}")
+
+
+def int32_on_device(what: str, device: int, *tensors) -> None:
+    """The same, and those that are not contiguous int32 tensors."""
+    import torch
+    i32 = torch.int32
+    for t in tensors:
+        if t.dtype is not i32 or not t.is_contiguous() or t.get_device() != device:
+            on_device(what, device, t)
+            raise TFError(TF_ERR_INVALID_ARG, f"{what}: lists, lengths and tables are contiguous int32 tensors")

@@ -11,15 +11,14 @@
 //   gather_kernel       per request: the tokens that anything is said of, in their order,
 //                       as entries (how often, in the prompt, bias)
 //   logit_rules_kernel  the rows, once in and once out: a chunk waits in shared memory, gets
-//                       the values of its few entries there, and is masked and compared
-//   best_token_kernel   the best of a row's chunks
+//                       the values of its few entries there, and is masked and compared; the
+//                       row's last chunk to be done writes its token
 #include "tf_paged.cuh"
 
 using namespace tf;
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kGatherThreads = 1024;
 constexpr uint32_t kInPrompt = 0x80000000u, kDrafted = 0x40000000u, kCount = 0x3FFFFFFFu;
 constexpr int kMaxNodes = 256;
@@ -32,7 +31,9 @@ struct Gathered {
     int* begin;        // [B][chunks + 1]: the first entry of a chunk's tokens
     long long* base;   // [B]: a request's first entry
     uint4* entries;    // token, count and flags, bias; in the order of the tokens
-    unsigned long long* best;  // [T][chunks], of the second kernel
+    // of the second kernel, 0 at its start:
+    unsigned long long* best;  // [T]: the best of a row's chunks
+    uint32_t* done;            // [T]: how many there are
 };
 
 struct RulesParams {
@@ -113,7 +114,11 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
     const int bias0 = p.bias_count ? p.bias_starts[b] : 0, bias1 = p.bias_count ? p.bias_starts[b + 1] : 0;
     const int start = max(0, min(s0, p.T)), n = max(start, min(s1, p.T)) - start, used = min(n, p.max_query);
     if (n > used && tid == 0) atomicOr(p.err, kErrBadTree);
-    for (int j = tid; j < n; j += kGatherThreads) p.g.request[start + j] = j < used ? b : -1;
+    for (int j = tid; j < n; j += kGatherThreads) {
+        p.g.request[start + j] = j < used ? b : -1;
+        p.g.best[start + j] = 0ull;
+        p.g.done[start + j] = 0u;
+    }
     if (b == 0) {
         const int end = max(start, min(p.starts[p.B], p.T));
         for (int t = tid; t < start + p.T - end; t += kGatherThreads) p.g.request[t < start ? t : end + t - start] = -1;
@@ -416,6 +421,28 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
     uint4 first = make_uint4(0u, 0u, 0u, 0u);
     if (now.k0 + tid < now.k1) first = entries[now.k0 + tid];
 
+    int last_i = i0, last_row = 0, last_b = -1;  // of the chunk before
+    // One thread: the best of the chunks that are done, and, when a row is left, what it has of it to the
+    // row's; whoever brings a row's last chunk has all the others before it.
+    unsigned long long row_best = 0ull;
+    int row_chunks = 0;
+    auto take = [&](int next_row) {  // after chunk last_i, of row last_row
+        if (last_b >= 0) {
+            row_best = max(row_best, s_best[last_i & 1]);
+            ++row_chunks;
+        }
+        s_best[last_i & 1] = 0ull;
+        if (next_row == last_row || row_chunks == 0) return;
+        if (row_best) atomicMax(&p.g.best[last_row], row_best);
+        __threadfence();
+        if (atomicAdd(&p.g.done[last_row], (uint32_t)row_chunks) + row_chunks == (uint32_t)p.chunks) {
+            __threadfence();
+            const unsigned long long best = atomicMax(&p.g.best[last_row], 0ull);
+            p.tokens[last_row] = best ? (int)(0xFFFFFFFFu - (uint32_t)best) : -1;
+        }
+        row_best = 0ull;
+        row_chunks = 0;
+    };
     int from = 0;
 #pragma unroll 1
     for (int i = i0; i < i1; ++i) {
@@ -428,10 +455,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncthreads();  // the chunk is here, and the one before has been read
         load_ahead(i + kStages - 1);
-        if (i > i0 && tid == 0) {  // the chunk before's best
-            p.g.best[i - 1] = s_best[(i - 1) & 1];
-            s_best[(i - 1) & 1] = 0ull;
-        }
+        if (i > i0 && tid == 0 && p.tokens) take(at.row);
         uint32_t* const known = s_known[i & 1];
         const bool any = now.k0 < now.k1;
         if constexpr (kRounds)
@@ -574,6 +598,9 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
                 if (lane == 0 && top) atomicMax(&s_best[i & 1], (unsigned long long)top << 32 | low);
             }
         }
+        last_i = i;
+        last_row = at.row;
+        last_b = b;
         if (next_b != b) {
             b = next_b;
             look_up_request();
@@ -583,19 +610,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
         if (more) at.advance(p);
     }
     __syncthreads();
-    if (tid == 0 && i0 < i1) p.g.best[i1 - 1] = s_best[(i1 - 1) & 1];
-}
-
-// A warp a row: the best of its chunks.
-__global__ void __launch_bounds__(kThreads) best_token_kernel(const __grid_constant__ RulesParams p) {
-    griddep_wait();
-    griddep_launch_dependents();
-    const int lane = threadIdx.x & 31, row = (blockIdx.x * kThreads + threadIdx.x) >> 5;
-    if (row >= p.T || p.g.request[row] < 0) return;
-    unsigned long long best = 0ull;
-    for (int c = lane; c < p.chunks; c += 32) best = max(best, p.g.best[(long long)row * p.chunks + c]);
-    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) p.tokens[row] = best ? (int)(0xFFFFFFFFu - (uint32_t)best) : -1;
+    if (tid == 0 && i0 < i1 && p.tokens) take(-1);
 }
 
 // As many CTAs as are resident at once, or as there are chunks.
@@ -622,7 +637,7 @@ inline int chunks_of(uint32_t V, tf_dtype dtype) {
 
 // The workspace, for any type of logits; places are 16-byte aligned.
 struct RulesLayout {
-    size_t request, begin, base, entries, best, bytes;
+    size_t request, begin, base, entries, best, done, bytes;
 };
 RulesLayout layout_of(uint32_t T, uint32_t V, uint32_t B, uint32_t max_history, uint32_t bias_count) {
     RulesLayout l;
@@ -637,7 +652,8 @@ RulesLayout layout_of(uint32_t T, uint32_t V, uint32_t B, uint32_t max_history, 
     l.begin = take((size_t)B * (chunks + 1) * sizeof(int));
     l.base = take((size_t)B * sizeof(long long));
     l.entries = take(((size_t)B * max_history + bias_count + T) * sizeof(uint4));
-    l.best = take((size_t)T * chunks * sizeof(unsigned long long));
+    l.best = take((size_t)T * sizeof(unsigned long long));
+    l.done = take((size_t)T * sizeof(uint32_t));
     l.bytes = at;
     return l;
 }
@@ -725,6 +741,7 @@ tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t log
     p.g.base = reinterpret_cast<long long*>(w + l.base);
     p.g.entries = reinterpret_cast<uint4*>(w + l.entries);
     p.g.best = reinterpret_cast<unsigned long long*>(w + l.best);
+    p.g.done = reinterpret_cast<uint32_t*>(w + l.done);
     p.err = ctx->d_err;
     p.V = (int)V;
     p.T = (int)T;
@@ -755,7 +772,6 @@ tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t log
         e = dtype == TF_DTYPE_F32   ? launch_rows<float>(p, ctx->device, ctx->num_sms, cs)
             : dtype == TF_DTYPE_F16 ? launch_rows<__half>(p, ctx->device, ctx->num_sms, cs)
                                     : launch_rows<__nv_bfloat16>(p, ctx->device, ctx->num_sms, cs);
-    if (e == cudaSuccess && tokens) e = launch_overlapped(best_token_kernel, (T + 7) / 8, kThreads, 0, cs, p);
     return cuda_check(ctx, e, name);
 }
 

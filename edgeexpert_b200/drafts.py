@@ -5,18 +5,18 @@ tokens of each request at once and keeps the way that the model itself chose.
 * ``TreeAttention.encode``     attention of the nodes over prefix, history and ancestors
 * ``DraftAccept.encode``       the walk down each tree; kept nodes' K and V moved into place
 
-and, between the last two, ``LogitRules.encode`` of sampling.py.  No counterpart
-in the reference, which decodes one token at a time.  Everything stays on the
-device, so a step can be captured in a CUDA graph.
+and, between the last two, ``LogitRules.encode`` of sampling.py; ``DraftDecoder``
+is the decoder of paged.py with all four.  No counterpart in the reference, which
+decodes one token at a time.  Everything stays on the device, so a step can be
+captured in a CUDA graph.
 """
 from __future__ import annotations
 
 import torch
 
-from ._lib import Context, TFError, TF_ERR_INVALID_ARG, lib, on_device
-from .paged import PagedKV, PagedKVLayers, _heads, _int32, _stream
-
-_I32 = torch.int32
+from ._lib import Context, TFError, TF_ERR_INVALID_ARG, int32_on_device, lib, on_device, raw_stream
+from .paged import PagedDecoder, PagedKV, PagedKVCache, PagedKVLayers, _heads
+from .sampling import LogitRules
 
 
 class DraftTree:
@@ -32,13 +32,13 @@ class DraftTree:
         Writes positions [T] (position_base + history + depth) and ancestors [T][words], a bit for every
         node on the way from the root, the node's own among them; rows of no request get -1 and 0."""
         T, B = parents.numel(), seq_lens.numel()
-        _int32("DraftTree.encode_plan", parents, seq_lens, token_starts, positions, ancestors)
+        device = self.ctx.device
+        int32_on_device("DraftTree.encode_plan", device, parents, seq_lens, token_starts, positions, ancestors)
         if positions.numel() != T or ancestors.dim() != 2 or ancestors.shape[0] != T or token_starts.numel() != B + 1:
             raise TFError(TF_ERR_INVALID_ARG, "DraftTree.encode_plan: sizes of the tensors do not agree")
-        on_device("DraftTree.encode_plan", self.ctx.device, parents, seq_lens, token_starts, positions, ancestors)
         st = self.call(self.ctx.handle, parents.data_ptr(), seq_lens.data_ptr(), token_starts.data_ptr(), B, max_query,
                        T, position_base, positions.data_ptr(), ancestors.data_ptr(), ancestors.shape[1],
-                       _stream(stream, self.ctx.device))
+                       raw_stream(stream, device))
         if st:
             self.ctx.check(st, "DraftTree.encode_plan")
 
@@ -67,29 +67,29 @@ class TreeAttention:
         B = seq_lens.numel()
         if q.dtype != kv.dtype or out.dtype != kv.dtype or out.shape != q.shape or hd != kv.head_dim:
             raise TFError(TF_ERR_INVALID_ARG, "TreeAttention.encode: q, out and the cache do not agree")
-        _int32("TreeAttention.encode", page_table, seq_lens, token_starts, ancestors)
+        what, device = "TreeAttention.encode", self.ctx.device
+        int32_on_device(what, device, page_table, seq_lens, token_starts, ancestors)
         if (page_table.dim() != 2 or page_table.shape[0] != B or token_starts.numel() != B + 1 or ancestors.dim() != 2
                 or ancestors.shape[0] != T):
             raise TFError(TF_ERR_INVALID_ARG, "TreeAttention.encode: sizes of the tensors do not agree")
         if prefix_len:
             if prefix_pages is None or prefix_pages.numel() * kv.page_size < prefix_len:
                 raise TFError(TF_ERR_INVALID_ARG, "TreeAttention.encode: too few prefix pages")
-            _int32("TreeAttention.encode", prefix_pages)
+            int32_on_device(what, device, prefix_pages)
         if positions is not None:
-            _int32("TreeAttention.encode", positions)
+            int32_on_device(what, device, positions)
             if positions.numel() != T:
                 raise TFError(TF_ERR_INVALID_ARG, "TreeAttention.encode: a position for every token")
         if lse is not None and (lse.dtype != torch.float32 or lse.numel() != T * nq or not lse.is_contiguous()):
             raise TFError(TF_ERR_INVALID_ARG, "TreeAttention.encode: lse must be contiguous float32 [T][heads]")
-        on_device("TreeAttention.encode", self.ctx.device, q, kv.k, kv.v, page_table, seq_lens, token_starts, ancestors,
-                  out, workspace, prefix_pages, positions, lse)
+        on_device(what, device, q, kv.k, kv.v, out, workspace, lse)
         st = self.call(
             self.ctx.handle, q.data_ptr(), _heads(q, "q"), kv.ref, prefix_pages.data_ptr() if prefix_len else None,
             prefix_len, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), token_starts.data_ptr(), B,
             ancestors.data_ptr(), ancestors.shape[1], None if positions is None else positions.data_ptr(), max_query, T,
             nq, hd ** -0.5 if scale is None else scale, window, out.data_ptr(), _heads(out, "out"),
             None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.nbytes,
-            _stream(stream, self.ctx.device))
+            raw_stream(stream, device))
         if st:
             self.ctx.check(st, "TreeAttention.encode")
 
@@ -109,29 +109,119 @@ class DraftAccept:
         counts, targets [requests] and paths, tokens [requests][max_query]: how many nodes are kept and
         which, the new tokens, and the lengths for KVPages.  `layers`: the pools in which the kept nodes'
         K and V move to the positions behind the history (page_table: the requests' pages)."""
-        what = "DraftAccept.encode"
+        what, device = "DraftAccept.encode", self.ctx.device
         T, B = token_ids.numel(), seq_lens.numel()
-        _int32(what, token_ids, parents, choices, seq_lens, token_starts, counts, paths, tokens, targets)
+        int32_on_device(what, device, token_ids, parents, choices, seq_lens, token_starts, counts, paths, tokens, targets)
         if (parents.numel() != T or choices.numel() != T or token_starts.numel() != B + 1 or counts.numel() != B
                 or targets.numel() != B or paths.numel() != B * max_query or tokens.numel() != B * max_query):
             raise TFError(TF_ERR_INVALID_ARG, f"{what}: sizes of the tensors do not agree")
         if given is not None:
-            _int32(what, given)
+            int32_on_device(what, device, given)
             if given.numel() != B:
                 raise TFError(TF_ERR_INVALID_ARG, f"{what}: given is one number a request")
-        on_device(what, self.ctx.device, token_ids, parents, choices, seq_lens, token_starts, counts, paths, tokens,
-                  targets, given)
         n = 0 if layers is None else layers.layers
         if n:
             if page_table is None or page_table.dim() != 2 or page_table.shape[0] != B:
                 raise TFError(TF_ERR_INVALID_ARG, f"{what}: pools need the requests' page table")
-            _int32(what, page_table)
-            on_device(what, self.ctx.device, layers.k, layers.v, page_table)
+            int32_on_device(what, device, page_table)
+            on_device(what, device, layers.k, layers.v)
         st = self.call(self.ctx.handle, token_ids.data_ptr(), parents.data_ptr(), choices.data_ptr(),
                        None if given is None else given.data_ptr(), seq_lens.data_ptr(), token_starts.data_ptr(), B,
                        max_query, T, counts.data_ptr(), paths.data_ptr(), tokens.data_ptr(), targets.data_ptr(),
                        layers.ref if n else None, layers.layer_stride if n else 0, n,
                        page_table.data_ptr() if n else None, page_table.shape[1] if n else 0,
-                       _stream(stream, self.ctx.device))
+                       raw_stream(stream, device))
         if st:
             self.ctx.check(st, what)
+
+
+class DraftDecoder(PagedDecoder):
+    """PagedDecoder with steps that check drafted trees: `draft` adds the nodes of each request's tree,
+    chooses a token after every one, keeps the way that the choices take from the root, and gives the
+    pages of the others back.  `step` is as before."""
+
+    def __init__(self, weights, T: int, cache: PagedKVCache, max_query: int = 1, context: Context | None = None,
+                 device=None):
+        super().__init__(weights, T, cache, max_query, context, device)
+        if max_query > 256:
+            raise TFError(TF_ERR_INVALID_ARG, "DraftDecoder: a tree has up to 256 nodes")
+        dev, B = self.q.device, cache.num_requests
+
+        def i32(*shape):
+            return torch.zeros(shape, dtype=torch.int32, device=dev)
+
+        self.tree, self.tree_attention = DraftTree(self.ctx), TreeAttention(self.ctx)
+        self.rules, self.accept = LogitRules(self.ctx), DraftAccept(self.ctx)
+        self.parents, self.node_positions, self.ancestors = i32(T), i32(T), i32(T, -(-max_query // 32))
+        self.counts, self.targets = i32(B), i32(B)
+        self.paths, self.new_tokens = i32(B, max_query), i32(B, max_query)
+        self.draft_starts, self.draft_state = i32(B + 1), i32(4)
+        self.rules_workspace = None
+        self._drafting = False
+
+    def _row_positions(self):
+        return self.node_positions if self._drafting else super()._row_positions()
+
+    def _attend_rows(self, q, i: int, out, stream):
+        if not self._drafting:
+            return super()._attend_rows(q, i, out, stream)
+        kv = self.kv
+        self.tree_attention.encode(q, kv.layer[i], kv.page_table, kv.seq_lens, kv.token_starts, self.ancestors, out,
+                                   self.workspace, prefix_pages=kv.prefix_pages, prefix_len=kv.prefix_len,
+                                   max_query=self.max_query, scale=1.0, stream=stream)
+
+    def _workspace_bytes(self) -> int:
+        kv = self.kv
+        return max(super()._workspace_bytes(), self.tree_attention.workspace_bytes(
+            kv.layer[0], self.cfg.num_q_heads, self.T, kv.num_requests, kv.prefix_len, self.max_query))
+
+    def draft(self, token_ids, parents, targets, given=None, rules: dict | None = None, stream=None):
+        """token_ids, targets: as in step, the tokens of a request being the nodes of its tree (up to
+        max_query).  parents: of each token the index of its parent among its request's, below its own,
+        or -1 for the root (the first).  given (optional): how many leading tokens of each request are
+        known and kept without a look, a prompt's for instance; 1, the root, without it.  rules: what
+        LogitRules.encode takes for the requests (history, repetition, biases, allowed for every row ...); the
+        drafted tokens count as said on their way down.  self.logits then holds the logits under the
+        rules, self.tokens the choice after every node.
+
+        Returns (counts, new_tokens), on the device: how many nodes of each request are kept, and
+        [requests][max_query] the counts - given + 1 tokens that are new, -1 behind them.  The last of
+        them is not in the cache yet: it is the next root.  self.paths: which nodes are kept.  The cache
+        then holds the kept nodes alone; rows i of this step were tokens draft_starts[b] .. of request b,
+        and draft_state is what free_state was after they were added."""
+        kv = self.kv
+        more = {} if given is None else dict(given=given)
+        self._check_step("DraftDecoder.draft", token_ids, targets, parents=parents, **more)
+        if parents.numel() != token_ids.numel() or (given is not None and given.numel() != kv.num_requests):
+            raise TFError(TF_ERR_INVALID_ARG, "DraftDecoder.draft: a parent for every token, given for every request")
+        with torch.cuda.stream(stream):  # (None: the current one)
+            self._make_workspace()
+            at = self._resize(token_ids, targets, stream)
+            if at is None:
+                self.parents.fill_(-1)
+            else:
+                self.parents.copy_(torch.where(kv.requests >= 0, parents[at], -1))
+            self.draft_starts.copy_(kv.token_starts)
+            self.draft_state.copy_(kv.free_state)
+            self.tree.encode_plan(self.parents, kv.seq_lens, kv.token_starts, self.node_positions, self.ancestors,
+                                  self.max_query, position_base=kv.prefix_len, stream=stream)
+            if rules is not None:
+                history, biases = rules.get("history"), rules.get("bias_tokens")
+                need = self.rules.workspace_bytes(self.T, self.cfg.vocab, kv.num_requests,
+                                                  0 if history is None else history.shape[1],
+                                                  0 if biases is None else biases.numel())
+                if self.rules_workspace is None or self.rules_workspace.nbytes < need:
+                    self.rules_workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
+        self._drafting = True
+        try:
+            self._run_rows(stream)
+        finally:
+            self._drafting = False
+        if rules is not None:
+            self.rules.encode(self.logits, self.logits, kv.token_starts, self.rules_workspace, max_query=self.max_query,
+                              token_ids=self.ids, ancestors=self.ancestors, tokens=self.tokens, stream=stream, **rules)
+        self.accept.encode(self.ids, self.parents, self.tokens, kv.seq_lens, kv.token_starts, self.counts, self.paths,
+                           self.new_tokens, self.targets, self.max_query, given=given, layers=kv.layers,
+                           page_table=kv.page_table, stream=stream)
+        kv.resize(self.targets, stream)
+        return self.counts, self.new_tokens

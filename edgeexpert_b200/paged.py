@@ -16,7 +16,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import Context, PagedKVDesc, TFError, TF_ERR_INVALID_ARG, TF_OK, lib, status_string
+from ._lib import Context, PagedKVDesc, TFError, TF_ERR_INVALID_ARG, TF_OK, lib, raw_stream as _stream, status_string
 from .decoder import Decoder
 
 _I32 = torch.int32
@@ -24,14 +24,6 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _MAX_STEP = 256  # rows that tf_lm_head_greedy takes
 _SCALINGS = {None: 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4}
-
-
-def _stream(stream, device: int) -> int:
-    """The raw stream of an encode call (these calls are made once a layer: the
-    stream objects of torch would cost as much as the launch)."""
-    if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device)
-    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def _heads(t, what: str) -> int:
@@ -298,16 +290,29 @@ class PagedDecoder(Decoder):
         self._proj(L.v, self.normed, self.v_rows, stream)
         q = self.q.view(T, nq, hd)
         self.rope.encode(q, self.k_rows.view(T, nkv, hd), self.v_rows.view(T, nkv, hd), q, kv.layer[i], kv.slots,
-                         kv.positions, self.inv_freq, attention_factor=self.rope_factor, q_weight=L.q_norm,
+                         self._row_positions(), self.inv_freq, attention_factor=self.rope_factor, q_weight=L.q_norm,
                          k_weight=L.k_norm, norm=True, eps=cfg.eps, stream=stream)
-        self.attention.encode(q, kv.layer[i], kv.page_table, kv.seq_lens, kv.token_starts, self.attn.view(T, nq, hd),
-                              self.workspace, prefix_pages=kv.prefix_pages, prefix_len=kv.prefix_len,
-                              max_query=self.max_query, scale=1.0, stream=stream)
+        self._attend_rows(q, i, self.attn.view(T, nq, hd), stream)
+
+    def _row_positions(self):
+        return self.kv.positions
+
+    def _attend_rows(self, q, i: int, out, stream):
+        kv = self.kv
+        self.attention.encode(q, kv.layer[i], kv.page_table, kv.seq_lens, kv.token_starts, out, self.workspace,
+                              prefix_pages=kv.prefix_pages, prefix_len=kv.prefix_len, max_query=self.max_query, scale=1.0,
+                              stream=stream)
+
+    def _workspace_bytes(self) -> int:
+        kv = self.kv
+        return self.attention.workspace_bytes(kv.layer[0], self.cfg.num_q_heads, self.T, kv.num_requests, kv.prefix_len,
+                                              self.max_query)
 
     def _resize(self, token_ids, targets, stream):
         """The page tables brought to `targets`, and self.ids = the tokens of the requests that
         were granted.  The list holds the tokens of all that asked, the rows those of the granted
-        ones alone; a request whose tokens the list does not hold to the end is refused."""
+        ones alone; a request whose tokens the list does not hold to the end is refused.  Returns
+        every row's place in the list (0 for padding, None for an empty list)."""
         kv, n = self.kv, token_ids.numel()
         before = kv.seq_lens.clone()
         asked = torch.maximum(targets, before) - before
@@ -316,9 +321,10 @@ class PagedDecoder(Decoder):
         first = ends - asked - before - kv.prefix_len  # + a token's position = its place in the list
         if n == 0:
             self.ids.zero_()
-            return
+            return None
         at = (first[kv.requests.clamp(min=0)] + kv.positions).clamp_(0, n - 1)
         torch.mul(token_ids[at], kv.requests >= 0, out=self.ids)
+        return at
 
     def step(self, token_ids, targets, stream=None):
         """token_ids (up to T): the tokens to add, request after request, of every request that
@@ -327,19 +333,25 @@ class PagedDecoder(Decoder):
         counts before later requests' pages all the same); the others get their own tokens.  Next
         tokens in self.tokens, row by row of the tokens added: row i is position kv.positions[i]
         of request kv.requests[i], and kv.free_state tells how many requests were refused."""
-        kv = self.kv
-        for t, what in ((token_ids, "token_ids"), (targets, "targets")):
-            if t.dtype is not _I32 or t.dim() != 1 or t.device != self.ids.device:
-                raise TFError(TF_ERR_INVALID_ARG,
-                              f"PagedDecoder.step: {what} must be a vector of int32 on {self.ids.device}")
-        if token_ids.numel() > self.T or targets.numel() != kv.num_requests:
-            raise TFError(TF_ERR_INVALID_ARG, "PagedDecoder.step: up to T tokens, a target per request")
-        need = self.attention.workspace_bytes(kv.layer[0], self.cfg.num_q_heads, self.T, kv.num_requests, kv.prefix_len,
-                                              self.max_query)
+        self._check_step("PagedDecoder.step", token_ids, targets)
         with torch.cuda.stream(stream):  # (None: the current one)
-            if self.workspace is None or self.workspace.nbytes < need:
-                self.workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
+            self._make_workspace()
             self._resize(token_ids, targets, stream)
+        return self._run_rows(stream)
+
+    def _check_step(self, name: str, token_ids, targets, **more):
+        for what, t in dict(token_ids=token_ids, targets=targets, **more).items():
+            if t.dtype is not _I32 or t.dim() != 1 or t.device != self.ids.device:
+                raise TFError(TF_ERR_INVALID_ARG, f"{name}: {what} must be a vector of int32 on {self.ids.device}")
+        if token_ids.numel() > self.T or targets.numel() != self.kv.num_requests:
+            raise TFError(TF_ERR_INVALID_ARG, f"{name}: up to T tokens, a target per request")
+
+    def _make_workspace(self):
+        need = self._workspace_bytes()
+        if self.workspace is None or self.workspace.nbytes < need:
+            self.workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
+
+    def _run_rows(self, stream):
         self.launches = 0
         self.embed(self.ids, stream)
         for i in range(self.cfg.layers):

@@ -9,7 +9,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import (Context, LogitRulesDesc, TF_ERR_INVALID_ARG, TFError, lib, on_device, ptr, stream_ptr)
+from ._lib import Context, LogitRulesDesc, TF_ERR_INVALID_ARG, TFError, lib, ptr, raw_stream, stream_ptr
 
 _LOGITS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -67,17 +67,26 @@ class LogitRules:
         requests' entries)."""
         return int(lib().tf_logit_rules_workspace_bytes(rows, vocab, requests, history, biases))
 
-    @staticmethod
-    def _vectors(n: int, dtype, what: str, *tensors):
-        for t in tensors:
-            if t is not None and (t.dtype is not dtype or t.numel() != n or not t.is_contiguous()):
-                raise TFError(TF_ERR_INVALID_ARG, f"LogitRules.encode: {what}: {n} contiguous values of {dtype}")
+    def _place(self, t, dtype, n: int, what: str):
+        """Where a vector of n values is (None: nowhere)."""
+        if t is None:
+            return None
+        if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+            raise TFError(TF_ERR_INVALID_ARG, f"LogitRules.encode: {what}: {n} contiguous values of {dtype}")
+        return self._here(t, what)
 
-    @staticmethod
-    def _matrix(t, rows, what: str):
-        if t.dtype is not torch.int32 or t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (
+    def _matrix(self, t, rows: int, what: str):
+        """Where an int32 matrix is."""
+        if t.dtype is not torch.int32 or t.dim() != 2 or (rows >= 0 and t.shape[0] != rows) or (
                 t.shape[1] > 1 and t.stride(1) != 1):
             raise TFError(TF_ERR_INVALID_ARG, f"LogitRules.encode: {what} must be an int32 matrix, rows contiguous")
+        return self._here(t, what)
+
+    def _here(self, t, what: str):
+        if t.get_device() != self.ctx.device:
+            raise TFError(TF_ERR_INVALID_ARG, f"LogitRules.encode: {what} on {t.device}, the context is on "
+                          f"cuda:{self.ctx.device}")
+        return t.data_ptr()
 
     def encode(self, logits, out, token_starts, workspace, max_query: int = 1, history=None, history_lens=None,
                prompt_lens=None, repetition=None, presence=None, frequency=None, bias_starts=None, bias_tokens=None,
@@ -89,53 +98,51 @@ class LogitRules:
         request b are bias_starts[b] .. bias_starts[b+1].  allowed: rows of 32 tokens a word, allowed_rows which
         of them is a row's (-1: none).  token_ids [T], ancestors [T][words]: a drafted tree's tokens, each row's
         way being part of its output.  tokens (optional): int32 [T], the best token of each row or -1."""
-        what, i32 = "LogitRules.encode", torch.int32
+        def refuse(why):
+            raise TFError(TF_ERR_INVALID_ARG, "LogitRules.encode: " + why)
+
+        i32, f32, place = torch.int32, torch.float32, self._place
         if logits.dim() != 2 or out.shape != logits.shape or out.dtype is not logits.dtype or logits.dtype not in _LOGITS:
-            raise TFError(TF_ERR_INVALID_ARG, f"{what}: logits and out are [rows][vocab] of one float type")
+            refuse("logits and out are [rows][vocab] of one float type")
         T, V = logits.shape
         if V > 1 and (logits.stride(1) != 1 or out.stride(1) != 1):
-            raise TFError(TF_ERR_INVALID_ARG, f"{what}: rows must be contiguous")
+            refuse("rows must be contiguous")
         B = token_starts.numel() - 1
-        self._vectors(B + 1, i32, "token_starts and bias_starts", token_starts, bias_starts)
-        self._vectors(B, i32, "history_lens and prompt_lens", history_lens, prompt_lens)
-        self._vectors(B, torch.float32, "repetition, presence and frequency", repetition, presence, frequency)
-        self._vectors(T, i32, "allowed_rows, token_ids and tokens", allowed_rows, token_ids, tokens)
-        on_device(what, self.ctx.device, logits, out, token_starts, workspace, history, history_lens, prompt_lens,
-                  repetition, presence, frequency, bias_starts, bias_tokens, bias_values, allowed, allowed_rows,
-                  token_ids, ancestors, tokens)
-        if (history is None) != (history_lens is None) or (prompt_lens is not None and history is None):
-            raise TFError(TF_ERR_INVALID_ARG, f"{what}: a history and its lengths go together")
-        if (bias_starts is None) != (bias_tokens is None) or (bias_tokens is None) != (bias_values is None):
-            raise TFError(TF_ERR_INVALID_ARG, f"{what}: biases have starts, tokens and values")
-        if (token_ids is None) != (ancestors is None):
-            raise TFError(TF_ERR_INVALID_ARG, f"{what}: drafted tokens and their ancestors go together")
-        if allowed_rows is not None and allowed is None:
-            raise TFError(TF_ERR_INVALID_ARG, f"{what}: rows of no allowed tokens")
-
-        def at(t):
-            return None if t is None else t.data_ptr()
-
-        d = LogitRulesDesc(at(history), at(history_lens), at(prompt_lens), at(repetition), at(presence), at(frequency),
-                           at(bias_starts), at(bias_tokens), at(bias_values), at(allowed), at(allowed_rows),
-                           at(token_ids), at(ancestors))
+        d = LogitRulesDesc()
         if history is not None:
-            self._matrix(history, B, "history")
-            d.history_stride, d.max_history = history.stride(0), history.shape[1]
-        if bias_tokens is not None:
-            n = bias_tokens.numel()
-            self._vectors(n, i32, "bias_tokens", bias_tokens)
-            self._vectors(n, torch.float32, "bias_values", bias_values)
-            d.bias_count = n
+            if history_lens is None:
+                refuse("a history has lengths")
+            d.history, d.history_stride, d.max_history = self._matrix(history, B, "history"), history.stride(0), history.shape[1]
+            d.history_lens = place(history_lens, i32, B, "history_lens")
+            d.prompt_lens = place(prompt_lens, i32, B, "prompt_lens")
+        elif history_lens is not None or prompt_lens is not None:
+            refuse("lengths of no history")
+        d.repetition = place(repetition, f32, B, "repetition")
+        d.presence = place(presence, f32, B, "presence")
+        d.frequency = place(frequency, f32, B, "frequency")
+        if bias_starts is not None or bias_tokens is not None or bias_values is not None:
+            if bias_starts is None or bias_tokens is None or bias_values is None:
+                refuse("biases have starts, tokens and values")
+            n = d.bias_count = bias_tokens.numel()
+            d.bias_starts = place(bias_starts, i32, B + 1, "bias_starts")
+            d.bias_tokens = place(bias_tokens, i32, n, "bias_tokens")
+            d.bias_values = place(bias_values, f32, n, "bias_values")
         if allowed is not None:
-            self._matrix(allowed, None, "allowed")
+            d.allowed, d.allowed_stride, d.allowed_count = self._matrix(allowed, -1, "allowed"), allowed.stride(0), allowed.shape[0]
             if allowed.shape[1] * 32 < V:
-                raise TFError(TF_ERR_INVALID_ARG, f"{what}: allowed must have a bit for every token")
-            d.allowed_stride, d.allowed_count = allowed.stride(0), allowed.shape[0]
-        if ancestors is not None:
-            if ancestors.dtype is not i32 or ancestors.dim() != 2 or ancestors.shape[0] != T or not ancestors.is_contiguous():
-                raise TFError(TF_ERR_INVALID_ARG, f"{what}: ancestors are a contiguous int32 [rows][words]")
+                refuse("allowed must have a bit for every token")
+            d.allowed_rows = place(allowed_rows, i32, T, "allowed_rows")
+        elif allowed_rows is not None:
+            refuse("rows of no allowed tokens")
+        if token_ids is not None or ancestors is not None:
+            if token_ids is None or ancestors is None or ancestors.dim() != 2:
+                refuse("drafted tokens and their ancestors [rows][words] go together")
             d.words = ancestors.shape[1]
-        st = self.call(self.ctx.handle, logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0),
-                       _LOGITS[logits.dtype], V, T, token_starts.data_ptr(), B, max_query, C.byref(d), at(tokens),
-                       workspace.data_ptr(), workspace.nbytes, stream_ptr(stream))
-        self.ctx.check(st, what)
+            d.token_ids = place(token_ids, i32, T, "token_ids")
+            d.ancestors = place(ancestors, i32, T * d.words, "ancestors")
+        st = self.call(self.ctx.handle, self._here(logits, "logits"), logits.stride(0), self._here(out, "out"), out.stride(0),
+                       _LOGITS[logits.dtype], V, T, place(token_starts, i32, B + 1, "token_starts"), B, max_query, C.byref(d),
+                       place(tokens, i32, T, "tokens"), self._here(workspace, "workspace"), workspace.nbytes,
+                       raw_stream(stream, self.ctx.device))
+        if st:
+            self.ctx.check(st, "LogitRules.encode")

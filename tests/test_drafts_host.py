@@ -35,3 +35,7 @@ def test_tensors_elsewhere_are_refused():
     _lib.on_device("x", -1, t, None)  # (-1: host memory)
     with pytest.raises(_lib.TFError):
         _lib.on_device("x", 0, None, t)
+    _lib.int32_on_device("x", -1, t.int())
+    for bad in (t, t.long(), torch.zeros(2, 2, dtype=torch.int32).t()[:1]):
+        with pytest.raises(_lib.TFError):
+            _lib.int32_on_device("x", -1, bad)
