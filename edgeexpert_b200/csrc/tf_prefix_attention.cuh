@@ -202,20 +202,12 @@ struct Pair<__half> {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
-    static __device__ __forceinline__ uint32_t scaled(uint32_t x, float f) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&x));
-        return pack(v.x * f, v.y * f);
-    }
 };
 template <>
 struct Pair<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    static __device__ __forceinline__ uint32_t scaled(uint32_t x, float f) {
-        const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
-        return pack(v.x * f, v.y * f);
     }
 };
 

@@ -88,6 +88,29 @@ __device__ __noinline__ void attend_alone(const AttnParams<T, kTree>& p, int b, 
 __host__ __device__ constexpr float few_unit_ns(int hd) { return 16.f * 4.f * hd / 43.6f; }
 __host__ __device__ constexpr float many_unit_ns(int hd) { return hd > 128 ? 1700.f : (hd > 64 ? 2300.f : 900.f); }
 
+// kTree: which segment unit u0 is in, where that begins and what its row tiles have; told by the one
+// thread that has it among its requests [b0, b1), whose first unit is `before`.
+template <typename T, int HD>
+__device__ __forceinline__ void find_tree_segment(const AttnParams<T, true>& p, int u0, int b0, int b1, int before,
+                                                  int& seg, int& at, int& units) {
+    const TreeSegment prefix = tree_segment<T, HD>(p, -1);
+    if (threadIdx.x == 0 && u0 < tree_slots(p, prefix)) {
+        seg = -1;
+        at = 0;
+        units = prefix.units;
+    }
+    for (int b = b0; b < b1; ++b) {
+        const TreeSegment s = tree_segment<T, HD>(p, b);
+        const int slots = tree_slots(p, s);
+        if (u0 >= before && u0 < before + slots) {
+            seg = b;
+            at = before;
+            units = s.units;
+        }
+        before += slots;
+    }
+}
+
 // All parts of all rows, one CTA per SM.  Every CTA sums the units of both kinds
 // over the batch and finds its share: the first CTAs take the tensor cores' jobs,
 // as many as these need to finish when the others have streamed the rest.
@@ -146,23 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
             __shared__ TensorBarriers bar;
             const int u0 = unit_begin(cta, many, many_ctas), u1 = unit_begin(cta + 1, many, many_ctas);
             if constexpr (kTree) {
-                const TreeSegment pre = tree_segment<T, HD>(p, -1);
-                if (threadIdx.x == 0 && u0 < tree_slots(p, pre)) {
-                    s_tile = -1;
-                    s_tile_at = 0;
-                    s_tile_units = pre.units;
-                }
-                int at = many_before;
-                for (int b = b0; b < b1; ++b) {
-                    const TreeSegment s = tree_segment<T, HD>(p, b);
-                    const int units = tree_slots(p, s);
-                    if (u0 >= at && u0 < at + units) {
-                        s_tile = b;
-                        s_tile_at = at;
-                        s_tile_units = s.units;
-                    }
-                    at += units;
-                }
+                find_tree_segment<T, HD>(p, u0, b0, b1, many_before, s_tile, s_tile_at, s_tile_units);
             } else if (per_row_tile) {
                 if (threadIdx.x == 0) {
                     s_tile = u0 / per_row_tile;
@@ -230,6 +237,41 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
     cur.rt = in / cur.tiles % cur.row_tiles;
     cur.kvh = in / cur.tiles / cur.row_tiles;
     stream_warp<T, HD, NT>(p, smem + warp * S::kTiles * S::kTile, full + warp * S::kTiles, cur, u0, u1, worker);
+}
+
+// kTree, requests of more than eight rows among them: everything on the tensor cores, without the
+// streaming warps' code and without counting their units.  A few requests of one or two nodes beside
+// such trees stream no faster than this (61 requests of 1 to 5 nodes, eight query heads a KV head: 39
+// us with those of one node streamed, their warps ending long after the tiles, 30 this way); 200
+// requests of which one has more take 225 instead of 156 us (16 / 8 heads of 256).
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) tree_tiles_kernel(const __grid_constant__ AttnParams<T, true> p) {
+    extern __shared__ uint8_t raw[];
+    __shared__ int red[32], s_seg, s_at, s_units;
+    __shared__ TensorBarriers bar;
+    griddep_wait();
+    griddep_launch_dependents();  // the joining kernel may read what this one may
+    const int per = (p.B + kThreads - 1) / kThreads;
+    const int b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
+    if (p.window) {  // the first prefix position that any row sees
+        if (threadIdx.x == 0) shared_prefix_first() = p.prefix_len;
+        __syncthreads();
+        int first = p.prefix_len;
+        for (int b = b0; b < b1; ++b) {
+            const Request r = request_of(p, b);
+            if (r.used) first = min(first, seen_from(p, r));
+        }
+        if (first < p.prefix_len) atomicMin(&shared_prefix_first(), first);
+        __syncthreads();
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.prefix_first = prefix_first(p);
+    }
+    int before;
+    const int units = all_tree_units<T, HD>(p, red, b0, b1, before), ctas = min((int)gridDim.x, units), cta = blockIdx.x;
+    if (cta >= ctas) return;
+    const int u0 = unit_begin(cta, units, ctas), u1 = unit_begin(cta + 1, units, ctas);
+    find_tree_segment<T, HD>(p, u0, b0, b1, before, s_seg, s_at, s_units);
+    __syncthreads();
+    tensor_cta<T, HD>(p, (smem_u32(raw) + 1023u) & ~1023u, bar, u0, u1, s_seg, s_at, s_units, cta);
 }
 
 // The parts of one row: own keys' first and cont, then (prefix or tensor
@@ -440,6 +482,7 @@ constexpr int kFewRows = 64, kFewPrefixRows = 32;
 struct Shape {
     int hd, nt, few_rows;
     bool prefix_few, tensor;  // tensor: there may be work for the tensor cores
+    bool tiles;               // trees: everything is
     int many_above;
 };
 
@@ -450,10 +493,11 @@ Shape shape_of_call(const tf_paged_kv* kv, uint32_t nq, uint32_t T, uint32_t pre
     Shape s;
     s.hd = kv->head_dim <= 64 ? 64 : (kv->head_dim <= 128 ? 128 : (kv->head_dim <= 256 ? 256 : 512));
     s.nt = own <= 8 || tree ? 1 : std::min(4, 512 / s.hd);
+    s.tiles = tree && s.hd <= 256 && own > 8;
     s.few_rows = s.nt * 8;
     const bool can = s.hd <= 256;
-    s.prefix_few = !can || T * G <= kFewPrefixRows;
-    s.many_above = can ? (tree ? s.few_rows : kFewRows) : 0x7FFFFFFF;
+    s.prefix_few = !can || (T * G <= kFewPrefixRows && !s.tiles);
+    s.many_above = !can ? 0x7FFFFFFF : (s.tiles ? 0 : (tree ? s.few_rows : kFewRows));
     s.tensor = can && ((prefix_len && !s.prefix_few) || own > s.many_above);
     return s;
 }
@@ -524,11 +568,28 @@ tf_status launch_parts(tf_context* ctx, const AttnParams<T, kTree>& p, cudaStrea
                       name);
 }
 
+template <typename T, int HD>
+tf_status launch_tiles(tf_context* ctx, const AttnParams<T, true>& p, cudaStream_t cs, const char* name) {
+    constexpr int kSmem = TensorShape<HD>::kSmem;
+    static bool configured[64] = {};  // per instantiation, per device
+    const int dev = ctx->device & 63;
+    if (!configured[dev]) {
+        cudaError_t e =
+            cudaFuncSetAttribute(tree_tiles_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e != cudaSuccess) return cuda_check(ctx, e, name);
+        configured[dev] = true;
+    }
+    return cuda_check(ctx, launch_overlapped(tree_tiles_kernel<T, HD>, ctx->num_sms, kThreads, kSmem, cs, p), name);
+}
+
 template <typename T, bool kTree>
 tf_status launch(tf_context* ctx, const AttnParams<T, kTree>& p, const Shape& s, cudaStream_t cs, const char* name) {
     tf_status st = TF_OK;
     auto parts = [&](auto hd, auto nt) {
         constexpr int HD = decltype(hd)::value, NT = kTree ? 1 : decltype(nt)::value;
+        if constexpr (HD <= 256 && kTree) {
+            if (s.tiles) return launch_tiles<T, HD>(ctx, p, cs, name);
+        }
         if constexpr (HD <= 256) {
             if (s.tensor) return launch_parts<T, HD, NT, true>(ctx, p, cs, name);
         }

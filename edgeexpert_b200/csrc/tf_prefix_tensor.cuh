@@ -299,16 +299,12 @@ __device__ __forceinline__ bool wait_unless(uint64_t* bar, uint32_t parity, vola
 }
 
 // kTree: the weights of a unit's N keys for a row (the calling thread's), in place of its scores at
-// column `scol`, and m and d brought up to date; false if a wait gave up.  The row sees keys [lo, hi) and,
-// from key `node_at` on, the nodes of its `ancestors`, up to key `end`.
-// A tree's jobs are short (a few units) and so are a CTA's (twenty or thirty units), and code is fetched
-// anew by every launch: the N scores of a row at once, unrolled, took 5 to 9 us the first time and 1.0 to
-// 1.7 us a unit of 128 keys from then on.  So 64 keys at a time by one short loop and in one pass: weights
-// are formed with the reference m that there is, and where a maximum has outgrown it by more than 2^8 the
-// new one is a whole power of two away, so that weights that have been rounded already are moved to it
-// without another error.  P of keys 64 w .. is written over scores that have been read.
-// Out of line, so that a warp without work can run it too, beforehand and to no end (`dry`): the code is then
-// on its way while the rows wait for their queries.
+// column `scol`, and m and d brought up to date; ok 0 if a wait gave up.  The row sees keys [lo, hi) and,
+// from key `node_at` on, the nodes of its `ancestors`, up to key `end`.  P is written over the scores.
+// Out of line, for two reasons: a row's N scores in registers beside all that a row keeps were spilled
+// (every unit of 128 keys took three times as long), and a warp without work can run it too, beforehand
+// and to no end (`dry`): a CTA's trees are twenty or thirty units, code is fetched anew by every launch,
+// and the first unit took 5 to 9 us, now 1.5 to 3.
 struct TreeSums {
     float m, d;
     int ok;
@@ -317,80 +313,69 @@ template <typename T, int N, int HD>
 __device__ __noinline__ TreeSums tree_weights(const uint32_t* ancestors, int words, int node_at, int lo, int hi, int end,
                                               uint32_t scol, uint32_t ocol, float sc, float m, float d, bool dry,
                                               uint64_t* o_done, uint32_t parity, volatile int* dead, uint32_t* err) {
-    // 32 keys from key k on that the row sees, as bits
-    auto seen = [&](int k) {
-        const int a = max(0, lo - k), z = min(32, hi - k);
-        uint32_t bits = z > a ? (0xFFFFFFFFu >> (32 - (z - a))) << a : 0u;
-        if (k + 32 > node_at) {
+    float s[N];
+#pragma unroll
+    for (int i = 0; i < N; i += 32) tmem_ld32_async(scol + i, s + i);
+    // the keys that the row sees, as bits
+    uint32_t see[N / 32];
+    bool all = !dry;
+#pragma unroll
+    for (int w = 0; w < N / 32; ++w) {
+        const int a = max(0, lo - 32 * w), z = min(32, hi - 32 * w);
+        see[w] = z > a ? (0xFFFFFFFFu >> (32 - (z - a))) << a : 0u;
+        if (32 * w + 32 > node_at) {
             // 32 bits from node `at` on; what lies before node 0 or behind the words is not set
-            const int at = k - node_at, word = at >> 5, left = end - k;
+            const int at = 32 * w - node_at, word = at >> 5, left = end - 32 * w;
             const uint32_t x = word >= 0 && word < words ? ancestors[word] : 0u;
             const uint32_t y = word >= -1 && word + 1 < words ? ancestors[word + 1] : 0u;
             const uint32_t nodes = __funnelshift_r(x, y, at & 31);
-            bits |= left >= 32 ? nodes : (left > 0 ? nodes & ((1u << left) - 1u) : 0u);
+            see[w] |= left >= 32 ? nodes : (left > 0 ? nodes & ((1u << left) - 1u) : 0u);
         }
-        return bits;
-    };
+        all &= see[w] == 0xFFFFFFFFu;
+    }
+    tmem_ld_wait(s);
+    if (!__all_sync(0xffffffffu, all)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = see[i / 32] >> (i & 31) & 1u ? s[i] : -INFINITY;
+    }
+    float top4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int i = 4; i < N; ++i) top4[i & 3] = fmaxf(top4[i & 3], s[i]);
+    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
+    if (__any_sync(0xffffffffu, top > m + 8.f) && !dry) {
+        const float now = fmaxf(m, top);
+        const float f = m == -INFINITY ? 1.f : exp2_approx(m - now);
+        d *= f;
+        m = now;
+        if (o_done) {  // O of the units before
+            if (!__all_sync(0xffffffffu, wait_unless(o_done, parity, dead, err))) return {m, d, 0};
+            tc_fence_after();
 #pragma unroll 1
-    for (int w = 0; w < N / 64; ++w) {
-        const uint32_t bits[2] = {seen(64 * w), dry ? 0u : seen(64 * w + 32)};
-        float s[64];
-        tmem_ld32_async(scol + 64 * w, s);
-        tmem_ld32_async(scol + 64 * w + 32, s + 32);
-        tmem_ld_wait(s);
-        if (!__all_sync(0xffffffffu, (bits[0] & bits[1]) == 0xFFFFFFFFu)) {
+            for (int i = 0; i < HD; i += 32) {
+                float o[32];
+                tmem_ld32_async(ocol + i, o);
+                tmem_ld_wait(o);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) s[i] = bits[i / 32] >> (i & 31) & 1u ? s[i] : -INFINITY;
-        }
-        float top4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < 64; ++i) top4[i & 3] = fmaxf(top4[i & 3], s[i]);
-        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
-        const bool grown = top > m + 8.f && !dry;
-        if (__any_sync(0xffffffffu, grown)) {
-            const float now = grown ? floorf(top) : m;
-            const float f = !grown || m == -INFINITY ? 1.f : exp2_approx(m - now);
-            d *= f;
-            m = now;
-            if (w) {  // this unit's weights so far
-                tmem_wait_st();
-#pragma unroll 1
-                for (int i = 0; i < 32 * w; i += 16) {
-                    uint32_t x[16];
-                    tmem_ld16(scol + i, x);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = Pair<T>::scaled(x[e], f);
-                    tmem_st16(scol + i, x);
-                }
-            }
-            if (o_done) {  // O of the units before
-                if (!__all_sync(0xffffffffu, wait_unless(o_done, parity, dead, err))) return {m, d, 0};
-                tc_fence_after();
-#pragma unroll 1
-                for (int i = 0; i < HD; i += 32) {
-                    float o[32];
-                    tmem_ld32_async(ocol + i, o);
-                    tmem_ld_wait(o);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] *= f;
-                    tmem_st32(ocol + i, reinterpret_cast<uint32_t*>(o));
-                }
+                for (int e = 0; e < 32; ++e) o[e] *= f;
+                tmem_st32(ocol + i, reinterpret_cast<uint32_t*>(o));
             }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float d4[4] = {0.f, 0.f, 0.f, 0.f};
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float d4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; i += 64) {
         uint32_t weights[32];
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-            const float a = exp2_approx(fmaf(s[i], sc, -ref)), z = exp2_approx(fmaf(s[i + 1], sc, -ref));
-            d4[i & 2] += a;
-            d4[(i & 2) + 1] += z;
-            weights[i / 2] = Pair<T>::pack(a, z);
+        for (int e = 0; e < 64; e += 2) {
+            const float a = exp2_approx(fmaf(s[i + e], sc, -ref)), z = exp2_approx(fmaf(s[i + e + 1], sc, -ref));
+            d4[e & 2] += a;
+            d4[(e & 2) + 1] += z;
+            weights[e / 2] = Pair<T>::pack(a, z);
         }
-        if (!dry) tmem_st32(scol + 32 * w, weights);
-        d += (d4[0] + d4[1]) + (d4[2] + d4[3]);
+        if (!dry) tmem_st32(scol + i / 2, weights);
     }
-    return {m, d, 1};
+    return {m, d + ((d4[0] + d4[1]) + (d4[2] + d4[3])), 1};
 }
 
 struct TensorBarriers {
