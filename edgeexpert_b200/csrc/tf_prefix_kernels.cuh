@@ -610,7 +610,9 @@ tf_status launch(tf_context* ctx, const AttnParams<T, kTree>& p, const Shape& s,
     if (st) return st;
     // a warp per row while that fills the GPU; then more rows a CTA, in four rounds of CTAs
     const int rows = p.T_tokens * p.nq;
-    const int per = std::min(kJoinRows, std::max(8, (rows / (ctx->num_sms * 12) + 7) / 8 * 8));
+    // (trees: in one round, since to find a row's request takes a bisection, which the first round does
+    // while the parts are still computed: 11520 rows join in 11 us, 16 in four rounds)
+    const int per = std::min(kJoinRows, std::max(8, (rows / (ctx->num_sms * (kTree ? 3 : 12)) + 7) / 8 * 8));
     const unsigned ctas = (unsigned)((rows + per - 1) / per);
     cudaError_t e;
     if (s.hd <= 128)

@@ -301,16 +301,12 @@ __device__ __forceinline__ bool wait_unless(uint64_t* bar, uint32_t parity, vola
 // kTree: the weights of a unit's N keys for a row (the calling thread's), in place of its scores at
 // column `scol`, and m and d brought up to date; ok 0 if a wait gave up.  The row sees keys [lo, hi) and,
 // from key `node_at` on, the nodes of its `ancestors`, up to key `end`.  P is written over the scores.
-// Out of line, for two reasons: a row's N scores in registers beside all that a row keeps were spilled
-// (every unit of 128 keys took three times as long), and a warp without work can run it too, beforehand
-// and to no end (`dry`): a CTA's trees are twenty or thirty units, code is fetched anew by every launch,
-// and the first unit took 5 to 9 us, now 1.5 to 3.
 struct TreeSums {
     float m, d;
     int ok;
 };
 template <typename T, int N, int HD>
-__device__ __noinline__ TreeSums tree_weights(const uint32_t* ancestors, int words, int node_at, int lo, int hi, int end,
+__device__ __forceinline__ TreeSums tree_weights(const uint32_t* ancestors, int words, int node_at, int lo, int hi, int end,
                                               uint32_t scol, uint32_t ocol, float sc, float m, float d, bool dry,
                                               uint64_t* o_done, uint32_t parity, volatile int* dead, uint32_t* err) {
     float s[N];
@@ -393,7 +389,12 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                                            int tile0, int tile_at, int tile_units, int worker) {
     using S = TensorShape<HD>;
     constexpr int N = S::kKeys;
-    const int warp = threadIdx.x >> 5;
+    // kTree: the warp without work goes with the rows' up to the weights of a unit, waits for nothing and
+    // leaves no trace.  A CTA's trees are twenty or thirty units, code is fetched anew by every launch, and
+    // the first unit took 5 to 9 us; it takes 1.5 to 3 when that has been done while the rows wait for
+    // their queries.
+    const bool ahead = kTree && threadIdx.x >> 5 > 6;
+    const int warp = ahead ? threadIdx.x >> 5 & 3 : threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kSlots; ++i) {
             for (int kv = 0; kv < 2; ++kv) {
@@ -495,11 +496,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
     auto after = [&](const Job& j, int u) { return kTree ? j.at + kJobUnits + j.units : u + j.to - j.from; };
 
     if (warp > 6) {
-        if constexpr (kTree) {  // no work: see tree_weights
-            const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            tree_weights<T, N, HD>(p.ancestors, 0, N, 0, N, N, mine + S::kColS, mine + S::kColO, 0.f, 0.f, 0.f, true,
-                                   nullptr, 0, &bar.dead, p.err);
-        }
+        // no work
     } else if (warp >= 5) {
         // ---- loaders: warp 5 K, warp 6 V, tile after tile -------------------------------
         const int kv = warp - 5;
@@ -618,18 +615,26 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
         // a commit covers all earlier MMAs, so the scores of unit uc being there means that
         // the phase before the one waited for here (unit uc - 3) is over.
         auto o_ready = [&]() { return wait_warp(&bar.o_done[(uc - 1) & 1], ((uc - 1) >> 1) & 1); };
-        Job job = first_job();
+        Job job = ahead ? Job{0x7FFFFFFF, 0, 1, 0, 1, -1, 1, 0} : first_job();  // (ahead: a tile behind all rows)
         for (int u = u0; ok && u < u1 && job.from < job.to;) {
             const long long row = (long long)job.tile * kTcRows + threadIdx.x;
             bool exists = row < (long long)p.T_tokens * p.G;
-            int t = exists ? (int)(row / p.G) : 0;
-            const int h = job.kvh * p.G + (int)(row % p.G);
+            int t, h;
+            if (kTree) {
+                t = exists ? token_of(p, (int)row) : 0;
+                h = job.kvh * p.G + (exists ? (int)row - t * p.G : 0);
+            } else {
+                t = exists ? (int)(row / p.G) : 0;
+                h = job.kvh * p.G + (int)(row % p.G);
+            }
             int b = p.B, row_lo = 0, row_hi = 0, node0 = 0x7FFFFFFF;
             bool own = false;  // its own keys are this kernel's too (kTree: are the job's)
             if (kTree && job.seg >= 0) {
                 const Request r = request_of(p, job.seg);
                 exists = row < (long long)r.used * p.G;
-                t = exists ? r.start + (int)(row / p.G) : 0;
+                t = exists ? token_of(p, (int)row) : 0;
+                h = job.kvh * p.G + (exists ? (int)row - t * p.G : 0);
+                t += exists ? r.start : 0;
                 node0 = r.len - r.n;
                 if (exists) b = job.seg;
             } else if (exists) {
@@ -649,13 +654,14 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
             // nothing: their results go nowhere (a row of a product does not depend on another)
             const bool warp_live = !kTree || __any_sync(0xffffffffu, live);
             if (kTree && !live) row_hi = 0x7FFFFFFF;
-            {  // Q to tensor memory
+            if (!ahead) {  // Q to tensor memory
                 const T* q = p.q + t * p.q_stride + (long long)h * p.hd;
+                constexpr int kTogether = kTree ? HD / 2 : 32;  // words whose loads are in flight together
 #pragma unroll
-                for (int c = 0; c < HD / 2; c += 32) {
-                    uint32_t w[32];
+                for (int c = 0; c < HD / 2; c += kTogether) {
+                    uint32_t w[kTogether];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < kTogether / 4; ++i) {
                         uint4 x = make_uint4(0u, 0u, 0u, 0u);
                         if (live && c * 2 + i * 8 < p.hd) x = *reinterpret_cast<const uint4*>(q + c * 2 + i * 8);
                         w[4 * i] = x.x;
@@ -663,7 +669,8 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                         w[4 * i + 2] = x.z;
                         w[4 * i + 3] = x.w;
                     }
-                    tmem_st32(mine + S::kColQ + c, w);
+#pragma unroll
+                    for (int i = 0; i < kTogether; i += 32) tmem_st32(mine + S::kColQ + c + i, w + i);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -673,7 +680,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
             TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from, job.seg);
             for (int x = job.from; x < job.to; ++x, ++uc) {
                 const int buf = uc & 1;
-                ok = wait_warp(&bar.s_full[buf], (uc >> 1) & 1);
+                if (!ahead) ok = wait_warp(&bar.s_full[buf], (uc >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t scol = mine + S::kColS + buf * N;
@@ -687,16 +694,16 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 lo = max(0, lo - key0);
                 hi = min(min(hi, c.hi) - key0, N);
                 if constexpr (kTree) {
-                    if (warp_live) {
+                    if (warp_live || ahead) {
                         const int node_at = live ? node0 - key0 : N;
                         uint64_t* const before = x > job.from ? &bar.o_done[(uc - 1) & 1] : nullptr;
                         const TreeSums sums = tree_weights<T, N, HD>(
                             p.ancestors + (long long)t * p.words, p.words, node_at, lo, hi, min(N, c.hi - key0), scol,
-                            mine + S::kColO, sc, m, d, false, before, ((uc - 1) >> 1) & 1, &bar.dead, p.err);
+                            mine + S::kColO, sc, m, d, ahead, before, ((uc - 1) >> 1) & 1, &bar.dead, p.err);
                         m = sums.m;
                         d = sums.d;
                         ok = sums.ok != 0;
-                        if (!ok) break;
+                        if (!ok || ahead) break;
                         tmem_wait_st();
                     }
                     tc_fence_before();
@@ -765,6 +772,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 mbar_arrive(&bar.p_full[buf]);
                 if (x + 1 < job.to) tensor_advance<T, HD>(p, job.tile, c);
             }
+            if (ahead) break;
             // ---- the job's part, or the result where nothing else belongs to it ------
             ok = ok && o_ready();
             if (!ok) break;
