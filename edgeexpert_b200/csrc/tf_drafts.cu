@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_con
     if (node && i >= given) {
         if (parent < -1 || parent >= i)
             atomicOr(p.err, kErrBadTree);
-        else if (parent >= given - 1 && token == s_choice[parent])
+        else if (parent >= given - 1 && token == s_choice[parent] && token >= 0)
             atomicMin(&s_next[parent], i);
     }
     __syncthreads();

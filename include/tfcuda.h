@@ -684,8 +684,9 @@ TF_API tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint6
 
 /* Down every tree: of the node at hand, the first child whose token is the choice made there
  * (choices[t], by any sampler, so the kept tokens are distributed as without drafts) is kept and is
- * the next at hand.  given (int32[B], NULL: 1): so many leading nodes are a chain of known tokens (the
- * root, or the rest of a prompt) that is kept without a look; the walk begins at the last of them.
+ * the next at hand; a negative choice (no token) ends the way.  given (int32[B], NULL: 1): so many
+ * leading nodes are a chain of known tokens (the root, or the rest of a prompt) that is kept without a
+ * look; the walk begins at the last of them.
  * Outputs, int32:
  *   counts[b]           nodes kept (0 for a request without tokens)
  *   paths[b][max_query] their indices among the request's nodes, -1 behind them

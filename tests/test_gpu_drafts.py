@@ -501,6 +501,18 @@ def test_accept_of_chains_in_place(cuda):
     no_device_error()
 
 
+def test_no_choice_ends_the_way(cuda):
+    """A choice of -1 is no token, and meets no node, whatever was drafted."""
+    d = Drafts([4], [4], 1, 2, 64, 4, seed=3, vocab=1)
+    d.trees[0] = np.array([-1, 0, 1, 2])
+    d.drafted[0] = np.array([0, 0, -1, 0])
+    d.choices[0] = np.array([0, -1, 0, 0])
+    counts, paths, tokens, targets = d.run(4)
+    assert counts.tolist() == [2] and paths.tolist() == [[0, 1, -1, -1]] and tokens.tolist() == [[0, -1, -1, -1]]
+    assert targets.tolist() == [2]
+    no_device_error()
+
+
 def test_accept_of_bad_trees_and_pages(cuda):
     """A parent that is not earlier is nobody's; nodes beyond the bound and pages outside the pool are
     reported, and what they hold is not moved."""
