@@ -210,8 +210,7 @@ class DraftDecoder(PagedDecoder):
                 need = self.rules.workspace_bytes(self.T, self.cfg.vocab, kv.num_requests,
                                                   0 if history is None else history.shape[1],
                                                   0 if biases is None else biases.numel())
-                if self.rules_workspace is None or self.rules_workspace.nbytes < need:
-                    self.rules_workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
+                self.rules_workspace = self._larger(self.rules_workspace, need)
         self._drafting = True
         try:
             self._run_rows(stream)

@@ -279,7 +279,7 @@ class PagedDecoder(Decoder):
                                     for _ in range(2))
         self.inv_freq, self.rope_factor = rope_frequencies(cfg.head_dim, cfg.rope_theta, device=dev)
         self.rope, self.attention = RotaryKVWrite(self.ctx), SharedPrefixAttention(self.ctx)
-        self.workspace = None
+        self.workspace, self._workspaces = None, []
         self.ids = torch.zeros(T, dtype=_I32, device=dev)  # the tokens of a step's rows
 
     def _attend(self, i: int, position, stream):
@@ -347,9 +347,18 @@ class PagedDecoder(Decoder):
             raise TFError(TF_ERR_INVALID_ARG, f"{name}: up to T tokens, a target per request")
 
     def _make_workspace(self):
-        need = self._workspace_bytes()
-        if self.workspace is None or self.workspace.nbytes < need:
-            self.workspace = torch.empty(need, dtype=torch.uint8, device=self.q.device)
+        self.workspace = self._larger(self.workspace, self._workspace_bytes())
+
+    def _larger(self, workspace, need: int):
+        """`workspace`, or one of `need` bytes in its place.  The old one stays: a step that was captured
+        in a graph goes on writing there.  Each is at least twice the one before, so that all of them
+        together are at most twice the last, however slowly the need grows."""
+        if workspace is not None:
+            if workspace.nbytes >= need:
+                return workspace
+            need = max(need, 2 * workspace.nbytes)
+        self._workspaces.append(torch.empty(need, dtype=torch.uint8, device=self.q.device))
+        return self._workspaces[-1]
 
     def _run_rows(self, stream):
         self.launches = 0

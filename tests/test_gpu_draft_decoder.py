@@ -327,6 +327,36 @@ def test_a_round_in_a_graph(cuda, model):
     del graph
 
 
+def test_a_captured_round_outlives_larger_ones(cuda, model):
+    """A step with longer histories than a captured one's takes a workspace of its own: the captured step's
+    stays where it is."""
+    weights, _ = model
+    dec, cache = make(weights, 1, 8, 4, 8, 4, 4)
+    short, history = dict(history=i32([[5] * 8]), history_lens=i32([8])), i32([[6] * 3000])
+    ids, parents, targets = i32([1, 2]), i32([-1, 0]), i32([2])
+    dec.draft(ids, parents, targets, rules=short)
+    cache.resize(i32([0]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dec.draft(ids, parents, targets, rules=short)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, small = (dec.tokens[:2].tolist(), dec.logits[:2].clone()), dec.rules_workspace
+    cache.resize(i32([0]))
+    dec.draft(ids, parents, targets, rules=dict(history=history, history_lens=i32([3000])))
+    assert dec.rules_workspace.data_ptr() != small.data_ptr() and any(w is small for w in dec._workspaces)
+    del small
+    for _ in range(3):
+        torch.full((1 << 16,), 255, dtype=torch.uint8, device="cuda")
+    cache.resize(i32([0]))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert dec.tokens[:2].tolist() == want[0] and torch.equal(dec.logits[:2], want[1])
+    no_device_error()
+    del graph
+
+
 def test_refusals(cuda, model):
     from edgeexpert_b200._lib import TFError
     from edgeexpert_b200.drafts import DraftDecoder
