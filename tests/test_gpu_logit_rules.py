@@ -170,6 +170,9 @@ CASES = [
     dict(counts=[9], V=70001, dtype="fp16", factors=False, trees=True),
     dict(counts=[4, 4], V=31, dtype="bf16", prompt=1.0),
     dict(counts=[4, 4], V=12289, dtype="fp32", prompt=0.0, trees=True),
+    # the largest vocabulary, and more different tokens than are counted at once
+    dict(counts=[2, 1], V=393216, dtype="fp16", history=(60000, 60000), biases=3000, grammar="some"),
+    dict(counts=[1, 3], V=393213, dtype="fp32", history=(50000, 60000), biases=3000, trees=True),
 ]
 
 
@@ -227,6 +230,26 @@ def test_ties_infinities_and_nan(cuda, dtype):
     assert torch.equal(out.nan_to_num(3.0), z.nan_to_num(3.0)) and torch.equal(out.isnan(), z.isnan())
     # (-0 is below +0 in no comparison: the lower token of the two)
     assert chosen.tolist() == [0, 4100, 3, -1, -1, 0, V - 1, 1, 17, 18000]
+
+
+def test_the_quotient_is_that_of_fp32(cuda):
+    """Any bits of a logit and of a repetition penalty: the same as the fp32 division and product by themselves,
+    bit for bit (NaN: some NaN; a zero keeps no sign, since a bias of 0 is added)."""
+    V, rng = 50000, np.random.default_rng(11)
+    reps = np.concatenate([rng.integers(0, 2 ** 32, 20, dtype=np.uint64).astype(np.uint32).view(np.float32),
+                           np.float32([1.1, 1.3, 3, 1e-38, 1e-45, 3e38, 0, -2, np.inf, np.nextafter(np.float32(1), 2)])])
+    B = len(reps)
+    rows = Rows([1] * B, V, "fp32", history=(V, V), prompt=1.0, factors=False)
+    rows.history[:] = np.arange(V)
+    rows.rep = reps
+    z = rng.integers(0, 2 ** 32, (B, V), dtype=np.uint64).astype(np.uint32).view(np.float32)
+    z[:, :V // 2] = (rng.standard_normal((B, V // 2)) * 10).astype(np.float32)
+    rows.logits.copy_(torch.from_numpy(z))
+    out, _ = rows.run()
+    with np.errstate(all="ignore"):
+        want = np.where(z > 0, z / reps[:, None], z * reps[:, None])
+    np.testing.assert_array_equal(out.cpu().numpy(), want)
+    no_device_error()
 
 
 def test_the_last_bias_of_a_token_counts(cuda):
