@@ -203,13 +203,26 @@ class DraftDecoder(PagedDecoder):
                 self.parents.copy_(torch.where(kv.requests >= 0, parents[at], -1))
             self.draft_starts.copy_(kv.token_starts)
             self.draft_state.copy_(kv.free_state)
-            self.tree.encode_plan(self.parents, kv.seq_lens, kv.token_starts, self.node_positions, self.ancestors,
-                                  self.max_query, position_base=kv.prefix_len, stream=stream)
-            if rules is not None:
-                history, biases = rules.get("history"), rules.get("bias_tokens")
-                need = self.rules.workspace_bytes(self.T, self.cfg.vocab, kv.num_requests,
-                                                  0 if history is None else history.shape[1],
-                                                  0 if biases is None else biases.numel())
+        try:
+            self._check_nodes(given, rules, stream)
+        except Exception:  # a refused step leaves the requests as long as they were
+            with torch.cuda.stream(stream):
+                kv.resize(kv.seq_lens - (self.draft_starts[1:] - self.draft_starts[:-1]), stream)
+            raise
+        kv.resize(self.targets, stream)
+        return self.counts, self.new_tokens
+
+    def _check_nodes(self, given, rules, stream):
+        """The nodes' positions, logits, choices and ways; self.targets: the lengths with the kept ones."""
+        kv = self.kv
+        self.tree.encode_plan(self.parents, kv.seq_lens, kv.token_starts, self.node_positions, self.ancestors,
+                              self.max_query, position_base=kv.prefix_len, stream=stream)
+        if rules is not None:
+            history, biases = rules.get("history"), rules.get("bias_tokens")
+            need = self.rules.workspace_bytes(self.T, self.cfg.vocab, kv.num_requests,
+                                              0 if history is None else history.shape[1],
+                                              0 if biases is None else biases.numel())
+            with torch.cuda.stream(stream):
                 self.rules_workspace = self._larger(self.rules_workspace, need)
         self._drafting = True
         try:
@@ -222,5 +235,3 @@ class DraftDecoder(PagedDecoder):
         self.accept.encode(self.ids, self.parents, self.tokens, kv.seq_lens, kv.token_starts, self.counts, self.paths,
                            self.new_tokens, self.targets, self.max_query, given=given, layers=kv.layers,
                            page_table=kv.page_table, stream=stream)
-        kv.resize(self.targets, stream)
-        return self.counts, self.new_tokens

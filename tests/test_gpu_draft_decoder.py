@@ -374,6 +374,12 @@ def test_refusals(cuda, model):
         DraftDecoder(weights, 8, cache, max_query=257)
     assert cache.seq_lens.tolist() == [0, 0]
     dec.draft(ids, parents, targets)
+    kept, free = cache.seq_lens.tolist(), cache.free_state[1].item()
+    for bad in (dict(repetition=torch.ones(3, device="cuda")), dict(temperature=1), dict(history=i32([[1], [2]])),
+                dict(allowed=i32(np.zeros((1, 1)))), dict(tokens=ids)):  # found when the nodes are there
+        with pytest.raises((TFError, TypeError)):
+            dec.draft(ids, parents, cache.seq_lens + i32([2, 1]), rules=bad)
+        assert cache.seq_lens.tolist() == kept and cache.free_state[1].item() == free
     dec.draft(ids[:0], parents[:0], i32([-1, -1]))  # nothing to do
     assert dec.counts.tolist() == [0, 0]
     no_device_error()
