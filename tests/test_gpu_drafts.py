@@ -501,6 +501,25 @@ def test_accept_of_chains_in_place(cuda):
     no_device_error()
 
 
+@pytest.mark.parametrize("layer_stride,page_stride", [((1 << 32) + 8, 64 * 64), (16 * 64, 1 << 30)])
+def test_accept_far_into_the_pools(cuda, layer_stride, page_stride):
+    """Elements beyond 2^32 of the first: by the layers' distance and by the pages'."""
+    d = Drafts([8, 5], [20, 5], 2, 2, 32, 16, seed=5, vocab=1)
+    layers, pages = d.k.shape[:2]
+    extent = (layers - 1) * layer_stride + (pages - 1) * page_stride + 16 * 64
+    answer, k, v = d.expected(8)
+    assert any(p >= 0 and p != i for path in answer[1] for i, p in enumerate(path))  # (something moves)
+    near, far = (d.k, d.v), []
+    for x in near:
+        far.append(torch.empty(extent, dtype=x.dtype, device="cuda").as_strided(x.shape, (layer_stride, page_stride, 64, 32, 1)))
+        far[-1].copy_(x)
+    d.k, d.v = far
+    for g, a in zip(d.run(8), answer):
+        assert np.array_equal(g, a)
+    assert torch.equal(d.k, k) and torch.equal(d.v, v)
+    no_device_error()
+
+
 def test_no_choice_ends_the_way(cuda):
     """A choice of -1 is no token, and meets no node, whatever was drafted."""
     d = Drafts([4], [4], 1, 2, 64, 4, seed=3, vocab=1)
