@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_parts_kernel(const __gr
 
 // kTree, requests of more than eight rows among them: everything on the tensor cores, without the
 // streaming warps' code and without counting their units.  A few requests of one or two nodes beside
-// such trees stream no faster than this (61 requests of 1 to 5 nodes, eight query heads a KV head: 39
-// us with those of one node streamed, their warps ending long after the tiles, 30 this way); 200
+// such trees stream no faster than this (61 requests of 1 to 5 nodes, eight query heads a KV head: 55
+// us with those of one node streamed, their warps ending long after the tiles, 39 this way); 200
 // requests of which one has more take 225 instead of 156 us (16 / 8 heads of 256).
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) tree_tiles_kernel(const __grid_constant__ AttnParams<T, true> p) {

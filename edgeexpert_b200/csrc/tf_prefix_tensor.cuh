@@ -235,7 +235,9 @@ struct TreeSegment {
     int row_tiles, units;
 };
 // kTree: what a job costs besides its units (Q in, the pipeline filled and drained, O out), as units:
-// the work is dealt by both, so that CTAs with many short jobs get fewer.
+// the work is dealt by both, so that CTAs with many short jobs get fewer.  24 trees of 20 to 40 behind
+// 4096 shared positions and up to 1000 of their own (16 / 4 heads of 128): 82 us; with 1 113, with 3 91,
+// with 12 86.  16 trees of 16 behind up to 4096 (16 / 8 heads of 256): 78, 96, 82 and 82.
 constexpr int kJobUnits = 6;
 template <typename T, bool kTree>
 __device__ __forceinline__ int tree_slots(const AttnParams<T, kTree>& p, const TreeSegment& s) {
@@ -307,14 +309,14 @@ struct TreeSums {
 };
 template <typename T, int N, int HD>
 __device__ __forceinline__ TreeSums tree_weights(const uint32_t* ancestors, int words, int node_at, int lo, int hi, int end,
-                                              uint32_t scol, uint32_t ocol, float sc, float m, float d, bool dry,
+                                              uint32_t scol, uint32_t ocol, float sc, float m, float d,
                                               uint64_t* o_done, uint32_t parity, volatile int* dead, uint32_t* err) {
     float s[N];
 #pragma unroll
     for (int i = 0; i < N; i += 32) tmem_ld32_async(scol + i, s + i);
     // the keys that the row sees, as bits
     uint32_t see[N / 32];
-    bool all = !dry;
+    bool all = true;
 #pragma unroll
     for (int w = 0; w < N / 32; ++w) {
         const int a = max(0, lo - 32 * w), z = min(32, hi - 32 * w);
@@ -338,7 +340,7 @@ __device__ __forceinline__ TreeSums tree_weights(const uint32_t* ancestors, int 
 #pragma unroll
     for (int i = 4; i < N; ++i) top4[i & 3] = fmaxf(top4[i & 3], s[i]);
     const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
-    if (__any_sync(0xffffffffu, top > m + 8.f) && !dry) {
+    if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float now = fmaxf(m, top);
         const float f = m == -INFINITY ? 1.f : exp2_approx(m - now);
         d *= f;
@@ -369,7 +371,7 @@ __device__ __forceinline__ TreeSums tree_weights(const uint32_t* ancestors, int 
             d4[(e & 2) + 1] += z;
             weights[e / 2] = Pair<T>::pack(a, z);
         }
-        if (!dry) tmem_st32(scol + i / 2, weights);
+        tmem_st32(scol + i / 2, weights);
     }
     return {m, d + ((d4[0] + d4[1]) + (d4[2] + d4[3])), 1};
 }
@@ -389,12 +391,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                                            int tile0, int tile_at, int tile_units, int worker) {
     using S = TensorShape<HD>;
     constexpr int N = S::kKeys;
-    // kTree: the warp without work goes with the rows' up to the weights of a unit, waits for nothing and
-    // leaves no trace.  A CTA's trees are twenty or thirty units, code is fetched anew by every launch, and
-    // the first unit took 5 to 9 us; it takes 1.5 to 3 when that has been done while the rows wait for
-    // their queries.
-    const bool ahead = kTree && threadIdx.x >> 5 > 6;
-    const int warp = ahead ? threadIdx.x >> 5 & 3 : threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kSlots; ++i) {
             for (int kv = 0; kv < 2; ++kv) {
@@ -615,7 +612,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
         // a commit covers all earlier MMAs, so the scores of unit uc being there means that
         // the phase before the one waited for here (unit uc - 3) is over.
         auto o_ready = [&]() { return wait_warp(&bar.o_done[(uc - 1) & 1], ((uc - 1) >> 1) & 1); };
-        Job job = ahead ? Job{0x7FFFFFFF, 0, 1, 0, 1, -1, 1, 0} : first_job();  // (ahead: a tile behind all rows)
+        Job job = first_job();
         for (int u = u0; ok && u < u1 && job.from < job.to;) {
             const long long row = (long long)job.tile * kTcRows + threadIdx.x;
             bool exists = row < (long long)p.T_tokens * p.G;
@@ -654,7 +651,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
             // nothing: their results go nowhere (a row of a product does not depend on another)
             const bool warp_live = !kTree || __any_sync(0xffffffffu, live);
             if (kTree && !live) row_hi = 0x7FFFFFFF;
-            if (!ahead) {  // Q to tensor memory
+            {  // Q to tensor memory
                 const T* q = p.q + t * p.q_stride + (long long)h * p.hd;
                 constexpr int kTogether = kTree ? HD / 2 : 32;  // words whose loads are in flight together
 #pragma unroll
@@ -680,7 +677,7 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
             TensorCursor c = tensor_begin<T, HD>(p, job.tile, job.from, job.seg);
             for (int x = job.from; x < job.to; ++x, ++uc) {
                 const int buf = uc & 1;
-                if (!ahead) ok = wait_warp(&bar.s_full[buf], (uc >> 1) & 1);
+                ok = wait_warp(&bar.s_full[buf], (uc >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t scol = mine + S::kColS + buf * N;
@@ -694,16 +691,16 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 lo = max(0, lo - key0);
                 hi = min(min(hi, c.hi) - key0, N);
                 if constexpr (kTree) {
-                    if (warp_live || ahead) {
+                    if (warp_live) {
                         const int node_at = live ? node0 - key0 : N;
                         uint64_t* const before = x > job.from ? &bar.o_done[(uc - 1) & 1] : nullptr;
                         const TreeSums sums = tree_weights<T, N, HD>(
                             p.ancestors + (long long)t * p.words, p.words, node_at, lo, hi, min(N, c.hi - key0), scol,
-                            mine + S::kColO, sc, m, d, ahead, before, ((uc - 1) >> 1) & 1, &bar.dead, p.err);
+                            mine + S::kColO, sc, m, d, before, ((uc - 1) >> 1) & 1, &bar.dead, p.err);
                         m = sums.m;
                         d = sums.d;
                         ok = sums.ok != 0;
-                        if (!ok || ahead) break;
+                        if (!ok) break;
                         tmem_wait_st();
                     }
                     tc_fence_before();
@@ -772,7 +769,6 @@ __device__ __forceinline__ void tensor_cta(const AttnParams<T, kTree>& p, uint32
                 mbar_arrive(&bar.p_full[buf]);
                 if (x + 1 < job.to) tensor_advance<T, HD>(p, job.tile, c);
             }
-            if (ahead) break;
             // ---- the job's part, or the result where nothing else belongs to it ------
             ok = ok && o_ready();
             if (!ok) break;
