@@ -35,7 +35,8 @@ struct PlanParams {
 // One CTA a request, one thread a node.  With up(i) a node that i's bits do not go
 // beyond yet, bits(i) |= bits(up(i)), up(i) = up(up(i)) doubles the length of way
 // covered, so a tree of 256 takes eight steps at most, whatever its shape; the depth
-// is the number of bits.
+// is the number of bits.  Bound by its launch: 1.7 us for one tree of 12, 2.2 us for 301
+// of up to 64, one after another in a graph.
 template <int W>
 __global__ void __launch_bounds__(W * 32) tree_plan_kernel(const PlanParams p) {
     __shared__ uint32_t bits[W * 32][W];
@@ -121,6 +122,8 @@ struct AcceptParams {
 // position path[k] to k of the request's own.  A thread takes its column's moves in order
 // and loads a few before it stores the first: what a store overwrites (k) is the source
 // of an earlier move than any that is still to be loaded (path[j] >= j > k).
+// One tree of 12 in 30 layers: 2.8 us, latency; 32 of 8 to 24, 42 MB in and out of L2: 6.8 us,
+// 6.2 TB/s (one after another in a graph).
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptParams p) {
     __shared__ int s_next[kMaxNodes], s_path[kMaxNodes], s_choice[kMaxNodes], s_count, s_same;
     __shared__ long long s_from[kMaxNodes], s_to[kMaxNodes];
