@@ -300,6 +300,33 @@ __device__ __forceinline__ bool wait_unless(uint64_t* bar, uint32_t parity, vola
     return true;
 }
 
+// Two fp32 numbers in one instruction, each as by itself.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 each_of(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // kTree: the weights of a unit's N keys for a row (the calling thread's), in place of its scores at
 // column `scol`, and m and d brought up to date; ok 0 if a wait gave up.  The row sees keys [lo, hi) and,
 // from key `node_at` on, the nodes of its `ancestors`, up to key `end`.  P is written over the scores.
@@ -338,7 +365,7 @@ __device__ __forceinline__ TreeSums tree_weights(const uint32_t* ancestors, int 
     }
     float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-    for (int i = 4; i < N; ++i) top4[i & 3] = fmaxf(top4[i & 3], s[i]);
+    for (int i = 4; i < N; i += 2) top4[i >> 1 & 3] = max_of(top4[i >> 1 & 3], s[i], s[i + 1]);
     const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
     if (__any_sync(0xffffffffu, top > m + 8.f)) {
         const float now = fmaxf(m, top);
@@ -360,20 +387,22 @@ __device__ __forceinline__ TreeSums tree_weights(const uint32_t* ancestors, int 
         }
     }
     const float ref = m == -INFINITY ? 0.f : m;
-    float d4[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint64_t sc2 = two(sc, sc), ref2 = two(-ref, -ref);
+    uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
     for (int i = 0; i < N; i += 64) {
         uint32_t weights[32];
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
-            const float a = exp2_approx(fmaf(s[i + e], sc, -ref)), z = exp2_approx(fmaf(s[i + e + 1], sc, -ref));
-            d4[e & 2] += a;
-            d4[(e & 2) + 1] += z;
+            const float2 x = each_of(fma_two(two(s[i + e], s[i + e + 1]), sc2, ref2));
+            const float a = exp2_approx(x.x), z = exp2_approx(x.y);
+            sums[e >> 1 & 1] = add_two(sums[e >> 1 & 1], two(a, z));
             weights[e / 2] = Pair<T>::pack(a, z);
         }
         tmem_st32(scol + i / 2, weights);
     }
-    return {m, d + ((d4[0] + d4[1]) + (d4[2] + d4[3])), 1};
+    const float2 sum = each_of(add_two(sums[0], sums[1]));
+    return {m, d + (sum.x + sum.y), 1};
 }
 
 struct TensorBarriers {
