@@ -350,6 +350,47 @@ def test_tree_attention_in_a_graph(cuda):
         batch.both = keep
 
 
+def test_tree_attention_calls_at_once(cuda):
+    """Two batches on two streams at the same time, each with a workspace of its own; nothing waits between."""
+    from edgeexpert_b200.drafts import TreeAttention
+    from edgeexpert_b200.paged import PagedKV
+    op, calls = TreeAttention(), []
+    for spec in ((513, [60, 131, 20, 900], [20, 40, 20, 1], 16, 4, 128, "bf16", 32), (0, [700, 30], [12, 9], 16, 8, 256, "fp16", 16)):
+        x = TreeBatch(*spec, seed=len(calls))
+        want, _ = x.run()
+        kv, mq, T, nq = PagedKV(x.k, x.v), max(x.counts), len(x.q), x.q.shape[1]
+        ws = torch.empty(op.workspace_bytes(kv, nq, T, len(x.lens), x.P, mq), dtype=torch.uint8, device="cuda")
+        prefix = i32(x.prefix_pages) if x.P else None
+        args = (x.q, kv, i32(x.table), i32(x.lens), i32(x.starts), x.ancestors)
+        calls.append((x, want, args, ws, prefix, mq, torch.cuda.Stream(), [torch.full_like(x.q, 7.0) for _ in range(20)]))
+    torch.cuda.synchronize()
+    for i in range(20):
+        for x, _, args, ws, prefix, mq, stream, outs in calls:
+            op.encode(*args, outs[i], ws, prefix_pages=prefix, prefix_len=x.P, max_query=mq, scale=x.scale, stream=stream)
+    torch.cuda.synchronize()
+    for _, want, *_, outs in calls:
+        assert all(torch.equal(out, want) for out in outs)
+    no_device_error()
+
+
+def test_no_tokens(cuda):
+    """A step in which nobody has a token: every operator takes it and writes what it has to."""
+    from edgeexpert_b200.drafts import DraftAccept, DraftTree, TreeAttention
+    from edgeexpert_b200.paged import PagedKV
+    none, starts, lens = i32([]), i32([0, 0, 0]), i32([5, 0])
+    DraftTree().encode_plan(none, lens, starts, none.clone(), i32(np.zeros((0, 1))), 4)
+    k = torch.zeros(2, 16, 2, 64, dtype=torch.float16, device="cuda")
+    op, kv, q = TreeAttention(), PagedKV(k, k.clone()), torch.zeros(0, 4, 64, dtype=torch.float16, device="cuda")
+    ws = torch.empty(max(16, op.workspace_bytes(kv, 4, 0, 2, 0, 4)), dtype=torch.uint8, device="cuda")
+    op.encode(q, kv, i32([[0], [-1]]), lens, starts, i32(np.zeros((0, 1))), q.clone(), ws, max_query=4)
+    counts, targets, paths, tokens = i32([7, 7]), i32([7, 7]), i32(np.full((2, 4), 7)), i32(np.full((2, 4), 7))
+    DraftAccept().encode(none, none, none, lens, starts, counts, paths, tokens, targets, max_query=4)
+    torch.cuda.synchronize()
+    assert counts.tolist() == [0, 0] and targets.tolist() == [-1, -1]
+    assert (paths == -1).all() and (tokens == -1).all()
+    no_device_error()
+
+
 def test_tree_attention_refusals(cuda):
     from edgeexpert_b200._lib import TFError
     from edgeexpert_b200.drafts import TreeAttention

@@ -290,6 +290,30 @@ def test_rules_in_a_graph(cuda):
         now.check(out, tokens)
 
 
+def test_calls_at_once_and_no_rows(cuda):
+    """Two batches on two streams at the same time, each with a workspace of its own; a batch of no rows."""
+    from edgeexpert_b200.sampling import LogitRules
+    op, calls = LogitRules(), []
+    for rows in (Rows([3, 30, 1], 50001, "bf16", history=(0, 3000), seed=1), Rows([1] * 9, 70000, "fp32", history=(9, 90), seed=2)):
+        want, chosen = rows.run()
+        ws = torch.empty(rows.workspace(op, len(rows.logits)), dtype=torch.uint8, device="cuda")
+        kw = dict(history=i32(rows.history), history_lens=i32(rows.lens), prompt_lens=i32(rows.prompt), max_query=30)
+        kw.update((n, torch.from_numpy(x).cuda()) for n, x in (("repetition", rows.rep), ("presence", rows.pres),
+                                                               ("frequency", rows.freq)))
+        outs = [(torch.full_like(rows.logits, 7.0), i32(np.full(len(rows.logits), 77))) for _ in range(20)]
+        calls.append((rows, want, chosen, ws, kw, i32(rows.starts), torch.cuda.Stream(), outs))
+    torch.cuda.synchronize()
+    for i in range(20):
+        for rows, _, _, ws, kw, starts, stream, outs in calls:
+            op.encode(rows.logits, outs[i][0], starts, ws, tokens=outs[i][1], stream=stream, **kw)
+    torch.cuda.synchronize()
+    for _, want, chosen, *_, outs in calls:
+        assert all(torch.equal(o, want) and torch.equal(t, chosen) for o, t in outs)
+    z = torch.zeros(0, 64, device="cuda")
+    op.encode(z, z, i32([0, 0]), calls[0][3], tokens=i32([]))
+    no_device_error()
+
+
 def test_lists_that_the_kernel_bounds(cuda):
     """Rows beyond the bound, masks that do not exist, lengths beyond their lists: reported or cut, not read."""
     rows = Rows([4, 2], 500, "fp32", history=(5, 5), biases=3)
