@@ -436,6 +436,16 @@ struct Place {
     __device__ __forceinline__ uint32_t barred(const Stage<T>& s, int g) const { return ~bits_of(s.mask, g) & ((1u << N) - 1u); }
 };
 
+// z / r, rounded as fp32 divides, without a branch (r_inverse: 1 / r in 64 bits).  z * r_inverse is off by
+// 2^-52 of the quotient at the most; a step of Newton's, whose remainder is exact, leaves no error but the
+// rounding to 64 bits.  That is no matter for the rounding to fp32: a quotient of two 24-bit numbers is on
+// a middle between two fp32 numbers, and then 64 bits hold it (only below the smallest normal number,
+// since a middle above has 25 bits), or 2^-49 of itself or more away.  Infinities have no remainder.
+__device__ __forceinline__ float quotient(float z, float r, double r_inverse) {
+    const double q = (double)z * r_inverse, rest = fma(-q, (double)r, (double)z), better = fma(rest, r_inverse, q);
+    return (float)(better == better ? better : q);
+}
+
 // How often a token was drafted on a row's way through its request's tree of `most` nodes at the most.
 __device__ __noinline__ int drafted_before(const int* starts, int rows, int most, const uint32_t* way, const int* ids,
                                            int token) {
@@ -452,12 +462,9 @@ __device__ __noinline__ int drafted_before(const int* starts, int rows, int most
 // The chunks of all rows, one after the other, are dealt evenly to the CTAs, which have the next
 // kStages - 1 of them on their way.  Bound by memory: the logits in and out.  A row's entries are
 // applied to the chunk in shared memory, four a thread together and without a branch, those of the
-// next chunk loaded meanwhile.  z / repetition is z * (1 / repetition) in 64 bits: a quotient of two
-// 24-bit numbers is 2^-49 of itself or more away from every middle between two fp32 numbers (or on
-// it), and the product is off by 2^-52 at the most, so it rounds as the quotient does.  The largest
-// value is looked for by granules, its place in the granule once a chunk.  Logits of 16 bits: an
-// entry's value is compared before it is rounded, and its place is left out of the comparison of
-// the others.
+// next chunk loaded meanwhile.  The largest value is looked for by granules, its place in the granule
+// once a chunk.  Logits of 16 bits: an entry's value is compared before it is rounded, and its place
+// is left out of the comparison of the others.
 // 256 rows of 262144 fp32 logits: 102 us, 5.3 TB/s; 64 rows without rules: 6.1 TB/s.
 // A CTA a chunk, whose dependent loads (request, entries, mask) lay between its logits and its end,
 // left the memory at 0.55 of its rate.  This one with 256 threads and four granules each took 1.4
@@ -610,7 +617,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
 #pragma unroll
                 for (int u = 0; u < kRead; ++u) {
                     const uint32_t e = x[u].x - (uint32_t)c0, count = x[u].y & kCount;
-                    const float divided = (float)((double)z[u] * rep_inverse), times = __fmul_rn(z[u], rep);
+                    const float divided = quotient(z[u], rep, rep_inverse), times = __fmul_rn(z[u], rep);
                     float r = count || (x[u].y & kInPrompt) ? (z[u] > 0.f ? divided : times) : z[u];
                     r = __fsub_rn(r, __fmul_rn(freq, (float)count));
                     r = count ? __fsub_rn(r, pres) : r;

@@ -252,6 +252,21 @@ def test_the_quotient_is_that_of_fp32(cuda):
     no_device_error()
 
 
+def test_quotients_half_way_between_the_smallest_numbers(cuda):
+    """Odd multiples of half the penalty, in steps of 2^-149: every quotient lies on a middle and goes to the
+    even neighbour."""
+    V, reps = 4000, np.float32([98, 150, 196, 206, 334, 6, 1022, 3998])
+    rows = Rows([1] * len(reps), V, "fp32", history=(V, V), prompt=1.0, factors=False)
+    rows.history[:] = np.arange(V)
+    rows.rep = reps
+    odd = np.arange(1, 2 * V, 2)
+    z = (odd[None] * (reps[:, None].astype(np.int64) // 2) * 2.0 ** -149).astype(np.float32)
+    rows.logits.copy_(torch.from_numpy(z))
+    out, _ = rows.run()
+    np.testing.assert_array_equal(out.cpu().numpy(), z / reps[:, None])
+    no_device_error()
+
+
 def test_the_last_bias_of_a_token_counts(cuda):
     rows = Rows([1, 1], 100, "fp32", history=(0, 0), factors=False)
     rows.bias = (np.array([0, 4, 7]), np.array([5, 5, 9, 5, 9, 100, -1]), np.array([1, 2, 3, 40, 50, 6, 7], np.float32))
