@@ -43,7 +43,8 @@ __device__ __noinline__ void attend_alone(const AttnParams<T, kTree>& p, int b, 
     int lo, hi;
     seen_by(p, r, j, lo, hi);
     const int end = kTree ? p.prefix_len + r.len : hi, node0 = p.prefix_len + r.len - r.n;
-    for (int pos = lo; pos < end; ++pos) {
+    // (kTree: positions far ahead leave nothing of the history, and the nodes all the same)
+    for (int pos = kTree ? min(lo, hi) : lo; pos < end; ++pos) {
         if (kTree && pos >= hi && !sees_node(p.ancestors + (long long)t * p.words, p.words, pos - node0)) continue;
         const bool shared = pos < p.prefix_len;
         const int at = shared ? pos : pos - p.prefix_len, in_page = at / p.kv.page_size;

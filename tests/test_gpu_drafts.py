@@ -286,6 +286,26 @@ def test_nodes_that_others_see(cuda, counts, hd):
         assert not np.isfinite(out[t][hit][..., 0]).any() and not np.isfinite(lse[t][hit][:, 2:4]).any()
 
 
+@pytest.mark.parametrize("counts,hd", [([6, 3], 256), ([40, 9], 128), ([3, 5], 64), ([3, 2], 512)])
+def test_windows_that_have_left_the_history(cuda, counts, hd):
+    """Positions far ahead of the history: the nodes alone are seen, also by rows that are computed by
+    themselves because a node beside them is infinite."""
+    lens = [c + 13 + 5 * i for i, c in enumerate(counts)]
+    trees = [np.minimum(np.arange(n) - 1, 1) for n in counts]  # 0 - 1 - {2, 3, ...}
+    batch = TreeBatch(40, lens, counts, 8, 4, hd, "fp16", 16, seed=12, masks=masks_of(trees))
+    batch.at = [a + 5000 for a in batch.at]
+    batch.positions = i32(np.concatenate(batch.at))
+    batch.check(*batch.run(window=64), window=64)
+    at = lens[0] - 1  # the last node of the first tree
+    batch.v[int(batch.table[0, at // 16]), at % 16] = float("inf")
+    out, _ = batch.run(window=64)
+    for b, n in enumerate(counts):
+        t, _, _, ro, _, A, s = batch.reference(b, 64)
+        fine = np.arange(n) != (n - 1 if b == 0 else -1)
+        assert (np.abs(f64(out)[t] - ro)[fine] <= ((2 * U[torch.float16] + 2 * s + 16 * E32) * A + 1e-4)[fine]).all()
+    no_device_error()
+
+
 def test_chains_are_the_causal_batch(cuda):
     """A chain's ancestors are all nodes before it: the ragged batch's causal attention."""
     counts = [5, 1, 3]
