@@ -592,6 +592,10 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
 
         // ---- the entries ---------------------------------------------------------------------
         if (any) {
+            // Places count from the row's own first token here: what the chunk has before it is of the row
+            // before, and the token of no entry (~0) is beyond any place, however the row lies.
+            T* const own = stage.x + lo;
+            const uint32_t own_first = (uint32_t)(c0 + lo), own_len = (uint32_t)(hi - lo);
             float said_best = -INFINITY;  // (of equals the first, which is the lower token)
             int said_token = 0;
 #pragma unroll 1
@@ -602,27 +606,27 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
                 uint32_t drafted = 0u;
 #pragma unroll
                 for (int u = 0; u < kRead; ++u) {
-                    const uint32_t e = x[u].x - (uint32_t)c0;
-                    z[u] = e < (uint32_t)hi ? to_float(stage.x[e]) : NAN;
+                    const uint32_t e = x[u].x - own_first;
+                    z[u] = e < own_len ? to_float(own[e]) : NAN;
                     drafted |= x[u].y & kDrafted;
                 }
                 if (drafted) {
 #pragma unroll
                     for (int u = 0; u < kRead; ++u)
-                        if ((x[u].y & kDrafted) && x[u].x - (uint32_t)c0 < (uint32_t)hi)
+                        if ((x[u].y & kDrafted) && x[u].x - own_first < own_len)
                             x[u].y += drafted_before(p.starts + b, p.T, min(p.max_query, p.words * 32),
                                                      p.ancestors + (long long)at.row * p.words, p.token_ids, (int)x[u].x);
                 }
                 float top = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < kRead; ++u) {
-                    const uint32_t e = x[u].x - (uint32_t)c0, count = x[u].y & kCount;
+                    const uint32_t e = x[u].x - own_first, count = x[u].y & kCount;
                     const float divided = quotient(z[u], rep, rep_inverse), times = __fmul_rn(z[u], rep);
                     float r = count || (x[u].y & kInPrompt) ? (z[u] > 0.f ? divided : times) : z[u];
                     r = __fsub_rn(r, __fmul_rn(freq, (float)count));
                     r = count ? __fsub_rn(r, pres) : r;
                     r = __fadd_rn(r, __uint_as_float(x[u].z));
-                    if (e < (uint32_t)hi) stage.x[e] = rounded<T>(r);
+                    if (e < own_len) own[e] = rounded<T>(r);
                     z[u] = r;
                     top = fmaxf(top, r);
                 }
