@@ -155,7 +155,7 @@ class DraftDecoder(PagedDecoder):
         self.parents, self.node_positions, self.ancestors = i32(T), i32(T), i32(T, -(-max_query // 32))
         self.counts, self.targets = i32(B), i32(B)
         self.paths, self.new_tokens = i32(B, max_query), i32(B, max_query)
-        self.draft_starts, self.draft_state = i32(B + 1), i32(4)
+        self.draft_starts, self.draft_state, self.mask_rows = i32(B + 1), i32(4), i32(T)
         self.rules_workspace = None
         self._drafting = False
 
@@ -180,9 +180,11 @@ class DraftDecoder(PagedDecoder):
         max_query).  parents: of each token the index of its parent among its request's, below its own,
         or -1 for the root (the first).  given (optional): how many leading tokens of each request are
         known and kept without a look, a prompt's for instance; 1, the root, without it.  rules: what
-        LogitRules.encode takes for the requests (history, repetition, biases, allowed for every row ...); the
-        drafted tokens count as said on their way down.  self.logits then holds the logits under the
-        rules, self.tokens the choice after every node.
+        LogitRules.encode takes for the requests (history, repetition, biases, allowed ...); allowed_rows is
+        of each token of the list the row of `allowed` that holds for the choice after it, -1: none (without
+        allowed_rows token t's row is t), whichever requests are refused.  The drafted tokens count as said
+        on their way down.  self.logits then holds the logits under the rules, self.tokens the choice after
+        every node.
 
         Returns (counts, new_tokens), on the device: how many nodes of each request are kept, and
         [requests][max_query] the counts - given + 1 tokens that are new, -1 behind them.  The last of
@@ -194,6 +196,11 @@ class DraftDecoder(PagedDecoder):
         self._check_step("DraftDecoder.draft", token_ids, targets, parents=parents, **more)
         if parents.numel() != token_ids.numel() or (given is not None and given.numel() != kv.num_requests):
             raise TFError(TF_ERR_INVALID_ARG, "DraftDecoder.draft: a parent for every token, given for every request")
+        allowed, rows = (None, None) if rules is None else (rules.get("allowed"), rules.get("allowed_rows"))
+        if rows is not None:
+            self._check_step("DraftDecoder.draft", token_ids, targets, allowed_rows=rows)
+        if (allowed if rows is None else rows) is not None and len(allowed if rows is None else rows) < len(token_ids):
+            raise TFError(TF_ERR_INVALID_ARG, "DraftDecoder.draft: a row of allowed tokens for every token")
         with torch.cuda.stream(stream):  # (None: the current one)
             self._make_workspace()
             at = self._resize(token_ids, targets, stream)
@@ -201,6 +208,12 @@ class DraftDecoder(PagedDecoder):
                 self.parents.fill_(-1)
             else:
                 self.parents.copy_(torch.where(kv.requests >= 0, parents[at], -1))
+            if allowed is not None:  # from the list's order to the rows of those that were granted
+                if at is None:
+                    self.mask_rows.fill_(-1)
+                else:
+                    self.mask_rows.copy_(torch.where(kv.requests >= 0, at if rows is None else rows[at], -1))
+                rules = {**rules, "allowed_rows": self.mask_rows}
             self.draft_starts.copy_(kv.token_starts)
             self.draft_state.copy_(kv.free_state)
         try:
