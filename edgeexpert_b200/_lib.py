@@ -100,7 +100,8 @@ class LogitRulesDesc(C.Structure):
         "history", "history_lens", "prompt_lens", "repetition", "presence", "frequency", "bias_starts", "bias_tokens",
         "bias_values", "allowed", "allowed_rows", "token_ids", "ancestors")] + [
         (n, C.c_uint64) for n in ("history_stride", "allowed_stride")] + [
-        (n, C.c_uint32) for n in ("max_history", "bias_count", "allowed_count", "words")]
+        (n, C.c_uint32) for n in ("max_history", "bias_count", "allowed_count", "words")] + [
+        ("prompt_nodes", C.c_void_p)]
 
 
 _P = C.c_void_p

@@ -2,7 +2,8 @@
 // logits of a ragged batch, and the token that is best under them (tf_logit_rules_apply).
 //
 // For a row of request b, with c = how often a token was said (in the output and on the
-// row's way through its drafted tree) and `known` = said or in the prompt:
+// row's way through its drafted tree, where its first nodes may be a prompt's) and `known` = said or in
+// the prompt:
 //   z = logit;  known: z = z > 0 ? z / repetition : z * repetition;
 //   z -= frequency * c;  c > 0: z -= presence;  z += bias;  not allowed: -infinity.
 // Each step is rounded to fp32 by itself (no contraction), so what a user computes with
@@ -57,6 +58,7 @@ struct RulesParams {
     const int* allowed_rows;
     const int* token_ids;
     const uint32_t* ancestors;
+    const int* prompt_nodes;
     int* tokens;
     Gathered g;
     uint32_t* err;
@@ -137,6 +139,7 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
     griddep_launch_dependents();  // after the wait: the next kernel may read the logits at once
     const int s0 = p.starts[b], s1 = p.starts[b + 1];
     const int lens = p.history ? p.history_lens[b] : 0, prompts = p.prompt_lens ? p.prompt_lens[b] : 0;
+    const int first_nodes = p.prompt_nodes ? p.prompt_nodes[b] : 0;
     const int bias0 = p.bias_count ? p.bias_starts[b] : 0, bias1 = p.bias_count ? p.bias_starts[b + 1] : 0;
     const int start = max(0, min(s0, p.T)), n = max(start, min(s1, p.T)) - start, used = min(n, p.max_query);
     if (n > used && tid == 0) atomicOr(p.err, kErrBadTree);
@@ -151,6 +154,7 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
     }
     if (used == 0) return;
     const int nodes = p.token_ids ? min(used, p.words * 32) : 0;
+    const bool in_prompt = tid < first_nodes;  // this thread's node
     const int len = max(0, min(lens, p.max_history)), prompt = max(0, min(prompts, len));
     const int b0 = max(0, min(bias0, p.bias_count)), b1 = max(b0, min(bias1, p.bias_count));
     // what the threads need of the lists, all of it asked for at once
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
     history.each([&](int token, int at) { mark(at < prompt ? asked : known, token); });
     if (b0 + tid < b1) mark(known, bias_token);
     for (int i = b0 + kGatherThreads + tid; i < b1; i += kGatherThreads) mark(known, p.bias_tokens[i]);
-    if (tid < nodes) mark(known, drafted);
+    if (tid < nodes) mark(in_prompt ? asked : known, drafted);
     __syncthreads();
 
     // ranks: thread i has the words [i * per, (i + 1) * per)
@@ -239,14 +243,14 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
         if (tid < nodes)
             with_rank(drafted, [&](uint32_t k) {
                 token_of[k] = (uint32_t)drafted;
-                atomicOr(&said[k], kDrafted);
+                if (!in_prompt) atomicOr(&said[k], kDrafted);
             });
         __syncthreads();
 #pragma unroll 4
         for (int k = tid; k < ranks; k += kGatherThreads) {
             const uint32_t e = token_of[k];
-            const bool in_prompt = asked[e >> 5] >> (e & 31) & 1u;
-            p.g.entries[base + k0 + k] = make_uint4(e, said[k] | (in_prompt ? kInPrompt : 0u), 0u, 0u);
+            const uint32_t flag = asked[e >> 5] >> (e & 31) & 1u ? kInPrompt : 0u;
+            p.g.entries[base + k0 + k] = make_uint4(e, said[k] | flag, 0u, 0u);
         }
         __syncthreads();
         if (b0 < b1 || k0 + p.window < listed) {
@@ -446,15 +450,17 @@ __device__ __forceinline__ float quotient(float z, float r, double r_inverse) {
     return (float)(better == better ? better : q);
 }
 
-// How often a token was drafted on a row's way through its request's tree of `most` nodes at the most.
-__device__ __noinline__ int drafted_before(const int* starts, int rows, int most, const uint32_t* way, const int* ids,
-                                           int token) {
+// How often a token was drafted on a row's way through its request's tree of `most` nodes at the most,
+// the prompt's left out.
+__device__ __noinline__ int drafted_before(const int* starts, int rows, int most, const int* prompt_nodes,
+                                           const uint32_t* way, const int* ids, int token) {
     const int start = max(0, min(starts[0], rows)), nodes = min(min(max(start, starts[1]), rows) - start, most);
+    const int first = prompt_nodes ? *prompt_nodes : 0;
     int count = 0;
     for (int w = 0; w * 32 < nodes; ++w)
         for (uint32_t m = way[w]; m; m &= m - 1) {
             const int j = w * 32 + __ffs(m) - 1;
-            if (j < nodes) count += ids[start + j] == token;
+            if (j >= first && j < nodes) count += ids[start + j] == token;
         }
     return count;
 }
@@ -615,6 +621,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
                     for (int u = 0; u < kRead; ++u)
                         if ((x[u].y & kDrafted) && x[u].x - own_first < own_len)
                             x[u].y += drafted_before(p.starts + b, p.T, min(p.max_query, p.words * 32),
+                                                     p.prompt_nodes ? p.prompt_nodes + b : nullptr,
                                                      p.ancestors + (long long)at.row * p.words, p.token_ids, (int)x[u].x);
                 }
                 float top = -INFINITY;
@@ -820,6 +827,8 @@ tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t log
         return fail(ctx, TF_ERR_INVALID_ARG, "%s: a row of allowed tokens for every row", name);
     if (!r.token_ids != !r.ancestors)
         return fail(ctx, TF_ERR_INVALID_ARG, "%s: drafted tokens and their ancestors go together", name);
+    if (r.prompt_nodes && !r.token_ids)
+        return fail(ctx, TF_ERR_INVALID_ARG, "%s: a prompt among no drafted tokens", name);
     if (r.token_ids && (max_query > (uint32_t)kMaxNodes || r.words > 0xFFFFu || r.words * 32 < max_query))
         return fail(ctx, TF_ERR_INVALID_ARG, "%s: trees of up to %d nodes, a bit for each", name, kMaxNodes);
     const size_t size = dtype == TF_DTYPE_F32 ? 4 : 2;
@@ -827,7 +836,7 @@ tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t log
         return fail(ctx, TF_ERR_MISALIGNED, "%s: logits and out aligned to their elements", name);
     const void* all[] = {token_starts, r.history, r.history_lens, r.prompt_lens, r.repetition, r.presence, r.frequency,
                          r.bias_starts, r.bias_tokens, r.bias_values, r.allowed, r.allowed_rows, r.token_ids,
-                         r.ancestors, tokens};
+                         r.ancestors, r.prompt_nodes, tokens};
     for (const void* ptr : all)
         if (!aligned4(ptr)) return fail(ctx, TF_ERR_MISALIGNED, "%s: pointers must be 4-byte aligned", name);
     const uint32_t max_history = r.history ? r.max_history : 0;
@@ -856,6 +865,7 @@ tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t log
     p.allowed_rows = static_cast<const int*>(r.allowed_rows);
     p.token_ids = static_cast<const int*>(r.token_ids);
     p.ancestors = static_cast<const uint32_t*>(r.ancestors);
+    p.prompt_nodes = static_cast<const int*>(r.prompt_nodes);
     p.tokens = static_cast<int*>(tokens);
     uint8_t* const w = static_cast<uint8_t*>(workspace);
     p.g.request = reinterpret_cast<int*>(w + l.request);

@@ -182,9 +182,11 @@ class DraftDecoder(PagedDecoder):
         known and kept without a look, a prompt's for instance; 1, the root, without it.  rules: what
         LogitRules.encode takes for the requests (history, repetition, biases, allowed ...); allowed_rows is
         of each token of the list the row of `allowed` that holds for the choice after it, -1: none (without
-        allowed_rows token t's row is t), whichever requests are refused.  The drafted tokens count as said
-        on their way down.  self.logits then holds the logits under the rules, self.tokens the choice after
-        every node.
+        allowed_rows token t's row is t), whichever requests are refused.  The tokens, the root's too, count
+        as said on their way down, so that `history` ends before the root; those of a request whose given is
+        above 1 count as its prompt (prompt_nodes says otherwise: of each request how many of its first
+        tokens are the prompt's, 1 for a prompt of one token, 0 for known tokens of the output).  self.logits
+        then holds the logits under the rules, self.tokens the choice after every node.
 
         Returns (counts, new_tokens), on the device: how many nodes of each request are kept, and
         [requests][max_query] the counts - given + 1 tokens that are new, -1 behind them.  The last of
@@ -214,6 +216,8 @@ class DraftDecoder(PagedDecoder):
                 else:
                     self.mask_rows.copy_(torch.where(kv.requests >= 0, at if rows is None else rows[at], -1))
                 rules = {**rules, "allowed_rows": self.mask_rows}
+            if rules is not None and given is not None and rules.get("prompt_nodes") is None:
+                rules = {**rules, "prompt_nodes": torch.where(given > 1, given, 0)}
             self.draft_starts.copy_(kv.token_starts)
             self.draft_state.copy_(kv.free_state)
         try:

@@ -91,13 +91,15 @@ class LogitRules:
     def encode(self, logits, out, token_starts, workspace, max_query: int = 1, history=None, history_lens=None,
                prompt_lens=None, repetition=None, presence=None, frequency=None, bias_starts=None, bias_tokens=None,
                bias_values=None, allowed=None, allowed_rows=None, token_ids=None, ancestors=None, tokens=None,
-               stream=None):
+               stream=None, prompt_nodes=None):
         """logits, out [T][vocab] (out may be logits): rows token_starts[b] .. token_starts[b+1] are request
         b's.  history [requests][longest] with history_lens: the requests' tokens, the first prompt_lens of
         them their prompts.  repetition, presence, frequency: float32, one a request.  bias_*: the entries of
         request b are bias_starts[b] .. bias_starts[b+1].  allowed: rows of 32 tokens a word, allowed_rows which
         of them is a row's (-1: none).  token_ids [T], ancestors [T][words]: a drafted tree's tokens, each row's
-        way being part of its output.  tokens (optional): int32 [T], the best token of each row or -1."""
+        way being part of its output (so that a history ends before the root); prompt_nodes [requests]: so many
+        of the first nodes are the prompt's instead.  tokens (optional): int32 [T], the best token of each row
+        or -1."""
         def refuse(why):
             raise TFError(TF_ERR_INVALID_ARG, "LogitRules.encode: " + why)
 
@@ -140,6 +142,9 @@ class LogitRules:
             d.words = ancestors.shape[1]
             d.token_ids = place(token_ids, i32, T, "token_ids")
             d.ancestors = place(ancestors, i32, T * d.words, "ancestors")
+            d.prompt_nodes = place(prompt_nodes, i32, B, "prompt_nodes")
+        elif prompt_nodes is not None:
+            refuse("a prompt among no drafted tokens")
         st = self.call(self.ctx.handle, self._here(logits, "logits"), logits.stride(0), self._here(out, "out"), out.stride(0),
                        _LOGITS[logits.dtype], V, T, place(token_starts, i32, B + 1, "token_starts"), B, max_query, C.byref(d),
                        place(tokens, i32, T, "tokens"), self._here(workspace, "workspace"), workspace.nbytes,

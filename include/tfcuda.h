@@ -642,7 +642,9 @@ TF_API tf_status tf_tree_attention(tf_context* ctx, const void* q, uint64_t q_st
  *   allowed (uint32[allowed_count][allowed_stride]): bit v (word v / 32) = token v is allowed;
  *     allowed_rows (int32[T]): the row's row of allowed, -1: none (NULL: row t)
  *   token_ids (int32[T]) and ancestors (uint32[T][words]): the tokens of a drafted tree; the tokens of a
- *     row's ancestors are part of its output
+ *     row's ancestors (its own among them: a history ends before the root) are part of its output
+ *   prompt_nodes (int32[B], with the two): so many of the request's first nodes are part of its prompt
+ *     instead, for all of its rows
  * Tokens outside [0, V) have no effect. */
 typedef struct {
     const void* history;
@@ -660,6 +662,7 @@ typedef struct {
     const void* ancestors;
     uint64_t history_stride, allowed_stride;
     uint32_t max_history, bias_count, allowed_count, words;
+    const void* prompt_nodes;
 } tf_logit_rules;
 
 /* For every row and token v, c = how often v is in the row's output:

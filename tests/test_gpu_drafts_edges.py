@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from test_gpu_draft_decoder import VOCAB, Round, make, model, padded  # noqa: F401 (model: a fixture)
+from test_gpu_drafts import way, words_of
 from test_gpu_logit_rules import Rows
 from test_gpu_paged import i32, no_device_error
 
@@ -61,6 +62,94 @@ def test_nothing_is_left_beside_larger_rows(cuda, dtype, offset):
     out, chosen = rows.run(logits=view)
     rows.check(out, chosen)
     assert chosen.tolist() == [3, 3, 3, -1, 39, 39]
+    no_device_error()
+
+
+# ------------------------------------------------ prompts among the nodes ----
+def prompts_as_history(rows, first):
+    """The same rules with the first nodes' tokens in the history's prompt, and no tokens of their own."""
+    n = np.minimum(first, rows.counts).clip(0)
+    wide = np.full((len(n), rows.history.shape[1] + max(n)), -1)
+    drafted = rows.drafted.copy()
+    for b, k in enumerate(n):
+        at, cut = rows.starts[b], rows.prompt[b]
+        line = np.concatenate([rows.history[b, :cut], drafted[at:at + k], rows.history[b, cut:]])
+        wide[b, :len(line)] = line
+        drafted[at:at + k] = -1
+    rows.history, rows.lens, rows.prompt, rows.drafted = wide, rows.lens + n, rows.prompt + n, drafted
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("counts,first,V", [([5, 9, 1, 1, 0, 7], [3, 1, 1, 0, 2, 99], 1000), ([60, 256], [40, -3], 97),
+                                            ([12], [12], 20001)])
+def test_first_nodes_that_are_a_prompt(cuda, dtype, counts, first, V):
+    """The same bits as with those tokens in the history's prompt, and these are the definition's."""
+    from edgeexpert_b200.sampling import LogitRules
+    op, rows = LogitRules(), Rows(counts, V, dtype, history=(0, 20), prompt=0.3, biases=5, trees=True, seed=V)
+    T, B = len(rows.logits), len(counts)
+    f32 = [torch.from_numpy(x).cuda() for x in (rows.rep, rows.pres, rows.freq, rows.bias[2])]
+    out, tokens = torch.full_like(rows.logits, 7.0), i32(np.full(T, 77))
+    ws = torch.empty(rows.workspace(op, T), dtype=torch.uint8, device="cuda")
+    op.encode(rows.logits, out, i32(rows.starts), ws, max_query=max(counts), history=i32(rows.history),
+              history_lens=i32(rows.lens), prompt_lens=i32(rows.prompt), repetition=f32[0], presence=f32[1],
+              frequency=f32[2], bias_starts=i32(rows.bias[0]), bias_tokens=i32(rows.bias[1]), bias_values=f32[3],
+              token_ids=i32(rows.drafted), ancestors=words_of(rows.masks, -(-max(counts) // 32)), tokens=tokens,
+              prompt_nodes=i32(first))
+    prompts_as_history(rows, np.array(first))
+    want, chosen = rows.run()
+    rows.check(want, chosen)
+    assert torch.equal(out, want) and torch.equal(tokens, chosen)
+    no_device_error()
+
+
+def test_prompt_nodes_refusals(cuda):
+    from edgeexpert_b200._lib import TFError
+    from edgeexpert_b200.sampling import LogitRules
+    op, z = LogitRules(), torch.zeros(2, 64, device="cuda")
+    ws = torch.empty(op.workspace_bytes(2, 64, 2), dtype=torch.uint8, device="cuda")
+    one = i32([1, 1])
+    for bad in (dict(prompt_nodes=one), dict(prompt_nodes=one[:1], token_ids=one, ancestors=one[:, None]),
+                dict(prompt_nodes=one.long(), token_ids=one, ancestors=one[:, None]),
+                dict(prompt_nodes=one.cpu(), token_ids=one, ancestors=one[:, None])):
+        with pytest.raises(TFError):
+            op.encode(z, z, i32([0, 1, 2]), ws, **bad)
+    no_device_error()
+
+
+@pytest.mark.parametrize("given,prompt_nodes,asked", [([5, 1, 3], None, [5, 0, 3]), (None, None, [0, 0, 0]),
+                                                      ([5, 1, 3], [5, 1, 0], [5, 1, 0])])
+def test_a_prompt_in_a_step_is_no_output(cuda, model, given, prompt_nodes, asked):  # noqa: F811
+    """Logits under penalties are the plain step's after fp32 steps of the definition: on a prompt's tokens the
+    repetition penalty alone, on the others of a row's way all of them."""
+    weights, _ = model
+    rng = np.random.default_rng(3)
+    counts = [9, 6, 7]
+    trees = [np.concatenate([np.arange(g) - 1, rng.integers(g - 1, np.arange(g, n))])
+             for g, n in zip(given or [1, 1, 1], counts)]
+    tokens = rng.integers(6, size=22)  # few, so that they come again
+    dec, cache = make(weights, 3, 24, 4, 24, 4, 16)
+    rep, pres, freq = np.float32([1.25, 2, 1.5]), np.float32([0.5, 1, -0.25]), np.float32([0.25, -0.5, 2])
+    kw = dict(given=None if given is None else i32(given))
+    args = i32(tokens), i32(np.concatenate(trees)), i32(counts)
+    dec.draft(*args, **kw)
+    plain = dec.logits[:22].cpu().numpy().copy()
+    cache.resize(i32([0, 0, 0]))
+    rules = dict(zip(("repetition", "presence", "frequency"), (torch.from_numpy(x).cuda() for x in (rep, pres, freq))))
+    if prompt_nodes is not None:
+        rules["prompt_nodes"] = i32(prompt_nodes)
+    dec.draft(*args, **kw, rules=rules)
+    got, starts = dec.logits[:22].cpu().numpy(), np.concatenate([[0], np.cumsum(counts)])
+    for b, tree in enumerate(trees):
+        ids = tokens[starts[b]:starts[b + 1]].tolist()
+        for i in range(len(tree)):
+            prompt, said = ids[:asked[b]], [ids[j] for j in way(tree, i) if j >= asked[b]]
+            want = plain[starts[b] + i].copy()
+            for t in set(prompt + said):
+                z, c = want[t], np.float32(said.count(t))
+                z = z / rep[b] if z > 0 else z * rep[b]
+                want[t] = z - freq[b] * c - (pres[b] if c else np.float32(0))
+            np.testing.assert_array_equal(got[starts[b] + i], want)
+            assert int(dec.tokens[starts[b] + i]) == int(want.argmax())
     no_device_error()
 
 
