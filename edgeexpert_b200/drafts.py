@@ -152,6 +152,8 @@ class DraftDecoder(PagedDecoder):
 
         self.tree, self.tree_attention = DraftTree(self.ctx), TreeAttention(self.ctx)
         self.rules, self.accept = LogitRules(self.ctx), DraftAccept(self.ctx)
+        self.rules_checks = LogitRules(self.ctx)
+        self.rules_checks.call = lambda *args: 0  # the rules' checks alone, before a step changes anything
         self.parents, self.node_positions, self.ancestors = i32(T), i32(T), i32(T, -(-max_query // 32))
         self.counts, self.targets = i32(B), i32(B)
         self.paths, self.new_tokens = i32(B, max_query), i32(B, max_query)
@@ -205,6 +207,13 @@ class DraftDecoder(PagedDecoder):
             raise TFError(TF_ERR_INVALID_ARG, "DraftDecoder.draft: a row of allowed tokens for every token")
         with torch.cuda.stream(stream):  # (None: the current one)
             self._make_workspace()
+            if rules is not None:
+                if allowed is not None:
+                    rules = {**rules, "allowed_rows": self.mask_rows}
+                if given is not None and rules.get("prompt_nodes") is None:
+                    rules = {**rules, "prompt_nodes": torch.where(given > 1, given, 0)}
+                self._make_rules_workspace(rules)
+                self._apply(self.rules_checks, rules, stream)
             at = self._resize(token_ids, targets, stream)
             if at is None:
                 self.parents.fill_(-1)
@@ -215,40 +224,42 @@ class DraftDecoder(PagedDecoder):
                     self.mask_rows.fill_(-1)
                 else:
                     self.mask_rows.copy_(torch.where(kv.requests >= 0, at if rows is None else rows[at], -1))
-                rules = {**rules, "allowed_rows": self.mask_rows}
-            if rules is not None and given is not None and rules.get("prompt_nodes") is None:
-                rules = {**rules, "prompt_nodes": torch.where(given > 1, given, 0)}
             self.draft_starts.copy_(kv.token_starts)
             self.draft_state.copy_(kv.free_state)
         try:
             self._check_nodes(given, rules, stream)
-        except Exception:  # a refused step leaves the requests as long as they were
+        except Exception:  # what does not fail for the step's arguments, which are checked: no nodes are left
             with torch.cuda.stream(stream):
                 kv.resize(kv.seq_lens - (self.draft_starts[1:] - self.draft_starts[:-1]), stream)
             raise
         kv.resize(self.targets, stream)
         return self.counts, self.new_tokens
 
+    def _make_rules_workspace(self, rules):
+        history, biases = rules.get("history"), rules.get("bias_tokens")
+        need = self.rules.workspace_bytes(self.T, self.cfg.vocab, self.kv.num_requests,
+                                          0 if history is None else history.shape[-1],
+                                          0 if biases is None else biases.numel())
+        if need == 0:
+            raise TFError(TF_ERR_INVALID_ARG, f"DraftDecoder.draft: no rules for {self.cfg.vocab} tokens")
+        self.rules_workspace = self._larger(self.rules_workspace, need)
+
+    def _apply(self, operator: LogitRules, rules, stream):
+        operator.encode(self.logits, self.logits, self.kv.token_starts, self.rules_workspace, max_query=self.max_query,
+                        token_ids=self.ids, ancestors=self.ancestors, tokens=self.tokens, stream=stream, **rules)
+
     def _check_nodes(self, given, rules, stream):
         """The nodes' positions, logits, choices and ways; self.targets: the lengths with the kept ones."""
         kv = self.kv
         self.tree.encode_plan(self.parents, kv.seq_lens, kv.token_starts, self.node_positions, self.ancestors,
                               self.max_query, position_base=kv.prefix_len, stream=stream)
-        if rules is not None:
-            history, biases = rules.get("history"), rules.get("bias_tokens")
-            need = self.rules.workspace_bytes(self.T, self.cfg.vocab, kv.num_requests,
-                                              0 if history is None else history.shape[1],
-                                              0 if biases is None else biases.numel())
-            with torch.cuda.stream(stream):
-                self.rules_workspace = self._larger(self.rules_workspace, need)
         self._drafting = True
         try:
             self._run_rows(stream)
         finally:
             self._drafting = False
         if rules is not None:
-            self.rules.encode(self.logits, self.logits, kv.token_starts, self.rules_workspace, max_query=self.max_query,
-                              token_ids=self.ids, ancestors=self.ancestors, tokens=self.tokens, stream=stream, **rules)
+            self._apply(self.rules, rules, stream)
         self.accept.encode(self.ids, self.parents, self.tokens, kv.seq_lens, kv.token_starts, self.counts, self.paths,
                            self.new_tokens, self.targets, self.max_query, given=given, layers=kv.layers,
                            page_table=kv.page_table, stream=stream)

@@ -211,3 +211,33 @@ def test_masks_for_too_few_tokens_are_refused(cuda, model):  # noqa: F811
     dec.draft(ids, parents, targets, rules=dict(allowed=bits))  # a row of the step is nobody's
     assert dec.tokens[:3].tolist() == [-1] * 3 and dec.counts.tolist() == [1]
     no_device_error()
+
+
+def test_refused_rules_change_nothing(cuda, model):  # noqa: F811
+    """A step whose rules are refused shortens no request that its targets would shorten, and moves no page."""
+    from edgeexpert_b200._lib import TFError
+    weights, _ = model
+    dec, cache = make(weights, 3, 24, 6, 24, 4, 8)
+    ids, parents = i32(np.arange(20)), i32([-1, 0, 0, 2, 1] * 4)
+    dec.draft(ids[:15], parents[:15], i32([5, 5, 5]), given=i32([5, 5, 5]))
+
+    def state():
+        torch.cuda.synchronize()
+        return [t.clone() for t in (cache.seq_lens, cache.page_table, cache.free_ring, cache.free_state)]
+
+    before = state()
+    assert before[0].tolist() == [5, 5, 5]
+    f, words = torch.ones(3, device="cuda"), -(-VOCAB // 32)
+    bits = i32(np.full((5, words), -1))
+    for bad in (dict(repetition=f[:2]), dict(presence=f.double()), dict(frequency=f.cpu()), dict(temperature=1.0),
+                dict(history=i32(np.zeros((3, 4)))), dict(history=i32(np.zeros((1, 4))).expand(3, 4), history_lens=i32([4] * 3)),
+                dict(history=i32(np.zeros(3)), history_lens=i32([0] * 3)), dict(allowed=bits[:1].expand(5, words)),
+                dict(allowed=bits[:, :-1]), dict(allowed=bits[:4]), dict(allowed=bits, allowed_rows=i32([0])),
+                dict(bias_tokens=i32([1])), dict(prompt_nodes=i32([1])), dict(prompt_nodes=f), dict(tokens=ids),
+                dict(bias_starts=i32([0, 0, 0, 1]), bias_tokens=i32([1]), bias_values=f[:0])):
+        with pytest.raises((TFError, TypeError)):
+            dec.draft(ids[:5], parents[:5], i32([2, 10, 0]), rules=bad)
+        assert all(torch.equal(a, b) for a, b in zip(before, state())), bad
+    dec.draft(ids[:5], parents[:5], i32([2, 10, 0]), rules=dict(allowed=bits, repetition=f))
+    assert cache.seq_lens.tolist()[0] == 2 and cache.seq_lens.tolist()[1] >= 6 and cache.seq_lens.tolist()[2] == 0
+    no_device_error()
