@@ -75,10 +75,11 @@ class LogitRules:
             raise TFError(TF_ERR_INVALID_ARG, f"LogitRules.encode: {what}: {n} contiguous values of {dtype}")
         return self._here(t, what)
 
-    def _matrix(self, t, rows: int, least: int, what: str):
-        """Where an int32 matrix is, whose rows have `least` values of their own."""
+    def _matrix(self, t, rows: int, what: str, least: int | None = None):
+        """Where an int32 matrix is, whose rows have all of their values, or the first `least`, to themselves."""
         if t.dtype is not torch.int32 or t.dim() != 2 or (rows >= 0 and t.shape[0] != rows) or (
-                t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < least):
+                t.shape[1] > 1 and t.stride(1) != 1) or (
+                t.shape[0] > 1 and t.stride(0) < (t.shape[1] if least is None else least)):
             raise TFError(TF_ERR_INVALID_ARG, f"LogitRules.encode: {what} must be an int32 matrix, rows contiguous")
         return self._here(t, what)
 
@@ -114,7 +115,7 @@ class LogitRules:
         if history is not None:
             if history_lens is None:
                 refuse("a history has lengths")
-            d.history, d.history_stride, d.max_history = self._matrix(history, B, history.shape[-1], "history"), history.stride(0), history.shape[1]
+            d.history, d.history_stride, d.max_history = self._matrix(history, B, "history"), history.stride(0), history.shape[1]
             d.history_lens = place(history_lens, i32, B, "history_lens")
             d.prompt_lens = place(prompt_lens, i32, B, "prompt_lens")
         elif history_lens is not None or prompt_lens is not None:
@@ -130,10 +131,14 @@ class LogitRules:
             d.bias_tokens = place(bias_tokens, i32, n, "bias_tokens")
             d.bias_values = place(bias_values, f32, n, "bias_values")
         if allowed is not None:
-            d.allowed, d.allowed_stride, d.allowed_count = self._matrix(allowed, -1, -(-V // 32), "allowed"), allowed.stride(0), allowed.shape[0]
+            d.allowed, d.allowed_stride, d.allowed_count = self._matrix(allowed, -1, "allowed", -(-V // 32)), allowed.stride(0), allowed.shape[0]
             if allowed.shape[1] * 32 < V:
                 refuse("allowed must have a bit for every token")
             d.allowed_rows = place(allowed_rows, i32, T, "allowed_rows")
+            if not allowed.shape[0]:  # (an empty tensor is nowhere: a place that is not read, since no row is there)
+                if T and allowed_rows is None:
+                    refuse("a row of allowed tokens for every row")
+                d.allowed, d.allowed_stride = d.allowed_rows, 0
         elif allowed_rows is not None:
             refuse("rows of no allowed tokens")
         if token_ids is not None or ancestors is not None:

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_gpu_draft_decoder import VOCAB, Round, make, model, padded  # noqa: F401 (model: a fixture)
-from test_gpu_drafts import way, words_of
+from test_gpu_drafts import flags, way, words_of
 from test_gpu_logit_rules import Rows
 from test_gpu_paged import i32, no_device_error
 
@@ -62,6 +62,25 @@ def test_nothing_is_left_beside_larger_rows(cuda, dtype, offset):
     out, chosen = rows.run(logits=view)
     rows.check(out, chosen)
     assert chosen.tolist() == [3, 3, 3, -1, 39, 39]
+    no_device_error()
+
+
+def test_masks_without_a_row(cuda):
+    """No rows of allowed tokens are rows for nobody: refused, or, where rows are named, reported."""
+    from edgeexpert_b200._lib import TFError
+    from edgeexpert_b200.sampling import LogitRules
+    op, z = LogitRules(), torch.randn(3, 70, device="cuda")
+    ws = torch.empty(op.workspace_bytes(3, 70, 3), dtype=torch.uint8, device="cuda")
+    out, starts, nobody = torch.empty_like(z), i32([0, 1, 2, 3]), torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+    with pytest.raises(TFError):
+        op.encode(z, out, starts, ws, allowed=nobody)
+    op.encode(z, out, starts, ws, allowed=nobody, allowed_rows=i32([-1, -1, -1]))
+    torch.cuda.synchronize()
+    assert torch.equal(out, z)
+    no_device_error()
+    op.encode(z, out, starts, ws, allowed=nobody, allowed_rows=i32([-1, 0, -1]))
+    assert flags() and torch.equal(out, z)
+    op.encode(z[:0], out[:0], i32([0, 0]), ws, allowed=nobody)
     no_device_error()
 
 
