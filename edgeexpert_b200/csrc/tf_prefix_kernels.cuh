@@ -698,9 +698,13 @@ tf_status attention_call(tf_context* ctx, const tf_paged_kv* kv, const Attention
     }
     const uint64_t G = num_q_heads / kv->num_kv_heads;
     const Shape shape = shape_of_call(kv, num_q_heads, T, prefix_len, max_query, kTree);
-    const uint64_t row_tiles = T * G / shape.few_rows + std::min<uint64_t>(T, num_requests);
-    const uint64_t tiles = (uint64_t)max_pages * kv->page_size / 16 + prefix_len / 16 + 2;
-    if (row_tiles * (tiles + (kTree ? kJobUnits : 0)) * kv->num_kv_heads > 0x7FFFFFFFull)
+    // an int counts the units: streamed ones, smaller than the tensor cores', or, of tiles alone, theirs (a row
+    // tile has two jobs at most, prefix and own keys)
+    const uint64_t unit_rows = shape.tiles ? kTcRows : shape.few_rows;
+    const uint64_t unit_keys = !shape.tiles ? 16 : (shape.hd > 128 ? TensorShape<256>::kKeys : TensorShape<128>::kKeys);
+    const uint64_t row_tiles = T * G / unit_rows + std::min<uint64_t>(T, num_requests);
+    const uint64_t tiles = (uint64_t)max_pages * kv->page_size / unit_keys + prefix_len / unit_keys + 2;
+    if (row_tiles * (tiles + (kTree ? 2 * kJobUnits : 0)) * kv->num_kv_heads > 0x7FFFFFFFull)
         return fail(ctx, TF_ERR_UNSUPPORTED_SHAPE, "%s: too many keys", name);
     const Layout l = layout_of(ctx, kv, num_q_heads, T, shape);
     const size_t need = l.bytes;

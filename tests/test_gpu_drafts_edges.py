@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_gpu_draft_decoder import VOCAB, Round, make, model, padded  # noqa: F401 (model: a fixture)
-from test_gpu_drafts import flags, way, words_of
+from test_gpu_drafts import TreeBatch, flags, way, words_of
 from test_gpu_logit_rules import Rows
 from test_gpu_paged import i32, no_device_error
 
@@ -169,6 +169,18 @@ def test_a_prompt_in_a_step_is_no_output(cuda, model, given, prompt_nodes, asked
                 want[t] = z - freq[b] * c - (pres[b] if c else np.float32(0))
             np.testing.assert_array_equal(got[starts[b] + i], want)
             assert int(dec.tokens[starts[b] + i]) == int(want.argmax())
+    no_device_error()
+
+
+# -------------------------------------------------------------- attention ----
+def test_trees_of_many_nodes_behind_wide_tables(cuda):
+    """65 trees of 64 under tables of a million positions: what the tables could hold counts by tiles of 128 rows
+    and the keys of a unit, and the answer is that of tables as wide as the requests are long."""
+    batch = TreeBatch(20, [64 + 3 * b for b in range(65)], [64] * 65, 64, 8, 64, "bf16", 16)
+    out, lse = batch.run()
+    batch.table = np.concatenate([batch.table, np.full((65, 65536 - batch.table.shape[1]), -1)], 1)
+    wide, lse_wide = batch.run()
+    assert torch.equal(wide, out) and torch.equal(lse_wide, lse)
     no_device_error()
 
 
