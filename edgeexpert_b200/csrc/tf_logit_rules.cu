@@ -33,6 +33,8 @@ struct Gathered {
     long long* base;   // [B]: a request's first entry
     uint4* entries;    // token, count and flags, bias; in the order of the tokens
     uint32_t* known;   // [B][known_words]: the tokens with an entry (for logits of 16 bits)
+    int* output_ids;   // [T]: the drafted tokens, -1 in the place of a prompt's (if there are prompts among
+                       // them; to look at prompt_nodes again would take the rows 2 us of 120)
     // of the second kernel, 0 at its start:
     unsigned long long* best;  // [T]: the best of a row's chunks
     uint32_t* done;            // [T]: how many there are
@@ -59,6 +61,7 @@ struct RulesParams {
     const int* token_ids;
     const uint32_t* ancestors;
     const int* prompt_nodes;
+    const int* output_ids;  // token_ids, or what is gathered of them
     int* tokens;
     Gathered g;
     uint32_t* err;
@@ -139,7 +142,6 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
     griddep_launch_dependents();  // after the wait: the next kernel may read the logits at once
     const int s0 = p.starts[b], s1 = p.starts[b + 1];
     const int lens = p.history ? p.history_lens[b] : 0, prompts = p.prompt_lens ? p.prompt_lens[b] : 0;
-    const int first_nodes = p.prompt_nodes ? p.prompt_nodes[b] : 0;
     const int bias0 = p.bias_count ? p.bias_starts[b] : 0, bias1 = p.bias_count ? p.bias_starts[b + 1] : 0;
     const int start = max(0, min(s0, p.T)), n = max(start, min(s1, p.T)) - start, used = min(n, p.max_query);
     if (n > used && tid == 0) atomicOr(p.err, kErrBadTree);
@@ -154,7 +156,6 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
     }
     if (used == 0) return;
     const int nodes = p.token_ids ? min(used, p.words * 32) : 0;
-    const bool in_prompt = tid < first_nodes;  // this thread's node
     const int len = max(0, min(lens, p.max_history)), prompt = max(0, min(prompts, len));
     const int b0 = max(0, min(bias0, p.bias_count)), b1 = max(b0, min(bias1, p.bias_count));
     // what the threads need of the lists, all of it asked for at once
@@ -180,7 +181,14 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
     history.each([&](int token, int at) { mark(at < prompt ? asked : known, token); });
     if (b0 + tid < b1) mark(known, bias_token);
     for (int i = b0 + kGatherThreads + tid; i < b1; i += kGatherThreads) mark(known, p.bias_tokens[i]);
-    if (tid < nodes) mark(in_prompt ? asked : known, drafted);
+    if (tid < nodes) {
+        mark(known, drafted);
+        if (p.prompt_nodes) {
+            const bool in_prompt = tid < p.prompt_nodes[b];
+            if (in_prompt) mark(asked, drafted);
+            p.g.output_ids[start + tid] = in_prompt ? -1 : drafted;
+        }
+    }
     __syncthreads();
 
     // ranks: thread i has the words [i * per, (i + 1) * per)
@@ -243,14 +251,14 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
         if (tid < nodes)
             with_rank(drafted, [&](uint32_t k) {
                 token_of[k] = (uint32_t)drafted;
-                if (!in_prompt) atomicOr(&said[k], kDrafted);
+                atomicOr(&said[k], kDrafted);
             });
         __syncthreads();
 #pragma unroll 4
         for (int k = tid; k < ranks; k += kGatherThreads) {
             const uint32_t e = token_of[k];
-            const uint32_t flag = asked[e >> 5] >> (e & 31) & 1u ? kInPrompt : 0u;
-            p.g.entries[base + k0 + k] = make_uint4(e, said[k] | flag, 0u, 0u);
+            const bool in_prompt = asked[e >> 5] >> (e & 31) & 1u;
+            p.g.entries[base + k0 + k] = make_uint4(e, said[k] | (in_prompt ? kInPrompt : 0u), 0u, 0u);
         }
         __syncthreads();
         if (b0 < b1 || k0 + p.window < listed) {
@@ -336,6 +344,10 @@ constexpr int kStages = 3;  // chunks of a CTA in shared memory
 template <typename T>
 constexpr int kChunk = kFly * kRowThreads * Vec<T>::N;  // 4096 or 8192 tokens
 constexpr int kRead = 4;    // entries that a thread loads at once
+// In the place of an entry that there is not.  Its distance to a chunk's first token, unsigned, is beyond
+// any chunk, also where that token is up to seven before the row's own (~0 came round to those, which are
+// another row's); an entry's token is not below the row's first.
+constexpr uint32_t kNoToken = 0x7FFFFFFFu;
 
 __device__ __forceinline__ float largest(const Vec<float>& x) {  // (NaN is passed over)
     return fmaxf(fmaxf(x.e[0], x.e[1]), fmaxf(x.e[2], x.e[3]));
@@ -450,17 +462,15 @@ __device__ __forceinline__ float quotient(float z, float r, double r_inverse) {
     return (float)(better == better ? better : q);
 }
 
-// How often a token was drafted on a row's way through its request's tree of `most` nodes at the most,
-// the prompt's left out.
-__device__ __noinline__ int drafted_before(const int* starts, int rows, int most, const int* prompt_nodes,
-                                           const uint32_t* way, const int* ids, int token) {
+// How often a token was drafted on a row's way through its request's tree of `most` nodes at the most.
+__device__ __noinline__ int drafted_before(const int* starts, int rows, int most, const uint32_t* way, const int* ids,
+                                           int token) {
     const int start = max(0, min(starts[0], rows)), nodes = min(min(max(start, starts[1]), rows) - start, most);
-    const int first = prompt_nodes ? *prompt_nodes : 0;
     int count = 0;
     for (int w = 0; w * 32 < nodes; ++w)
         for (uint32_t m = way[w]; m; m &= m - 1) {
             const int j = w * 32 + __ffs(m) - 1;
-            if (j >= first && j < nodes) count += ids[start + j] == token;
+            if (j < nodes) count += ids[start + j] == token;
         }
     return count;
 }
@@ -553,7 +563,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
     auto fetch = [&](uint4 (&x)[kRead], int k, int k1) {
 #pragma unroll
         for (int u = 0; u < kRead; ++u)
-            x[u] = k + u * kRowThreads < k1 ? p.g.entries[base + k + u * kRowThreads] : make_uint4(~0u, 0u, 0u, 0u);
+            x[u] = k + u * kRowThreads < k1 ? p.g.entries[base + k + u * kRowThreads] : make_uint4(kNoToken, 0u, 0u, 0u);
     };
     fetch(x, now.k0 + tid, now.k1);
 
@@ -598,10 +608,6 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
 
         // ---- the entries ---------------------------------------------------------------------
         if (any) {
-            // Places count from the row's own first token here: what the chunk has before it is of the row
-            // before, and the token of no entry (~0) is beyond any place, however the row lies.
-            T* const own = stage.x + lo;
-            const uint32_t own_first = (uint32_t)(c0 + lo), own_len = (uint32_t)(hi - lo);
             float said_best = -INFINITY;  // (of equals the first, which is the lower token)
             int said_token = 0;
 #pragma unroll 1
@@ -612,28 +618,27 @@ __global__ void __launch_bounds__(kRowThreads, 4) logit_rules_kernel(const __gri
                 uint32_t drafted = 0u;
 #pragma unroll
                 for (int u = 0; u < kRead; ++u) {
-                    const uint32_t e = x[u].x - own_first;
-                    z[u] = e < own_len ? to_float(own[e]) : NAN;
+                    const uint32_t e = x[u].x - (uint32_t)c0;
+                    z[u] = e < (uint32_t)hi ? to_float(stage.x[e]) : NAN;
                     drafted |= x[u].y & kDrafted;
                 }
                 if (drafted) {
 #pragma unroll
                     for (int u = 0; u < kRead; ++u)
-                        if ((x[u].y & kDrafted) && x[u].x - own_first < own_len)
+                        if ((x[u].y & kDrafted) && x[u].x - (uint32_t)c0 < (uint32_t)hi)
                             x[u].y += drafted_before(p.starts + b, p.T, min(p.max_query, p.words * 32),
-                                                     p.prompt_nodes ? p.prompt_nodes + b : nullptr,
-                                                     p.ancestors + (long long)at.row * p.words, p.token_ids, (int)x[u].x);
+                                                     p.ancestors + (long long)at.row * p.words, p.output_ids, (int)x[u].x);
                 }
                 float top = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < kRead; ++u) {
-                    const uint32_t e = x[u].x - own_first, count = x[u].y & kCount;
+                    const uint32_t e = x[u].x - (uint32_t)c0, count = x[u].y & kCount;
                     const float divided = quotient(z[u], rep, rep_inverse), times = __fmul_rn(z[u], rep);
                     float r = count || (x[u].y & kInPrompt) ? (z[u] > 0.f ? divided : times) : z[u];
                     r = __fsub_rn(r, __fmul_rn(freq, (float)count));
                     r = count ? __fsub_rn(r, pres) : r;
                     r = __fadd_rn(r, __uint_as_float(x[u].z));
-                    if (e < own_len) own[e] = rounded<T>(r);
+                    if (e < (uint32_t)hi) stage.x[e] = rounded<T>(r);
                     z[u] = r;
                     top = fmaxf(top, r);
                 }
@@ -765,7 +770,7 @@ inline uint32_t known_words_of(uint32_t V) { return (V + 127) / 128 * 4; }
 
 // The workspace, for any type of logits; places are 16-byte aligned.
 struct RulesLayout {
-    size_t request, begin, base, entries, known, best, done, bytes;
+    size_t request, begin, base, entries, known, output_ids, best, done, bytes;
 };
 RulesLayout layout_of(uint32_t T, uint32_t V, uint32_t B, uint32_t max_history, uint32_t bias_count) {
     RulesLayout l;
@@ -781,6 +786,7 @@ RulesLayout layout_of(uint32_t T, uint32_t V, uint32_t B, uint32_t max_history, 
     l.base = take((size_t)B * sizeof(long long));
     l.entries = take(((size_t)B * max_history + bias_count + T) * sizeof(uint4));
     l.known = take((size_t)B * known_words_of(V) * sizeof(uint32_t));
+    l.output_ids = take((size_t)T * sizeof(int));
     l.best = take((size_t)T * sizeof(unsigned long long));
     l.done = take((size_t)T * sizeof(uint32_t));
     l.bytes = at;
@@ -873,6 +879,8 @@ tf_status tf_logit_rules_apply(tf_context* ctx, const void* logits, uint64_t log
     p.g.base = reinterpret_cast<long long*>(w + l.base);
     p.g.entries = reinterpret_cast<uint4*>(w + l.entries);
     p.g.known = reinterpret_cast<uint32_t*>(w + l.known);
+    p.g.output_ids = reinterpret_cast<int*>(w + l.output_ids);
+    p.output_ids = r.prompt_nodes ? p.g.output_ids : p.token_ids;
     p.g.best = reinterpret_cast<unsigned long long*>(w + l.best);
     p.g.done = reinterpret_cast<uint32_t*>(w + l.done);
     p.err = ctx->d_err;
