@@ -237,7 +237,10 @@ struct TreeSegment {
 // kTree: what a job costs besides its units (Q in, the pipeline filled and drained, O out), as units:
 // the work is dealt by both, so that CTAs with many short jobs get fewer.  24 trees of 20 to 40 behind
 // 4096 shared positions and up to 1000 of their own (16 / 4 heads of 128): 82 us; with 1 113, with 3 91,
-// with 12 86.  16 trees of 16 behind up to 4096 (16 / 8 heads of 256): 78, 96, 82 and 82.
+// with 12 86.  16 trees of 16 behind up to 4096 (16 / 8 heads of 256): 78, 96, 82 and 82.  Heads of 64,
+// whose units are 128 keys (16 / 2 heads, 6 / 1 / 3 / 12): 24 trees behind 4096 shared 72, 81, 70 and 74;
+// 16 of 16 behind up to 4096 30, 32, 31 and 33; 61 of 1 to 5 behind up to 3000 40, 39, 37 and 45, under a
+// window of 1024 35 with any.
 constexpr int kJobUnits = 6;
 template <typename T, bool kTree>
 __device__ __forceinline__ int tree_slots(const AttnParams<T, kTree>& p, const TreeSegment& s) {
@@ -327,8 +330,8 @@ __device__ __forceinline__ float max_of(float a, float b, float c) {
     return r;
 }
 
-// kTree: the weights of a unit's N keys for a row (the calling thread's), in place of its scores at
-// column `scol`, and m and d brought up to date; ok 0 if a wait gave up.  The row sees keys [lo, hi) and,
+// kTree: the weights of a unit's N keys for a row (the calling thread's), rounded to the cache's type for
+// the product with V (d sums them unrounded, as for prompts), in place of its scores at column `scol`, and m and d brought up to date; ok 0 if a wait gave up.  The row sees keys [lo, hi) and,
 // from key `node_at` on, the nodes of its `ancestors`, up to key `end`.  P is written over the scores.
 struct TreeSums {
     float m, d;

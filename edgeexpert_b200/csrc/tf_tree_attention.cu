@@ -5,12 +5,13 @@
 //   leaves and the nodes p whose bit is set in j's ancestors.
 // A row's nodes are its request's last positions, so only the units that reach them look
 // at bits; those before are history, seen whole or from the window's first position on.
-// Trees of more than eight rows per KV head go to tree_tiles_kernel (tcgen05), batches of
-// smaller ones to the streaming warps.
+// Batches whose bound on a request's nodes is above eight rows per KV head go to
+// tree_tiles_kernel (tcgen05), others to the streaming warps (200 single nodes behind up to
+// 2048, 1.68 GB: 269 us, 6.3 TB/s; 64 of 1 to 4 behind up to 4096, 1.08 GB: 182 us, 5.9 TB/s).
 // Measured (calls among others): 16 trees of 16 behind up to 4096 positions, 16 / 8 heads
 // of 256, 275 MB: 62 to 64 us, HBM inside the jobs; 4 of 60 to 64 behind 32 to 64 thousand,
-// 1.62 GB: 300 to 322 us, 5.0 to 5.4 TB/s; 24 of 20 to 40 behind 4096 shared, 16 / 4 heads
-// of 128: 73 us, bound by the tiles' way out of L2 and the ends of the jobs; one of 12
+// 1.62 GB: 300 to 333 us by machine, 4.9 to 5.4 TB/s; 24 of 20 to 40 behind 4096 shared, 16 / 4 heads
+// of 128: 73 to 76 us, bound by the tiles' way out of L2 and the ends of the jobs; one of 12
 // behind 700: 16.7 us, latency.  Two threads a row, with half the keys each: 0 to 4 % faster
 // for these 24, 3 % slower for the long histories, 5 % for one tree.
 #include "tf_prefix_kernels.cuh"
