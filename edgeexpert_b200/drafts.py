@@ -190,7 +190,8 @@ class DraftDecoder(PagedDecoder):
         tokens are the prompt's, 1 for a prompt of one token, 0 for known tokens of the output).  self.logits
         then holds the logits under the rules, self.tokens the choice after every node.
 
-        Returns (counts, new_tokens), on the device: how many nodes of each request are kept, and
+        Returns (counts, new_tokens), on the device and the decoder's own, for the next step writes there
+        again: how many nodes of each request are kept, and
         [requests][max_query] the counts - given + 1 tokens that are new, -1 behind them.  The last of
         them is not in the cache yet: it is the next root.  self.paths: which nodes are kept.  The cache
         then holds the kept nodes alone; rows i of this step were tokens draft_starts[b] .. of request b,

@@ -272,3 +272,31 @@ def test_refused_rules_change_nothing(cuda, model):  # noqa: F811
     dec.draft(ids[:5], parents[:5], i32([2, 10, 0]), rules=dict(allowed=bits, repetition=f))
     assert cache.seq_lens.tolist()[0] == 2 and cache.seq_lens.tolist()[1] >= 6 and cache.seq_lens.tolist()[2] == 0
     no_device_error()
+
+
+def test_a_step_by_another_stream(cuda, model):  # noqa: F811
+    """Prompts, trees, masks and penalties on a stream of their own, with the other stream busy: the same bits."""
+    weights, _ = model
+    rng = np.random.default_rng(12)
+    r = Round(rng, [rng.integers(VOCAB, size=n) for n in (4, 1, 6)], (5, 9, 0))
+    bits, rows = r.masks()
+    f = [torch.tensor(x, device="cuda") for x in ([1.5, 2.0, 1.25], [0.5, 0.25, 1.0], [0.25, 0.5, 0.125])]
+    given, answers = i32([len(k) for k in r.known]), []
+    rules = dict(allowed=torch.from_numpy(bits).cuda(), allowed_rows=i32(rows), repetition=f[0], presence=f[1], frequency=f[2])
+    args = i32(np.concatenate(r.tokens)), i32(np.concatenate(r.trees)), i32([len(t) for t in r.tokens])
+    for stream in (None, torch.cuda.Stream()):
+        dec, cache = make(weights, 3, 24, 6, 32, 4, 16)
+        noise = torch.randn(2000, 2000, device="cuda")
+        torch.cuda.synchronize()
+        if stream is not None:
+            for _ in range(20):
+                noise = noise @ noise / 50
+        dec.draft(*args, given=given, rules=rules, stream=stream)
+        torch.cuda.synchronize()
+        n = sum(map(len, r.tokens))
+        answers.append([x.clone() for x in (dec.counts, dec.new_tokens, dec.logits[:n], cache.seq_lens, cache.k, cache.v)])
+    assert all(torch.equal(a, b) for a, b in zip(*answers))
+    for b in range(3):
+        path, fresh = r.expected(b)
+        assert answers[0][0].tolist()[b] == len(path) and answers[0][1][b, :len(fresh)].tolist() == fresh
+    no_device_error()
